@@ -701,6 +701,8 @@ int64_t num_sms() { return kapsl::gemm_num_sms(); }
 
 }  // namespace
 
+void register_latent(pybind11::module_& m);  // bindings_latent.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "kapsl_sdk_b200 sm_100a kernels";
   m.def("rmsnorm", &rmsnorm, "RMSNorm (optionally residual += x first)", py::arg("out"), py::arg("x"),
@@ -755,5 +757,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("symm_close", &symm_close);
   m.def("tensor_from_ptr", &tensor_from_ptr);
   m.def("launch_count", &launch_count, "kernels launched through this library so far");
+  register_latent(m);
   m.def("num_sms", &num_sms);
 }

@@ -19,6 +19,76 @@ void launch_rope_kv_write(__nv_bfloat16* qkv, int64_t qkv_stride, const int32_t*
                           const float* cos_sin, __nv_bfloat16* k_cache, __nv_bfloat16* v_cache, int T, int Hq,
                           int Hkv, int D, int block_size, cudaStream_t st);
 
+// Rotary positions of strided heads x [T, H, D] -> y (rope.cu).  P = width of the cos | sin
+// table = rotated dims, from `offset`; strides in elements.
+struct RopeArgs {
+  const void* x = nullptr;
+  void* y = nullptr;
+  int64_t xs_t = 0, xs_h = 0, ys_t = 0, ys_h = 0;
+  const int32_t* positions = nullptr;
+  const float* cos_sin = nullptr;
+  int max_pos = 0;
+  int64_t T = 0;
+  int H = 0, D = 0, P = 0, offset = 0;
+  bool interleaved = false, in_place = false;
+  int* err = nullptr;
+};
+void launch_rope(const RopeArgs& a, int dtype, cudaStream_t st);  // dtype: 0 bf16, 1 fp16, 2 fp32
+// latent cache write: RopeArgs holds the query heads' rotary part (D = P = 64)
+void launch_rope_latent_write(const RopeArgs& a, const __nv_bfloat16* kv, int64_t kv_stride, const int64_t* slots,
+                              const __nv_bfloat16* w, float eps, __nv_bfloat16* cache, int64_t num_slots, int R,
+                              cudaStream_t st);
+
+// Latent attention over a paged cache [blocks, page, R + 64] (latent_decode.cu, latent_prefill.cu).
+// Head products with the key and value expansions w [H, 256, R]:
+//   absorb: qa[b, h, :R] = q[b, h, :128] . w[h, :128], qa[b, h, R:] = q[b, h, 128:]
+//   out:    out[b, h, :] = w[h, 128:] . o[b, h, :R]
+struct LatentDecode {
+  const __nv_bfloat16* q = nullptr;  // [B, H * 192], pitch q_stride
+  int64_t q_stride = 0;
+  const __nv_bfloat16* cache = nullptr;
+  int64_t num_blocks = 0;
+  int page = 0, R = 0;
+  const __nv_bfloat16* w = nullptr;
+  const int32_t* block_tables = nullptr;
+  int max_blocks = 0;
+  const int32_t* ctx_lens = nullptr;
+  __nv_bfloat16* out = nullptr;  // [B, H * 128], pitch out_stride
+  int64_t out_stride = 0;
+  int B = 0, H = 0, nsplit = 1;
+  float scale = 0.f;
+  void* workspace = nullptr;  // latent_decode_workspace_bytes
+  int* err = nullptr;
+};
+int latent_decode_num_splits(int B, int H, int R, int max_ctx, int num_sms);
+size_t latent_decode_workspace_bytes(int B, int H, int R, int nsplit);
+void launch_latent_decode(const LatentDecode& a, cudaStream_t st);
+
+// Copies each sequence's context rows out of the paged cache into rows [S.kv_start, + ctx)
+// of `rows` [total, R + 64]; pad rows up to the next multiple of 16 are zero.
+void launch_latent_gather(const __nv_bfloat16* cache, int64_t num_blocks, int page, int R, const int32_t* seq_info,
+                          int nseq, const int32_t* block_tables, int max_blocks, __nv_bfloat16* rows, int64_t total,
+                          int* err, cudaStream_t st);
+// Causal attention of the chunk over expanded keys and values: kv [total, heads * 256]
+// (key 128 | value 128 a head), shared rotary keys rows[:, R:].
+struct LatentPrefill {
+  const __nv_bfloat16* q = nullptr;  // first of these heads: [T, heads * 192], pitch q_stride
+  int64_t q_stride = 0, T = 0;
+  const __nv_bfloat16* kv = nullptr;
+  int64_t kv_stride = 0, kv_rows = 0;
+  const __nv_bfloat16* rows = nullptr;
+  int R = 0;
+  const int32_t* work = nullptr;      // [nwork, 2] = (sequence, first token of the tile)
+  int nwork = 0;
+  const int32_t* seq_info = nullptr;  // [S, 5] = (first q row, tokens, context, block-table row, first kv row)
+  __nv_bfloat16* out = nullptr;
+  int64_t out_stride = 0;
+  int heads = 0;
+  float scale = 0.f;
+  int* err = nullptr;
+};
+void launch_latent_prefill(const LatentPrefill& a, cudaStream_t st);
+
 void launch_silu_mul(__nv_bfloat16* out, const __nv_bfloat16* x, int T, int F, cudaStream_t st);
 
 // rows t < n_src with src_rows[t] >= 0 read their token id from prev_tokens[src_rows[t]]

@@ -8,7 +8,8 @@ them as the oracle.
 from __future__ import annotations
 
 import math
-from typing import Optional
+from dataclasses import dataclass
+from typing import Optional, Sequence
 
 import torch
 
@@ -53,6 +54,9 @@ DEVICE_ERRORS = {
     50: "vocab-parallel sampler: a peer's candidates did not arrive",
     **{c: "Q4_K GEMM pipeline wait ran out" for c in range(60, 67)},
     **{c: "tcgen05 prefill attention pipeline wait ran out" for c in range(71, 79)},
+    80: "rotary positions: a position lies outside the cos/sin table (its row was not rotated)",
+    81: "latent cache write: a slot lies outside the cache (its row was not written)",
+    82: "latent attention: a block table entry lies outside the cache (its keys were skipped)",
 }
 
 
@@ -84,6 +88,40 @@ def rope_kv_write(qkv: torch.Tensor, positions: torch.Tensor, slots: Optional[to
                   head_dim: int) -> None:
     """Rotate q and k of ``qkv`` in place and write k, v into the paged cache."""
     cuda_ops().rope_kv_write(qkv, positions, slots, cos_sin, k_cache, v_cache, num_heads, num_kv_heads, head_dim)
+
+
+def rope(x: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor, offset: int = 0, interleaved: bool = False,
+         out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Rotary positions of the heads of ``x`` [T, H, D] (bf16, fp16 or fp32; any token and head
+    strides): the dims ``[offset, offset + P)`` of every head turn by their token's angles,
+    the others are copied.  ``cos_sin`` [positions, P] comes from
+    :func:`~kapsl_sdk_b200.ops.reference.rope_cos_sin` (scaled tables included), so its
+    width is the rotated part.  Pairs are ``(i, i + P/2)``, or ``(2i, 2i + 1)`` with
+    ``interleaved``.  ``out=x`` rotates in place.  A position outside the table leaves its
+    row unrotated and records device error 80."""
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    cuda_ops().rope(out, x, positions, cos_sin, int(offset), bool(interleaved), error_buffer(x.device))
+    return out
+
+
+def rope_latent_write(q_rope: torch.Tensor, kv: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor,
+                      cos_sin: torch.Tensor, weight: torch.Tensor, eps: float, cache: torch.Tensor,
+                      interleaved: bool = False, q_out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """One step's cache write of latent attention, with the queries' rotation.
+
+    ``kv`` [T, R + 64] (R 256 or 512) is a token's compressed row: the first R values are RMS-normed
+    with ``weight``, the last 64 rotated by ``positions``, and the row goes to
+    ``cache`` [blocks, page, R + 64] at ``slots[t]`` = block * page + offset (a negative slot
+    writes nothing; one past the cache is skipped and records device error 81).
+    ``q_rope`` [T, H, 64], the rotary part of the query heads (usually a view
+    ``q.view(T, H, 192)[..., 128:]``), is rotated in place, or into ``q_out``.
+    Two tokens of one call must not share a slot."""
+    if q_out is None:
+        q_out = q_rope
+    cuda_ops().rope_latent_write(q_rope, q_out, kv, positions, slots, cos_sin, weight, float(eps), cache,
+                                 bool(interleaved), error_buffer(q_rope.device))
+    return q_out
 
 
 def silu_mul(x: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -296,6 +334,119 @@ def prefill_tc_tile(num_heads: int, num_kv_heads: int) -> int:
     """Query tokens per CTA of the tcgen05 prefill kernel: its 128 MMA rows hold
     every query head of one KV head for floor(128 / group) tokens."""
     return 128 // (num_heads // num_kv_heads)
+
+
+# ------------------------------------------------------------ latent attention
+def latent_decode_attention(q: torch.Tensor, cache: torch.Tensor, w_kv_b: torch.Tensor, block_tables: torch.Tensor,
+                            ctx_lens: torch.Tensor, num_heads: int, scale: Optional[float] = None,
+                            out: Optional[torch.Tensor] = None, num_splits: int = 0,
+                            max_ctx: Optional[int] = None) -> torch.Tensor:
+    """Latent attention of one query token per row, absorbed form.
+
+    ``cache`` [blocks, page, R + 64] holds one row a token (:func:`rope_latent_write`; R 256 or
+    512, pages of 16, 32 or 64).  ``w_kv_b`` [H * 256, R] expands a latent to every head's
+    128 key and 128 value dims; here its key half moves to the query's side and its value
+    half is applied to the attended latents, so nothing is expanded per cached token.
+    ``q`` [B, H * 192] has 128 position-free and 64 rotated dims a head; ``out`` is
+    [B, H * 128].  Rows with ``ctx_lens`` 0 (a padded batch) give zeros.  ``max_ctx`` (a host
+    number, default the block tables' width) only chooses how many splits the context is cut into.
+    A block table entry outside the cache is skipped and records device error 82."""
+    if scale is None:
+        scale = 1.0 / math.sqrt(192)
+    B = q.shape[0]
+    if out is None:
+        out = torch.empty(B, num_heads * 128, dtype=q.dtype, device=q.device)
+    c = cuda_ops()
+    R = cache.shape[-1] - 64
+    if num_splits <= 0:
+        mc = int(max_ctx) if max_ctx is not None else int(block_tables.shape[-1]) * int(cache.shape[1])
+        num_splits = int(c.latent_num_splits(B, num_heads, R, mc))
+    ws = torch.empty(max(1, int(c.latent_workspace_bytes(B, num_heads, R, num_splits))), dtype=torch.uint8,
+                     device=q.device)
+    c.latent_decode_attention(q, cache, w_kv_b, block_tables, ctx_lens, out, num_heads, float(scale), num_splits, ws,
+                              error_buffer(q.device))
+    return out
+
+
+LATENT_PREFILL_TILE = 256  # query tokens a CTA of the expanded-form attention handles
+LATENT_KV_BYTES = 2 << 30  # expanded keys and values held at once; more heads go in further passes
+
+
+@dataclass
+class LatentPrefillPlan:
+    """Tile list and sequence table of one :func:`latent_prefill_attention` call."""
+    work: torch.Tensor      # int32 [n, 2]: (sequence, first token of the tile)
+    seq_info: torch.Tensor  # int32 [S, 5]: (first q row, tokens, context, block-table row, first kv row)
+    rows: int               # q rows up to the last sequence's end
+    tables: int             # block-table rows read
+    max_ctx: int
+    kv_rows: int            # context rows of all sequences, each padded to a multiple of 16
+
+
+def latent_prefill_plan(q_lens: Sequence[int], ctx_lens: Sequence[int], device, q_start: int = 0,
+                        bt_start: int = 0) -> LatentPrefillPlan:
+    """Plan of chunks of ``q_lens[s]`` new tokens at the end of contexts of ``ctx_lens[s]`` tokens
+    (new ones included).  Their q rows follow each other from ``q_start``, their block
+    tables from row ``bt_start`` (a mixed batch has its decode rows first).  The tables are
+    device tensors: reuse them for every layer of a step."""
+    q_lens, ctx_lens = [int(n) for n in q_lens], [int(n) for n in ctx_lens]
+    if len(q_lens) != len(ctx_lens):
+        raise ValueError("latent_prefill_plan: q_lens and ctx_lens differ in length")
+    if q_start < 0 or bt_start < 0:
+        raise ValueError("latent_prefill_plan: negative start")
+    info, work, row, kv = [], [], int(q_start), 0
+    for s, (n, ctx) in enumerate(zip(q_lens, ctx_lens)):
+        if n < 0 or n > ctx:
+            raise ValueError(f"latent_prefill_plan: sequence {s} has {n} new tokens in a context of {ctx}")
+        if n == 0:  # nothing asks for its context
+            ctx = 0
+        info.append((row, n, ctx, bt_start + s, kv))
+        work += [(ctx - n + min(n, t0 + LATENT_PREFILL_TILE), s, t0) for t0 in range(0, n, LATENT_PREFILL_TILE)]
+        row += n
+        kv += -(-ctx // 16) * 16
+    if row >= 2 ** 31 or kv >= 2 ** 31:
+        raise ValueError("latent_prefill_plan: too many rows")
+    work.sort(key=lambda w: -w[0])  # the tiles with the most keys start first
+    dev = torch.device(device)
+    t = torch.tensor([v for w in work for v in w[1:]] + [v for i in info for v in i], dtype=torch.int32).to(dev)
+    return LatentPrefillPlan(work=t[:2 * len(work)].view(-1, 2), seq_info=t[2 * len(work):].view(-1, 5), rows=row,
+                             tables=bt_start + len(info) if info else 0, max_ctx=max([i[2] for i in info], default=0),
+                             kv_rows=kv)
+
+
+def latent_prefill_attention(q: torch.Tensor, cache: torch.Tensor, w_kv_b: torch.Tensor, plan: LatentPrefillPlan,
+                             block_tables: torch.Tensor, num_heads: int, scale: Optional[float] = None,
+                             out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Causal latent attention of chunks of new tokens over the paged latent cache, expanded form.
+
+    The new tokens' rows are in ``cache`` already; arguments as in
+    :func:`latent_decode_attention`, with ``plan`` from :func:`latent_prefill_plan`.  The
+    context's latents are gathered from their pages and expanded by ``w_kv_b`` to keys and
+    values (at most ``LATENT_KV_BYTES`` of them at a time, in passes over the heads).
+    ``out`` rows outside the plan's sequences keep what they held (zeros when ``out`` is
+    allocated here)."""
+    if scale is None:
+        scale = 1.0 / math.sqrt(192)
+    if out is None:
+        out = torch.zeros(q.shape[0], num_heads * 128, dtype=q.dtype, device=q.device)
+    c = cuda_ops()
+    c.check_latent_prefill(q, cache, w_kv_b, block_tables, out, num_heads, plan.rows, plan.tables, plan.max_ctx)
+    if plan.work.shape[0] == 0:
+        return out
+    err = error_buffer(q.device)
+    R = cache.shape[2] - 64
+    rows = torch.empty(plan.kv_rows, R + 64, dtype=torch.bfloat16, device=q.device)
+    c.latent_gather(cache, plan.seq_info, block_tables, rows, err)
+    w = w_kv_b.view(num_heads * 256, R)
+    step = max(1, min(num_heads, LATENT_KV_BYTES // (plan.kv_rows * 512)))
+    kv_buf = torch.empty(plan.kv_rows * step * 256, dtype=torch.bfloat16, device=q.device)
+    for h0 in range(0, num_heads, step):
+        n = min(step, num_heads - h0)
+        kv = kv_buf[:plan.kv_rows * n * 256].view(plan.kv_rows, n * 256)
+        c.gemm(rows[:, :R], w[h0 * 256:(h0 + n) * 256], kv, EPI_PLAIN, None, None, None, err, 0, 0)
+        c.latent_prefill(q[:, h0 * 192:(h0 + n) * 192], kv, rows, plan.work, plan.seq_info,
+                         out[:, h0 * 128:(h0 + n) * 128], n, float(scale), err)
+    return out
 
 
 SAMPLE_MAX_TOP_K = 1024  # top_k above this (or 0, with T > 0) takes the whole-vocabulary path

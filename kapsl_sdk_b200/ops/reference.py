@@ -110,6 +110,43 @@ def apply_rope(x: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor) 
     return torch.cat([x1 * c - x2 * s, x2 * c + x1 * s], dim=-1)
 
 
+def rope(x: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor, offset: int = 0,
+         interleaved: bool = False) -> torch.Tensor:
+    """x [T, H, D]: dims [offset, offset + P) of every head rotated, P = the table's width;
+    pairs (i, i + P/2), or (2i, 2i + 1) with ``interleaved``."""
+    P = cos_sin.shape[1]
+    y = x.float().clone()
+    part = y[..., offset:offset + P]
+    if interleaved:
+        part = torch.cat([part[..., 0::2], part[..., 1::2]], -1)
+    part = apply_rope(part, positions, cos_sin)
+    if interleaved:
+        part = torch.stack(part.chunk(2, -1), -1).flatten(-2)
+    y[..., offset:offset + P] = part
+    return y
+
+
+def latent_row(kv: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor, weight: torch.Tensor, eps: float,
+               interleaved: bool = False) -> torch.Tensor:
+    """Latent cache rows of kv [T, R + 64]: normed latent, rotated shared key."""
+    R = weight.numel()
+    c, _ = rmsnorm(kv[:, :R], weight, eps)
+    k = rope(kv[:, None, R:], positions, cos_sin, interleaved=interleaved)[:, 0]
+    return torch.cat([c, k], -1)
+
+
+def latent_attention(q: torch.Tensor, rows: torch.Tensor, w_kv_b: torch.Tensor, scale: float) -> torch.Tensor:
+    """One sequence's latent attention, expanded form: q [n, H, 192] are the last n of the
+    tokens whose cache rows are rows [ctx, R + 64]; w_kv_b [H * 256, R].  -> [n, H, 128]"""
+    H, R = q.shape[1], rows.shape[1] - 64
+    kv = torch.einsum("tr,hdr->thd", rows[:, :R].float(), w_kv_b.float().view(H, 256, R))
+    k = torch.cat([kv[..., :128], rows[:, None, R:].float().expand(-1, H, -1)], -1)
+    s = torch.einsum("qhd,khd->hqk", q.float(), k) * scale
+    pos = torch.arange(rows.shape[0] - q.shape[0], rows.shape[0], device=q.device)
+    s = s.masked_fill(torch.arange(rows.shape[0], device=q.device)[None, :] > pos[:, None], float("-inf"))
+    return torch.einsum("hqk,khd->qhd", torch.softmax(s, -1), kv[..., 128:])
+
+
 def silu_mul(x: torch.Tensor) -> torch.Tensor:
     F = x.shape[-1] // 2
     g, u = x[..., :F].float(), x[..., F:].float()

@@ -1,0 +1,68 @@
+"""Latent attention's plans and plain forms on the CPU (no GPU needed)."""
+import math
+
+import pytest
+import torch
+
+from kapsl_sdk_b200 import ops
+from kapsl_sdk_b200.ops import reference as ref
+
+
+def test_plan_rows_and_tiles():
+    p = ops.latent_prefill_plan([300, 0, 1, 17], [557, 40, 900, 17], device="cpu", q_start=5, bt_start=2)
+    # contexts start at multiples of 16; a sequence without new tokens needs no context
+    assert p.seq_info.tolist() == [[5, 300, 557, 2, 0], [305, 0, 0, 3, 560], [305, 1, 900, 4, 560],
+                                   [306, 17, 17, 5, 1472]]
+    assert (p.rows, p.tables, p.max_ctx, p.kv_rows) == (323, 6, 900, 1504)
+    # every query row in exactly one tile, most keys first
+    got = [(s, t) for s, t in p.work.tolist()]
+    assert got == [(2, 0), (0, 256), (0, 0), (3, 0)]
+
+
+def test_plan_of_nothing():
+    p = ops.latent_prefill_plan([], [], device="cpu")
+    assert p.work.shape == (0, 2) and p.seq_info.shape == (0, 5) and p.kv_rows == 0 and p.tables == 0
+    p = ops.latent_prefill_plan([0, 0], [0, 7], device="cpu")
+    assert p.work.shape == (0, 2) and p.kv_rows == 0
+
+
+@pytest.mark.parametrize("q_lens,ctx_lens", [([5], [4]), ([-1], [4]), ([1, 2], [3])])
+def test_plan_refuses(q_lens, ctx_lens):
+    with pytest.raises(ValueError):
+        ops.latent_prefill_plan(q_lens, ctx_lens, device="cpu")
+    with pytest.raises(ValueError):
+        ops.latent_prefill_plan([1], [1], device="cpu", q_start=-1)
+
+
+def test_reference_rope_layouts():
+    # the interleaved layout is the half layout of permuted dims
+    g = torch.Generator().manual_seed(0)
+    x = torch.randn(9, 3, 80, generator=g)
+    pos = torch.randint(0, 50, (9,), generator=g)
+    cs = ref.rope_cos_sin(50, 32, 10000.0)
+    il = ref.rope(x, pos, cs, offset=16, interleaved=True)
+    assert torch.equal(il[..., :16], x[..., :16]) and torch.equal(il[..., 48:], x[..., 48:])
+    perm = torch.cat([torch.arange(0, 32, 2), torch.arange(1, 32, 2)])
+    half = ref.rope(x[..., 16:48][..., perm], pos, cs)
+    assert torch.equal(il[..., 16:48][..., perm], half)
+    # against the complex product, in 64 bits
+    z = torch.view_as_complex(x[..., 16:48].double().reshape(9, 3, 16, 2))
+    c = cs[pos].double()
+    y = torch.view_as_real(z * torch.complex(c[:, None, :16], c[:, None, 16:])).reshape(9, 3, 32)
+    assert (il[..., 16:48] - y).abs().max() < 4 * 2.0 ** -24 * 8
+
+
+def test_reference_forms_agree():
+    """The absorbed order of the products gives the expanded form's result."""
+    g = torch.Generator().manual_seed(1)
+    H, R, ctx, n = 3, 256, 37, 5
+    q = torch.randn(n, H, 192, generator=g).double()
+    rows = torch.randn(ctx, R + 64, generator=g).double()
+    w = (torch.randn(H, 256, R, generator=g) / math.sqrt(R)).double()
+    got = ref.latent_attention(q, rows, w.reshape(-1, R), 0.07)
+    for i in range(n):
+        c = rows[:ctx - n + i + 1]
+        qa = torch.cat([torch.einsum("hd,hdr->hr", q[i, :, :128], w[:, :128]), q[i, :, 128:]], -1)
+        o = torch.softmax(qa @ c.T * 0.07, -1) @ c[:, :R]
+        exp = torch.einsum("hr,hvr->hv", o, w[:, 128:])
+        assert (got[i].double() - exp).abs().max() < 1e-4

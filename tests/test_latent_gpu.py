@@ -1,0 +1,589 @@
+"""Rotary positions, the latent cache write and both forms of latent attention against
+plain 64-bit implementations.
+
+Tolerances.  A rounding to a type with unit u = eps / 2 errs by at most u relative, and as
+the errors of many roundings are independent and spread over [-u, u], each counts with a
+standard deviation of at most u / sqrt(3).  For attention the test carries the
+variance of every rounding that the kernels make (listed at each oracle) to the
+output in 64 bits and allows 8 standard deviations: an error of the kernel's own, a
+key too many or too few, a wrong page or a wrong weight is far outside.
+fp32 sums of up to 600 terms err by at most 600 * 2^-24 < 2^-14 of the terms' absolute sum.
+"""
+import math
+import random
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = torch.finfo(torch.bfloat16).eps / 2
+F32 = 2.0 ** -14
+NAN = float("nan")
+
+
+@pytest.fixture(scope="module")
+def dev():
+    from kapsl_sdk_b200._ext import cuda_ops
+
+    cuda_ops()
+    return torch.device("cuda", 0)
+
+
+def within(got, exp, tol):
+    err = (got.double() - exp).abs()
+    assert torch.isfinite(got.double()).all()
+    bad = int((err > tol).sum())
+    worst = float((err / tol.clamp_min(1e-30)).max()) if err.numel() else 0.0
+    assert bad == 0, f"{bad} values off, worst {worst:.3g} x"
+
+
+def no_error(dev):
+    from kapsl_sdk_b200 import ops
+
+    torch.cuda.synchronize()
+    assert ops.check_errors(dev) == 0
+
+
+# ------------------------------------------------------------------------------ rope
+def rope64(x, pos, cs, offset, interleaved):
+    y = x.double().clone()
+    P = cs.shape[1]
+    v = y[..., offset:offset + P]
+    c, s = cs[pos.long()].double()[:, None, :P // 2], cs[pos.long()].double()[:, None, P // 2:]
+    a, b = (v[..., 0::2], v[..., 1::2]) if interleaved else (v[..., :P // 2], v[..., P // 2:])
+    ya, yb = a * c - b * s, b * c + a * s
+    mag = a.abs() + b.abs()
+    y[..., offset:offset + P] = torch.stack([ya, yb], -1).flatten(-2) if interleaved else torch.cat([ya, yb], -1)
+    m = torch.zeros_like(y)
+    m[..., offset:offset + P] = torch.stack([mag, mag], -1).flatten(-2) if interleaved else torch.cat([mag, mag], -1)
+    return y, m
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("T,H,D,P,offset", [(1, 1, 64, 64, 0), (5, 3, 192, 64, 128), (130, 28, 128, 32, 0),
+                                            (33, 7, 80, 16, 40), (9, 2, 37, 10, 5), (3, 5, 7, 2, 5), (2, 1, 2, 2, 0),
+                                            (17, 4, 256, 256, 0), (40, 1, 96, 24, 8)])
+def test_rope(dev, dtype, interleaved, T, H, D, P, offset):
+    """One rounding (u |y|) and two fp32 products and a sum (3 * 2^-24 of |a| + |b|).  Below the
+    smallest normal number t the values are t * eps apart whatever their size, so a rounding
+    there errs by up to t * eps / 2 = t * u (fp16: 2^-14 * 2^-11 = 2^-25)."""
+    from kapsl_sdk_b200 import ops
+    from kapsl_sdk_b200.ops import reference as ref
+
+    g = torch.Generator(device=dev).manual_seed(T * 31 + D)
+    u = torch.finfo(dtype).eps / 2
+    cs = ref.rope_cos_sin(500, P, 1e4, device=dev,
+                          scaling={"rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": 100})
+    pos = torch.randint(0, 500, (T,), generator=g, device=dev, dtype=torch.int32)
+    x = torch.randn(T, H, D, generator=g, device=dev).to(dtype)
+    exp, mag = rope64(x, pos, cs, offset, interleaved)
+    tol = u * exp.abs().clamp_min(torch.finfo(dtype).tiny) + 4 * 2.0 ** -24 * mag
+    keep = x.clone()
+    within(ops.rope(x, pos, cs, offset, interleaved), exp, tol)
+    assert torch.equal(x, keep)
+    # a strided view of a wider buffer, in place: nothing else moves
+    wide = torch.randn(T, H + 1, D + 3, generator=g, device=dev).to(dtype)
+    view = wide[:, 1:, 2:D + 2]
+    view.copy_(x)
+    before = wide.clone()
+    assert ops.rope(view, pos, cs, offset, interleaved, out=view) is view
+    within(view, exp, tol)
+    before[:, 1:, 2:D + 2] = view
+    assert torch.equal(wide, before)
+    # heads and tokens swapped in memory, into a strided out
+    xt = x.transpose(0, 1).contiguous().transpose(0, 1)
+    out = torch.full((T, H, D + 5), 7.0, device=dev, dtype=dtype)
+    ops.rope(xt, pos, cs, offset, interleaved, out=out[..., :D])
+    within(out[..., :D], exp, tol)
+    assert bool((out[..., D:] == 7.0).all())
+    # one head shared by all (expanded)
+    e = x[:, :1].expand(T, H, D)
+    within(ops.rope(e, pos, cs, offset, interleaved), rope64(e, pos, cs, offset, interleaved)[0],
+           u * 2 * e.abs().amax() + 1e-5)
+    no_error(dev)
+
+
+def test_rope_empty_and_positions_outside(dev):
+    from kapsl_sdk_b200 import ops
+    from kapsl_sdk_b200.ops import reference as ref
+
+    cs = ref.rope_cos_sin(10, 32, 1e4, device=dev)
+    x = torch.randn(4, 2, 64, device=dev, dtype=torch.bfloat16)
+    assert ops.rope(x[:0], torch.zeros(0, dtype=torch.int32, device=dev), cs).shape == (0, 2, 64)
+    assert ops.rope(x[:, :0], torch.zeros(4, dtype=torch.int32, device=dev), cs).shape == (4, 0, 64)
+    pos = torch.tensor([3, 10, -1, 9], device=dev, dtype=torch.int32)
+    y = ops.rope(x, pos, cs)
+    torch.cuda.synchronize()
+    assert ops.check_errors(dev) == 80 and "position" in ops.describe_error(80)
+    assert torch.equal(y[1:3], x[1:3]) and not torch.equal(y[0], x[0]) and not torch.equal(y[3], x[3])
+
+
+def test_rope_refuses(dev):
+    from kapsl_sdk_b200 import ops
+    from kapsl_sdk_b200.ops import reference as ref
+
+    cs = ref.rope_cos_sin(10, 32, 1e4, device=dev)
+    x = torch.randn(4, 2, 64, device=dev, dtype=torch.bfloat16)
+    pos = torch.zeros(4, dtype=torch.int32, device=dev)
+    for bad in (lambda: ops.rope(x.cpu(), pos, cs), lambda: ops.rope(x.double(), pos, cs),
+                lambda: ops.rope(x, pos.long(), cs), lambda: ops.rope(x, pos[:3], cs), lambda: ops.rope(x, pos.cpu(), cs),
+                lambda: ops.rope(x, pos, cs, offset=33), lambda: ops.rope(x, pos, cs, offset=-1),
+                lambda: ops.rope(x, pos, cs[:, :31]), lambda: ops.rope(x, pos, cs.half()),
+                lambda: ops.rope(x[0], pos, cs), lambda: ops.rope(x.transpose(1, 2), pos, cs),
+                lambda: ops.rope(x, pos, cs, out=torch.empty_like(x[:3])),
+                lambda: ops.rope(x, pos, cs, out=torch.empty_like(x.float())),
+                lambda: ops.rope(x[:, :, :32], pos, cs, out=x[:, :, 16:48]),
+                lambda: ops.rope(x, pos, cs, out=x[:1].expand(4, 2, 64)),
+                lambda: ops.rope(x[:, :1].expand(4, 2, 64), pos, cs, out=x[:, :1].expand(4, 2, 64))):
+        with pytest.raises((RuntimeError, TypeError)):
+            bad()
+    no_error(dev)
+
+
+# ------------------------------------------------------------------------ cache write
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("T,H,R,page", [(1, 1, 512, 16), (7, 28, 512, 16), (130, 128, 256, 32), (65, 3, 512, 64),
+                                        (300, 20, 256, 16)])
+def test_rope_latent_write(dev, interleaved, T, H, R, page):
+    """Latents: one rounding of x * inv * w in fp32 (the mean of R squares errs by less than
+    (R / 32 + 5) 2^-24, rsqrt and three products by 2^-21 in all); keys as in test_rope."""
+    from kapsl_sdk_b200 import ops
+    from kapsl_sdk_b200.ops import reference as ref
+
+    g = torch.Generator(device=dev).manual_seed(T + R)
+
+    def rn(*s):
+        return torch.randn(*s, generator=g, device=dev).to(torch.bfloat16)
+
+    cs = ref.rope_cos_sin(700, 64, 1e4, device=dev)
+    pos = torch.randint(0, 700, (T,), generator=g, device=dev, dtype=torch.int32)
+    blocks = T // page + 3
+    slots = torch.randperm(blocks * page, generator=g, device=dev)[:T].contiguous()
+    if T > 4:
+        slots[2] = -1
+    cache = rn(blocks, page, R + 64)
+    q, kvw, w = rn(T, H, 192), rn(T, R + 64 + 8), rn(R)
+    kv = kvw[:, :R + 64]
+    kv[0] = 0  # a row of zeros stays finite
+    before, q0 = cache.clone(), q.clone()
+    c = kv[:, :R].double()
+    lat = c / (c.pow(2).mean(1, keepdim=True) + 1e-6).sqrt() * w.double()
+    key, kmag = rope64(kv[:, None, R:], pos, cs, 0, interleaved)
+    q_exp, q_mag = rope64(q[..., 128:], pos, cs, 0, interleaved)
+    exp = torch.cat([lat, key[:, 0]], 1)
+    tol = torch.cat([lat.abs() * (U + 2.0 ** -18), U * key[:, 0].abs() + 2.0 ** -22 * kmag[:, 0]], 1)
+    q_tol = U * q_exp.abs() + 2.0 ** -22 * q_mag
+    q_out = torch.full((T, H, 72), 5.0, device=dev, dtype=torch.bfloat16)
+    ops.rope_latent_write(q[..., 128:], kv, pos, slots, cs, w, 1e-6, cache, interleaved, q_out=q_out[..., :64])
+    assert torch.equal(q, q0) and bool((q_out[..., 64:] == 5.0).all())
+    within(q_out[..., :64], q_exp, q_tol)
+    used = (slots >= 0).nonzero().flatten()
+    flat = cache.view(-1, R + 64)
+    within(flat[slots[used]], exp[used], tol[used])
+    flat[slots[used]] = before.view(-1, R + 64)[slots[used]]
+    assert torch.equal(cache, before)  # other rows as they were
+    ops.rope_latent_write(q[..., 128:], kv, pos, slots, cs, w, 1e-6, cache, interleaved)
+    within(q[..., 128:], q_exp, q_tol)
+    assert torch.equal(q[..., :128], q0[..., :128])
+    no_error(dev)
+
+
+def test_rope_latent_write_bounds_and_refusals(dev):
+    from kapsl_sdk_b200 import ops
+    from kapsl_sdk_b200.ops import reference as ref
+
+    def z(*s, dt=torch.bfloat16):
+        return torch.zeros(*s, device=dev, dtype=dt)
+
+    cs = ref.rope_cos_sin(10, 64, 1e4, device=dev)
+    cache, w = z(2, 16, 576), z(512) + 1
+    q = torch.randn(3, 2, 64, device=dev).to(torch.bfloat16)
+    kv, pos = z(3, 576) + 1, z(3, dt=torch.int32)
+    slots = torch.tensor([0, 32, 31], device=dev)  # 32 rows: the second lies outside
+    ops.rope_latent_write(q, kv, pos, slots, cs, w, 1e-6, cache)
+    torch.cuda.synchronize()
+    assert ops.check_errors(dev) == 81
+    assert bool((cache.view(32, 576)[[0, 31]] != 0).all()) and bool((cache.view(32, 576)[1:31] == 0).all())
+    ops.rope_latent_write(q[:0], kv[:0], pos[:0], slots[:0], cs, w, 1e-6, cache)
+    bad = [dict(q=z(3, 2, 32)), dict(q=q.float()), dict(kv=z(3, 575)), dict(kv=z(2, 576)), dict(kv=z(3, 576).float()),
+           dict(cache=z(2, 16, 448)), dict(cache=z(2, 8, 576)), dict(cache=z(2, 16, 640)[..., :576]), dict(w=z(256)),
+           dict(slots=slots.int()), dict(slots=slots[:2]), dict(pos=pos[:2]), dict(cs=cs[:, :32].contiguous()),
+           dict(q_out=z(3, 1, 64)), dict(q_out=z(3, 2, 65)[..., :64]), dict(kv=cache.view(32, 576)[:3])]
+    for kw in bad:
+        a = dict(q=q, kv=kv, pos=pos, slots=slots, cs=cs, w=w, cache=cache, q_out=None)
+        a.update(kw)
+        with pytest.raises((RuntimeError, TypeError)):
+            ops.rope_latent_write(a["q"], a["kv"], a["pos"], a["slots"], a["cs"], a["w"], 1e-6, a["cache"],
+                                  q_out=a["q_out"])
+    no_error(dev)
+
+
+# -------------------------------------------------------------------------- attention
+class Cache:
+    """Ragged contexts in permuted pages; what no sequence owns is NaN."""
+
+    def __init__(self, dev, lens, R, page, seed, spare=2):
+        g = torch.Generator(device=dev).manual_seed(seed)
+        r = random.Random(seed)
+        need = [-(-n // page) for n in lens]
+        total = sum(need) + spare
+        ids = list(range(total))
+        r.shuffle(ids)
+        self.cache = torch.full((total, page, R + 64), NAN, device=dev, dtype=torch.bfloat16)
+        self.bt = torch.zeros(len(lens), max(need + [1]) + 1, dtype=torch.int32)
+        self.rows, at = [], 0
+        flat = self.cache.view(-1, R + 64)
+        for i, n in enumerate(lens):
+            self.bt[i, :need[i]] = torch.tensor(ids[at:at + need[i]], dtype=torch.int32)
+            at += need[i]
+            rows = torch.randn(n, R + 64, generator=g, device=dev).to(torch.bfloat16)
+            j = torch.arange(n)
+            flat[(self.bt[i, j // page].long() * page + j % page).to(dev)] = rows
+            self.rows.append(rows)
+        self.bt = self.bt.to(dev)
+        self.ctx = torch.tensor(lens, dtype=torch.int32, device=dev)
+        self.g = g
+
+    def randn(self, *s, std=1.0):
+        return (torch.randn(*s, generator=self.g, device=self.cache.device) * std).to(torch.bfloat16)
+
+
+def decode64(q, rows, w, scale):
+    """q [H, 192], rows [ctx, R + 64], w [H, 256, R] -> out [H, 128] and its standard deviation
+    under the roundings of qa, p, o and out to bf16."""
+    H, R = w.shape[0], w.shape[2]
+    if rows.shape[0] == 0:
+        z = torch.zeros(H, 128, dtype=torch.float64, device=q.device)
+        return z, z
+    q, rows, w = q.double(), rows.double(), w.double()
+    c = rows[:, :R]
+    qn = torch.einsum("hd,hdr->hr", q[:, :128], w[:, :128])
+    s = (qn @ c.T + q[:, 128:] @ rows[:, R:].T) * scale
+    p = torch.softmax(s, -1)
+    o = p @ c
+    out = torch.einsum("hr,hvr->hv", o, w[:, 128:])
+    v = torch.einsum("kr,hvr->hkv", c, w[:, 128:])
+    dev_v = p[..., None] * (v - out[:, None])  # d out / d s_j
+    grad = torch.einsum("hkv,kr->hvr", dev_v, c) * scale  # d out / d qa_r
+    var = torch.einsum("hvr,hr->hv", grad ** 2, qn ** 2)
+    var += torch.einsum("hk,hkv->hv", p ** 2, v ** 2)
+    var += torch.einsum("hr,hvr->hv", o ** 2, w[:, 128:] ** 2)
+    var += out ** 2
+    slop = F32 * torch.einsum("hk,hkv->hv", p, v.abs())
+    return out, 8 * U / math.sqrt(3) * var.sqrt() + slop
+
+
+def prefill64(q, rows, w, scale):
+    """q [n, H, 192] at the end of rows [ctx, R + 64] -> out [n, H, 128] and its tolerance under the
+    roundings of k, v, p and out to bf16."""
+    n, H, _ = q.shape
+    ctx, R = rows.shape[0], w.shape[2]
+    q, rows, w = q.double(), rows.double(), w.double()
+    out = torch.empty(n, H, 128, dtype=torch.float64, device=q.device)
+    tol = torch.empty_like(out)
+    seen = torch.arange(ctx, device=q.device)[None] <= torch.arange(ctx - n, ctx, device=q.device)[:, None]
+    for h in range(H):
+        kn, v = rows[:, :R] @ w[h, :128].T, rows[:, :R] @ w[h, 128:].T
+        s = (q[:, h, :128] @ kn.T + q[:, h, 128:] @ rows[:, R:].T) * scale
+        p = torch.softmax(s.masked_fill(~seen, -math.inf), -1)
+        o = p @ v
+        ds2 = (q[:, h, :128] ** 2 @ (kn ** 2).T) * scale ** 2  # variance of s_j in units of u^2 / 3
+        a = p ** 2 * ds2
+        var = a @ v ** 2 - 2 * o * (a @ v) + o ** 2 * a.sum(1, keepdim=True)
+        var += 2 * (p ** 2 @ v ** 2) + o ** 2
+        out[:, h] = o
+        tol[:, h] = 8 * U / math.sqrt(3) * var.clamp_min(0).sqrt() + F32 * (p @ v.abs())
+    return out, tol
+
+
+LENS = [1, 15, 16, 17, 0, 63, 64, 65, 127, 128, 129, 300, 1000]
+
+
+@pytest.mark.parametrize("H,R,page,splits", [(1, 512, 16, 0), (3, 256, 64, 1), (8, 512, 64, 3), (17, 512, 32, 0),
+                                             (28, 512, 16, 7), (64, 512, 16, 1), (65, 256, 16, 2), (128, 512, 32, 0),
+                                             (33, 256, 32, 64)])
+def test_decode(dev, H, R, page, splits):
+    from kapsl_sdk_b200 import ops
+
+    k = Cache(dev, LENS, R, page, H * 7 + R)
+    B = len(LENS)
+    qw = k.randn(B, H * 192 + 16, std=1.5)
+    q = qw[:, 8:H * 192 + 8]  # a view of wider rows
+    w = k.randn(H, 256, R, std=1 / math.sqrt(R))
+    scale = 1 / math.sqrt(192)
+    out = torch.full((B, H * 128 + 8), 3.0, device=dev, dtype=torch.bfloat16)
+    ops.latent_decode_attention(q, k.cache, w, k.bt, k.ctx, H, out=out[:, :H * 128], num_splits=splits, max_ctx=1000)
+    no_error(dev)
+    assert bool((out[:, H * 128:] == 3.0).all())
+    for b in range(B):
+        exp, tol = decode64(q[b].view(H, 192), k.rows[b], w, scale)
+        within(out[b, :H * 128].view(H, 128), exp, tol)
+
+
+def test_decode_large_logits(dev):
+    """A running maximum that moves by far more than one tile's spread, in both directions."""
+    from kapsl_sdk_b200 import ops
+
+    H, R, lens = 9, 512, [700, 640, 129]
+    k = Cache(dev, lens, R, 16, 5)
+    q = k.randn(3, H * 192)
+    w = k.randn(H, 256, R, std=1 / math.sqrt(R))
+    flat = k.cache.view(-1, R + 64)
+    for b, n in enumerate(lens):  # grow (b = 0), shrink (1) or spike (2) along the context
+        f = torch.linspace(0.1, 6.0, n, device=dev) if b == 0 else torch.linspace(6.0, 0.1, n, device=dev)
+        if b == 2:
+            f = torch.full((n,), 0.2, device=dev)
+            f[128] = 8.0
+        rows = (k.rows[b].float() * f[:, None]).to(torch.bfloat16)
+        j = torch.arange(n, device=dev)
+        flat[k.bt[b, j // 16].long() * 16 + j % 16] = rows
+        k.rows[b] = rows
+    for splits in (1, 3):
+        out = ops.latent_decode_attention(q, k.cache, w, k.bt, k.ctx, H, num_splits=splits)
+        no_error(dev)
+        for b in range(3):
+            exp, tol = decode64(q[b].view(H, 192), k.rows[b], w, 1 / math.sqrt(192))
+            within(out[b].view(H, 128), exp, tol)
+
+
+def test_decode_pages_outside(dev):
+    """A table entry outside the cache records an error; other rows are untouched by it."""
+    from kapsl_sdk_b200 import ops
+
+    k = Cache(dev, [40, 50], 512, 16, 3)
+    q, w = k.randn(2, 5 * 192), k.randn(5, 256, 512, std=0.04)
+    good = ops.latent_decode_attention(q, k.cache, w, k.bt, k.ctx, 5)
+    no_error(dev)
+    for bad in (-1, k.cache.shape[0], 2 ** 31 - 1):
+        bt = k.bt.clone()
+        bt[0, 1] = bad
+        out = ops.latent_decode_attention(q, k.cache, w, bt, k.ctx, 5)
+        torch.cuda.synchronize()
+        assert ops.check_errors(dev) == 82
+        assert torch.equal(out[1], good[1])
+    # a context longer than its table is cut to the table
+    ctx = torch.tensor([40, 10 ** 9], dtype=torch.int32, device=dev)
+    out = ops.latent_decode_attention(q[1:], k.cache, w, k.bt[1:, :3].contiguous(), ctx[1:], 5, max_ctx=64)
+    torch.cuda.synchronize()
+    exp, tol = decode64(q[1].view(5, 192), k.rows[1][:48], w, 1 / math.sqrt(192))
+    within(out[0].view(5, 128), exp, tol)
+    no_error(dev)
+
+
+def test_decode_refuses(dev):
+    from kapsl_sdk_b200 import ops
+
+    k = Cache(dev, [40, 50], 512, 16, 3)
+    q, w = k.randn(2, 5 * 192), k.randn(5, 256, 512, std=0.04)
+    a0 = dict(q=q, cache=k.cache, w=w, bt=k.bt, ctx=k.ctx, H=5, out=None, num_splits=0)
+    for kw in (dict(q=q.float()), dict(q=q[:, :-1]), dict(q=q.cpu()), dict(cache=k.cache[..., :448].contiguous()),
+               dict(cache=k.cache.float()), dict(cache=k.cache[:, :8].contiguous()), dict(w=w[:4]), dict(H=4),
+               dict(w=w[..., :256].contiguous()), dict(w=w.transpose(1, 2)), dict(bt=k.bt.long()), dict(bt=k.bt[:1]),
+               dict(ctx=k.ctx.long()), dict(ctx=k.ctx[:1]), dict(out=q[:, :5 * 128]), dict(num_splits=65),
+               dict(out=torch.empty(2, 5 * 128, device=dev)), dict(q=k.randn(2, 5 * 192 + 1)[:, 1:]), dict(H=0)):
+        a = dict(a0)
+        a.update(kw)
+        with pytest.raises((RuntimeError, TypeError, ValueError)):
+            ops.latent_decode_attention(a["q"], a["cache"], a["w"], a["bt"], a["ctx"], a["H"], out=a["out"],
+                                        num_splits=a["num_splits"])
+    assert ops.latent_decode_attention(q[:0], k.cache, w, k.bt, k.ctx, 5).shape == (0, 640)
+    no_error(dev)
+
+
+PREFILLS = [([1], [1]), ([17], [17]), ([130], [130]), ([128, 256], [128, 300]), ([300, 0, 1, 64], [557, 9, 900, 64]),
+            ([257, 129, 5, 385], [257, 513, 1000, 400])]
+
+
+@pytest.mark.parametrize("q_lens,ctx_lens", PREFILLS)
+@pytest.mark.parametrize("H,R,page", [(1, 512, 16), (5, 256, 64), (28, 512, 32)])
+def test_prefill(dev, q_lens, ctx_lens, H, R, page):
+    from kapsl_sdk_b200 import ops
+
+    k = Cache(dev, ctx_lens, R, page, H + len(q_lens))
+    T, q0 = sum(q_lens) + 5, 3  # rows before and behind the sequences
+    qw = k.randn(T, H * 192 + 8, std=1.5)
+    q = qw[:, :H * 192]
+    w = k.randn(H * 256, R, std=1 / math.sqrt(R))
+    out = torch.full((T, H * 128 + 8), 3.0, device=dev, dtype=torch.bfloat16)
+    bt = torch.cat([k.bt.new_full((2, k.bt.shape[1]), -1), k.bt])
+    plan = ops.latent_prefill_plan(q_lens, ctx_lens, dev, q_start=q0, bt_start=2)
+    ops.latent_prefill_attention(q, k.cache, w, plan, bt, H, out=out[:, :H * 128])
+    no_error(dev)
+    at = q0
+    for i, n in enumerate(q_lens):
+        if n:
+            exp, tol = prefill64(q[at:at + n].view(n, H, 192), k.rows[i], w.view(H, 256, R), 1 / math.sqrt(192))
+            within(out[at:at + n, :H * 128].view(n, H, 128), exp, tol)
+        at += n
+    assert bool((out[:q0] == 3.0).all()) and bool((out[at:] == 3.0).all()) and bool((out[:, H * 128:] == 3.0).all())
+
+
+def test_prefill_passes_over_heads(dev, monkeypatch):
+    """A small bound on the expanded rows cuts the heads into passes, the last one shorter."""
+    from kapsl_sdk_b200 import ops
+
+    k = Cache(dev, [200, 90], 512, 16, 11)
+    H = 7
+    q, w = k.randn(200, H * 192), k.randn(H * 256, 512, std=0.05)
+    plan = ops.latent_prefill_plan([110, 90], [200, 90], dev)
+    one = ops.latent_prefill_attention(q, k.cache, w, plan, k.bt, H)
+    monkeypatch.setattr(ops, "LATENT_KV_BYTES", plan.kv_rows * 512 * 3)
+    assert torch.equal(one, ops.latent_prefill_attention(q, k.cache, w, plan, k.bt, H))
+    no_error(dev)
+
+
+def test_prefill_large_logits(dev):
+    from kapsl_sdk_b200 import ops
+
+    H, R, n = 2, 512, 520
+    k = Cache(dev, [n], R, 16, 6)
+    f = torch.linspace(0.1, 5.0, n, device=dev)
+    f[300:] = f[300:].flip(0)
+    rows = (k.rows[0].float() * f[:, None]).to(torch.bfloat16)
+    j = torch.arange(n, device=dev)
+    k.cache.view(-1, R + 64)[k.bt[0, j // 16].long() * 16 + j % 16] = rows
+    q, w = k.randn(n, H * 192), k.randn(H * 256, R, std=1 / math.sqrt(R))
+    out = ops.latent_prefill_attention(q, k.cache, w, ops.latent_prefill_plan([n], [n], dev), k.bt, H)
+    no_error(dev)
+    exp, tol = prefill64(q.view(n, H, 192), rows, w.view(H, 256, R), 1 / math.sqrt(192))
+    within(out.view(n, H, 128), exp, tol)
+
+
+def test_prefill_pages_outside_and_refusals(dev):
+    from kapsl_sdk_b200 import ops
+
+    k = Cache(dev, [40, 50], 512, 16, 3)
+    q, w = k.randn(50, 5 * 192), k.randn(5, 256, 512, std=0.04)
+    plan = ops.latent_prefill_plan([20, 30], [40, 50], dev)
+    good = ops.latent_prefill_attention(q, k.cache, w, plan, k.bt, 5)
+    no_error(dev)
+    for bad in (-1, k.cache.shape[0], 2 ** 31 - 1):
+        bt = k.bt.clone()
+        bt[0, 1] = bad
+        out = ops.latent_prefill_attention(q, k.cache, w, plan, bt, 5)
+        torch.cuda.synchronize()
+        assert ops.check_errors(dev) == 82
+        assert torch.equal(out[20:], good[20:]) and torch.isfinite(out.float()).all()
+    wide = ops.latent_prefill_plan([20, 30], [40, 5000], dev)
+    for bad in (lambda: ops.latent_prefill_attention(q[:49], k.cache, w, plan, k.bt, 5),
+                lambda: ops.latent_prefill_attention(q, k.cache, w, plan, k.bt[:1], 5),
+                lambda: ops.latent_prefill_attention(q, k.cache, w, wide, k.bt, 5),
+                lambda: ops.latent_prefill_attention(q, k.cache, w, plan, k.bt, 4),
+                lambda: ops.latent_prefill_attention(q.float(), k.cache, w, plan, k.bt, 5),
+                lambda: ops.latent_prefill_attention(q, k.cache.float(), w, plan, k.bt, 5),
+                lambda: ops.latent_prefill_attention(q, k.cache, w[:4], plan, k.bt, 5),
+                lambda: ops.latent_prefill_attention(q, k.cache, w, plan, k.bt, 5, out=q[:, :640])):
+        with pytest.raises((RuntimeError, TypeError)):
+            bad()
+    empty = ops.latent_prefill_plan([0], [0], dev)
+    assert bool((ops.latent_prefill_attention(q, k.cache, w, empty, k.bt, 5) == 0).all())
+    no_error(dev)
+
+
+def test_graphs_streams_and_repeats(dev):
+    """Two captured graphs replayed in turn and eager calls on two streams give the eager results."""
+    from kapsl_sdk_b200 import ops
+
+    H, R = 20, 512
+    k = Cache(dev, [300, 77, 0, 1000], R, 16, 9)
+    w = k.randn(H * 256, R, std=1 / math.sqrt(R))
+    qd, qp = k.randn(4, H * 192), k.randn(177, H * 192)
+    plan = ops.latent_prefill_plan([100, 77], [300, 77], dev)
+
+    def decode():
+        return ops.latent_decode_attention(qd, k.cache, w, k.bt, k.ctx, H, max_ctx=1000)
+
+    def prefill():
+        return ops.latent_prefill_attention(qp, k.cache, w, plan, k.bt, H)
+
+    decode(), prefill()
+    torch.cuda.synchronize()
+    graphs = []
+    for fn in (decode, prefill):
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            o = fn()
+        graphs.append((gr, o, fn))
+    for rep in range(3):
+        qd.copy_(k.randn(4, H * 192))
+        qp.copy_(k.randn(177, H * 192))
+        exp = [fn().clone() for _, _, fn in graphs]
+        for gr, _, _ in graphs:
+            gr.replay()
+        torch.cuda.synchronize()
+        for (_, o, _), e in zip(graphs, exp):
+            assert torch.equal(o, e)
+    s = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for rep in range(4):
+        for i, fn in enumerate((decode, prefill)):
+            s[i].wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s[i]):
+                got[i].append(fn())
+    torch.cuda.synchronize()
+    for i in range(2):
+        for o in got[i]:
+            assert torch.equal(o, exp[i])
+    no_error(dev)
+
+
+def test_layer_run_together(dev):
+    """A latent-attention layer as a serving loop drives it: two prefill chunks of one sequence
+    beside a whole prompt of another, then decode steps of both, against a 64-bit layer that
+    sees the full sequences.  The cache holds bf16 rows, which the oracle rounds likewise."""
+    from kapsl_sdk_b200 import ops
+    from kapsl_sdk_b200.ops import reference as ref
+
+    g = torch.Generator(device=dev).manual_seed(4)
+    H, R, page, lens = 5, 256, 16, [90, 41]
+
+    def rn(*s, std=1.0):
+        return (torch.randn(*s, generator=g, device=dev) * std).to(torch.bfloat16)
+
+    w, wn = rn(H * 256, R, std=1 / math.sqrt(R)), 1 + rn(R, std=0.1)
+    cs = ref.rope_cos_sin(200, 64, 1e4, device=dev)
+    Q = [rn(n, H * 192, std=1.5) for n in lens]
+    KV = [rn(n, R + 64) for n in lens]
+    cache = torch.full((14, page, R + 64), NAN, device=dev, dtype=torch.bfloat16)
+    bt = torch.randperm(14, generator=g, device=dev).int()[:12].view(2, 6).contiguous()
+    scale = 0.06
+    outs = [[], []]
+    done = [0, 0]
+
+    def step(news, prefill):
+        rows = [(s, done[s] + i) for s, n in enumerate(news) for i in range(n)]
+        q = torch.cat([Q[s][done[s]:done[s] + n] for s, n in enumerate(news)]).clone()
+        kv = torch.cat([KV[s][done[s]:done[s] + n] for s, n in enumerate(news)])
+        pos = torch.tensor([p for _, p in rows], dtype=torch.int32, device=dev)
+        slots = torch.tensor([int(bt[s, p // page]) * page + p % page for s, p in rows], device=dev)
+        ops.rope_latent_write(q.view(-1, H, 192)[..., 128:], kv, pos, slots, cs, wn, 1e-5, cache, interleaved=True)
+        for s, n in enumerate(news):
+            done[s] += n
+        if prefill:
+            plan = ops.latent_prefill_plan(news, done, dev)
+            o = ops.latent_prefill_attention(q, cache, w, plan, bt, H, scale=scale)
+        else:
+            ctx = torch.tensor(done, dtype=torch.int32, device=dev)
+            o = ops.latent_decode_attention(q, cache, w, bt, ctx, H, scale=scale, max_ctx=max(done))
+        for s, n in enumerate(news):
+            outs[s].append(o[:n])
+            o = o[n:]
+
+    step([50, 0], True)
+    step([30, 31], True)
+    for _ in range(10):
+        step([1, 1], False)
+    no_error(dev)
+    for s, n in enumerate(lens):
+        pos = torch.arange(n, device=dev)
+        rows = ref.latent_row(KV[s], pos, cs, wn, 1e-5, interleaved=True).to(torch.bfloat16)
+        q = ref.rope(Q[s].view(n, H, 192), pos, cs, offset=128, interleaved=True).to(torch.bfloat16)
+        got = torch.cat(outs[s]).view(n, H, 128)
+        exp, tol = prefill64(q, rows, w.view(H, 256, R), scale)
+        first = n - 10
+        within(got[:first], exp[:first], tol[:first])
+        for i in range(first, n):
+            e, t = decode64(q[i], rows[:i + 1], w.view(H, 256, R), scale)
+            within(got[i], e, t)
