@@ -100,7 +100,7 @@ void rope(Tensor y, Tensor x, Tensor positions, Tensor cos_sin, int64_t offset, 
 // cache [blocks, page, R + 64]; returns R
 int64_t check_cache(const char* op, const Tensor& cache, const Tensor& like) {
   check(cache, at::kBFloat16, like, op, "cache");
-  TORCH_CHECK(cache.dim() == 3 && cache.is_contiguous(), op, ": cache must be [blocks, page, R + 64] contiguous");
+  TORCH_CHECK(cache.dim() == 3 && cache.is_contiguous() && cache.size(0) >= 1, op, ": cache must be [blocks, page, R + 64] contiguous");
   const int64_t R = cache.size(2) - kRot, page = cache.size(1);
   TORCH_CHECK(R == 256 || R == 512, op, ": the latent must have 256 or 512 values (cache rows of 320 or 576), got rows of ",
               num(cache.size(2)));

@@ -56,7 +56,9 @@ DEVICE_ERRORS = {
     **{c: "tcgen05 prefill attention pipeline wait ran out" for c in range(71, 79)},
     80: "rotary positions: a position lies outside the cos/sin table (its row was not rotated)",
     81: "latent cache write: a slot lies outside the cache (its row was not written)",
-    82: "latent attention: a block table entry lies outside the cache (its keys were skipped)",
+    82: "latent attention: a block table entry lies outside the cache (its keys read as zeros)",
+    83: "latent decode attention: shared memory is not 1 KiB aligned",
+    **{c: "latent decode attention pipeline wait ran out" for c in range(84, 90)},
 }
 
 
@@ -350,7 +352,7 @@ def latent_decode_attention(q: torch.Tensor, cache: torch.Tensor, w_kv_b: torch.
     ``q`` [B, H * 192] has 128 position-free and 64 rotated dims a head; ``out`` is
     [B, H * 128].  Rows with ``ctx_lens`` 0 (a padded batch) give zeros.  ``max_ctx`` (a host
     number, default the block tables' width) only chooses how many splits the context is cut into.
-    A block table entry outside the cache is skipped and records device error 82."""
+    The keys of a block table entry outside the cache read as zeros, and device error 82 is recorded."""
     if scale is None:
         scale = 1.0 / math.sqrt(192)
     B = q.shape[0]
