@@ -144,12 +144,14 @@ void rope_latent_write(Tensor q, Tensor q_out, Tensor kv, Tensor positions, Tens
                                   (float)eps, bf(cache), cache.size(0) * cache.size(1), (int)R, cur_stream());
 }
 
-int64_t latent_num_splits(int64_t B, int64_t H, int64_t R, int64_t max_ctx) {
-  return kapsl::latent_decode_num_splits((int)B, (int)H, (int)R, (int)max_ctx, kapsl::gemm_num_sms());
-}
-
-int64_t latent_workspace_bytes(int64_t B, int64_t H, int64_t R, int64_t nsplit) {
-  return (int64_t)kapsl::latent_decode_workspace_bytes((int)B, (int)H, (int)R, (int)nsplit);
+// Workspace of latent_decode_attention for these rows of q.
+int64_t latent_workspace_bytes(Tensor q, int64_t H, int64_t R, int64_t max_ctx) {
+  TORCH_CHECK(q.is_cuda() && q.dim() == 2 && q.size(0) <= 65535 && H >= 1 && H <= 1024 && (R == 256 || R == 512),
+              "latent_decode_attention: q, num_heads or the cache's row width out of range");
+  const c10::cuda::CUDAGuard g(q.device());
+  return (int64_t)kapsl::latent_decode_workspace_bytes((int)q.size(0), (int)H, (int)R,
+                                                       (int)std::min<int64_t>(std::max<int64_t>(max_ctx, 0), INT32_MAX),
+                                                       kapsl::gemm_num_sms());
 }
 
 // q / out [rows, heads * width] and w [H, 256, R]
@@ -171,7 +173,7 @@ void check_heads(const char* op, const Tensor& q, const Tensor& w, const Tensor&
 }
 
 void latent_decode_attention(Tensor q, Tensor cache, Tensor w, Tensor block_tables, Tensor ctx_lens, Tensor out,
-                             int64_t H, double scale, int64_t nsplit, Tensor workspace, Tensor err) {
+                             int64_t H, double scale, int64_t max_ctx, Tensor workspace, Tensor err) {
   const char* op = "latent_decode_attention";
   TORCH_CHECK(q.is_cuda(), op, ": q must be a CUDA tensor");
   check(q, at::kBFloat16, q, op, "q");
@@ -186,10 +188,9 @@ void latent_decode_attention(Tensor q, Tensor cache, Tensor w, Tensor block_tabl
   check(ctx_lens, at::kInt, q, op, "ctx_lens");
   TORCH_CHECK(ctx_lens.dim() == 1 && ctx_lens.is_contiguous() && ctx_lens.size(0) >= B, op,
               ": ctx_lens must hold an int32 per row");
-  TORCH_CHECK(nsplit >= 1 && nsplit <= 64, op, ": num_splits must be 1 to 64");
   TORCH_CHECK(B <= 65535, op, ": at most 65535 rows");
   check(workspace, at::kByte, q, op, "workspace");
-  TORCH_CHECK(workspace.is_contiguous() && workspace.numel() >= latent_workspace_bytes(B, H, R, nsplit) &&
+  TORCH_CHECK(workspace.is_contiguous() && workspace.numel() >= latent_workspace_bytes(q, H, R, max_ctx) &&
                   (reinterpret_cast<uintptr_t>(workspace.data_ptr()) & 127) == 0,
               op, ": workspace too small or not 128-byte aligned");
   check(err, at::kInt, q, op, "err");
@@ -209,7 +210,8 @@ void latent_decode_attention(Tensor q, Tensor cache, Tensor w, Tensor block_tabl
   a.out_stride = out.stride(0);
   a.B = (int)B;
   a.H = (int)H;
-  a.nsplit = (int)nsplit;
+  a.max_ctx = (int)std::min<int64_t>(std::max<int64_t>(max_ctx, 0), INT32_MAX);
+  a.num_sms = kapsl::gemm_num_sms();
   a.scale = (float)scale;
   a.workspace = workspace.data_ptr();
   a.err = err.data_ptr<int>();
@@ -302,7 +304,6 @@ void register_latent(pybind11::module_& m) {
   m.def("rope", &rope, "rotary positions of strided heads (half / interleaved, part of the head)");
   m.def("rope_latent_write", &rope_latent_write, "latent norm + rotary key -> paged latent cache, query rotary part");
   m.def("latent_decode_attention", &latent_decode_attention, "absorbed latent attention over a paged cache");
-  m.def("latent_num_splits", &latent_num_splits);
   m.def("latent_workspace_bytes", &latent_workspace_bytes);
   m.def("latent_gather", &latent_gather, "context rows of every sequence out of the paged latent cache");
   m.def("check_latent_prefill", &check_latent_prefill);

@@ -55,13 +55,13 @@ struct LatentDecode {
   const int32_t* ctx_lens = nullptr;
   __nv_bfloat16* out = nullptr;  // [B, H * 128], pitch out_stride
   int64_t out_stride = 0;
-  int B = 0, H = 0, nsplit = 1;
+  int B = 0, H = 0;
+  int max_ctx = 0, num_sms = 1;  // choose the number of CTAs only
   float scale = 0.f;
   void* workspace = nullptr;  // latent_decode_workspace_bytes
   int* err = nullptr;
 };
-int latent_decode_num_splits(int B, int H, int R, int max_ctx, int num_sms);
-size_t latent_decode_workspace_bytes(int B, int H, int R, int nsplit);
+size_t latent_decode_workspace_bytes(int B, int H, int R, int max_ctx, int num_sms);
 void launch_latent_decode(const LatentDecode& a, cudaStream_t st);
 
 // Copies each sequence's context rows out of the paged cache into rows [S.kv_start, + ctx)

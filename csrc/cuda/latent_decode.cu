@@ -7,8 +7,8 @@
 //   o_h = sum_j softmax(s)_j c_j,           out_h = V_h o_h,
 // so the cache is read once for all heads and nothing is expanded per token.
 //
-// Three launches: absorb (qa), attention over splits of the context (fp32 partials of
-// o), and one that joins the splits and applies V_h.
+// Three launches: absorb (qa, and the schedule), attention over pieces of the contexts (fp32
+// partials of o), and one that joins the pieces and applies V_h.
 #include <algorithm>
 
 #include "common.cuh"
@@ -23,26 +23,81 @@ using bf16 = __nv_bfloat16;
 namespace {
 
 constexpr int kNope = 128, kRot = 64, kVal = 128;
-constexpr int kMaxSplits = 64;
 constexpr float kLog2e = 1.4426950408889634f;
+
+// -------------------------------------------------------------------- schedule
+//
+// The tiles (64 keys) of all sequences form one line, and each CTA of a head tile takes an
+// equal stretch of it, whatever the lengths: stretches cross sequence ends, sequences
+// cross stretches.  A piece is the part of sequence b that CTA c holds; b + c grows along
+// the line, so it numbers the pieces' partial results.  Head tiles of the same
+// sequences run side by side (cache tiles are read from DRAM once).
+//
+// table: [0] tiles a CTA takes, [1 + b] first tile of sequence b, [1 + B] all tiles.
+// `quota` is at least a 32nd of the longest sequence: no row joins more than kMaxPieces.
+constexpr int kKeys = 64;
+constexpr int kMaxPieces = 33;
+
+__host__ __device__ constexpr int table_ints(int B) { return (B + 2 + 31) / 32 * 32; }
+
+__device__ __forceinline__ int seq_tiles(const int32_t* ctx_lens, int b, int limit) {
+  return (max(0, min(ctx_lens[b], limit)) + kKeys - 1) / kKeys;
+}
+
+// One block writes the table (`limit`: tokens the block tables hold).
+__device__ void write_schedule(const int32_t* __restrict__ ctx_lens, int B, int limit, int ctas, int32_t* table) {
+  __shared__ int sums[33], longest;
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5, nw = blockDim.x >> 5;
+  if (t == 0) longest = 0;
+  int base = 0;
+  for (int b0 = 0; b0 < B; b0 += blockDim.x) {
+    const int n = b0 + t < B ? seq_tiles(ctx_lens, b0 + t, limit) : 0;
+    int x = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    __syncthreads();
+    if (lane == 31) sums[warp] = x;
+    atomicMax(&longest, n);
+    __syncthreads();
+    int before = base;
+    for (int w = 0; w < nw; ++w) {
+      if (w < warp) before += sums[w];
+      base += sums[w];
+    }
+    if (b0 + t < B) table[1 + b0 + t] = before + x - n;
+  }
+  __syncthreads();
+  if (t == 0) {
+    table[1 + B] = base;
+    table[0] = max(1, max((base + ctas - 1) / ctas, (longest + 31) / 32));
+  }
+}
 
 // ------------------------------------------------------------------ attention
 //
-// One CTA per (split, up to 64 heads, sequence).  The products are transposed so
-// that the heads are the MMA's N, which may be 16, 32 or 64 without wasted rows:
+// A CTA works on up to 64 heads.  The products are transposed so that the heads are the
+// MMA's N, which may be 16, 32 or 64 without wasted rows:
 //   S^T [64 keys, heads] = K . qa^T    (M = 64, K tile K-major)
 //   O^T [R dims, heads] += c^T . P^T   (M = 128 x R / 128; the same K tile read MN-major)
 // so a key tile is loaded once and serves both products, and O^T of 64 heads takes 256
 // of the 512 TMEM columns, which leaves room for two S^T tiles.
 //
-// Warp 0 loads 64-key tiles by TMA into a ring, warp 1 issues the MMAs, warps 2-5
-// do the softmax: a tile's column maxima by register/shuffle exchange and shared
-// memory, P rounded to bf16 (the operand type of the second product; the row sums are
-// of the fp32 values).  The running maximum is raised, and O^T rescaled in TMEM, only
-// when a score exceeds it by 2^8: p <= 256 loses nothing in bf16 or fp32, and the
-// final division uses the same maximum.  Keys past the context have p = 0 and their
-// cache rows are cleared in shared memory, since 0 * NaN of a stale row would count.
-constexpr int kKeys = 64;
+// Warp 0 loads the tiles by TMA, in groups of 128 latent dims (the rotary dims with the
+// first) with barriers of their own: the scores of a group start when it lands, and its
+// slot is free again when the second product has read it.  Warp 1 issues the MMAs from one
+// elected thread (elect.sync: issued from `lane == 0` the same MMAs took 44 cycles each
+// instead of the 23-48 of their operands).  Warps 2-5 do the softmax.
+//
+// Softmax: scores are compared with the running maximum; only when one exceeds it by 2^8
+// (a vote over the four warps) is the maximum raised - column maxima by register and
+// shared-memory exchange - and O^T rescaled in TMEM.  p <= 256 loses nothing in bf16 or
+// fp32, and the final division uses the same maximum.  P is rounded to bf16, the operand
+// type of the second product; the row sums are of the fp32 values.  Keys past the context
+// have p = 0 and their cache rows are cleared in shared memory, since 0 * NaN of a
+// stale row would count.
 constexpr int kSoft = 4;  // softmax warps
 constexpr int kThreads = (2 + kSoft) * 32;
 constexpr float kRaise = 8.f;
@@ -51,7 +106,8 @@ template <int R, int NT>
 struct Shape {
   static constexpr int W = R + kRot;
   static constexpr int kChunks = W / 64;
-  static constexpr uint32_t kChunkBytes = kKeys * 128;        // 64 keys x 64 dims
+  static constexpr int kGroups = R / 128;
+  static constexpr uint32_t kChunkBytes = kKeys * 128;  // 64 keys x 64 dims
   static constexpr uint32_t kTileBytes = kChunks * kChunkBytes;
   static constexpr uint32_t kQChunk = NT * 128;
   static constexpr uint32_t kQBytes = kChunks * kQChunk;
@@ -65,8 +121,9 @@ struct DecodeSmem {
   alignas(1024) uint8_t k[S::kStages][S::kTileBytes];
   alignas(1024) uint8_t q[S::kQBytes];
   alignas(1024) uint8_t p[S::kP];
-  float red[2][kSoft][NT];  // per warp column maxima (tiles alternate), then sums
-  uint64_t q_full, kv_full[S::kStages], kv_empty[S::kStages], s_full[2], s_free[2], p_full, pv_done, drained;
+  float red[kSoft][NT];  // per warp column maxima, or sums
+  uint64_t q_full, q_empty, kv_full[S::kStages][S::kGroups], kv_empty[S::kStages][S::kGroups], s_full[2], s_free[2],
+      p_full, pv_done, drained;
   uint32_t tmem_base;
   volatile int abort_flag;
 };
@@ -89,6 +146,15 @@ __device__ __forceinline__ bool wait_or_abort(Smem& s, uint64_t* bar, uint32_t p
 }
 
 __device__ __forceinline__ void soft_barrier() { asm volatile("bar.sync 1, %0;" ::"n"(kSoft * 32) : "memory"); }
+__device__ __forceinline__ bool soft_any(bool v) {  // any thread of the softmax warps
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 q, %1, 0;\n\tbar.red.or.pred p, 1, %2, q;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r)
+      : "r"((uint32_t)v), "n"(kSoft * 32)
+      : "memory");
+  return r != 0;
+}
 
 // Reduces v[n] over the 8 lanes that share lane % 4 (rows of an accumulator fragment)
 // and leaves in v[0 .. out) the results of columns `first ..`: each step a lane keeps half of
@@ -130,30 +196,48 @@ __device__ __forceinline__ void columns16(const float (&v)[V], int c, float (&ou
     out[n] = __shfl_sync(0xffffffffu, v[((c + n) >> 3) * 2 + (n & 1)], (n & 7) >> 1);
 }
 
+// A CTA's stretch of the line, piece by piece.
+struct Pieces {
+  const int32_t* start;  // table + 1
+  int at, end, b;
+  __device__ Pieces(const int32_t* table, int B, int c) : start(table + 1) {
+    const int quota = table[0], all = table[1 + B];
+    at = min((int64_t)c * quota, (int64_t)all);
+    end = min(at + quota, all);
+    int lo = 0, hi = B - 1;  // last sequence that starts at or before `at`
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) / 2;
+      if (start[mid] <= at) lo = mid;
+      else hi = mid - 1;
+    }
+    b = lo;
+  }
+  __device__ bool more() const { return at < end; }
+  __device__ int first() const { return at - start[b]; }             // tile within the sequence
+  __device__ int tiles() const { return min(end, start[b + 1]) - at; }
+  __device__ void next() {
+    at = min(end, start[b + 1]);
+    while (at < end && start[b + 1] <= at) ++b;  // sequences without keys take no tiles
+  }
+};
+
 template <int R, int NT>
 __global__ void __launch_bounds__(kThreads, 1)
     latent_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap c_map,
                        int64_t num_blocks, int page, const int32_t* __restrict__ block_tables, int max_blocks,
-                       const int32_t* __restrict__ ctx_lens, float* __restrict__ part_o,
-                       float* __restrict__ part_lse, int H, int heads_per_cta, int nsplit, float scale_log2,
-                       int* __restrict__ err) {
+                       const int32_t* __restrict__ ctx_lens, const int32_t* __restrict__ table,
+                       float* __restrict__ part_o, float* __restrict__ part_lse, int B, int H, int heads_per_cta,
+                       int head_tiles, float scale_log2, int* __restrict__ err) {
   griddep_entry();
   using S = Shape<R, NT>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   DecodeSmem<R, NT>& s = *reinterpret_cast<DecodeSmem<R, NT>*>(smem_raw);
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int split = blockIdx.x, b = blockIdx.z;
-  const int h0 = blockIdx.y * heads_per_cta, nheads = min(heads_per_cta, H - h0);
-  const int ctx = max(0, min(ctx_lens[b], max_blocks * page));
-  const int tiles_all = (ctx + kKeys - 1) / kKeys;
-  const int per = (tiles_all + nsplit - 1) / nsplit;
-  const int tile0 = split * per;
-  const int ntiles = max(0, min(tiles_all, tile0 + per) - tile0);
-  const int64_t part0 = ((int64_t)b * H + h0) * nsplit + split;  // + head * nsplit
-  if (ntiles == 0) {
-    if (threadIdx.x < nheads) part_lse[part0 + (int64_t)threadIdx.x * nsplit] = -INFINITY;
-    return;
-  }
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
+  const int ht = blockIdx.x % head_tiles, c = blockIdx.x / head_tiles;
+  const int ctas = gridDim.x / head_tiles;
+  const int h0 = ht * heads_per_cta, nheads = min(heads_per_cta, H - h0);
+  Pieces pc(table, B, c);
+  if (!pc.more()) return;
   if (smem_u32(smem_raw) & 1023) {  // the swizzled tiles need it
     if (threadIdx.x == 0) atomicCAS(err, 0, 83);
     return;
@@ -162,10 +246,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) {
     s.abort_flag = 0;
     mbar_init(&s.q_full, 1);
-    for (int i = 0; i < S::kStages; ++i) {
-      mbar_init(&s.kv_full[i], 1);
-      mbar_init(&s.kv_empty[i], 1);
-    }
+    mbar_init(&s.q_empty, 1);
+    for (int i = 0; i < S::kStages; ++i)
+      for (int g = 0; g < S::kGroups; ++g) {
+        mbar_init(&s.kv_full[i][g], 1);
+        mbar_init(&s.kv_empty[i][g], 1);
+      }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s.s_full[i], 1);
       mbar_init(&s.s_free[i], kSoft * 32);
@@ -179,105 +265,143 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = s.tmem_base;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, s.tmem_base, 0);
   const uint32_t tmem_o = tmem + 2 * NT;
 
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer
     const int pages = kKeys / page;  // per tile: 1, 2 or 4
-    const int32_t* bt = block_tables + (int64_t)b * max_blocks;
-    const int nblk = (ctx + page - 1) / page;
     const int oob = (int)(num_blocks * page);  // a row past the cache reads as zeros
-    if (lane == 0) mbar_arrive_expect_tx(&s.q_full, S::kQBytes);
-    __syncwarp();
-    if (lane < S::kChunks) tma_load_2d(s.q + lane * S::kQChunk, &q_map, &s.q_full, lane * 64, b * H + h0);
-    int sent = 0;
-    for (; sent < ntiles; ++sent) {
-      const int st = sent % S::kStages;
-      int y = oob;  // lane l < pages: first row of the tile's page l
-      const int j = (tile0 + sent) * pages + lane;
-      if (lane < pages && j < nblk) {
-        const int blk = bt[j];
-        if (blk >= 0 && blk < num_blocks) {
-          y = blk * page;
-        } else {
-          atomicCAS(err, 0, 82);
-        }
-      }
-      bool ok = !s.abort_flag;
-      if (ok && sent >= S::kStages) ok = wait_or_abort(s, &s.kv_empty[st], (sent / S::kStages - 1) & 1, err, 84);
+    int sent = 0, nq = 0;
+    bool ok = true;
+    // lane l < pages: first row of page l of a tile
+    auto page_row = [&](int b, int tile) {
+      const int j = tile * pages + lane;
+      const int nblk = (min(ctx_lens[b], max_blocks * page) + page - 1) / page;
+      if (lane >= pages || j >= nblk) return oob;
+      const int blk = block_tables[(int64_t)b * max_blocks + j];
+      if (blk >= 0 && blk < num_blocks) return blk * page;
+      atomicCAS(err, 0, 82);
+      return oob;
+    };
+    for (; ok && pc.more(); pc.next()) {
+      const int b = pc.b, t0 = pc.first(), n = pc.tiles();
+      int y = page_row(b, t0);
+      if (nq > 0) ok = wait_or_abort(s, &s.q_empty, (nq - 1) & 1, err, 84);
       if (!__all_sync(0xffffffffu, ok)) break;
-      if (lane == 0) mbar_arrive_expect_tx(&s.kv_full[st], S::kTileBytes);
+      if (lane == 0) mbar_arrive_expect_tx(&s.q_full, S::kQBytes);
       __syncwarp();
-      for (int i0 = 0; i0 < pages * S::kChunks; i0 += 32) {
-        const int i = i0 + lane, pg = min(i / S::kChunks, pages - 1), c = i % S::kChunks;
-        const int yy = __shfl_sync(0xffffffffu, y, pg);
-        if (i < pages * S::kChunks)
-          tma_load_2d(s.k[st] + c * S::kChunkBytes + pg * page * 128, &c_map, &s.kv_full[st], c * 64, yy);
+      if (lane < S::kChunks) tma_load_2d(s.q + lane * S::kQChunk, &q_map, &s.q_full, lane * 64, b * H + h0);
+      ++nq;
+      for (int i = 0; i < n; ++i, ++sent) {
+        const int st = sent % S::kStages;
+        const int y_next = i + 1 < n ? page_row(b, t0 + i + 1) : oob;
+#pragma unroll
+        for (int g = 0; g < S::kGroups; ++g) {
+          if (sent >= S::kStages) ok = ok && wait_or_abort(s, &s.kv_empty[st][g], (sent / S::kStages - 1) & 1, err, 84);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          const int nch = g == 0 ? 3 : 2;
+          if (lane == 0) mbar_arrive_expect_tx(&s.kv_full[st][g], nch * S::kChunkBytes);
+          __syncwarp();
+          const int pg = min(lane / nch, pages - 1);
+          const int ch = lane % nch == 2 ? S::kChunks - 1 : 2 * g + lane % nch;
+          const int yy = __shfl_sync(0xffffffffu, y, pg);
+          if (lane < pages * nch)
+            tma_load_2d(s.k[st] + ch * S::kChunkBytes + pg * page * 128, &c_map, &s.kv_full[st][g], ch * 64, yy);
+        }
+        if (!ok) break;
+        y = y_next;
       }
     }
     // the copies in flight end before the CTA does, on the way out of a time-out too
+    // (a group of the tile at hand may not have been sent: its wait then ends at once or
+    // at the bound)
     if (lane == 0) {
-      mbar_wait_sleep(&s.q_full, 0);
+      if (nq > 0) mbar_wait_sleep(&s.q_full, (nq - 1) & 1);
       for (int i = max(0, sent - S::kStages); i < sent; ++i)
-        mbar_wait_sleep(&s.kv_full[i % S::kStages], (i / S::kStages) & 1);
+        for (int g = 0; g < S::kGroups; ++g) mbar_wait_sleep(&s.kv_full[i % S::kStages][g], (i / S::kStages) & 1);
+      if (!ok)
+        for (int g = 0; g < S::kGroups; ++g)
+          mbar_wait_sleep(&s.kv_full[sent % S::kStages][g], (sent / S::kStages) & 1, 10000000ull);
     }
   } else if (warp == 1) {
     // -------------------------------------------------------------- MMA issuer
-    if (lane == 0) {
+    if (elect_one()) {
       constexpr uint32_t idesc_s = idesc_bf16<64, NT>();
       constexpr uint32_t idesc_o = idesc_bf16<128, NT>() | kIdescAMn | kIdescBMn;
       const uint32_t q_addr = smem_u32(s.q), p_addr = smem_u32(s.p);
-      auto issue_s = [&](int j) {  // the tile has landed
-        tc_fence_after();
-        const uint32_t k_addr = smem_u32(s.k[j % S::kStages]);
+      // two cursors over the same tiles: scores (sc) and second products (pv)
+      Pieces sp = pc;
+      int sc = 0, grp = 0, left_s = sp.tiles(), nq = 0;
+      bool s_open = false, q_open = false, first_s = true;
+      const int total = pc.end - pc.at;
+      int left_p = pc.tiles();
+      bool first_p = true;
+      uint64_t t_last = globaltimer_ns();
+      for (int pv = 0; pv < total;) {
+        bool moved = false;
+        if (sc < total) {
+          if (!q_open && mbar_try_wait(&s.q_full, nq & 1)) q_open = true;
+          if (!s_open && (sc < 2 || mbar_try_wait(&s.s_free[sc & 1], ((sc >> 1) - 1) & 1))) s_open = true;
+          const int st = sc % S::kStages;
+          if (q_open && s_open && mbar_try_wait(&s.kv_full[st][grp], (sc / S::kStages) & 1)) {
+            tc_fence_after();
+            const uint32_t k_addr = smem_u32(s.k[st]);
+            auto chunk = [&](int ch, bool fresh) {
 #pragma unroll
-        for (int c = 0; c < S::kChunks; ++c)
-#pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            mma_bf16(tmem + (j & 1) * NT, smem_desc_sw128(k_addr + c * S::kChunkBytes + kk * 32),
-                     smem_desc_sw128(q_addr + c * S::kQChunk + kk * 32), idesc_s, c + kk > 0);
-        mma_commit(&s.s_full[j & 1]);
-      };
-      auto full = [&](int j) -> uint64_t* { return &s.kv_full[j % S::kStages]; };
-      auto full_ph = [&](int j) -> uint32_t { return (j / S::kStages) & 1; };
-      bool ok = wait_or_abort(s, &s.q_full, 0, err, 85) && wait_or_abort(s, full(0), 0, err, 85);
-      if (ok) issue_s(0);
-      for (int j = 0; ok && j < ntiles; ++j) {
-        // the next tile's scores as soon as it has landed, this tile's second product as
-        // soon as P is there, whichever comes first
-        bool next = j + 1 >= ntiles, p_ready = false;
-        const uint64_t t_start = globaltimer_ns();
-        while (!p_ready) {
-          if (!next && mbar_try_wait(full(j + 1), full_ph(j + 1)) &&
-              (j + 1 < 2 || mbar_try_wait(&s.s_free[(j + 1) & 1], (((j + 1) >> 1) - 1) & 1))) {
-            issue_s(j + 1);
-            next = true;
-          }
-          p_ready = mbar_try_wait(&s.p_full, j & 1);
-          if (!p_ready && (s.abort_flag || globaltimer_ns() - t_start > 2000000000ull)) {
-            if (!s.abort_flag) atomicCAS(err, 0, 86);
-            s.abort_flag = 1;
-            ok = false;
-            break;
+              for (int kk = 0; kk < 4; ++kk)
+                mma_bf16(tmem + (sc & 1) * NT, smem_desc_sw128(k_addr + ch * S::kChunkBytes + kk * 32),
+                         smem_desc_sw128(q_addr + ch * S::kQChunk + kk * 32), idesc_s, !(fresh && kk == 0));
+            };
+            chunk(2 * grp, grp == 0);
+            chunk(2 * grp + 1, false);
+            if (grp == 0) chunk(S::kChunks - 1, false);
+            if (++grp == S::kGroups) {
+              mma_commit(&s.s_full[sc & 1]);
+              grp = 0;
+              ++sc;
+              s_open = false;
+              if (--left_s == 0) {  // the piece's last scores: its queries are free
+                mma_commit(&s.q_empty);
+                ++nq;
+                q_open = false;
+                sp.next();
+                left_s = sp.more() ? sp.tiles() : 0;
+              }
+            }
+            moved = true;
           }
         }
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t k_addr = smem_u32(s.k[j % S::kStages]);
+        if (pv < sc && mbar_try_wait(&s.p_full, pv & 1)) {
+          tc_fence_after();
+          const int st = pv % S::kStages;
+          const uint32_t k_addr = smem_u32(s.k[st]);
 #pragma unroll
-        for (int m = 0; m < R / 128; ++m)
+          for (int m = 0; m < S::kGroups; ++m) {
 #pragma unroll
-          for (int kk = 0; kk < kKeys / 16; ++kk)
-            mma_bf16(tmem_o + m * NT,
-                     smem_desc_mn_sw128(k_addr + 2 * m * S::kChunkBytes + kk * 2048, S::kChunkBytes, 1024),
-                     smem_desc_mn_sw128(p_addr + kk * 2048, 1024, 1024), idesc_o, j > 0 || kk > 0);
-        mma_commit(&s.pv_done);
-        mma_commit(&s.kv_empty[j % S::kStages]);
-        if (!next) {
-          ok = wait_or_abort(s, full(j + 1), full_ph(j + 1), err, 85) &&
-               (j + 1 < 2 || wait_or_abort(s, &s.s_free[(j + 1) & 1], (((j + 1) >> 1) - 1) & 1, err, 87));
-          if (ok) issue_s(j + 1);
+            for (int kk = 0; kk < kKeys / 16; ++kk)
+              mma_bf16(tmem_o + m * NT,
+                       smem_desc_mn_sw128(k_addr + 2 * m * S::kChunkBytes + kk * 2048, S::kChunkBytes, 1024),
+                       smem_desc_mn_sw128(p_addr + kk * 2048, 1024, 1024), idesc_o, !(first_p && kk == 0));
+            mma_commit(&s.kv_empty[st][m]);
+          }
+          mma_commit(&s.pv_done);
+          first_p = false;
+          ++pv;
+          if (--left_p == 0) {
+            pc.next();
+            left_p = pc.more() ? pc.tiles() : 0;
+            first_p = true;
+          }
+          moved = true;
+        }
+        if (moved) {
+          t_last = globaltimer_ns();
+        } else if (s.abort_flag || globaltimer_ns() - t_last > 2000000000ull) {
+          if (!s.abort_flag) atomicCAS(err, 0, 86);
+          s.abort_flag = 1;
+          break;
         }
       }
       // every MMA issued has finished before the tensor memory is freed
@@ -289,144 +413,140 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int quad = warp & 3;  // TMEM lane quadrant
     const int sw = warp - 2;
     constexpr int V = NT / 4;  // columns a thread holds
+    constexpr int VF = V >= 8 ? V / 8 : 1;
     const int row = quad * 16 + (lane >> 2);  // keys row and row + 8 of the tile
     const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
-    float m_ref[V], l[V];
+    int tile = 0;  // of the CTA
+    for (; pc.more(); pc.next()) {
+      const int b = pc.b, n_tiles = pc.tiles();
+      const int left = min(ctx_lens[b], max_blocks * page) - pc.first() * kKeys;  // keys from the piece's first on
+      float m_ref[V], l[V];
 #pragma unroll
-    for (int n = 0; n < V; ++n) m_ref[n] = -INFINITY, l[n] = 0.f;
-    for (int i = 0; i < ntiles; ++i) {
-      wait_or_abort(s, &s.s_full[i & 1], (i >> 1) & 1, err, 88);
-      __syncwarp();
-      tc_fence_after();
-      float v[NT / 8][4];
-      tmem_ld_frag<NT / 8>(tmem + lane_off + (i & 1) * NT, v);
-      tc_fence_before();
-      mbar_arrive(&s.s_free[i & 1]);
-      const int valid = ctx - (tile0 + i) * kKeys;  // keys of this tile
-      const bool in0 = row < valid, in1 = row + 8 < valid;
-      float mx[V];
-#pragma unroll
-      for (int n = 0; n < V; ++n) {
-        float& a = v[n >> 1][n & 1];
-        float& c = v[n >> 1][2 + (n & 1)];
-        a = in0 ? a * scale_log2 : -INFINITY;
-        c = in1 ? c * scale_log2 : -INFINITY;
-        mx[n] = fmaxf(a, c);
-      }
-      const int first = reduce_columns<V>(mx, [](float x, float y) { return fmaxf(x, y); });
-      constexpr int VF = V >= 8 ? V / 8 : 1;
-#pragma unroll
-      for (int n = 0; n < VF; ++n) s.red[i & 1][sw][frag_col(first + n)] = mx[n];
-      soft_barrier();
-      float mt[V];
-      bool raise = false;
-#pragma unroll
-      for (int g = 0; g < V / 2; ++g) {
-        const int c = g * 8 + (lane & 3) * 2;
-        float2 x = *reinterpret_cast<const float2*>(&s.red[i & 1][0][c]);
-#pragma unroll
-        for (int w = 1; w < kSoft; ++w) {
-          const float2 y = *reinterpret_cast<const float2*>(&s.red[i & 1][w][c]);
-          x.x = fmaxf(x.x, y.x), x.y = fmaxf(x.y, y.y);
-        }
-        mt[2 * g] = x.x, mt[2 * g + 1] = x.y;
-        raise |= x.x > m_ref[2 * g] + kRaise || x.y > m_ref[2 * g + 1] + kRaise;
-      }
-      // every warp sees every column, so all of them decide alike
-      raise = __any_sync(0xffffffffu, raise);
-      if (i > 0) wait_or_abort(s, &s.pv_done, (i - 1) & 1, err, 89);
-      __syncwarp();
-      if (raise) {
+      for (int n = 0; n < V; ++n) m_ref[n] = -INFINITY, l[n] = 0.f;
+      for (int i = 0; i < n_tiles; ++i, ++tile) {
+        wait_or_abort(s, &s.s_full[tile & 1], (tile >> 1) & 1, err, 88);
+        __syncwarp();
+        tc_fence_after();
+        float v[NT / 8][4];
+        tmem_ld_frag<NT / 8>(tmem + lane_off + (tile & 1) * NT, v);
+        tc_fence_before();
+        mbar_arrive(&s.s_free[tile & 1]);
+        const int valid = left - i * kKeys;  // keys of this tile
+        const bool in0 = row < valid, in1 = row + 8 < valid;
+        bool over = false;
 #pragma unroll
         for (int n = 0; n < V; ++n) {
-          const float mn = fmaxf(m_ref[n], mt[n]);
-          mt[n] = mn == -INFINITY ? 1.f : exp2f(m_ref[n] - mn);  // now the factor
-          m_ref[n] = mn;
-          l[n] *= mt[n];
+          float& a = v[n >> 1][n & 1];
+          float& d = v[n >> 1][2 + (n & 1)];
+          a = in0 ? a * scale_log2 : -INFINITY;
+          d = in1 ? d * scale_log2 : -INFINITY;
+          over |= fmaxf(a, d) > m_ref[n] + kRaise;
         }
-        if (i > 0) {
-          tc_fence_after();
+        const bool raise = soft_any(over);
+        if (tile > 0) wait_or_abort(s, &s.pv_done, (tile - 1) & 1, err, 89);  // P is free, O^T at rest
+        __syncwarp();
+        if (raise) {
+          float mx[V];
 #pragma unroll
-          for (int c = 0; c < NT; c += 16) {
-            float f[16];
-            columns16(mt, c, f);
-#pragma unroll 1
-            for (int m = 0; m < R / 128; ++m) {
-              float o[16];
-              uint32_t u[16];
-              const uint32_t at = tmem_o + lane_off + m * NT + c;
-              tmem_ld16(at, o);
+          for (int n = 0; n < V; ++n) mx[n] = fmaxf(v[n >> 1][n & 1], v[n >> 1][2 + (n & 1)]);
+          const int first = reduce_columns<V>(mx, [](float x, float y) { return fmaxf(x, y); });
 #pragma unroll
-              for (int n = 0; n < 16; ++n) u[n] = __float_as_uint(o[n] * f[n]);
-              tmem_st16(at, u);
-            }
+          for (int n = 0; n < VF; ++n) s.red[sw][frag_col(first + n)] = mx[n];
+          soft_barrier();
+          float f[V];
+#pragma unroll
+          for (int n = 0; n < V; ++n) {
+            const int col = frag_col(n);
+            const float mn = fmaxf(fmaxf(fmaxf(s.red[0][col], s.red[1][col]), fmaxf(s.red[2][col], s.red[3][col])), m_ref[n]);
+            f[n] = mn == -INFINITY ? 1.f : exp2f(m_ref[n] - mn);
+            m_ref[n] = mn;
+            l[n] *= f[n];
           }
-          tmem_wait_st();
-        }
-      }
+          if (i > 0) {
+            tc_fence_after();
 #pragma unroll
-      for (int g = 0; g < V / 2; ++g) {
-        const float m0 = m_ref[2 * g] == -INFINITY ? 0.f : m_ref[2 * g];
-        const float m1 = m_ref[2 * g + 1] == -INFINITY ? 0.f : m_ref[2 * g + 1];
-        const float a0 = exp2f(v[g][0] - m0), a1 = exp2f(v[g][1] - m1);
-        const float b0 = exp2f(v[g][2] - m0), b1 = exp2f(v[g][3] - m1);
-        l[2 * g] += a0 + b0;
-        l[2 * g + 1] += a1 + b1;
-        uint8_t* dst = s.p + (lane & 3) * 4;
-        *reinterpret_cast<uint32_t*>(dst + sw128_offset(row, g)) = pack_bf16(a0, a1);
-        *reinterpret_cast<uint32_t*>(dst + sw128_offset(row + 8, g)) = pack_bf16(b0, b1);
-      }
-      if (valid < kKeys) {  // the last tile: rows past the context
-        wait_or_abort(s, &s.kv_full[i % S::kStages], (i / S::kStages) & 1, err, 88);
-        uint8_t* kt = s.k[i % S::kStages];
-        const int t = threadIdx.x - 64, per_row = R / 8;  // 16-byte vectors of a row's latent
-        for (int e = t; e < (kKeys - valid) * per_row; e += kSoft * 32) {
-          const int r = valid + e / per_row, x = e % per_row;
-          *reinterpret_cast<uint4*>(kt + (x >> 3) * S::kChunkBytes + r * 128 + (x & 7) * 16) = make_uint4(0, 0, 0, 0);
-        }
-      }
-      fence_proxy_async_smem();
-      tc_fence_before();
-      mbar_arrive(&s.p_full);
-    }
-    wait_or_abort(s, &s.pv_done, (ntiles - 1) & 1, err, 89);
-    __syncwarp();
-    tc_fence_after();
-    float (&red)[kSoft][NT] = s.red[ntiles & 1];  // the last tile's maxima are in the other one
-    {
-      float part[V];
-#pragma unroll
-      for (int n = 0; n < V; ++n) part[n] = l[n];
-      const int first = reduce_columns<V>(part, [](float x, float y) { return x + y; });
-      constexpr int VF = V >= 8 ? V / 8 : 1;
-#pragma unroll
-      for (int n = 0; n < VF; ++n) red[sw][frag_col(first + n)] = part[n];
-    }
-    soft_barrier();
-#pragma unroll
-    for (int n = 0; n < V; ++n) {
-      const int c = frag_col(n);
-      float sum = 0.f;
-#pragma unroll
-      for (int w = 0; w < kSoft; ++w) sum += red[w][c];
-      l[n] = sum == 0.f ? 0.f : 1.f / sum;
-      if (sw == 0 && lane < 4 && c < nheads)
-        part_lse[part0 + (int64_t)c * nsplit] = sum == 0.f ? -INFINITY : m_ref[n] + log2f(sum);
-    }
-#pragma unroll
-    for (int c = 0; c < NT; c += 16) {
-      float f[16];
-      columns16(l, c, f);
+            for (int col = 0; col < NT; col += 16) {
+              float fc[16];
+              columns16(f, col, fc);
 #pragma unroll 1
-      for (int m = 0; m < R / 128; ++m) {
-        float o[16];
-        tmem_ld16(tmem_o + lane_off + m * NT + c, o);
-        // a warp writes 32 consecutive dims of one head at a time
-        float* dst = part_o + (part0 + (int64_t)c * nsplit) * R + m * 128 + quad * 32 + lane;
+              for (int m = 0; m < S::kGroups; ++m) {
+                float o[16];
+                uint32_t u[16];
+                const uint32_t at = tmem_o + lane_off + m * NT + col;
+                tmem_ld16(at, o);
 #pragma unroll
-        for (int n = 0; n < 16; ++n)
-          if (c + n < nheads) dst[(int64_t)n * nsplit * R] = o[n] * f[n];
+                for (int n = 0; n < 16; ++n) u[n] = __float_as_uint(o[n] * fc[n]);
+                tmem_st16(at, u);
+              }
+            }
+            tmem_wait_st();
+          }
+        }
+#pragma unroll
+        for (int g = 0; g < V / 2; ++g) {
+          const float m0 = m_ref[2 * g] == -INFINITY ? 0.f : m_ref[2 * g];
+          const float m1 = m_ref[2 * g + 1] == -INFINITY ? 0.f : m_ref[2 * g + 1];
+          const float a0 = exp2f(v[g][0] - m0), a1 = exp2f(v[g][1] - m1);
+          const float b0 = exp2f(v[g][2] - m0), b1 = exp2f(v[g][3] - m1);
+          l[2 * g] += a0 + b0;
+          l[2 * g + 1] += a1 + b1;
+          uint8_t* dst = s.p + (lane & 3) * 4;
+          *reinterpret_cast<uint32_t*>(dst + sw128_offset(row, g)) = pack_bf16(a0, a1);
+          *reinterpret_cast<uint32_t*>(dst + sw128_offset(row + 8, g)) = pack_bf16(b0, b1);
+        }
+        if (valid < kKeys) {  // the sequence's last tile: rows past the context
+          const int st = tile % S::kStages;
+          for (int g = 0; g < S::kGroups; ++g)
+            wait_or_abort(s, &s.kv_full[st][g], (tile / S::kStages) & 1, err, 88);
+          const int t = threadIdx.x - 64, per_row = R / 8;  // 16-byte vectors of a row's latent
+          for (int e = t; e < (kKeys - valid) * per_row; e += kSoft * 32) {
+            const int r = valid + e / per_row, x = e % per_row;
+            *reinterpret_cast<uint4*>(s.k[st] + (x >> 3) * S::kChunkBytes + r * 128 + (x & 7) * 16) = make_uint4(0, 0, 0, 0);
+          }
+        }
+        fence_proxy_async_smem();
+        tc_fence_before();
+        mbar_arrive(&s.p_full);
       }
+      // ---- the piece's partial result
+      wait_or_abort(s, &s.pv_done, (tile - 1) & 1, err, 89);
+      __syncwarp();
+      tc_fence_after();
+      const int64_t slot = ((int64_t)ht * (B + ctas) + b + c) * heads_per_cta;
+      {
+        float part[V];
+#pragma unroll
+        for (int n = 0; n < V; ++n) part[n] = l[n];
+        const int first = reduce_columns<V>(part, [](float x, float y) { return x + y; });
+#pragma unroll
+        for (int n = 0; n < VF; ++n) s.red[sw][frag_col(first + n)] = part[n];
+      }
+      soft_barrier();
+#pragma unroll
+      for (int n = 0; n < V; ++n) {
+        const int col = frag_col(n);
+        const float sum = s.red[0][col] + s.red[1][col] + s.red[2][col] + s.red[3][col];
+        l[n] = sum == 0.f ? 0.f : 1.f / sum;
+        if (sw == 0 && lane < 4 && col < nheads) part_lse[slot + col] = sum == 0.f ? -INFINITY : m_ref[n] + log2f(sum);
+      }
+      soft_barrier();  // the sums have been read: the next piece may write here
+#pragma unroll
+      for (int col = 0; col < NT; col += 16) {
+        if (col >= nheads) break;
+        float f[16];
+        columns16(l, col, f);
+#pragma unroll 1
+        for (int m = 0; m < S::kGroups; ++m) {
+          float o[16];
+          tmem_ld16(tmem_o + lane_off + m * NT + col, o);
+          // a warp writes 32 consecutive dims of one head at a time
+          float* dst = part_o + (slot + col) * R + m * 128 + quad * 32 + lane;
+#pragma unroll
+          for (int n = 0; n < 16; ++n)
+            if (col + n < nheads) dst[n * R] = o[n] * f[n];
+        }
+      }
+      tc_fence_before();  // O^T has been read: ordered before the next p_full
     }
   }
   tc_fence_before();
@@ -455,8 +575,11 @@ __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0
 template <int R, int MROWS>
 __global__ void __launch_bounds__(128) latent_absorb_kernel(const bf16* __restrict__ q, int64_t q_stride,
                                                             const bf16* __restrict__ w, bf16* __restrict__ qa, int B,
-                                                            int H) {
+                                                            int H, const int32_t* __restrict__ ctx_lens, int limit,
+                                                            int ctas, int32_t* __restrict__ table) {
   griddep_entry();
+  if (blockIdx.x == gridDim.x - 1 && blockIdx.y == 0 && blockIdx.z == 0)
+    write_schedule(ctx_lens, B, limit, ctas, table);
   constexpr int kPitchW = 64 + 8, kPitchX = kNope + 8;  // 16 bytes of padding: conflict-free ldmatrix
   __shared__ __align__(16) bf16 ws[kNope * kPitchW];
   __shared__ __align__(16) bf16 xs[MROWS * kPitchX];
@@ -509,72 +632,95 @@ __global__ void __launch_bounds__(128) latent_absorb_kernel(const bf16* __restri
       }
 }
 
-// Joins the splits and applies V_h: out[b, h, n] = sum_r o[b, h, r] w[h, 128 + n, r] with
-//   o = sum_s 2^(lse_s - M) o_s / sum_s 2^(lse_s - M).
+// Joins the pieces and applies V_h: out[b, h, n] = sum_r o[b, h, r] w[h, 128 + n, r] with
+//   o = sum_c 2^(lse_c - M) o_c / sum_c 2^(lse_c - M)  over the pieces c of sequence b.
 // o enters the product as hi + lo, two bf16 whose sum keeps 16 bits of it: the
 // second MMA costs nothing beside the loads, and one rounding less reaches the output.
-// One CTA per (NCOLS columns, head, MROWS rows), K in chunks of 128.
-template <int R, int MROWS, int NCOLS>
-__global__ void __launch_bounds__(MROWS == 64 ? 256 : 128)
+// One CTA per (NCOLS columns, head, MROWS rows), K in chunks of 128; the next chunk's
+// partials are in registers and its weights under way while one is multiplied.
+template <int R, int MROWS, int NCOLS, int THREADS>
+__global__ void __launch_bounds__(THREADS)
     latent_out_kernel(const float* __restrict__ part_o, const float* __restrict__ part_lse,
-                      const bf16* __restrict__ w, bf16* __restrict__ out, int64_t out_stride, int B, int H,
-                      int nsplit) {
+                      const int32_t* __restrict__ table, const bf16* __restrict__ w, bf16* __restrict__ out,
+                      int64_t out_stride, int B, int H, int heads_per_cta, int ctas) {
   griddep_entry();
-  constexpr int kThr = MROWS == 64 ? 256 : 128;
   constexpr int kPitch = 128 + 8;
   constexpr int kSteps = R / 128;
+  constexpr int kX = MROWS * 32 / THREADS;  // float4 a thread joins per chunk
   extern __shared__ __align__(16) uint8_t raw[];
   bf16* ws = reinterpret_cast<bf16*>(raw);             // [2][NCOLS][kPitch]
   bf16* xh = ws + 2 * NCOLS * kPitch;                  // [MROWS][kPitch]
   bf16* xl = xh + MROWS * kPitch;
-  float* wt = reinterpret_cast<float*>(xl + MROWS * kPitch);  // [MROWS][nsplit] split weights
+  float* wt = reinterpret_cast<float*>(xl + MROWS * kPitch);   // [MROWS][kMaxPieces] weights
+  int* np = reinterpret_cast<int*>(wt + MROWS * kMaxPieces);   // [MROWS] pieces
+  int64_t* src0 = reinterpret_cast<int64_t*>(np + MROWS);      // [MROWS] first piece's partial
   const int n0 = blockIdx.x * NCOLS, h = blockIdx.y, b0 = blockIdx.z * MROWS;
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
+  const int ht = h / heads_per_cta, hh = h % heads_per_cta;
   const bf16* wv = w + ((int64_t)h * (kNope + kVal) + kNope + n0) * R;
   auto load_w = [&](int c) {
-    for (int i = t; i < NCOLS * 16; i += kThr)
+    for (int i = t; i < NCOLS * 16; i += THREADS)
       cp16(ws + ((c & 1) * NCOLS + (i >> 4)) * kPitch + (i & 15) * 8, wv + (int64_t)(i >> 4) * R + c * 128 + (i & 15) * 8);
     cp_commit();
   };
   load_w(0);
-  for (int r = warp; r < MROWS; r += kThr / 32) {  // a warp per row
+  const int quota = table[0];
+  for (int r = warp; r < MROWS; r += THREADS / 32) {  // a warp per row
     const int b = b0 + r;
-    const float* lse = part_lse + ((int64_t)min(b, B - 1) * H + h) * nsplit;
-    const float a0 = lane < nsplit ? lse[lane] : -INFINITY, a1 = lane + 32 < nsplit ? lse[lane + 32] : -INFINITY;
+    int n = 0;
+    int64_t slot = 0;
+    if (b < B) {
+      const int s0 = table[1 + b], s1 = table[2 + b];
+      const int c0 = s0 / quota;
+      n = s1 > s0 ? min((s1 - 1) / quota - c0 + 1, kMaxPieces) : 0;
+      slot = ((int64_t)ht * (B + ctas) + b + c0) * heads_per_cta + hh;
+    }
+    const float a0 = lane < n ? part_lse[slot + (int64_t)lane * heads_per_cta] : -INFINITY;
+    const float a1 = lane + 32 < n ? part_lse[slot + (int64_t)(lane + 32) * heads_per_cta] : -INFINITY;
     const float M = warp_max(fmaxf(a0, a1));
-    // no split has a key: weights 0; a NaN in any split reaches the row
+    // no piece has a finite score: weights 0; a NaN in any piece reaches the row
     const float e0 = M == -INFINITY && a0 == a0 ? 0.f : exp2f(a0 - M), e1 = M == -INFINITY && a1 == a1 ? 0.f : exp2f(a1 - M);
     const float L = warp_sum(e0 + e1);
     const float inv = L == 0.f ? 0.f : 1.f / L;
-    if (lane < nsplit) wt[r * nsplit + lane] = e0 * inv;
-    if (lane + 32 < nsplit) wt[r * nsplit + lane + 32] = e1 * inv;
+    if (lane < n) wt[r * kMaxPieces + lane] = e0 * inv;
+    if (lane + 32 < n) wt[r * kMaxPieces + lane + 32] = e1 * inv;
+    if (lane == 0) np[r] = n, src0[r] = slot * R;
   }
-  constexpr int WN = MROWS == 64 ? NCOLS / 2 : NCOLS / 4;  // columns a warp
-  constexpr int NT8 = WN / 8;
-  const int r0 = MROWS == 64 ? (warp & 3) * 16 : 0, c0 = (MROWS == 64 ? warp >> 2 : warp) * WN;
+  constexpr int MW = MROWS / 16, NW = THREADS / 32 / MW;  // warps along rows and columns
+  constexpr int NT8 = NCOLS / NW / 8;
+  const int r0 = (warp % MW) * 16, c0 = (warp / MW) * (NCOLS / NW);
+  const int64_t pstride = (int64_t)heads_per_cta * R;
+  float4 x[kX];
+  auto load_x = [&](int c) {
+#pragma unroll
+    for (int i = 0; i < kX; ++i) {
+      const int r = (i * THREADS + t) >> 5;
+      const float* src = part_o + src0[r] + c * 128 + lane * 4;
+      const int n = np[r];
+      float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+      for (int p = 0; p < n; ++p) {
+        const float f = wt[r * kMaxPieces + p];
+        const float4 y = *reinterpret_cast<const float4*>(src + p * pstride);
+        a.x += f * y.x, a.y += f * y.y, a.z += f * y.z, a.w += f * y.w;
+      }
+      x[i] = a;
+    }
+  };
   float acc[NT8][4] = {};
   __syncthreads();
+  load_x(0);
   for (int c = 0; c < kSteps; ++c) {
     if (c + 1 < kSteps) load_w(c + 1);
-    for (int i = t; i < MROWS * 32; i += kThr) {
-      const int r = i >> 5, k = (i & 31) * 4;
-      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (b0 + r < B) {
-        const float* src = part_o + (((int64_t)(b0 + r) * H + h) * nsplit) * R + c * 128 + k;
-        for (int s = 0; s < nsplit; ++s) {
-          const float f = wt[r * nsplit + s];
-          if (f != 0.f) {  // a split without keys wrote no partial
-            const float4 y = *reinterpret_cast<const float4*>(src + (int64_t)s * R);
-            x.x += f * y.x, x.y += f * y.y, x.z += f * y.z, x.w += f * y.w;
-          }
-        }
-      }
-      const uint32_t h0 = pack_bf16(x.x, x.y), h1 = pack_bf16(x.z, x.w);
+#pragma unroll
+    for (int i = 0; i < kX; ++i) {
+      const int r = (i * THREADS + t) >> 5;
+      const uint32_t h0 = pack_bf16(x[i].x, x[i].y), h1 = pack_bf16(x[i].z, x[i].w);
       const float2 f0 = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&h0));
       const float2 f1 = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&h1));
-      *reinterpret_cast<uint2*>(xh + r * kPitch + k) = make_uint2(h0, h1);
-      *reinterpret_cast<uint2*>(xl + r * kPitch + k) =
-          make_uint2(pack_bf16(x.x - f0.x, x.y - f0.y), pack_bf16(x.z - f1.x, x.w - f1.y));
+      *reinterpret_cast<uint2*>(xh + r * kPitch + lane * 4) = make_uint2(h0, h1);
+      *reinterpret_cast<uint2*>(xl + r * kPitch + lane * 4) =
+          make_uint2(pack_bf16(x[i].x - f0.x, x[i].y - f0.y), pack_bf16(x[i].z - f1.x, x[i].w - f1.y));
     }
     if (c + 1 < kSteps) {
       cp_wait<1>();
@@ -582,6 +728,7 @@ __global__ void __launch_bounds__(MROWS == 64 ? 256 : 128)
       cp_wait<0>();
     }
     __syncthreads();
+    if (c + 1 < kSteps) load_x(c + 1);
     const bf16* wc = ws + (c & 1) * NCOLS * kPitch;
 #pragma unroll
     for (int ks = 0; ks < 8; ++ks) {
@@ -613,75 +760,96 @@ __global__ void __launch_bounds__(MROWS == 64 ? 256 : 128)
     }
 }
 
-template <int R, int MROWS, int NCOLS>
-void run_out(const LatentDecode& a, const float* part_o, const float* part_lse, cudaStream_t st) {
-  auto kern = latent_out_kernel<R, MROWS, NCOLS>;
-  const size_t fixed = (size_t)(2 * NCOLS + 2 * MROWS) * 136 * 2;
+// Heads are cut into equal tiles of at most 64; each gets an equal share of the SMs, and
+// no more CTAs than B contexts of max_ctx tokens have tiles.
+struct Plan {
+  int head_tiles, heads_per_cta, ctas;
+  Plan(int B, int H, int max_ctx, int num_sms)
+      : head_tiles((H + 63) / 64), heads_per_cta((H + head_tiles - 1) / head_tiles) {
+    const int64_t tiles = (int64_t)B * std::max(1, max_ctx / kKeys + (max_ctx % kKeys != 0));
+    ctas = (int)std::max<int64_t>(1, std::min<int64_t>(num_sms / head_tiles, tiles));
+  }
+};
+
+// Workspace: qa, the schedule, the pieces' lse and o (each part 128-byte aligned).
+struct Layout {
+  size_t table, lse, part, bytes;
+  Layout(int B, int H, int R, const Plan& p) {
+    const size_t slots = (size_t)p.head_tiles * (B + p.ctas) * p.heads_per_cta;
+    auto up = [](size_t n) { return (n + 127) / 128 * 128; };
+    table = up((size_t)B * H * (R + kRot) * 2);
+    lse = table + up((size_t)table_ints(B) * 4);
+    part = lse + up(slots * 4);
+    bytes = part + slots * R * 4;
+  }
+};
+
+template <int R, int MROWS, int NCOLS, int THREADS>
+void run_out(const LatentDecode& a, const Plan& p, const float* part_o, const float* part_lse, const int32_t* table,
+             cudaStream_t st) {
+  auto kern = latent_out_kernel<R, MROWS, NCOLS, THREADS>;
+  constexpr size_t smem = (size_t)(2 * NCOLS + 2 * MROWS) * 136 * 2 + (size_t)MROWS * (kMaxPieces * 4 + 4 + 8);
   static std::atomic<uint64_t> attr_devs{0};
-  ensure_smem_attr(attr_devs, kern, fixed + (size_t)MROWS * kMaxSplits * 4);
-  launch_k(kern, dim3(kVal / NCOLS, a.H, (a.B + MROWS - 1) / MROWS), MROWS == 64 ? 256 : 128,
-           fixed + (size_t)MROWS * a.nsplit * 4, st, part_o, part_lse, a.w, a.out, a.out_stride, a.B, a.H, a.nsplit);
+  ensure_smem_attr(attr_devs, kern, smem);
+  launch_k(kern, dim3(kVal / NCOLS, a.H, (a.B + MROWS - 1) / MROWS), THREADS, smem, st, part_o, part_lse, table, a.w,
+           a.out, a.out_stride, a.B, a.H, p.heads_per_cta, p.ctas);
   KAPSL_LAUNCH_CHECK();
 }
 
 template <int R, int NT>
-void run_attn(const LatentDecode& a, const bf16* qa, float* part_o, float* part_lse, int head_tiles, cudaStream_t st) {
+void run_attn(const LatentDecode& a, const Plan& p, const bf16* qa, float* part_o, float* part_lse,
+              const int32_t* table, cudaStream_t st) {
   using S = Shape<R, NT>;
   auto kern = latent_attn_kernel<R, NT>;
-  const size_t smem = sizeof(DecodeSmem<R, NT>);
-  static_assert(sizeof(DecodeSmem<R, NT>) <= 232448, "shared memory of one CTA");
+  constexpr size_t smem = sizeof(DecodeSmem<R, NT>);
+  static_assert(smem <= 232448, "shared memory of one CTA");
   static std::atomic<uint64_t> attr_devs{0};
   ensure_smem_attr(attr_devs, kern, smem);
   const CUtensorMap tq = make_tmap_2d_bf16(qa, (uint64_t)a.B * a.H, S::W, S::W, NT, 64, true);
   const CUtensorMap tc = make_tmap_2d_bf16(a.cache, (uint64_t)a.num_blocks * a.page, S::W, S::W, a.page, 64, true);
-  launch_k(kern, dim3(a.nsplit, head_tiles, a.B), kThreads, smem, st, tq, tc, a.num_blocks, a.page, a.block_tables,
-           a.max_blocks, a.ctx_lens, part_o, part_lse, a.H, (a.H + head_tiles - 1) / head_tiles, a.nsplit,
+  launch_k(kern, dim3(p.ctas * p.head_tiles), kThreads, smem, st, tq, tc, a.num_blocks, a.page, a.block_tables,
+           a.max_blocks, a.ctx_lens, table, part_o, part_lse, a.B, a.H, p.heads_per_cta, p.head_tiles,
            a.scale * kLog2e, a.err);
   KAPSL_LAUNCH_CHECK();
 }
 
-int head_tiles_of(int H) { return (H + 63) / 64; }
-
 template <int R>
 void run(const LatentDecode& a, cudaStream_t st) {
-  bf16* qa = static_cast<bf16*>(a.workspace);
-  float* part_o = reinterpret_cast<float*>(qa + (int64_t)a.B * a.H * (R + kRot));
-  float* part_lse = part_o + (int64_t)a.B * a.H * a.nsplit * R;
+  const Plan p(a.B, a.H, a.max_ctx, a.num_sms);
+  const Layout l(a.B, a.H, R, p);
+  uint8_t* ws = static_cast<uint8_t*>(a.workspace);
+  bf16* qa = reinterpret_cast<bf16*>(ws);
+  int32_t* table = reinterpret_cast<int32_t*>(ws + l.table);
+  float* part_lse = reinterpret_cast<float*>(ws + l.lse);
+  float* part_o = reinterpret_cast<float*>(ws + l.part);
+  const int limit = a.max_blocks * a.page;
   if (a.B <= 16) {
-    launch_k(latent_absorb_kernel<R, 16>, dim3(R / 64, a.H, 1), 128, 0, st, a.q, a.q_stride, a.w, qa, a.B, a.H);
+    launch_k(latent_absorb_kernel<R, 16>, dim3(R / 64, a.H, 1), 128, 0, st, a.q, a.q_stride, a.w, qa, a.B, a.H,
+             a.ctx_lens, limit, p.ctas, table);
   } else {
     launch_k(latent_absorb_kernel<R, 64>, dim3(R / 64, a.H, (a.B + 63) / 64), 128, 0, st, a.q, a.q_stride, a.w, qa,
-             a.B, a.H);
+             a.B, a.H, a.ctx_lens, limit, p.ctas, table);
   }
   KAPSL_LAUNCH_CHECK();
-  const int ht = head_tiles_of(a.H), hpc = (a.H + ht - 1) / ht;
-  if (hpc <= 16) {
-    run_attn<R, 16>(a, qa, part_o, part_lse, ht, st);
-  } else if (hpc <= 32) {
-    run_attn<R, 32>(a, qa, part_o, part_lse, ht, st);
+  if (p.heads_per_cta <= 16) {
+    run_attn<R, 16>(a, p, qa, part_o, part_lse, table, st);
+  } else if (p.heads_per_cta <= 32) {
+    run_attn<R, 32>(a, p, qa, part_o, part_lse, table, st);
   } else {
-    run_attn<R, 64>(a, qa, part_o, part_lse, ht, st);
+    run_attn<R, 64>(a, p, qa, part_o, part_lse, table, st);
   }
   if (a.B <= 16) {
-    run_out<R, 16, 32>(a, part_o, part_lse, st);
+    run_out<R, 16, 32, 128>(a, p, part_o, part_lse, table, st);
   } else {
-    run_out<R, 64, 128>(a, part_o, part_lse, st);
+    run_out<R, 32, 128, 256>(a, p, part_o, part_lse, table, st);
   }
   note_launch(3);
 }
 
 }  // namespace
 
-int latent_decode_num_splits(int B, int H, int R, int max_ctx, int num_sms) {
-  const int ctas = std::max(1, B * head_tiles_of(std::max(1, H)));
-  int s = (4 * num_sms + ctas - 1) / ctas;
-  s = std::min(s, std::max(1, (max_ctx + 511) / 512));
-  return std::max(1, std::min(s, kMaxSplits));
-}
-
-size_t latent_decode_workspace_bytes(int B, int H, int R, int nsplit) {
-  const size_t bh = (size_t)B * H;
-  return bh * (R + kRot) * 2 + bh * nsplit * ((size_t)R + 1) * 4;
+size_t latent_decode_workspace_bytes(int B, int H, int R, int max_ctx, int num_sms) {
+  return Layout(B, H, R, Plan(B, H, max_ctx, num_sms)).bytes;
 }
 
 void launch_latent_decode(const LatentDecode& a, cudaStream_t st) {

@@ -341,8 +341,7 @@ def prefill_tc_tile(num_heads: int, num_kv_heads: int) -> int:
 # ------------------------------------------------------------ latent attention
 def latent_decode_attention(q: torch.Tensor, cache: torch.Tensor, w_kv_b: torch.Tensor, block_tables: torch.Tensor,
                             ctx_lens: torch.Tensor, num_heads: int, scale: Optional[float] = None,
-                            out: Optional[torch.Tensor] = None, num_splits: int = 0,
-                            max_ctx: Optional[int] = None) -> torch.Tensor:
+                            out: Optional[torch.Tensor] = None, max_ctx: Optional[int] = None) -> torch.Tensor:
     """Latent attention of one query token per row, absorbed form.
 
     ``cache`` [blocks, page, R + 64] holds one row a token (:func:`rope_latent_write`; R 256 or
@@ -351,21 +350,18 @@ def latent_decode_attention(q: torch.Tensor, cache: torch.Tensor, w_kv_b: torch.
     half is applied to the attended latents, so nothing is expanded per cached token.
     ``q`` [B, H * 192] has 128 position-free and 64 rotated dims a head; ``out`` is
     [B, H * 128].  Rows with ``ctx_lens`` 0 (a padded batch) give zeros.  ``max_ctx`` (a host
-    number, default the block tables' width) only chooses how many splits the context is cut into.
+    number, default the block tables' width) only bounds how many CTAs are launched.
     The keys of a block table entry outside the cache read as zeros, and device error 82 is recorded."""
     if scale is None:
         scale = 1.0 / math.sqrt(192)
-    B = q.shape[0]
     if out is None:
-        out = torch.empty(B, num_heads * 128, dtype=q.dtype, device=q.device)
+        out = torch.empty(q.shape[0], num_heads * 128, dtype=q.dtype, device=q.device)
+    if max_ctx is None:
+        max_ctx = block_tables.shape[-1] * cache.shape[1]
     c = cuda_ops()
-    R = cache.shape[-1] - 64
-    if num_splits <= 0:
-        mc = int(max_ctx) if max_ctx is not None else int(block_tables.shape[-1]) * int(cache.shape[1])
-        num_splits = int(c.latent_num_splits(B, num_heads, R, mc))
-    ws = torch.empty(max(1, int(c.latent_workspace_bytes(B, num_heads, R, num_splits))), dtype=torch.uint8,
+    ws = torch.empty(c.latent_workspace_bytes(q, num_heads, cache.shape[-1] - 64, max_ctx), dtype=torch.uint8,
                      device=q.device)
-    c.latent_decode_attention(q, cache, w_kv_b, block_tables, ctx_lens, out, num_heads, float(scale), num_splits, ws,
+    c.latent_decode_attention(q, cache, w_kv_b, block_tables, ctx_lens, out, num_heads, float(scale), max_ctx, ws,
                               error_buffer(q.device))
     return out
 

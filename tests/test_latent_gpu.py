@@ -301,10 +301,11 @@ def prefill64(q, rows, w, scale):
 LENS = [1, 15, 16, 17, 0, 63, 64, 65, 127, 128, 129, 300, 1000]
 
 
-@pytest.mark.parametrize("H,R,page,splits", [(1, 512, 16, 0), (3, 256, 64, 1), (8, 512, 64, 3), (17, 512, 32, 0),
-                                             (28, 512, 16, 7), (64, 512, 16, 1), (65, 256, 16, 2), (128, 512, 32, 0),
-                                             (33, 256, 32, 64)])
-def test_decode(dev, H, R, page, splits):
+@pytest.mark.parametrize("H,R,page,max_ctx", [(1, 512, 16, None), (3, 256, 64, 1), (8, 512, 64, 100),
+                                              (17, 512, 32, 1000), (28, 512, 16, 200), (64, 512, 16, None),
+                                              (65, 256, 16, 0), (128, 512, 32, 1000), (33, 256, 32, 64),
+                                              (200, 256, 16, None)])
+def test_decode(dev, H, R, page, max_ctx):
     from kapsl_sdk_b200 import ops
 
     k = Cache(dev, LENS, R, page, H * 7 + R)
@@ -314,12 +315,31 @@ def test_decode(dev, H, R, page, splits):
     w = k.randn(H, 256, R, std=1 / math.sqrt(R))
     scale = 1 / math.sqrt(192)
     out = torch.full((B, H * 128 + 8), 3.0, device=dev, dtype=torch.bfloat16)
-    ops.latent_decode_attention(q, k.cache, w, k.bt, k.ctx, H, out=out[:, :H * 128], num_splits=splits, max_ctx=1000)
+    ops.latent_decode_attention(q, k.cache, w, k.bt, k.ctx, H, out=out[:, :H * 128], max_ctx=max_ctx)
     no_error(dev)
     assert bool((out[:, H * 128:] == 3.0).all())
     for b in range(B):
         exp, tol = decode64(q[b].view(H, 192), k.rows[b], w, scale)
         within(out[b, :H * 128].view(H, 128), exp, tol)
+
+
+@pytest.mark.parametrize("B,H,hi", [(40, 5, 700), (300, 3, 130), (2, 7, 20000), (17, 70, 900)])
+def test_decode_ragged_batches(dev, B, H, hi):
+    """Stretches of the schedule that hold many sequences, and sequences cut into many pieces;
+    empty rows first, last and between."""
+    from kapsl_sdk_b200 import ops
+
+    r = random.Random(B)
+    lens = [0 if r.random() < 0.15 else r.randint(1, hi) for _ in range(B)]
+    if B > 2:
+        lens[0] = lens[-1] = 0
+    k = Cache(dev, lens, 512, 16, B + H)
+    q, w = k.randn(B, H * 192, std=1.5), k.randn(H, 256, 512, std=1 / math.sqrt(512))
+    out = ops.latent_decode_attention(q, k.cache, w, k.bt, k.ctx, H)
+    no_error(dev)
+    for b in sorted(r.sample(range(B), min(B, 24)) + [0, B - 1]):
+        exp, tol = decode64(q[b].view(H, 192), k.rows[b], w, 1 / math.sqrt(192))
+        within(out[b].view(H, 128), exp, tol)
 
 
 def test_decode_large_logits(dev):
@@ -340,8 +360,8 @@ def test_decode_large_logits(dev):
         j = torch.arange(n, device=dev)
         flat[k.bt[b, j // 16].long() * 16 + j % 16] = rows
         k.rows[b] = rows
-    for splits in (1, 3):
-        out = ops.latent_decode_attention(q, k.cache, w, k.bt, k.ctx, H, num_splits=splits)
+    for max_ctx in (None, 64, 200):  # pieces of one tile, of many, whole sequences
+        out = ops.latent_decode_attention(q, k.cache, w, k.bt, k.ctx, H, max_ctx=max_ctx)
         no_error(dev)
         for b in range(3):
             exp, tol = decode64(q[b].view(H, 192), k.rows[b], w, 1 / math.sqrt(192))
@@ -377,17 +397,16 @@ def test_decode_refuses(dev):
 
     k = Cache(dev, [40, 50], 512, 16, 3)
     q, w = k.randn(2, 5 * 192), k.randn(5, 256, 512, std=0.04)
-    a0 = dict(q=q, cache=k.cache, w=w, bt=k.bt, ctx=k.ctx, H=5, out=None, num_splits=0)
+    a0 = dict(q=q, cache=k.cache, w=w, bt=k.bt, ctx=k.ctx, H=5, out=None)
     for kw in (dict(q=q.float()), dict(q=q[:, :-1]), dict(q=q.cpu()), dict(cache=k.cache[..., :448].contiguous()),
                dict(cache=k.cache.float()), dict(cache=k.cache[:, :8].contiguous()), dict(w=w[:4]), dict(H=4),
                dict(w=w[..., :256].contiguous()), dict(w=w.transpose(1, 2)), dict(bt=k.bt.long()), dict(bt=k.bt[:1]),
-               dict(ctx=k.ctx.long()), dict(ctx=k.ctx[:1]), dict(out=q[:, :5 * 128]), dict(num_splits=65),
+               dict(ctx=k.ctx.long()), dict(ctx=k.ctx[:1]), dict(out=q[:, :5 * 128]),
                dict(out=torch.empty(2, 5 * 128, device=dev)), dict(q=k.randn(2, 5 * 192 + 1)[:, 1:]), dict(H=0)):
         a = dict(a0)
         a.update(kw)
         with pytest.raises((RuntimeError, TypeError, ValueError)):
-            ops.latent_decode_attention(a["q"], a["cache"], a["w"], a["bt"], a["ctx"], a["H"], out=a["out"],
-                                        num_splits=a["num_splits"])
+            ops.latent_decode_attention(a["q"], a["cache"], a["w"], a["bt"], a["ctx"], a["H"], out=a["out"])
     assert ops.latent_decode_attention(q[:0], k.cache, w, k.bt, k.ctx, 5).shape == (0, 640)
     no_error(dev)
 
