@@ -85,21 +85,26 @@ __device__ void write_schedule(const int32_t* __restrict__ ctx_lens, int B, int 
 // so a key tile is loaded once and serves both products, and O^T of 64 heads takes 256
 // of the 512 TMEM columns, which leaves room for two S^T tiles.
 //
-// Warp 0 loads the tiles by TMA, in groups of 128 latent dims (the rotary dims with the
-// first) with barriers of their own: the scores of a group start when it lands, and its
-// slot is free again when the second product has read it.  Warp 1 issues the MMAs from one
-// elected thread (elect.sync: issued from `lane == 0` the same MMAs took 44 cycles each
-// instead of the 23-48 of their operands).  Warps 2-5 do the softmax.
+// Tiles are loaded by TMA in groups of 128 latent dims (the rotary dims with the first),
+// one producer warp and one ring of barriers a group: the scores of a group start when it
+// lands, its slot is free again when the second product has read it.  One warp issues the
+// MMAs, four do the softmax.
 //
-// Softmax: scores are compared with the running maximum; only when one exceeds it by 2^8
-// (a vote over the four warps) is the maximum raised - column maxima by register and
-// shared-memory exchange - and O^T rescaled in TMEM.  p <= 256 loses nothing in bf16 or
+// Single-thread roles are entered by elect.sync.  Measured per SM: MMAs of M = 64, N = 16-64
+// issued from a `lane == 0` branch took 44 cycles each, elected 23-32; 2 KB boxes (16-token
+// pages) issued by nine lanes of one warp arrived at 17 B/clk, by one elected thread at 31, by
+// four warps' elected threads at 90 (8 KB boxes: 80).
+//
+// Softmax: scores (times log2 e) are compared with the running maximum; only when one
+// exceeds it by 8 (a vote over the four warps) is the maximum raised - column maxima by
+// register and shared-memory exchange - and O^T rescaled in TMEM.  p <= 256 loses nothing in bf16 or
 // fp32, and the final division uses the same maximum.  P is rounded to bf16, the operand
 // type of the second product; the row sums are of the fp32 values.  Keys past the context
 // have p = 0 and their cache rows are cleared in shared memory, since 0 * NaN of a
 // stale row would count.
 constexpr int kSoft = 4;  // softmax warps
-constexpr int kThreads = (2 + kSoft) * 32;
+template <int R>
+constexpr int kAttnThreads = (R / 128 + 1 + kSoft) * 32;
 constexpr float kRaise = 8.f;
 
 template <int R, int NT>
@@ -143,6 +148,12 @@ __device__ __forceinline__ bool wait_or_abort(Smem& s, uint64_t* bar, uint32_t p
     }
   }
   return false;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
 __device__ __forceinline__ void soft_barrier() { asm volatile("bar.sync 1, %0;" ::"n"(kSoft * 32) : "memory"); }
@@ -222,7 +233,7 @@ struct Pieces {
 };
 
 template <int R, int NT>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kAttnThreads<R>, 1)
     latent_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap c_map,
                        int64_t num_blocks, int page, const int32_t* __restrict__ block_tables, int max_blocks,
                        const int32_t* __restrict__ ctx_lens, const int32_t* __restrict__ table,
@@ -230,6 +241,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                        int head_tiles, float scale_log2, int* __restrict__ err) {
   griddep_entry();
   using S = Shape<R, NT>;
+  constexpr int kMma = S::kGroups;  // warps: producers, MMA issuer, softmax
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   DecodeSmem<R, NT>& s = *reinterpret_cast<DecodeSmem<R, NT>*>(smem_raw);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
@@ -254,22 +266,23 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s.s_full[i], 1);
-      mbar_init(&s.s_free[i], kSoft * 32);
+      mbar_init(&s.s_free[i], kSoft);
     }
-    mbar_init(&s.p_full, kSoft * 32);
+    mbar_init(&s.p_full, kSoft);
     mbar_init(&s.pv_done, 1);
     mbar_init(&s.drained, 1);
     fence_barrier_init();
   }
-  if (warp == 1) tmem_alloc(&s.tmem_base, 512);
+  if (warp == kMma) tmem_alloc(&s.tmem_base, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, s.tmem_base, 0);
   const uint32_t tmem_o = tmem + 2 * NT;
 
-  if (warp == 0) {
-    // ------------------------------------------------------------ TMA producer
+  if (warp < S::kGroups) {
+    // ------------------------------------------- TMA producer of dims [128 g, 128 g + 128)
+    const int g = warp;
     const int pages = kKeys / page;  // per tile: 1, 2 or 4
     const int oob = (int)(num_blocks * page);  // a row past the cache reads as zeros
     int sent = 0, nq = 0;
@@ -286,104 +299,100 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
     for (; ok && pc.more(); pc.next()) {
       const int b = pc.b, t0 = pc.first(), n = pc.tiles();
-      int y = page_row(b, t0);
-      if (nq > 0) ok = wait_or_abort(s, &s.q_empty, (nq - 1) & 1, err, 84);
-      if (!__all_sync(0xffffffffu, ok)) break;
-      if (lane == 0) mbar_arrive_expect_tx(&s.q_full, S::kQBytes);
-      __syncwarp();
-      if (lane < S::kChunks) tma_load_2d(s.q + lane * S::kQChunk, &q_map, &s.q_full, lane * 64, b * H + h0);
-      ++nq;
+      int y = page_row(b, t0), y1 = n > 1 ? page_row(b, t0 + 1) : oob;
+      if (g == 0) {
+        if (nq > 0) ok = wait_or_abort(s, &s.q_empty, (nq - 1) & 1, err, 84);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        if (elect_one()) {
+          mbar_arrive_expect_tx(&s.q_full, S::kQBytes);
+#pragma unroll
+          for (int ch = 0; ch < S::kChunks; ++ch)
+            tma_load_2d(s.q + ch * S::kQChunk, &q_map, &s.q_full, ch * 64, b * H + h0);
+        }
+        ++nq;
+      }
       for (int i = 0; i < n; ++i, ++sent) {
         const int st = sent % S::kStages;
-        const int y_next = i + 1 < n ? page_row(b, t0 + i + 1) : oob;
+        const int y2 = i + 2 < n ? page_row(b, t0 + i + 2) : oob;
+        int yy[4], zz[4];
 #pragma unroll
-        for (int g = 0; g < S::kGroups; ++g) {
-          if (sent >= S::kStages) ok = ok && wait_or_abort(s, &s.kv_empty[st][g], (sent / S::kStages - 1) & 1, err, 84);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          const int nch = g == 0 ? 3 : 2;
-          if (lane == 0) mbar_arrive_expect_tx(&s.kv_full[st][g], nch * S::kChunkBytes);
-          __syncwarp();
-          const int pg = min(lane / nch, pages - 1);
-          const int ch = lane % nch == 2 ? S::kChunks - 1 : 2 * g + lane % nch;
-          const int yy = __shfl_sync(0xffffffffu, y, pg);
-          if (lane < pages * nch)
-            tma_load_2d(s.k[st] + ch * S::kChunkBytes + pg * page * 128, &c_map, &s.kv_full[st][g], ch * 64, yy);
+        for (int pg = 0; pg < 4; ++pg) {
+          yy[pg] = __shfl_sync(0xffffffffu, y, pg);
+          zz[pg] = __shfl_sync(0xffffffffu, y1, pg);
         }
-        if (!ok) break;
-        y = y_next;
+        if (elect_one()) {  // the next tile comes into L2 while its slot is still in use
+#pragma unroll
+          for (int pg = 0; pg < 4; ++pg) {
+            if (pg < pages && zz[pg] < oob) {
+              tma_prefetch_2d(&c_map, 128 * g, zz[pg]);
+              tma_prefetch_2d(&c_map, 128 * g + 64, zz[pg]);
+              if (g == 0) tma_prefetch_2d(&c_map, R, zz[pg]);
+            }
+          }
+        }
+        __syncwarp();
+        if (sent >= S::kStages) ok = wait_or_abort(s, &s.kv_empty[st][g], (sent / S::kStages - 1) & 1, err, 84);
+        if (!__all_sync(0xffffffffu, ok)) {
+          ok = false;
+          break;
+        }
+        if (elect_one()) {
+          uint64_t* bar = &s.kv_full[st][g];
+          mbar_arrive_expect_tx(bar, (g == 0 ? 3 : 2) * S::kChunkBytes);
+#pragma unroll
+          for (int pg = 0; pg < 4; ++pg) {
+            if (pg < pages) {
+              uint8_t* dst = s.k[st] + pg * page * 128;
+              tma_load_2d(dst + 2 * g * S::kChunkBytes, &c_map, bar, 128 * g, yy[pg]);
+              tma_load_2d(dst + (2 * g + 1) * S::kChunkBytes, &c_map, bar, 128 * g + 64, yy[pg]);
+              if (g == 0) tma_load_2d(dst + (S::kChunks - 1) * S::kChunkBytes, &c_map, bar, R, yy[pg]);
+            }
+          }
+        }
+        __syncwarp();
+        y = y1;
+        y1 = y2;
       }
     }
     // the copies in flight end before the CTA does, on the way out of a time-out too
-    // (a group of the tile at hand may not have been sent: its wait then ends at once or
-    // at the bound)
     if (lane == 0) {
       if (nq > 0) mbar_wait_sleep(&s.q_full, (nq - 1) & 1);
       for (int i = max(0, sent - S::kStages); i < sent; ++i)
-        for (int g = 0; g < S::kGroups; ++g) mbar_wait_sleep(&s.kv_full[i % S::kStages][g], (i / S::kStages) & 1);
-      if (!ok)
-        for (int g = 0; g < S::kGroups; ++g)
-          mbar_wait_sleep(&s.kv_full[sent % S::kStages][g], (sent / S::kStages) & 1, 10000000ull);
+        mbar_wait_sleep(&s.kv_full[i % S::kStages][g], (i / S::kStages) & 1);
     }
-  } else if (warp == 1) {
+  } else if (warp == kMma) {
     // -------------------------------------------------------------- MMA issuer
     if (elect_one()) {
       constexpr uint32_t idesc_s = idesc_bf16<64, NT>();
       constexpr uint32_t idesc_o = idesc_bf16<128, NT>() | kIdescAMn | kIdescBMn;
-      const uint32_t q_addr = smem_u32(s.q), p_addr = smem_u32(s.p);
+      // Descriptors differ in the 14-bit address field only (16-byte units): one 64-bit base per
+      // operand and constant steps, so that an MMA costs two additions.
+      constexpr uint64_t kChunkStep = S::kChunkBytes >> 4, kTileStep = S::kTileBytes >> 4, kQStep = S::kQChunk >> 4;
+      const uint64_t k_desc = smem_desc_sw128(smem_u32(s.k[0])), q_desc = smem_desc_sw128(smem_u32(s.q));
+      const uint64_t v_desc = smem_desc_mn_sw128(smem_u32(s.k[0]), S::kChunkBytes, 1024);
+      const uint64_t p_desc = smem_desc_mn_sw128(smem_u32(s.p), 1024, 1024);
       // two cursors over the same tiles: scores (sc) and second products (pv)
       Pieces sp = pc;
       int sc = 0, grp = 0, left_s = sp.tiles(), nq = 0;
-      bool s_open = false, q_open = false, first_s = true;
+      bool s_open = true, q_open = false;
       const int total = pc.end - pc.at;
       int left_p = pc.tiles();
       bool first_p = true;
-      uint64_t t_last = globaltimer_ns();
+      uint64_t t_last = 0;
+      uint32_t idle = 0;
       for (int pv = 0; pv < total;) {
         bool moved = false;
-        if (sc < total) {
-          if (!q_open && mbar_try_wait(&s.q_full, nq & 1)) q_open = true;
-          if (!s_open && (sc < 2 || mbar_try_wait(&s.s_free[sc & 1], ((sc >> 1) - 1) & 1))) s_open = true;
-          const int st = sc % S::kStages;
-          if (q_open && s_open && mbar_try_wait(&s.kv_full[st][grp], (sc / S::kStages) & 1)) {
-            tc_fence_after();
-            const uint32_t k_addr = smem_u32(s.k[st]);
-            auto chunk = [&](int ch, bool fresh) {
-#pragma unroll
-              for (int kk = 0; kk < 4; ++kk)
-                mma_bf16(tmem + (sc & 1) * NT, smem_desc_sw128(k_addr + ch * S::kChunkBytes + kk * 32),
-                         smem_desc_sw128(q_addr + ch * S::kQChunk + kk * 32), idesc_s, !(fresh && kk == 0));
-            };
-            chunk(2 * grp, grp == 0);
-            chunk(2 * grp + 1, false);
-            if (grp == 0) chunk(S::kChunks - 1, false);
-            if (++grp == S::kGroups) {
-              mma_commit(&s.s_full[sc & 1]);
-              grp = 0;
-              ++sc;
-              s_open = false;
-              if (--left_s == 0) {  // the piece's last scores: its queries are free
-                mma_commit(&s.q_empty);
-                ++nq;
-                q_open = false;
-                sp.next();
-                left_s = sp.more() ? sp.tiles() : 0;
-              }
-            }
-            moved = true;
-          }
-        }
-        if (pv < sc && mbar_try_wait(&s.p_full, pv & 1)) {
+        // the second product first: it frees the slots that the next loads wait for
+        if (pv < sc && mbar_test_wait(&s.p_full, pv & 1)) {
           tc_fence_after();
           const int st = pv % S::kStages;
-          const uint32_t k_addr = smem_u32(s.k[st]);
+          const uint64_t v0 = v_desc + st * kTileStep;
 #pragma unroll
           for (int m = 0; m < S::kGroups; ++m) {
 #pragma unroll
             for (int kk = 0; kk < kKeys / 16; ++kk)
-              mma_bf16(tmem_o + m * NT,
-                       smem_desc_mn_sw128(k_addr + 2 * m * S::kChunkBytes + kk * 2048, S::kChunkBytes, 1024),
-                       smem_desc_mn_sw128(p_addr + kk * 2048, 1024, 1024), idesc_o, !(first_p && kk == 0));
+              mma_bf16(tmem_o + m * NT, v0 + 2 * m * kChunkStep + kk * 128, p_desc + kk * 128, idesc_o,
+                       !(first_p && kk == 0));
             mma_commit(&s.kv_empty[st][m]);
           }
           mma_commit(&s.pv_done);
@@ -396,12 +405,51 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           moved = true;
         }
+        if (sc < total) {
+          if (!q_open) q_open = mbar_test_wait(&s.q_full, nq & 1);
+          if (!s_open) s_open = mbar_test_wait(&s.s_free[sc & 1], ((sc >> 1) - 1) & 1);
+          const int st = sc % S::kStages;
+          if (q_open && s_open && mbar_test_wait(&s.kv_full[st][grp], (sc / S::kStages) & 1)) {
+            tc_fence_after();
+            const uint64_t k0 = k_desc + st * kTileStep, kg = k0 + 2 * grp * kChunkStep, qg = q_desc + 2 * grp * kQStep;
+            const uint32_t d = tmem + (sc & 1) * NT;
+            const uint32_t fresh = grp == 0;
+#pragma unroll
+            for (int ch = 0; ch < 2; ++ch)
+#pragma unroll
+              for (int kk = 0; kk < 4; ++kk)
+                mma_bf16(d, kg + ch * kChunkStep + kk * 2, qg + ch * kQStep + kk * 2, idesc_s, ch + kk > 0 || !fresh);
+            if (grp == 0)
+#pragma unroll
+              for (int kk = 0; kk < 4; ++kk)
+                mma_bf16(d, k0 + (S::kChunks - 1) * kChunkStep + kk * 2, q_desc + (S::kChunks - 1) * kQStep + kk * 2,
+                         idesc_s, 1);
+            if (++grp == S::kGroups) {
+              mma_commit(&s.s_full[sc & 1]);
+              grp = 0;
+              ++sc;
+              s_open = sc < 2;
+              if (--left_s == 0) {  // the piece's last scores: its queries are free
+                mma_commit(&s.q_empty);
+                ++nq;
+                q_open = false;
+                sp.next();
+                left_s = sp.more() ? sp.tiles() : 0;
+              }
+            }
+            moved = true;
+          }
+        }
         if (moved) {
-          t_last = globaltimer_ns();
-        } else if (s.abort_flag || globaltimer_ns() - t_last > 2000000000ull) {
-          if (!s.abort_flag) atomicCAS(err, 0, 86);
-          s.abort_flag = 1;
-          break;
+          idle = 0;
+        } else if ((++idle & 1023) == 0) {  // the clock is read rarely: it is slow
+          const uint64_t now = globaltimer_ns();
+          if (idle == 1024) t_last = now;
+          if (s.abort_flag || now - t_last > 2000000000ull) {
+            if (!s.abort_flag) atomicCAS(err, 0, 86);
+            s.abort_flag = 1;
+            break;
+          }
         }
       }
       // every MMA issued has finished before the tensor memory is freed
@@ -411,7 +459,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else {
     // ------------------------------------------------------- softmax, epilogue
     const int quad = warp & 3;  // TMEM lane quadrant
-    const int sw = warp - 2;
+    const int sw = warp - kMma - 1;
     constexpr int V = NT / 4;  // columns a thread holds
     constexpr int VF = V >= 8 ? V / 8 : 1;
     const int row = quad * 16 + (lane >> 2);  // keys row and row + 8 of the tile
@@ -422,7 +470,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int left = min(ctx_lens[b], max_blocks * page) - pc.first() * kKeys;  // keys from the piece's first on
       float m_ref[V], l[V];
 #pragma unroll
-      for (int n = 0; n < V; ++n) m_ref[n] = -INFINITY, l[n] = 0.f;
+      for (int n = 0; n < V; ++n) m_ref[n] = 0.f, l[n] = 0.f;
       for (int i = 0; i < n_tiles; ++i, ++tile) {
         wait_or_abort(s, &s.s_full[tile & 1], (tile >> 1) & 1, err, 88);
         __syncwarp();
@@ -430,26 +478,42 @@ __global__ void __launch_bounds__(kThreads, 1)
         float v[NT / 8][4];
         tmem_ld_frag<NT / 8>(tmem + lane_off + (tile & 1) * NT, v);
         tc_fence_before();
-        mbar_arrive(&s.s_free[tile & 1]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s.s_free[tile & 1]);  // one arrival a warp: 128 on one word serialise
         const int valid = left - i * kKeys;  // keys of this tile
         const bool in0 = row < valid, in1 = row + 8 < valid;
-        bool over = false;
+        float x[NT / 8][4], top = -INFINITY;
+        auto scores = [&](bool relative) {  // log2 scores, less the running maximum
 #pragma unroll
-        for (int n = 0; n < V; ++n) {
-          float& a = v[n >> 1][n & 1];
-          float& d = v[n >> 1][2 + (n & 1)];
-          a = in0 ? a * scale_log2 : -INFINITY;
-          d = in1 ? d * scale_log2 : -INFINITY;
-          over |= fmaxf(a, d) > m_ref[n] + kRaise;
-        }
-        const bool raise = soft_any(over);
+          for (int g = 0; g < NT / 8; ++g)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              x[g][e] = fmaf(v[g][e], scale_log2, relative ? -m_ref[2 * g + (e & 1)] : 0.f);
+          if (valid < kKeys) {
+#pragma unroll
+            for (int g = 0; g < NT / 8; ++g)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (!(e < 2 ? in0 : in1)) x[g][e] = -INFINITY;
+          }
+        };
+        scores(true);
+#pragma unroll
+        for (int g = 0; g < NT / 8; ++g)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            top = fmaxf(top, x[g][e]);
+            x[g][e] = ex2(x[g][e]);
+          }
+        const bool raise = soft_any(i == 0 || top > kRaise);
         if (tile > 0) wait_or_abort(s, &s.pv_done, (tile - 1) & 1, err, 89);  // P is free, O^T at rest
         __syncwarp();
         if (raise) {
           float mx[V];
+          scores(false);
 #pragma unroll
-          for (int n = 0; n < V; ++n) mx[n] = fmaxf(v[n >> 1][n & 1], v[n >> 1][2 + (n & 1)]);
-          const int first = reduce_columns<V>(mx, [](float x, float y) { return fmaxf(x, y); });
+          for (int n = 0; n < V; ++n) mx[n] = fmaxf(x[n >> 1][n & 1], x[n >> 1][2 + (n & 1)]);
+          const int first = reduce_columns<V>(mx, [](float a, float c) { return fmaxf(a, c); });
 #pragma unroll
           for (int n = 0; n < VF; ++n) s.red[sw][frag_col(first + n)] = mx[n];
           soft_barrier();
@@ -457,8 +521,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int n = 0; n < V; ++n) {
             const int col = frag_col(n);
-            const float mn = fmaxf(fmaxf(fmaxf(s.red[0][col], s.red[1][col]), fmaxf(s.red[2][col], s.red[3][col])), m_ref[n]);
-            f[n] = mn == -INFINITY ? 1.f : exp2f(m_ref[n] - mn);
+            float mn = fmaxf(fmaxf(s.red[0][col], s.red[1][col]), fmaxf(s.red[2][col], s.red[3][col]));
+            mn = i == 0 ? (mn == -INFINITY ? 0.f : mn) : fmaxf(mn, m_ref[n]);  // no finite score yet: any reference
+            f[n] = ex2(m_ref[n] - mn);
             m_ref[n] = mn;
             l[n] *= f[n];
           }
@@ -481,24 +546,25 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             tmem_wait_st();
           }
+          scores(true);
+#pragma unroll
+          for (int g = 0; g < NT / 8; ++g)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[g][e] = ex2(x[g][e]);
         }
 #pragma unroll
-        for (int g = 0; g < V / 2; ++g) {
-          const float m0 = m_ref[2 * g] == -INFINITY ? 0.f : m_ref[2 * g];
-          const float m1 = m_ref[2 * g + 1] == -INFINITY ? 0.f : m_ref[2 * g + 1];
-          const float a0 = exp2f(v[g][0] - m0), a1 = exp2f(v[g][1] - m1);
-          const float b0 = exp2f(v[g][2] - m0), b1 = exp2f(v[g][3] - m1);
-          l[2 * g] += a0 + b0;
-          l[2 * g + 1] += a1 + b1;
+        for (int g = 0; g < NT / 8; ++g) {
+          l[2 * g] += x[g][0] + x[g][2];
+          l[2 * g + 1] += x[g][1] + x[g][3];
           uint8_t* dst = s.p + (lane & 3) * 4;
-          *reinterpret_cast<uint32_t*>(dst + sw128_offset(row, g)) = pack_bf16(a0, a1);
-          *reinterpret_cast<uint32_t*>(dst + sw128_offset(row + 8, g)) = pack_bf16(b0, b1);
+          *reinterpret_cast<uint32_t*>(dst + sw128_offset(row, g)) = pack_bf16(x[g][0], x[g][1]);
+          *reinterpret_cast<uint32_t*>(dst + sw128_offset(row + 8, g)) = pack_bf16(x[g][2], x[g][3]);
         }
         if (valid < kKeys) {  // the sequence's last tile: rows past the context
           const int st = tile % S::kStages;
           for (int g = 0; g < S::kGroups; ++g)
             wait_or_abort(s, &s.kv_full[st][g], (tile / S::kStages) & 1, err, 88);
-          const int t = threadIdx.x - 64, per_row = R / 8;  // 16-byte vectors of a row's latent
+          const int t = sw * 32 + lane, per_row = R / 8;  // 16-byte vectors of a row's latent
           for (int e = t; e < (kKeys - valid) * per_row; e += kSoft * 32) {
             const int r = valid + e / per_row, x = e % per_row;
             *reinterpret_cast<uint4*>(s.k[st] + (x >> 3) * S::kChunkBytes + r * 128 + (x & 7) * 16) = make_uint4(0, 0, 0, 0);
@@ -506,7 +572,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         fence_proxy_async_smem();
         tc_fence_before();
-        mbar_arrive(&s.p_full);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s.p_full);
       }
       // ---- the piece's partial result
       wait_or_abort(s, &s.pv_done, (tile - 1) & 1, err, 89);
@@ -551,7 +618,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 1) {
+  if (warp == kMma) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
@@ -619,17 +686,22 @@ __global__ void __launch_bounds__(128) latent_absorb_kernel(const bf16* __restri
       mma_bf16_16816(acc[p][1], a, {bb[2], bb[3]});
     }
   }
+  __syncthreads();  // the result takes the queries' place, then leaves in whole 128-byte rows
 #pragma unroll
   for (int p = 0; p < NP; ++p)
 #pragma unroll
     for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int b = b0 + r0 + (lane >> 2) + e * 8;
-        if (b < B)
-          *reinterpret_cast<uint32_t*>(qa + ((int64_t)b * H + h) * (R + kRot) + n0 + c0 + p * 16 + nt * 8 + (lane & 3) * 2) =
-              pack_bf16(acc[p][nt][2 * e], acc[p][nt][2 * e + 1]);
-      }
+      for (int e = 0; e < 2; ++e)
+        *reinterpret_cast<uint32_t*>(xs + (r0 + (lane >> 2) + e * 8) * kPitchX + c0 + p * 16 + nt * 8 + (lane & 3) * 2) =
+            pack_bf16(acc[p][nt][2 * e], acc[p][nt][2 * e + 1]);
+  __syncthreads();
+  for (int i = t; i < MROWS * 8; i += 128) {
+    const int b = b0 + (i >> 3);
+    if (b < B)
+      *reinterpret_cast<uint4*>(qa + ((int64_t)b * H + h) * (R + kRot) + n0 + (i & 7) * 8) =
+          *reinterpret_cast<const uint4*>(xs + (i >> 3) * kPitchX + (i & 7) * 8);
+  }
 }
 
 // Joins the pieces and applies V_h: out[b, h, n] = sum_r o[b, h, r] w[h, 128 + n, r] with
@@ -691,20 +763,29 @@ __global__ void __launch_bounds__(THREADS)
   const int r0 = (warp % MW) * 16, c0 = (warp / MW) * (NCOLS / NW);
   const int64_t pstride = (int64_t)heads_per_cta * R;
   float4 x[kX];
+  // Pieces in the outer loop: the loads of the thread's kX rows are independent.
   auto load_x = [&](int c) {
+    int most = 0;
 #pragma unroll
     for (int i = 0; i < kX; ++i) {
-      const int r = (i * THREADS + t) >> 5;
-      const float* src = part_o + src0[r] + c * 128 + lane * 4;
-      const int n = np[r];
-      float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-      for (int p = 0; p < n; ++p) {
-        const float f = wt[r * kMaxPieces + p];
-        const float4 y = *reinterpret_cast<const float4*>(src + p * pstride);
-        a.x += f * y.x, a.y += f * y.y, a.z += f * y.z, a.w += f * y.w;
+      x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      most = max(most, np[(i * THREADS + t) >> 5]);
+    }
+#pragma unroll 2
+    for (int p = 0; p < most; ++p) {
+      float4 y[kX];
+#pragma unroll
+      for (int i = 0; i < kX; ++i) {
+        const int r = (i * THREADS + t) >> 5;
+        y[i] = p < np[r] ? *reinterpret_cast<const float4*>(part_o + src0[r] + p * pstride + c * 128 + lane * 4)
+                         : make_float4(0.f, 0.f, 0.f, 0.f);
       }
-      x[i] = a;
+#pragma unroll
+      for (int i = 0; i < kX; ++i) {
+        const float f = wt[((i * THREADS + t) >> 5) * kMaxPieces + p];
+        if (p < np[(i * THREADS + t) >> 5])
+          x[i].x += f * y[i].x, x[i].y += f * y[i].y, x[i].z += f * y[i].z, x[i].w += f * y[i].w;
+      }
     }
   };
   float acc[NT8][4] = {};
@@ -807,7 +888,7 @@ void run_attn(const LatentDecode& a, const Plan& p, const bf16* qa, float* part_
   ensure_smem_attr(attr_devs, kern, smem);
   const CUtensorMap tq = make_tmap_2d_bf16(qa, (uint64_t)a.B * a.H, S::W, S::W, NT, 64, true);
   const CUtensorMap tc = make_tmap_2d_bf16(a.cache, (uint64_t)a.num_blocks * a.page, S::W, S::W, a.page, 64, true);
-  launch_k(kern, dim3(p.ctas * p.head_tiles), kThreads, smem, st, tq, tc, a.num_blocks, a.page, a.block_tables,
+  launch_k(kern, dim3(p.ctas * p.head_tiles), kAttnThreads<R>, smem, st, tq, tc, a.num_blocks, a.page, a.block_tables,
            a.max_blocks, a.ctx_lens, table, part_o, part_lse, a.B, a.H, p.heads_per_cta, p.head_tiles,
            a.scale * kLog2e, a.err);
   KAPSL_LAUNCH_CHECK();
