@@ -7,8 +7,8 @@
 //   o_h = sum_j softmax(s)_j c_j,           out_h = V_h o_h,
 // so the cache is read once for all heads and nothing is expanded per token.
 //
-// Three launches: absorb (qa, and the schedule), attention over pieces of the contexts (fp32
-// partials of o), and one that joins the pieces and applies V_h.
+// Four launches: absorb (qa, and the schedule), attention over pieces of the contexts (fp32
+// partials of o), the join of the pieces, and the product with V_h.
 #include <algorithm>
 
 #include "common.cuh"
@@ -704,119 +704,109 @@ __global__ void __launch_bounds__(128) latent_absorb_kernel(const bf16* __restri
   }
 }
 
-// Joins the pieces and applies V_h: out[b, h, n] = sum_r o[b, h, r] w[h, 128 + n, r] with
-//   o = sum_c 2^(lse_c - M) o_c / sum_c 2^(lse_c - M)  over the pieces c of sequence b.
-// o enters the product as hi + lo, two bf16 whose sum keeps 16 bits of it: the
-// second MMA costs nothing beside the loads, and one rounding less reaches the output.
-// One CTA per (NCOLS columns, head, MROWS rows), K in chunks of 128; the next chunk's
-// partials are in registers and its weights under way while one is multiplied.
-template <int R, int MROWS, int NCOLS, int THREADS>
+// Joins a row's pieces: o[b, h] = sum_c 2^(lse_c - M) o_c / sum_c 2^(lse_c - M), written as hi + lo,
+// two bf16 whose sum keeps 16 bits of it: the product below then rounds nothing else.  One
+// thread per 8 dims, whole warps a row: the pieces' weights are spread over the lanes, four
+// pieces' loads are in flight at once.
+template <int R>
+__global__ void __launch_bounds__(128)
+    latent_join_kernel(const float* __restrict__ part_o, const float* __restrict__ part_lse,
+                       const int32_t* __restrict__ table, bf16* __restrict__ hi, bf16* __restrict__ lo, int B, int H,
+                       int heads_per_cta, int ctas) {
+  griddep_entry();
+  constexpr int kRowThreads = R / 8;
+  const int lane = threadIdx.x & 31;
+  const int64_t row = (int64_t)blockIdx.x * (128 / kRowThreads) + threadIdx.x / kRowThreads;  // b * H + h
+  if (row >= (int64_t)B * H) return;
+  const int k = threadIdx.x % kRowThreads * 8;
+  const int b = (int)(row / H), h = (int)(row % H), ht = h / heads_per_cta;
+  const int quota = table[0], s0 = table[1 + b], s1 = table[2 + b];
+  const int c0 = s0 / quota, n = s1 > s0 ? (s1 - 1) / quota - c0 + 1 : 0;
+  const int64_t slot = ((int64_t)ht * (B + ctas) + b + c0) * heads_per_cta + h % heads_per_cta;
+  const float* src = part_o + slot * R + k;
+  const int64_t step = (int64_t)heads_per_cta * R;
+  const float a0 = lane < n ? part_lse[slot + (int64_t)lane * heads_per_cta] : -INFINITY;
+  const float a1 = lane + 32 < n ? part_lse[slot + (int64_t)(lane + 32) * heads_per_cta] : -INFINITY;
+  float M = warp_max(fmaxf(a0, a1));
+  if (M == -INFINITY) M = 0.f;  // no finite score in the row: weights 0 (or NaN, which reaches the row)
+  const float e0 = ex2(a0 - M), e1 = ex2(a1 - M);
+  const float L = warp_sum(e0 + e1);
+  float x[8] = {};
+  for (int p0 = 0; p0 < n; p0 += 4) {
+    float4 y[4][2];
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      const float4* at = reinterpret_cast<const float4*>(src + min(p0 + p, n - 1) * step);  // weight 0 past the last
+      y[p][0] = at[0];
+      y[p][1] = at[1];
+    }
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      const float f = __shfl_sync(0xffffffffu, p0 < 32 ? e0 : e1, (p0 + p) & 31);
+      x[0] += f * y[p][0].x, x[1] += f * y[p][0].y, x[2] += f * y[p][0].z, x[3] += f * y[p][0].w;
+      x[4] += f * y[p][1].x, x[5] += f * y[p][1].y, x[6] += f * y[p][1].z, x[7] += f * y[p][1].w;
+    }
+  }
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  uint32_t top[4], low[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float u = x[2 * i] * inv, v = x[2 * i + 1] * inv;
+    top[i] = pack_bf16(u, v);
+    const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&top[i]));
+    low[i] = pack_bf16(u - f.x, v - f.y);
+  }
+  *reinterpret_cast<uint4*>(hi + row * R + k) = make_uint4(top[0], top[1], top[2], top[3]);
+  *reinterpret_cast<uint4*>(lo + row * R + k) = make_uint4(low[0], low[1], low[2], low[3]);
+}
+
+// out[b, h, n] = sum_r (hi + lo)[b, h, r] w[h, 128 + n, r].  One CTA per (NCOLS columns, head,
+// MROWS rows); K in chunks of 128 through STAGES shared-memory stages.
+template <int R, int MROWS, int NCOLS, int THREADS, int STAGES>
 __global__ void __launch_bounds__(THREADS)
-    latent_out_kernel(const float* __restrict__ part_o, const float* __restrict__ part_lse,
-                      const int32_t* __restrict__ table, const bf16* __restrict__ w, bf16* __restrict__ out,
-                      int64_t out_stride, int B, int H, int heads_per_cta, int ctas) {
+    latent_out_kernel(const bf16* __restrict__ hi, const bf16* __restrict__ lo, const bf16* __restrict__ w,
+                      bf16* __restrict__ out, int64_t out_stride, int B, int H) {
   griddep_entry();
   constexpr int kPitch = 128 + 8;
   constexpr int kSteps = R / 128;
-  constexpr int kX = MROWS * 32 / THREADS;  // float4 a thread joins per chunk
+  constexpr int kStage = (NCOLS + 2 * MROWS) * kPitch;
   extern __shared__ __align__(16) uint8_t raw[];
-  bf16* ws = reinterpret_cast<bf16*>(raw);             // [2][NCOLS][kPitch]
-  bf16* xh = ws + 2 * NCOLS * kPitch;                  // [MROWS][kPitch]
-  bf16* xl = xh + MROWS * kPitch;
-  float* wt = reinterpret_cast<float*>(xl + MROWS * kPitch);   // [MROWS][kMaxPieces] weights
-  int* np = reinterpret_cast<int*>(wt + MROWS * kMaxPieces);   // [MROWS] pieces
-  int64_t* src0 = reinterpret_cast<int64_t*>(np + MROWS);      // [MROWS] first piece's partial
+  bf16* sm = reinterpret_cast<bf16*>(raw);  // a stage: [NCOLS] w, [MROWS] hi, [MROWS] lo rows
   const int n0 = blockIdx.x * NCOLS, h = blockIdx.y, b0 = blockIdx.z * MROWS;
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
-  const int ht = h / heads_per_cta, hh = h % heads_per_cta;
   const bf16* wv = w + ((int64_t)h * (kNope + kVal) + kNope + n0) * R;
-  auto load_w = [&](int c) {
-    for (int i = t; i < NCOLS * 16; i += THREADS)
-      cp16(ws + ((c & 1) * NCOLS + (i >> 4)) * kPitch + (i & 15) * 8, wv + (int64_t)(i >> 4) * R + c * 128 + (i & 15) * 8);
+  auto load = [&](int c) {
+    if (c < kSteps) {
+      bf16* st = sm + (c % STAGES) * kStage;
+      for (int i = t; i < NCOLS * 16; i += THREADS)
+        cp16(st + (i >> 4) * kPitch + (i & 15) * 8, wv + (int64_t)(i >> 4) * R + c * 128 + (i & 15) * 8);
+      for (int i = t; i < 2 * MROWS * 16; i += THREADS) {
+        const int r = (i >> 4) % MROWS;
+        if (b0 + r < B)
+          cp16(st + (NCOLS + (i >> 4)) * kPitch + (i & 15) * 8,
+               (i >= MROWS * 16 ? lo : hi) + ((int64_t)(b0 + r) * H + h) * R + c * 128 + (i & 15) * 8);
+      }
+    }
     cp_commit();
   };
-  load_w(0);
-  const int quota = table[0];
-  for (int r = warp; r < MROWS; r += THREADS / 32) {  // a warp per row
-    const int b = b0 + r;
-    int n = 0;
-    int64_t slot = 0;
-    if (b < B) {
-      const int s0 = table[1 + b], s1 = table[2 + b];
-      const int c0 = s0 / quota;
-      n = s1 > s0 ? min((s1 - 1) / quota - c0 + 1, kMaxPieces) : 0;
-      slot = ((int64_t)ht * (B + ctas) + b + c0) * heads_per_cta + hh;
-    }
-    const float a0 = lane < n ? part_lse[slot + (int64_t)lane * heads_per_cta] : -INFINITY;
-    const float a1 = lane + 32 < n ? part_lse[slot + (int64_t)(lane + 32) * heads_per_cta] : -INFINITY;
-    const float M = warp_max(fmaxf(a0, a1));
-    // no piece has a finite score: weights 0; a NaN in any piece reaches the row
-    const float e0 = M == -INFINITY && a0 == a0 ? 0.f : exp2f(a0 - M), e1 = M == -INFINITY && a1 == a1 ? 0.f : exp2f(a1 - M);
-    const float L = warp_sum(e0 + e1);
-    const float inv = L == 0.f ? 0.f : 1.f / L;
-    if (lane < n) wt[r * kMaxPieces + lane] = e0 * inv;
-    if (lane + 32 < n) wt[r * kMaxPieces + lane + 32] = e1 * inv;
-    if (lane == 0) np[r] = n, src0[r] = slot * R;
-  }
+#pragma unroll
+  for (int c = 0; c < STAGES - 1; ++c) load(c);
   constexpr int MW = MROWS / 16, NW = THREADS / 32 / MW;  // warps along rows and columns
   constexpr int NT8 = NCOLS / NW / 8;
   const int r0 = (warp % MW) * 16, c0 = (warp / MW) * (NCOLS / NW);
-  const int64_t pstride = (int64_t)heads_per_cta * R;
-  float4 x[kX];
-  // Pieces in the outer loop: the loads of the thread's kX rows are independent.
-  auto load_x = [&](int c) {
-    int most = 0;
-#pragma unroll
-    for (int i = 0; i < kX; ++i) {
-      x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-      most = max(most, np[(i * THREADS + t) >> 5]);
-    }
-#pragma unroll 2
-    for (int p = 0; p < most; ++p) {
-      float4 y[kX];
-#pragma unroll
-      for (int i = 0; i < kX; ++i) {
-        const int r = (i * THREADS + t) >> 5;
-        y[i] = p < np[r] ? *reinterpret_cast<const float4*>(part_o + src0[r] + p * pstride + c * 128 + lane * 4)
-                         : make_float4(0.f, 0.f, 0.f, 0.f);
-      }
-#pragma unroll
-      for (int i = 0; i < kX; ++i) {
-        const float f = wt[((i * THREADS + t) >> 5) * kMaxPieces + p];
-        if (p < np[(i * THREADS + t) >> 5])
-          x[i].x += f * y[i].x, x[i].y += f * y[i].y, x[i].z += f * y[i].z, x[i].w += f * y[i].w;
-      }
-    }
-  };
   float acc[NT8][4] = {};
-  __syncthreads();
-  load_x(0);
   for (int c = 0; c < kSteps; ++c) {
-    if (c + 1 < kSteps) load_w(c + 1);
-#pragma unroll
-    for (int i = 0; i < kX; ++i) {
-      const int r = (i * THREADS + t) >> 5;
-      const uint32_t h0 = pack_bf16(x[i].x, x[i].y), h1 = pack_bf16(x[i].z, x[i].w);
-      const float2 f0 = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&h0));
-      const float2 f1 = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&h1));
-      *reinterpret_cast<uint2*>(xh + r * kPitch + lane * 4) = make_uint2(h0, h1);
-      *reinterpret_cast<uint2*>(xl + r * kPitch + lane * 4) =
-          make_uint2(pack_bf16(x[i].x - f0.x, x[i].y - f0.y), pack_bf16(x[i].z - f1.x, x[i].w - f1.y));
-    }
-    if (c + 1 < kSteps) {
-      cp_wait<1>();
-    } else {
-      cp_wait<0>();
-    }
-    __syncthreads();
-    if (c + 1 < kSteps) load_x(c + 1);
-    const bf16* wc = ws + (c & 1) * NCOLS * kPitch;
+    cp_wait<STAGES - 2>();
+    __syncthreads();  // the chunk is here, and the stage loaded next has been read
+    load(c + STAGES - 1);
+    const bf16* wc = sm + (c % STAGES) * kStage;
+    const bf16* xh = wc + NCOLS * kPitch;
 #pragma unroll
     for (int ks = 0; ks < 8; ++ks) {
       uint32_t ah[4], al[4];
       const int at = (r0 + (lane & 15)) * kPitch + ks * 16 + (lane >> 4) * 8;
       ldmatrix_x4(ah, smem_u32(xh + at));
-      ldmatrix_x4(al, smem_u32(xl + at));
+      ldmatrix_x4(al, smem_u32(xh + MROWS * kPitch + at));
 #pragma unroll
       for (int n = 0; n < NT8; ++n) {
         uint32_t bb[2];
@@ -828,7 +818,6 @@ __global__ void __launch_bounds__(THREADS)
         mma_bf16_16816(acc[n], al, bb);
       }
     }
-    __syncthreads();  // the x tile is rewritten next
   }
 #pragma unroll
   for (int n = 0; n < NT8; ++n)
@@ -852,28 +841,28 @@ struct Plan {
   }
 };
 
-// Workspace: qa, the schedule, the pieces' lse and o (each part 128-byte aligned).
+// Workspace: qa, the schedule, the joined rows' low halves, the pieces' lse and o (each part 128-byte aligned).
 struct Layout {
-  size_t table, lse, part, bytes;
+  size_t table, low, lse, part, bytes;
   Layout(int B, int H, int R, const Plan& p) {
     const size_t slots = (size_t)p.head_tiles * (B + p.ctas) * p.heads_per_cta;
     auto up = [](size_t n) { return (n + 127) / 128 * 128; };
     table = up((size_t)B * H * (R + kRot) * 2);
-    lse = table + up((size_t)table_ints(B) * 4);
+    low = table + up((size_t)table_ints(B) * 4);
+    lse = low + up((size_t)B * H * R * 2);
     part = lse + up(slots * 4);
     bytes = part + slots * R * 4;
   }
 };
 
-template <int R, int MROWS, int NCOLS, int THREADS>
-void run_out(const LatentDecode& a, const Plan& p, const float* part_o, const float* part_lse, const int32_t* table,
-             cudaStream_t st) {
-  auto kern = latent_out_kernel<R, MROWS, NCOLS, THREADS>;
-  constexpr size_t smem = (size_t)(2 * NCOLS + 2 * MROWS) * 136 * 2 + (size_t)MROWS * (kMaxPieces * 4 + 4 + 8);
+template <int R, int MROWS, int NCOLS, int THREADS, int STAGES>
+void run_out(const LatentDecode& a, const bf16* hi, const bf16* lo, cudaStream_t st) {
+  auto kern = latent_out_kernel<R, MROWS, NCOLS, THREADS, STAGES>;
+  constexpr size_t smem = (size_t)STAGES * (NCOLS + 2 * MROWS) * 136 * 2;
   static std::atomic<uint64_t> attr_devs{0};
   ensure_smem_attr(attr_devs, kern, smem);
-  launch_k(kern, dim3(kVal / NCOLS, a.H, (a.B + MROWS - 1) / MROWS), THREADS, smem, st, part_o, part_lse, table, a.w,
-           a.out, a.out_stride, a.B, a.H, p.heads_per_cta, p.ctas);
+  launch_k(kern, dim3(kVal / NCOLS, a.H, (a.B + MROWS - 1) / MROWS), THREADS, smem, st, hi, lo, a.w, a.out,
+           a.out_stride, a.B, a.H);
   KAPSL_LAUNCH_CHECK();
 }
 
@@ -919,12 +908,18 @@ void run(const LatentDecode& a, cudaStream_t st) {
   } else {
     run_attn<R, 64>(a, p, qa, part_o, part_lse, table, st);
   }
+  // qa has been read: the high halves take its place
+  bf16* lo = reinterpret_cast<bf16*>(ws + l.low);
+  const int64_t rows = (int64_t)a.B * a.H, per = 1024 / R;
+  launch_k(latent_join_kernel<R>, dim3((unsigned)((rows + per - 1) / per)), 128, 0, st, part_o, part_lse, table, qa,
+           lo, a.B, a.H, p.heads_per_cta, p.ctas);
+  KAPSL_LAUNCH_CHECK();
   if (a.B <= 16) {
-    run_out<R, 16, 32, 128>(a, p, part_o, part_lse, table, st);
+    run_out<R, 16, 32, 128, R / 128 + 1>(a, qa, lo, st);
   } else {
-    run_out<R, 32, 128, 256>(a, p, part_o, part_lse, table, st);
+    run_out<R, 32, 128, 256, 2>(a, qa, lo, st);
   }
-  note_launch(3);
+  note_launch(4);
 }
 
 }  // namespace
