@@ -56,6 +56,11 @@ inline void ensure_smem_attr(std::atomic<uint64_t>& done, Kernel* kern, size_t s
 // predecessor, so "previous grid done" implies "every earlier grid done".
 // launch_k() issues a kernel with the attribute that allows the early launch
 // (KAPSL_PDL=0 turns it off: plain stream order).
+//
+// A parameter that an earlier kernel writes is not declared `const T* __restrict__`: loads through
+// such a pointer count as loads of constant memory, and the compiler may move them above the
+// wait (seen with a schedule table read first thing in a kernel: a first run read what the
+// buffer held before).
 bool pdl_enabled();
 
 template <typename... KArgs, typename... Args>

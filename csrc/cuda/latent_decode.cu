@@ -45,7 +45,7 @@ __device__ __forceinline__ int seq_tiles(const int32_t* ctx_lens, int b, int lim
 }
 
 // One block writes the table (`limit`: tokens the block tables hold).
-__device__ void write_schedule(const int32_t* __restrict__ ctx_lens, int B, int limit, int ctas, int32_t* table) {
+__device__ void write_schedule(const int32_t* ctx_lens, int B, int limit, int ctas, int32_t* table) {
   __shared__ int sums[33], longest;
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5, nw = blockDim.x >> 5;
   if (t == 0) longest = 0;
@@ -235,10 +235,10 @@ struct Pieces {
 template <int R, int NT>
 __global__ void __launch_bounds__(kAttnThreads<R>, 1)
     latent_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap c_map,
-                       int64_t num_blocks, int page, const int32_t* __restrict__ block_tables, int max_blocks,
-                       const int32_t* __restrict__ ctx_lens, const int32_t* __restrict__ table,
-                       float* __restrict__ part_o, float* __restrict__ part_lse, int B, int H, int heads_per_cta,
-                       int head_tiles, float scale_log2, int* __restrict__ err) {
+                       int64_t num_blocks, int page, const int32_t* block_tables, int max_blocks,
+                       const int32_t* ctx_lens, const int32_t* table,
+                       float* part_o, float* part_lse, int B, int H, int heads_per_cta,
+                       int head_tiles, float scale_log2, int* err) {
   griddep_entry();
   using S = Shape<R, NT>;
   constexpr int kMma = S::kGroups;  // warps: producers, MMA issuer, softmax
@@ -640,10 +640,10 @@ __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0
 // qa[b, h, :R] = q[b, h, :128] . w[h, :128, :], qa[b, h, R:] = q[b, h, 128:].
 // One CTA per (64 columns, head, MROWS rows); qa is bf16, the tensor cores' operand type.
 template <int R, int MROWS>
-__global__ void __launch_bounds__(128) latent_absorb_kernel(const bf16* __restrict__ q, int64_t q_stride,
-                                                            const bf16* __restrict__ w, bf16* __restrict__ qa, int B,
-                                                            int H, const int32_t* __restrict__ ctx_lens, int limit,
-                                                            int ctas, int32_t* __restrict__ table) {
+__global__ void __launch_bounds__(128) latent_absorb_kernel(const bf16* q, int64_t q_stride,
+                                                            const bf16* w, bf16* qa, int B,
+                                                            int H, const int32_t* ctx_lens, int limit,
+                                                            int ctas, int32_t* table) {
   griddep_entry();
   if (blockIdx.x == gridDim.x - 1 && blockIdx.y == 0 && blockIdx.z == 0)
     write_schedule(ctx_lens, B, limit, ctas, table);
@@ -710,8 +710,8 @@ __global__ void __launch_bounds__(128) latent_absorb_kernel(const bf16* __restri
 // pieces' loads are in flight at once.
 template <int R>
 __global__ void __launch_bounds__(128)
-    latent_join_kernel(const float* __restrict__ part_o, const float* __restrict__ part_lse,
-                       const int32_t* __restrict__ table, bf16* __restrict__ hi, bf16* __restrict__ lo, int B, int H,
+    latent_join_kernel(const float* part_o, const float* part_lse,
+                       const int32_t* table, bf16* hi, bf16* lo, int B, int H,
                        int heads_per_cta, int ctas) {
   griddep_entry();
   constexpr int kRowThreads = R / 8;
@@ -764,8 +764,8 @@ __global__ void __launch_bounds__(128)
 // MROWS rows); K in chunks of 128 through STAGES shared-memory stages.
 template <int R, int MROWS, int NCOLS, int THREADS, int STAGES>
 __global__ void __launch_bounds__(THREADS)
-    latent_out_kernel(const bf16* __restrict__ hi, const bf16* __restrict__ lo, const bf16* __restrict__ w,
-                      bf16* __restrict__ out, int64_t out_stride, int B, int H) {
+    latent_out_kernel(const bf16* hi, const bf16* lo, const bf16* w,
+                      bf16* out, int64_t out_stride, int B, int H) {
   griddep_entry();
   constexpr int kPitch = 128 + 8;
   constexpr int kSteps = R / 128;

@@ -8,8 +8,10 @@
 
 #include "common.cuh"
 #include "kernels.h"
+#include "tcgen05.cuh"
 
 namespace kapsl {
+using namespace tc;
 
 using bf16 = __nv_bfloat16;
 
@@ -19,11 +21,11 @@ constexpr int kNope = 128, kRot = 64, kVal = 128;
 constexpr float kLog2e = 1.4426950408889634f;
 
 // One warp per output row; rows between sequences (padding to 16) become zero.
-__global__ void __launch_bounds__(256) latent_gather_kernel(const bf16* __restrict__ cache, int64_t num_blocks,
-                                                            int page, int W, const int32_t* __restrict__ seq_info,
-                                                            int nseq, const int32_t* __restrict__ block_tables,
-                                                            int max_blocks, bf16* __restrict__ rows, int64_t total,
-                                                            int* __restrict__ err) {
+__global__ void __launch_bounds__(256) latent_gather_kernel(const bf16* cache, int64_t num_blocks,
+                                                            int page, int W, const int32_t* seq_info,
+                                                            int nseq, const int32_t* block_tables,
+                                                            int max_blocks, bf16* rows, int64_t total,
+                                                            int* err) {
   griddep_entry();
   const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
@@ -48,40 +50,311 @@ __global__ void __launch_bounds__(256) latent_gather_kernel(const bf16* __restri
   for (int c = lane; c < W / 8; c += 32) dst[c] = src ? src[c] : make_uint4(0, 0, 0, 0);
 }
 
-// One warp per (token, head), keys one at a time.
-__global__ void __launch_bounds__(256) latent_prefill_kernel(const LatentPrefill a) {
-  griddep_entry();
-  const int seq = a.work[2 * blockIdx.x], t0 = a.work[2 * blockIdx.x + 1], h = blockIdx.y;
-  const int32_t* si = a.seq_info + 5 * seq;
-  const int row0 = si[0], n = si[1], ctx = si[2], kv0 = si[4];
-  const int lane = threadIdx.x & 31;
-  const int W = a.R + kRot;
-  for (int t = t0 + (threadIdx.x >> 5); t < min(n, t0 + 256); t += 8) {
-    const __nv_bfloat162* q = reinterpret_cast<const __nv_bfloat162*>(a.q + (int64_t)(row0 + t) * a.q_stride + h * 192);
-    const float2 q0 = __bfloat1622float2(q[lane]), q1 = __bfloat1622float2(q[32 + lane]),
-                 q2 = __bfloat1622float2(q[64 + lane]);
-    float2 o0 = make_float2(0.f, 0.f), o1 = o0;
-    float m = -INFINITY, l = 0.f;
-    const int last = ctx - n + t;
-    for (int j = 0; j <= last; ++j) {
-      const __nv_bfloat162* kv = reinterpret_cast<const __nv_bfloat162*>(a.kv + (int64_t)(kv0 + j) * a.kv_stride + h * 256);
-      const __nv_bfloat162* kr = reinterpret_cast<const __nv_bfloat162*>(a.rows + (int64_t)(kv0 + j) * W + a.R);
-      const float2 k0 = __bfloat1622float2(kv[lane]), k1 = __bfloat1622float2(kv[32 + lane]),
-                   k2 = __bfloat1622float2(kr[lane]);
-      const float s = a.scale * kLog2e *
-                      warp_sum(q0.x * k0.x + q0.y * k0.y + q1.x * k1.x + q1.y * k1.y + q2.x * k2.x + q2.y * k2.y);
-      const float2 v0 = __bfloat1622float2(kv[64 + lane]), v1 = __bfloat1622float2(kv[96 + lane]);
-      const float mn = fmaxf(m, s);
-      const float f = m == -INFINITY ? 0.f : exp2f(m - mn), p = mn == -INFINITY ? 0.f : exp2f(s - mn);
-      m = mn;
-      l = l * f + p;
-      o0 = make_float2(o0.x * f + p * v0.x, o0.y * f + p * v0.y);
-      o1 = make_float2(o1.x * f + p * v1.x, o1.y * f + p * v1.y);
+// ------------------------------------------------------------------ attention
+//
+// One CTA per (256 query tokens of a sequence, head): two tiles of 128 rows share every K and V
+// tile of 128 keys.  Per row tile t and key tile j:
+//   S_t = Q_t K_j^T     tcgen05.mma, K-major operands in shared memory -> 128 TMEM columns
+//   P_t = 2^(S_t - m)   one thread a row, packed to bf16 (the MMA's operand type; the row
+//                       sums are of the fp32 values) over S_t's columns
+//   O_t += P_t V_j      tcgen05.mma, P from TMEM, V MN-major from shared memory
+// The MMA thread issues PV_0(j), S_0(j+1), PV_1(j), S_1(j+1): while one row tile's softmax runs, the
+// tensor cores work on the other.  K (3 x 16 KB) and V (2 x 16 KB) tiles go through a
+// ring of eight 16 KB slots, 128 keys x 64 dims each.
+//
+// S_t(j + 1) is issued after PV_t(j) by the same thread, so once its scores are complete O_t is at
+// rest: the softmax warps themselves rescale it, and only when a score exceeds the running
+// maximum by 8 (in log2; p <= 256 loses nothing in bf16 or fp32).
+// Keys past a row's position have p = 0.  PV stops at the row tile's last key, rounded up
+// to 16; the rows there are the gather's zeros, so nothing behind a sequence is read.
+constexpr int kThreads = 384;  // warp 0 TMA, warp 1 MMA, warps 4-7 and 8-11 softmax of row tile 0 and 1
+constexpr int kSlots = 8;
+constexpr uint32_t kSlotBytes = 128 * 128;
+constexpr float kRaise = 8.f;
+
+struct alignas(1024) PrefillSmem {
+  uint8_t q[2][3][kSlotBytes];
+  uint8_t ring[kSlots][kSlotBytes];
+  uint64_t q_full, full[kSlots], empty[kSlots], s_full[2], p_full[2], o_full[2], drained;
+  uint32_t tmem_base;
+  volatile int abort_flag;
+};
+
+__device__ __forceinline__ bool wait_or_abort(PrefillSmem& s, uint64_t* bar, uint32_t parity, int* err, int code) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = globaltimer_ns();
+  while (!s.abort_flag) {
+    if (mbar_try_wait_sleep(bar, parity, 20000u)) return true;
+    if (globaltimer_ns() - t0 > 2000000000ull) {
+      atomicCAS(err, 0, code);
+      s.abort_flag = 1;
     }
-    const float inv = l > 0.f ? 1.f / l : 0.f;
-    __nv_bfloat162* dst = reinterpret_cast<__nv_bfloat162*>(a.out + (int64_t)(row0 + t) * a.out_stride + h * kVal);
-    dst[lane] = __floats2bfloat162_rn(o0.x * inv, o0.y * inv);
-    dst[32 + lane] = __floats2bfloat162_rn(o1.x * inv, o1.y * inv);
+  }
+  return false;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__global__ void __launch_bounds__(kThreads, 1)
+    latent_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap kv_map,
+                          const __grid_constant__ CUtensorMap rope_map, const int32_t* work,
+                          const int32_t* seq_info, int64_t q_rows, int R, float scale_log2,
+                          bf16* out, int64_t out_stride, int* err) {
+  griddep_entry();
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  PrefillSmem& s = *reinterpret_cast<PrefillSmem*>(smem_raw);
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
+  const int h = blockIdx.y;
+  const int32_t* si = seq_info + 5 * work[2 * blockIdx.x];
+  const int t0 = work[2 * blockIdx.x + 1];
+  const int row0 = si[0] + t0, n = si[1] - t0, pos0 = si[2] - si[1] + t0, kv0 = si[4];  // n: rows from t0 on
+  // keys and key tiles of the two row tiles
+  const int keys0 = pos0 + min(n, 128), keys1 = n > 128 ? pos0 + min(n, 256) : 0;
+  const int nt0 = (keys0 + 127) / 128, nt1 = (keys1 + 127) / 128, nt = max(nt0, nt1);
+  if ((smem_u32(smem_raw) & 1023) || row0 < 0 || row0 + min(n, 256) > q_rows || n <= 0) {
+    if (threadIdx.x == 0) atomicCAS(err, 0, 90);
+    return;
+  }
+
+  if (threadIdx.x == 0) {
+    s.abort_flag = 0;
+    mbar_init(&s.q_full, 1);
+    for (int i = 0; i < kSlots; ++i) {
+      mbar_init(&s.full[i], 1);
+      mbar_init(&s.empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s.s_full[i], 1);
+      mbar_init(&s.p_full[i], 4);
+      mbar_init(&s.o_full[i], 1);
+    }
+    mbar_init(&s.drained, 1);
+    fence_barrier_init();
+  }
+  if (warp == 1) tmem_alloc(&s.tmem_base, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = __shfl_sync(0xffffffffu, s.tmem_base, 0);  // S_0, S_1, O_0, O_1: 128 columns each
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ TMA producer
+    if (elect_one()) {
+      const int tiles_q = nt1 > 0 ? 2 : 1;
+      mbar_arrive_expect_tx(&s.q_full, tiles_q * 3 * kSlotBytes);
+      for (int t = 0; t < tiles_q; ++t)
+        for (int c = 0; c < 3; ++c) tma_load_2d(s.q[t][c], &q_map, &s.q_full, h * 192 + c * 64, row0 + t * 128);
+      int sent = 0;
+      bool ok = true;
+      for (int j = 0; ok && j < nt; ++j) {
+#pragma unroll
+        for (int c = 0; c < 5; ++c, ++sent) {  // key chunks 0, 1, rotary; value chunks 0, 1
+          const int slot = sent % kSlots;
+          if (sent >= kSlots && !wait_or_abort(s, &s.empty[slot], (sent / kSlots - 1) & 1, err, 91)) {
+            ok = false;
+            break;
+          }
+          mbar_arrive_expect_tx(&s.full[slot], kSlotBytes);
+          if (c == 2) {
+            tma_load_2d(s.ring[slot], &rope_map, &s.full[slot], R, kv0 + j * 128);
+          } else {
+            tma_load_2d(s.ring[slot], &kv_map, &s.full[slot], h * 256 + (c < 2 ? c : c - 1) * 64, kv0 + j * 128);
+          }
+        }
+      }
+      // the copies in flight end before the CTA does, on the way out of a time-out too
+      mbar_wait_sleep(&s.q_full, 0);
+      for (int i = max(0, sent - kSlots); i < sent; ++i) mbar_wait_sleep(&s.full[i % kSlots], (i / kSlots) & 1);
+    }
+  } else if (warp == 1) {
+    // -------------------------------------------------------------- MMA issuer
+    if (elect_one()) {
+      constexpr uint32_t idesc_s = idesc_bf16<128, 128>();
+      constexpr uint32_t idesc_o = idesc_bf16<128, 128>() | kIdescBMn;
+      constexpr uint64_t kSlotStep = kSlotBytes >> 4;
+      const uint64_t q_desc = smem_desc_sw128(smem_u32(s.q[0][0])), k_desc = smem_desc_sw128(smem_u32(s.ring[0]));
+      bool ok = wait_or_abort(s, &s.q_full, 0, err, 92);
+      auto landed = [&](int pos) { return wait_or_abort(s, &s.full[pos % kSlots], (pos / kSlots) & 1, err, 93); };
+      // scores of row tile t; the last user of the key slots frees them
+      auto issue_s = [&](int t, int j, bool last) {
+#pragma unroll
+        for (int c = 0; c < 3; ++c) {
+          ok = ok && landed(5 * j + c);
+          if (!ok) return;
+          tc_fence_after();
+          const uint64_t a = q_desc + (t * 3 + c) * kSlotStep, b = k_desc + ((5 * j + c) % kSlots) * kSlotStep;
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk) mma_bf16(tmem + t * 128, a + kk * 2, b + kk * 2, idesc_s, c + kk > 0);
+          if (last) mma_commit(&s.empty[(5 * j + c) % kSlots]);
+        }
+        mma_commit(&s.s_full[t]);
+      };
+      auto issue_pv = [&](int t, int j, int keys, bool last) {
+        ok = ok && landed(5 * j + 3) && landed(5 * j + 4);
+        ok = ok && wait_or_abort(s, &s.p_full[t], j & 1, err, 94);
+        if (!ok) return;
+        tc_fence_after();
+        // the two value chunks may wrap around the ring's end: one descriptor step between them
+        const int s0 = (5 * j + 3) % kSlots, s1 = (5 * j + 4) % kSlots;
+        const int steps = min(8, (keys - j * 128 + 15) / 16);
+        if (s1 > s0) {
+          const uint64_t v = smem_desc_mn_sw128(smem_u32(s.ring[s0]), kSlotBytes, 1024);
+#pragma unroll
+          for (int kk = 0; kk < 8; ++kk)
+            if (kk < steps)
+              mma_bf16_tmem_a(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, v + kk * 128, idesc_o, j + kk > 0);
+        } else {
+          constexpr uint32_t idesc_h = idesc_bf16<128, 64>() | kIdescBMn;
+          for (int c = 0; c < 2; ++c) {
+            const uint64_t v = smem_desc_mn_sw128(smem_u32(s.ring[c ? s1 : s0]), kSlotBytes, 1024);
+            for (int kk = 0; kk < steps; ++kk)
+              mma_bf16_tmem_a(tmem + 256 + t * 128 + c * 64, tmem + t * 128 + kk * 8, v + kk * 128, idesc_h, j + kk > 0);
+          }
+        }
+        if (last) {
+          mma_commit(&s.empty[s0]);
+          mma_commit(&s.empty[s1]);
+        }
+      };
+      const bool two = nt1 > 0;
+      issue_s(0, 0, !two);
+      if (two) issue_s(1, 0, true);
+      for (int j = 0; ok && j < nt; ++j) {
+        if (j < nt0) {
+          issue_pv(0, j, keys0, !two);
+          if (j + 1 == nt0) {
+            if (ok) mma_commit(&s.o_full[0]);
+          } else {
+            issue_s(0, j + 1, !two);
+          }
+        }
+        if (j < nt1) {
+          issue_pv(1, j, keys1, true);
+          if (j + 1 == nt1) {
+            if (ok) mma_commit(&s.o_full[1]);
+          } else {
+            issue_s(1, j + 1, true);
+          }
+        }
+      }
+      // every MMA issued has finished before the tensor memory is freed
+      mma_commit(&s.drained);
+      mbar_wait_sleep(&s.drained, 0);
+    }
+  } else if (warp >= 4) {
+    // ------------------------------------------------------- softmax, epilogue
+    const int t = (warp - 4) / 4, quad = warp & 3;
+    const int r = quad * 32 + lane;  // row of the tile
+    const int keys = t ? keys1 : keys0, tiles = t ? nt1 : nt0;
+    const int last_key = min(pos0 + t * 128 + r, keys - 1);  // this row's; rows past the chunk see the tile's keys
+    const uint32_t s_tmem = tmem + t * 128 + ((uint32_t)(quad * 32) << 16);
+    const uint32_t o_tmem = s_tmem + 256;
+    float m = 0.f, l = 0.f;
+    bool ok = true;
+    for (int j = 0; j < tiles; ++j) {
+      ok = wait_or_abort(s, &s.s_full[t], j & 1, err, 95);
+      if (!__all_sync(0xffffffffu, ok)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const int limit = last_key - j * 128;  // columns up to this one count
+      const bool masked = __any_sync(0xffffffffu, limit < 127);
+      uint32_t p[64];
+      float sum = 0.f;
+      // P of one tile relative to the running maximum; returns the largest score, relative
+      auto pass = [&]() {
+        float top = -INFINITY;
+        sum = 0.f;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          float v[32];
+          tmem_ld32w(s_tmem + c * 32, v);
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            const float x0 = c * 32 + i > limit && masked ? -INFINITY : fmaf(v[i], scale_log2, -m);
+            const float x1 = c * 32 + i + 1 > limit && masked ? -INFINITY : fmaf(v[i + 1], scale_log2, -m);
+            top = fmaxf(top, fmaxf(x0, x1));
+            const float p0 = ex2(x0), p1 = ex2(x1);
+            sum += p0 + p1;
+            p[c * 16 + i / 2] = pack_bf16(p0, p1);
+          }
+        }
+        return top;
+      };
+      float top;
+      if (j == 0) {  // nothing to be relative to yet
+        top = -INFINITY;
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          float v[32];
+          tmem_ld32w(s_tmem + c * 32, v);
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            top = fmaxf(top, c * 32 + i > limit ? -INFINITY : v[i] * scale_log2);
+        }
+        m = top == -INFINITY ? 0.f : top;
+        pass();
+      } else {
+        top = pass();
+        if (__any_sync(0xffffffffu, top > kRaise)) {
+          const float up = fmaxf(top, 0.f), f = ex2(-up);
+          m += up;
+          l *= f;
+#pragma unroll 1
+          for (int c = 0; c < 8; ++c) {
+            float o[16];
+            uint32_t u[16];
+            tmem_ld16(o_tmem + c * 16, o);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) u[i] = __float_as_uint(o[i] * f);
+            tmem_st16(o_tmem + c * 16, u);
+          }
+          pass();
+        }
+      }
+      l += sum;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t u[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) u[i] = p[c * 16 + i];
+        tmem_st16(s_tmem + c * 16, u);
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s.p_full[t]);
+    }
+    if (ok && tiles > 0) ok = wait_or_abort(s, &s.o_full[t], 0, err, 96);
+    if (__all_sync(0xffffffffu, ok && tiles > 0)) {
+      tc_fence_after();
+      const float inv = 1.f / l;
+      bf16* dst = out + (int64_t)(row0 + t * 128 + r) * out_stride + (int64_t)h * kVal;
+      const bool write = t * 128 + r < n;
+#pragma unroll 1
+      for (int c = 0; c < 8; ++c) {
+        float o[16];
+        tmem_ld16(o_tmem + c * 16, o);
+        if (write) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            *reinterpret_cast<uint4*>(dst + c * 16 + i * 8) =
+                make_uint4(pack_bf16(o[8 * i] * inv, o[8 * i + 1] * inv), pack_bf16(o[8 * i + 2] * inv, o[8 * i + 3] * inv),
+                           pack_bf16(o[8 * i + 4] * inv, o[8 * i + 5] * inv), pack_bf16(o[8 * i + 6] * inv, o[8 * i + 7] * inv));
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
   }
 }
 
@@ -99,7 +372,15 @@ void launch_latent_gather(const bf16* cache, int64_t num_blocks, int page, int R
 
 void launch_latent_prefill(const LatentPrefill& a, cudaStream_t st) {
   if (a.nwork == 0 || a.heads == 0) return;
-  launch_k(latent_prefill_kernel, dim3(a.nwork, a.heads), 256, 0, st, a);
+  const size_t smem = sizeof(PrefillSmem);
+  static_assert(sizeof(PrefillSmem) <= 232448, "shared memory of one CTA");
+  static std::atomic<uint64_t> attr_devs{0};
+  ensure_smem_attr(attr_devs, latent_prefill_kernel, smem);
+  const CUtensorMap tq = make_tmap_2d_bf16(a.q, a.T, (uint64_t)a.heads * (kNope + kRot), a.q_stride, 128, 64, true);
+  const CUtensorMap tkv = make_tmap_2d_bf16(a.kv, a.kv_rows, (uint64_t)a.heads * (kNope + kVal), a.kv_stride, 128, 64, true);
+  const CUtensorMap tr = make_tmap_2d_bf16(a.rows, a.kv_rows, a.R + kRot, a.R + kRot, 128, 64, true);
+  launch_k(latent_prefill_kernel, dim3(a.nwork, a.heads), kThreads, smem, st, tq, tkv, tr, a.work, a.seq_info, a.T, a.R,
+           a.scale * kLog2e, a.out, a.out_stride, a.err);
   KAPSL_LAUNCH_CHECK();
   note_launch();
 }

@@ -100,10 +100,10 @@ constexpr int kRopeRows = 4;
 
 template <class T, int N, bool IL>
 __global__ void __launch_bounds__(256) rope_kernel(const T* x, int64_t xs_t, int64_t xs_h, T* y, int64_t ys_t,
-                                                   int64_t ys_h, const int32_t* __restrict__ positions,
+                                                   int64_t ys_h, const int32_t* positions,
                                                    const float* __restrict__ cos_sin, int max_pos, int64_t rows,
                                                    int H, int D, int P, int offset, bool in_place,
-                                                   int* __restrict__ err) {
+                                                   int* err) {
   griddep_entry();
   const int half = P >> 1;
   const int nrot = IL ? P / N : half / N;
@@ -198,10 +198,10 @@ void rope_dispatch(const RopeArgs& a, cudaStream_t st) {
 // rotate the query heads.
 template <int R, bool IL>
 __global__ void __launch_bounds__(256) rope_latent_write_kernel(
-    const bf16* q, int64_t qs_t, int64_t qs_h, bf16* qo, int64_t qo_t, int64_t qo_h, const bf16* __restrict__ kv,
-    int64_t kv_stride, const int32_t* __restrict__ positions, const int64_t* __restrict__ slots,
-    const float* __restrict__ cos_sin, int max_pos, const bf16* __restrict__ w, float eps, bf16* __restrict__ cache,
-    int64_t num_slots, int H, int* __restrict__ err) {
+    const bf16* q, int64_t qs_t, int64_t qs_h, bf16* qo, int64_t qo_t, int64_t qo_h, const bf16* kv,
+    int64_t kv_stride, const int32_t* positions, const int64_t* slots,
+    const float* __restrict__ cos_sin, int max_pos, const bf16* __restrict__ w, float eps, bf16* cache,
+    int64_t num_slots, int H, int* err) {
   griddep_entry();
   constexpr int P = 64, N = 8, half = P / 2;
   constexpr int NU = IL ? P / N : half / N;  // rotating units a head

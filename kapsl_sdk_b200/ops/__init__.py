@@ -59,6 +59,8 @@ DEVICE_ERRORS = {
     82: "latent attention: a block table entry lies outside the cache (its keys read as zeros)",
     83: "latent decode attention: shared memory is not 1 KiB aligned",
     **{c: "latent decode attention pipeline wait ran out" for c in range(84, 90)},
+    90: "latent prefill attention: the plan's rows lie outside q, or shared memory is not 1 KiB aligned",
+    **{c: "latent prefill attention pipeline wait ran out" for c in range(91, 97)},
 }
 
 
