@@ -99,6 +99,66 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// Two fp32 values as one 64-bit operand of the packed instructions (one issue slot for both).
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// P of one row of a key tile relative to the running maximum m: 128 scores from TMEM, 64
+// packed bf16 pairs, their fp32 sum, and the largest relative score.  The load of the
+// next 32 columns is under way while 32 are worked on.
+template <bool MASKED>
+__device__ __forceinline__ float row_pass(uint32_t s_tmem, float scale_log2, float m, int limit, uint32_t (&p)[64],
+                                          float& sum) {
+  const uint64_t sc = pair(scale_log2, scale_log2), off = pair(-m, -m);
+  float top = -INFINITY;
+  uint64_t acc = pair(0.f, 0.f);
+  uint32_t v[2][32];
+  tmem_ld32_start(s_tmem, v[0]);
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    tmem_ld_wait(v[c & 1]);
+    if (c < 3) tmem_ld32_start(s_tmem + (c + 1) * 32, v[(c + 1) & 1]);
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) {
+      float x0, x1;
+      unpair(fma2(pair(__uint_as_float(v[c & 1][i]), __uint_as_float(v[c & 1][i + 1])), sc, off), x0, x1);
+      if (MASKED) {
+        if (c * 32 + i > limit) x0 = -INFINITY;
+        if (c * 32 + i + 1 > limit) x1 = -INFINITY;
+      }
+      top = max3(top, x0, x1);
+      const float p0 = ex2(x0), p1 = ex2(x1);
+      acc = add2(acc, pair(p0, p1));
+      p[c * 16 + i / 2] = pack_bf16(p0, p1);
+    }
+  }
+  float a, b;
+  unpair(acc, a, b);
+  sum = a + b;
+  return top;
+}
+
 __global__ void __launch_bounds__(kThreads, 1)
     latent_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap kv_map,
                           const __grid_constant__ CUtensorMap rope_map, const int32_t* work,
@@ -266,25 +326,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool masked = __any_sync(0xffffffffu, limit < 127);
       uint32_t p[64];
       float sum = 0.f;
-      // P of one tile relative to the running maximum; returns the largest score, relative
       auto pass = [&]() {
-        float top = -INFINITY;
-        sum = 0.f;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          float v[32];
-          tmem_ld32w(s_tmem + c * 32, v);
-#pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            const float x0 = c * 32 + i > limit && masked ? -INFINITY : fmaf(v[i], scale_log2, -m);
-            const float x1 = c * 32 + i + 1 > limit && masked ? -INFINITY : fmaf(v[i + 1], scale_log2, -m);
-            top = fmaxf(top, fmaxf(x0, x1));
-            const float p0 = ex2(x0), p1 = ex2(x1);
-            sum += p0 + p1;
-            p[c * 16 + i / 2] = pack_bf16(p0, p1);
-          }
-        }
-        return top;
+        return masked ? row_pass<true>(s_tmem, scale_log2, m, limit, p, sum)
+                      : row_pass<false>(s_tmem, scale_log2, m, limit, p, sum);
       };
       float top;
       if (j == 0) {  // nothing to be relative to yet
