@@ -75,22 +75,26 @@ constexpr float kRaise = 8.f;
 struct alignas(1024) PrefillSmem {
   uint8_t q[2][3][kSlotBytes];
   uint8_t ring[kSlots][kSlotBytes];
-  uint64_t q_full, full[kSlots], empty[kSlots], s_full[2], p_full[2], o_full[2], drained;
+  uint64_t q_full, k_full[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], drained;
   uint32_t tmem_base;
   volatile int abort_flag;
 };
 
 __device__ __forceinline__ bool wait_or_abort(PrefillSmem& s, uint64_t* bar, uint32_t parity, int* err, int code) {
-  if (mbar_try_wait(bar, parity)) return true;
-  const uint64_t t0 = globaltimer_ns();
-  while (!s.abort_flag) {
-    if (mbar_try_wait_sleep(bar, parity, 20000u)) return true;
-    if (globaltimer_ns() - t0 > 2000000000ull) {
-      atomicCAS(err, 0, code);
-      s.abort_flag = 1;
+  uint64_t t0 = 0;
+  for (uint32_t spin = 1;; ++spin) {  // the clock is read rarely: it is slow
+    if (mbar_test_wait(bar, parity)) return true;
+    if ((spin & 1023) == 0) {
+      const uint64_t now = globaltimer_ns();
+      if (t0 == 0) t0 = now;
+      if (s.abort_flag) return false;
+      if (now - t0 > 2000000000ull) {
+        atomicCAS(err, 0, code);
+        s.abort_flag = 1;
+        return false;
+      }
     }
   }
-  return false;
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -183,11 +187,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) {
     s.abort_flag = 0;
     mbar_init(&s.q_full, 1);
-    for (int i = 0; i < kSlots; ++i) {
-      mbar_init(&s.full[i], 1);
-      mbar_init(&s.empty[i], 1);
-    }
     for (int i = 0; i < 2; ++i) {
+      mbar_init(&s.k_full[i], 1);
+      mbar_init(&s.v_full[i], 1);
+      mbar_init(&s.v_empty[i], 1);
       mbar_init(&s.s_full[i], 1);
       mbar_init(&s.p_full[i], 4);
       mbar_init(&s.o_full[i], 1);
@@ -208,27 +211,32 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_arrive_expect_tx(&s.q_full, tiles_q * 3 * kSlotBytes);
       for (int t = 0; t < tiles_q; ++t)
         for (int c = 0; c < 3; ++c) tma_load_2d(s.q[t][c], &q_map, &s.q_full, h * 192 + c * 64, row0 + t * 128);
-      int sent = 0;
+      // Slots of tile j: keys 5j .. 5j + 2, values 5j + 3, 5j + 4 (mod 8).  Those of K_j were
+      // last used by K_{j-2} and V_{j-2}, those of V_j by K_{j-1}, which is free once the last row
+      // tile's scores of tile j - 1 are complete.
+      const int last = tiles_q - 1;
       bool ok = true;
-      for (int j = 0; ok && j < nt; ++j) {
-#pragma unroll
-        for (int c = 0; c < 5; ++c, ++sent) {  // key chunks 0, 1, rotary; value chunks 0, 1
-          const int slot = sent % kSlots;
-          if (sent >= kSlots && !wait_or_abort(s, &s.empty[slot], (sent / kSlots - 1) & 1, err, 91)) {
-            ok = false;
-            break;
-          }
-          mbar_arrive_expect_tx(&s.full[slot], kSlotBytes);
-          if (c == 2) {
-            tma_load_2d(s.ring[slot], &rope_map, &s.full[slot], R, kv0 + j * 128);
-          } else {
-            tma_load_2d(s.ring[slot], &kv_map, &s.full[slot], h * 256 + (c < 2 ? c : c - 1) * 64, kv0 + j * 128);
-          }
-        }
+      int j = 0;
+      for (; j < nt; ++j) {
+        if (j >= 2 && !wait_or_abort(s, &s.v_empty[j & 1], ((j >> 1) - 1) & 1, err, 91)) { ok = false; break; }
+        uint64_t* bar = &s.k_full[j & 1];
+        mbar_arrive_expect_tx(bar, 3 * kSlotBytes);
+        tma_load_2d(s.ring[(5 * j) % kSlots], &kv_map, bar, h * 256, kv0 + j * 128);
+        tma_load_2d(s.ring[(5 * j + 1) % kSlots], &kv_map, bar, h * 256 + 64, kv0 + j * 128);
+        tma_load_2d(s.ring[(5 * j + 2) % kSlots], &rope_map, bar, R, kv0 + j * 128);
+        if (j >= 1 && !wait_or_abort(s, &s.s_full[last], (j - 1) & 1, err, 91)) { ok = false; break; }
+        bar = &s.v_full[j & 1];
+        mbar_arrive_expect_tx(bar, 2 * kSlotBytes);
+        tma_load_2d(s.ring[(5 * j + 3) % kSlots], &kv_map, bar, h * 256 + 128, kv0 + j * 128);
+        tma_load_2d(s.ring[(5 * j + 4) % kSlots], &kv_map, bar, h * 256 + 192, kv0 + j * 128);
       }
       // the copies in flight end before the CTA does, on the way out of a time-out too
       mbar_wait_sleep(&s.q_full, 0);
-      for (int i = max(0, sent - kSlots); i < sent; ++i) mbar_wait_sleep(&s.full[i % kSlots], (i / kSlots) & 1);
+      for (int i = max(0, j - 2); i < j; ++i) {
+        mbar_wait_sleep(&s.k_full[i & 1], (i >> 1) & 1);
+        mbar_wait_sleep(&s.v_full[i & 1], (i >> 1) & 1);
+      }
+      if (!ok) mbar_wait_sleep(&s.k_full[j & 1], (j >> 1) & 1, 10000000ull);  // if it was sent
     }
   } else if (warp == 1) {
     // -------------------------------------------------------------- MMA issuer
@@ -237,59 +245,52 @@ __global__ void __launch_bounds__(kThreads, 1)
       constexpr uint32_t idesc_o = idesc_bf16<128, 128>() | kIdescBMn;
       constexpr uint64_t kSlotStep = kSlotBytes >> 4;
       const uint64_t q_desc = smem_desc_sw128(smem_u32(s.q[0][0])), k_desc = smem_desc_sw128(smem_u32(s.ring[0]));
+      const uint64_t v_desc = smem_desc_mn_sw128(smem_u32(s.ring[0]), kSlotBytes, 1024);
       bool ok = wait_or_abort(s, &s.q_full, 0, err, 92);
-      auto landed = [&](int pos) { return wait_or_abort(s, &s.full[pos % kSlots], (pos / kSlots) & 1, err, 93); };
-      // scores of row tile t; the last user of the key slots frees them
-      auto issue_s = [&](int t, int j, bool last) {
+      auto issue_s = [&](int t, int j) {  // scores of row tile t
+        ok = ok && wait_or_abort(s, &s.k_full[j & 1], (j >> 1) & 1, err, 93);
+        if (!ok) return;
+        tc_fence_after();
 #pragma unroll
         for (int c = 0; c < 3; ++c) {
-          ok = ok && landed(5 * j + c);
-          if (!ok) return;
-          tc_fence_after();
           const uint64_t a = q_desc + (t * 3 + c) * kSlotStep, b = k_desc + ((5 * j + c) % kSlots) * kSlotStep;
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk) mma_bf16(tmem + t * 128, a + kk * 2, b + kk * 2, idesc_s, c + kk > 0);
-          if (last) mma_commit(&s.empty[(5 * j + c) % kSlots]);
         }
         mma_commit(&s.s_full[t]);
       };
       auto issue_pv = [&](int t, int j, int keys, bool last) {
-        ok = ok && landed(5 * j + 3) && landed(5 * j + 4);
+        ok = ok && wait_or_abort(s, &s.v_full[j & 1], (j >> 1) & 1, err, 93);
         ok = ok && wait_or_abort(s, &s.p_full[t], j & 1, err, 94);
         if (!ok) return;
         tc_fence_after();
         // the two value chunks may wrap around the ring's end: one descriptor step between them
         const int s0 = (5 * j + 3) % kSlots, s1 = (5 * j + 4) % kSlots;
         const int steps = min(8, (keys - j * 128 + 15) / 16);
-        if (s1 > s0) {
-          const uint64_t v = smem_desc_mn_sw128(smem_u32(s.ring[s0]), kSlotBytes, 1024);
+        const uint64_t v = v_desc + s0 * kSlotStep;
+        if (s1 > s0 && steps == 8) {
 #pragma unroll
           for (int kk = 0; kk < 8; ++kk)
-            if (kk < steps)
-              mma_bf16_tmem_a(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, v + kk * 128, idesc_o, j + kk > 0);
+            mma_bf16_tmem_a(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, v + kk * 128, idesc_o, j + kk > 0);
         } else {
           constexpr uint32_t idesc_h = idesc_bf16<128, 64>() | kIdescBMn;
-          for (int c = 0; c < 2; ++c) {
-            const uint64_t v = smem_desc_mn_sw128(smem_u32(s.ring[c ? s1 : s0]), kSlotBytes, 1024);
+          for (int c = 0; c < 2; ++c)
             for (int kk = 0; kk < steps; ++kk)
-              mma_bf16_tmem_a(tmem + 256 + t * 128 + c * 64, tmem + t * 128 + kk * 8, v + kk * 128, idesc_h, j + kk > 0);
-          }
+              mma_bf16_tmem_a(tmem + 256 + t * 128 + c * 64, tmem + t * 128 + kk * 8,
+                              v_desc + (c ? s1 : s0) * kSlotStep + kk * 128, idesc_h, j + kk > 0);
         }
-        if (last) {
-          mma_commit(&s.empty[s0]);
-          mma_commit(&s.empty[s1]);
-        }
+        if (last) mma_commit(&s.v_empty[j & 1]);
       };
       const bool two = nt1 > 0;
-      issue_s(0, 0, !two);
-      if (two) issue_s(1, 0, true);
+      issue_s(0, 0);
+      if (two) issue_s(1, 0);
       for (int j = 0; ok && j < nt; ++j) {
         if (j < nt0) {
           issue_pv(0, j, keys0, !two);
           if (j + 1 == nt0) {
             if (ok) mma_commit(&s.o_full[0]);
           } else {
-            issue_s(0, j + 1, !two);
+            issue_s(0, j + 1);
           }
         }
         if (j < nt1) {
@@ -297,7 +298,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (j + 1 == nt1) {
             if (ok) mma_commit(&s.o_full[1]);
           } else {
-            issue_s(1, j + 1, true);
+            issue_s(1, j + 1);
           }
         }
       }
