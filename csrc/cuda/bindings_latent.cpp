@@ -218,21 +218,52 @@ void latent_decode_attention(Tensor q, Tensor cache, Tensor w, Tensor block_tabl
   kapsl::launch_latent_decode(a, cur_stream());
 }
 
-void latent_gather(Tensor cache, Tensor seq_info, Tensor block_tables, Tensor rows, Tensor err) {
-  const char* op = "latent_gather";
+// kv [n, heads * 256] and, where given, k_rope [n, 64] of the plan's context rows; w [heads * 256, R]
+void latent_expand(Tensor cache, Tensor w, Tensor work, Tensor seq_info, Tensor block_tables, Tensor kv,
+                   c10::optional<Tensor> k_rope, Tensor err) {
+  const char* op = "latent_expand";
   TORCH_CHECK(cache.is_cuda(), op, ": cache must be a CUDA tensor");
   const int64_t R = check_cache(op, cache, cache);
+  check(w, at::kBFloat16, cache, op, "w");
+  check(kv, at::kBFloat16, cache, op, "kv");
+  check(work, at::kInt, cache, op, "work");
   check(seq_info, at::kInt, cache, op, "seq_info");
-  TORCH_CHECK(seq_info.dim() == 2 && seq_info.size(1) == 5 && seq_info.is_contiguous(), op, ": seq_info [S, 5]");
   check(block_tables, at::kInt, cache, op, "block_tables");
-  TORCH_CHECK(block_tables.dim() == 2 && block_tables.is_contiguous(), op, ": block_tables [S, max_blocks]");
-  check(rows, at::kBFloat16, cache, op, "rows");
-  TORCH_CHECK(rows.dim() == 2 && rows.is_contiguous() && rows.size(1) == R + kRot, op, ": rows [n, R + 64]");
   check(err, at::kInt, cache, op, "err");
+  TORCH_CHECK(w.dim() == 2 && w.is_contiguous() && w.size(1) == R && w.size(0) % 256 == 0 && w.size(0) > 0, op,
+              ": w must be [heads * 256, R]");
+  const int64_t heads = w.size(0) / 256;
+  TORCH_CHECK(kv.dim() == 2 && kv.stride(1) == 1 && kv.size(1) == heads * 256 && kv.stride(0) >= kv.size(1), op,
+              ": kv must be [n, heads * 256]");
+  check_rows16(op, kv, "kv");
+  check_rows16(op, w, "w");
+  TORCH_CHECK(work.dim() == 2 && work.size(1) == 2 && work.is_contiguous(), op, ": work [n, 2]");
+  TORCH_CHECK(seq_info.dim() == 2 && seq_info.size(1) == 5 && seq_info.is_contiguous(), op, ": seq_info [S, 5]");
+  TORCH_CHECK(block_tables.dim() == 2 && block_tables.is_contiguous(), op, ": block_tables [S, max_blocks]");
+  kapsl::LatentExpand a;
+  if (k_rope.has_value()) {
+    check(*k_rope, at::kBFloat16, cache, op, "k_rope");
+    TORCH_CHECK(k_rope->dim() == 2 && k_rope->is_contiguous() && k_rope->size(1) == kRot && k_rope->size(0) == kv.size(0),
+                op, ": k_rope must be [n, 64]");
+    a.k_rope = bf(*k_rope);
+  }
   const c10::cuda::CUDAGuard g(cache.device());
-  kapsl::launch_latent_gather(bf(cache), cache.size(0), (int)cache.size(1), (int)R, seq_info.data_ptr<int32_t>(),
-                              (int)seq_info.size(0), block_tables.data_ptr<int32_t>(), (int)block_tables.size(1),
-                              bf(rows), rows.size(0), err.data_ptr<int>(), cur_stream());
+  a.cache = bf(cache);
+  a.num_blocks = cache.size(0);
+  a.page = (int)cache.size(1);
+  a.R = (int)R;
+  a.w = bf(w);
+  a.work = work.data_ptr<int32_t>();
+  a.nwork = (int)work.size(0);
+  a.seq_info = seq_info.data_ptr<int32_t>();
+  a.block_tables = block_tables.data_ptr<int32_t>();
+  a.max_blocks = (int)block_tables.size(1);
+  a.heads = (int)heads;
+  a.num_sms = kapsl::gemm_num_sms();
+  a.kv = bf(kv);
+  a.kv_stride = kv.stride(0);
+  a.err = err.data_ptr<int>();
+  kapsl::launch_latent_expand(a, cur_stream());
 }
 
 void check_latent_prefill(Tensor q, Tensor cache, Tensor w, Tensor block_tables, Tensor out, int64_t H, int64_t rows,
@@ -253,13 +284,13 @@ void check_latent_prefill(Tensor q, Tensor cache, Tensor w, Tensor block_tables,
 }
 
 // attention of `heads` heads: q / out already narrowed to them
-void latent_prefill(Tensor q, Tensor kv, Tensor rows, Tensor work, Tensor seq_info, Tensor out, int64_t heads,
+void latent_prefill(Tensor q, Tensor kv, Tensor k_rope, Tensor work, Tensor seq_info, Tensor out, int64_t heads,
                     double scale, Tensor err) {
   const char* op = "latent_prefill";
   TORCH_CHECK(q.is_cuda(), op, ": q must be a CUDA tensor");
   check(q, at::kBFloat16, q, op, "q");
   check(kv, at::kBFloat16, q, op, "kv");
-  check(rows, at::kBFloat16, q, op, "rows");
+  check(k_rope, at::kBFloat16, q, op, "k_rope");
   check(out, at::kBFloat16, q, op, "out");
   check(work, at::kInt, q, op, "work");
   check(seq_info, at::kInt, q, op, "seq_info");
@@ -267,15 +298,15 @@ void latent_prefill(Tensor q, Tensor kv, Tensor rows, Tensor work, Tensor seq_in
   TORCH_CHECK(heads >= 1 && heads <= 65535, op, ": heads out of range");
   TORCH_CHECK(q.dim() == 2 && q.stride(1) == 1 && q.size(1) == heads * (kNope + kRot), op, ": q [T, heads * 192]");
   TORCH_CHECK(kv.dim() == 2 && kv.stride(1) == 1 && kv.size(1) == heads * (kNope + kVal), op, ": kv [n, heads * 256]");
-  TORCH_CHECK(rows.dim() == 2 && rows.is_contiguous() && rows.size(1) > kRot && rows.size(0) == kv.size(0), op,
-              ": rows [n, R + 64]");
+  TORCH_CHECK(k_rope.dim() == 2 && k_rope.is_contiguous() && k_rope.size(1) == kRot && k_rope.size(0) == kv.size(0), op,
+              ": k_rope [n, 64]");
   TORCH_CHECK(out.dim() == 2 && out.stride(1) == 1 && out.size(1) == heads * kVal && out.size(0) == q.size(0), op,
               ": out [T, heads * 128]");
   TORCH_CHECK(work.dim() == 2 && work.size(1) == 2 && work.is_contiguous(), op, ": work [n, 2]");
   TORCH_CHECK(seq_info.dim() == 2 && seq_info.size(1) == 5 && seq_info.is_contiguous(), op, ": seq_info [S, 5]");
   check_rows16(op, q, "q");
   check_rows16(op, kv, "kv");
-  check_rows16(op, rows, "rows");
+  check_rows16(op, k_rope, "k_rope");
   check_rows16(op, out, "out");
   const c10::cuda::CUDAGuard g(q.device());
   kapsl::LatentPrefill a;
@@ -285,8 +316,7 @@ void latent_prefill(Tensor q, Tensor kv, Tensor rows, Tensor work, Tensor seq_in
   a.kv = bf(kv);
   a.kv_stride = kv.stride(0);
   a.kv_rows = kv.size(0);
-  a.rows = bf(rows);
-  a.R = (int)(rows.size(1) - kRot);
+  a.k_rope = bf(k_rope);
   a.work = work.data_ptr<int32_t>();
   a.nwork = (int)work.size(0);
   a.seq_info = seq_info.data_ptr<int32_t>();
@@ -305,7 +335,7 @@ void register_latent(pybind11::module_& m) {
   m.def("rope_latent_write", &rope_latent_write, "latent norm + rotary key -> paged latent cache, query rotary part");
   m.def("latent_decode_attention", &latent_decode_attention, "absorbed latent attention over a paged cache");
   m.def("latent_workspace_bytes", &latent_workspace_bytes);
-  m.def("latent_gather", &latent_gather, "context rows of every sequence out of the paged latent cache");
+  m.def("latent_expand", &latent_expand, "keys and values of every head from the paged latent cache");
   m.def("check_latent_prefill", &check_latent_prefill);
   m.def("latent_prefill", &latent_prefill, "causal attention over expanded latent keys and values");
 }

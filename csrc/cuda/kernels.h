@@ -64,20 +64,32 @@ struct LatentDecode {
 size_t latent_decode_workspace_bytes(int B, int H, int R, int max_ctx, int num_sms);
 void launch_latent_decode(const LatentDecode& a, cudaStream_t st);
 
-// Copies each sequence's context rows out of the paged cache into rows [S.kv_start, + ctx)
-// of `rows` [total, R + 64]; pad rows up to the next multiple of 16 are zero.
-void launch_latent_gather(const __nv_bfloat16* cache, int64_t num_blocks, int page, int R, const int32_t* seq_info,
-                          int nseq, const int32_t* block_tables, int max_blocks, __nv_bfloat16* rows, int64_t total,
-                          int* err, cudaStream_t st);
-// Causal attention of the chunk over expanded keys and values: kv [total, heads * 256]
-// (key 128 | value 128 a head), shared rotary keys rows[:, R:].
+// Expands each sequence's context rows to kv [total, heads * 256] (key 128 | value 128 a head) at
+// rows [S.kv_start, + ctx), and copies their rotary keys to k_rope [total, 64] (null: not
+// again); pad rows up to the next multiple of 16 are zero.
+struct LatentExpand {
+  const __nv_bfloat16* cache = nullptr;
+  int64_t num_blocks = 0;
+  int page = 0, R = 0;
+  const __nv_bfloat16* w = nullptr;   // [heads, 256, R]
+  const int32_t* work = nullptr;      // [nwork, 2] = (sequence, first of 128 context rows)
+  int nwork = 0;
+  const int32_t* seq_info = nullptr;  // as below
+  const int32_t* block_tables = nullptr;
+  int max_blocks = 0, heads = 0, num_sms = 1;
+  __nv_bfloat16* kv = nullptr;
+  int64_t kv_stride = 0;
+  __nv_bfloat16* k_rope = nullptr;
+  int* err = nullptr;
+};
+void launch_latent_expand(const LatentExpand& a, cudaStream_t st);
+// Causal attention of the chunk over expanded keys and values and the shared rotary keys.
 struct LatentPrefill {
   const __nv_bfloat16* q = nullptr;  // first of these heads: [T, heads * 192], pitch q_stride
   int64_t q_stride = 0, T = 0;
   const __nv_bfloat16* kv = nullptr;
   int64_t kv_stride = 0, kv_rows = 0;
-  const __nv_bfloat16* rows = nullptr;
-  int R = 0;
+  const __nv_bfloat16* k_rope = nullptr;  // [kv_rows, 64]
   const int32_t* work = nullptr;      // [nwork, 2] = (sequence, first token of the tile)
   int nwork = 0;
   const int32_t* seq_info = nullptr;  // [S, 5] = (first q row, tokens, context, block-table row, first kv row)

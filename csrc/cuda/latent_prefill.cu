@@ -1,8 +1,8 @@
 // Expanded latent attention: a chunk of new tokens over a paged latent cache.
 //
-// The context rows [c (R) | k_r (64)] are gathered out of the pages, one GEMM expands
-// them to every head's key and value rows (kv = c w_h^T, [128 | 128] a head), and the
-// attention runs with keys [k_h (128) | k_r (64, shared)] and values of 128:
+// One kernel expands the context rows [c (R) | k_r (64)] out of their pages to every head's key
+// and value rows (kv = w_h c, [128 | 128] a head), and the attention runs with keys
+// [k_h (128) | k_r (64, shared)] and values of 128:
 //   out_i = sum_j softmax_j(scale q_i . k_j) v_j  over j <= position of i.
 #include <algorithm>
 
@@ -20,34 +20,230 @@ namespace {
 constexpr int kNope = 128, kRot = 64, kVal = 128;
 constexpr float kLog2e = 1.4426950408889634f;
 
-// One warp per output row; rows between sequences (padding to 16) become zero.
-__global__ void __launch_bounds__(256) latent_gather_kernel(const bf16* cache, int64_t num_blocks,
-                                                            int page, int W, const int32_t* seq_info,
-                                                            int nseq, const int32_t* block_tables,
-                                                            int max_blocks, bf16* rows, int64_t total,
-                                                            int* err) {
-  griddep_entry();
-  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (row >= total) return;
-  int lo = 0, hi = nseq - 1;  // last sequence whose first row is <= row
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) / 2;
-    if (seq_info[mid * 5 + 4] <= row) lo = mid;
-    else hi = mid - 1;
-  }
-  const int j = (int)(row - seq_info[lo * 5 + 4]);
-  const uint4* src = nullptr;
-  if (j < seq_info[lo * 5 + 2]) {
-    const int blk = block_tables[(int64_t)seq_info[lo * 5 + 3] * max_blocks + j / page];
-    if (blk >= 0 && blk < num_blocks) {
-      src = reinterpret_cast<const uint4*>(cache + ((int64_t)blk * page + j % page) * W);
-    } else if (lane == 0) {
-      atomicCAS(err, 0, 82);
+// Bounded wait (2 s): polls the barrier, and reads the clock and the CTA's abort flag rarely
+// (both are slow beside a poll).  A time-out records `code` and ends the CTA's other waits.
+template <class Smem>
+__device__ __forceinline__ bool wait_or_abort(Smem& s, uint64_t* bar, uint32_t parity, int* err, int code) {
+  uint64_t t0 = 0;
+  for (uint32_t spin = 1;; ++spin) {
+    if (mbar_test_wait(bar, parity)) return true;
+    if ((spin & 1023) == 0) {
+      const uint64_t now = globaltimer_ns();
+      if (t0 == 0) t0 = now;
+      if (s.abort_flag) return false;
+      if (now - t0 > 2000000000ull) {
+        atomicCAS(err, 0, code);
+        s.abort_flag = 1;
+        return false;
+      }
     }
   }
-  uint4* dst = reinterpret_cast<uint4*>(rows + row * W);
-  for (int c = lane; c < W / 8; c += 32) dst[c] = src ? src[c] : make_uint4(0, 0, 0, 0);
+}
+
+// ------------------------------------------------------------------ expansion
+//
+// kv[row, head] = w_head (256 x R) . c_row for every context row: a GEMM whose A rows come straight
+// out of the pages.  A unit is (128 context rows of one sequence, head): M = 128, N = 256,
+// K = R.  The units, rows outermost, are cut into equal stretches, one a CTA; the rows stay in
+// shared memory while the heads' weights stream past them, and two accumulators of 256 TMEM
+// columns let one unit's epilogue run beside the next one's products.
+// The epilogue turns 32-row slabs in shared memory so that every global store instruction
+// writes whole 128-byte lines.  Rows behind a context (up to the next multiple of 16) are
+// written as zeros, whatever their page slots hold; the head-0 unit also copies the rows'
+// rotary keys.
+constexpr int kExpandThreads = 192;  // warp 0 TMA, warp 1 MMA, warps 2-5 epilogue
+constexpr int kSlabPitch = 144;      // 64 bf16 and 16 bytes against bank conflicts
+
+template <int R>
+struct alignas(1024) ExpandSmem {
+  static constexpr int kChunks = R / 64;
+  static constexpr int kStages = R == 512 ? 2 : 4;
+  uint8_t a[kChunks][128 * 128];
+  uint8_t b[kStages][256 * 128];
+  uint8_t slab[4][32 * kSlabPitch];
+  uint64_t a_full, a_empty, b_full[kStages], b_empty[kStages], acc_full[2], acc_empty[2], drained;
+  uint32_t tmem_base;
+  volatile int abort_flag;
+};
+
+// The `page`-row group of cache row j of a sequence: its first row, or the row past the cache.
+__device__ __forceinline__ int64_t page_row(const int32_t* bt, int j, int page, int64_t num_blocks, int* err) {
+  const int blk = bt[j / page];
+  if (blk >= 0 && blk < num_blocks) return (int64_t)blk * page;
+  atomicCAS(err, 0, 82);
+  return num_blocks * page;
+}
+
+template <int R>
+__global__ void __launch_bounds__(kExpandThreads, 1)
+    latent_expand_kernel(const __grid_constant__ CUtensorMap c_map, const __grid_constant__ CUtensorMap w_map,
+                         const bf16* cache, int64_t num_blocks, int page, const int32_t* work, int nwork,
+                         const int32_t* seq_info, const int32_t* block_tables, int max_blocks, int heads,
+                         bf16* kv, int64_t kv_stride, bf16* k_rope, int* err) {
+  griddep_entry();
+  using S = ExpandSmem<R>;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  S& s = *reinterpret_cast<S*>(smem_raw);
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
+  const int64_t units = (int64_t)nwork * heads;
+  const int64_t u0 = units * blockIdx.x / gridDim.x, u1 = units * (blockIdx.x + 1) / gridDim.x;
+  if (u0 >= u1) return;
+  if (smem_u32(smem_raw) & 1023) {
+    if (threadIdx.x == 0) atomicCAS(err, 0, 90);
+    return;
+  }
+  if (threadIdx.x == 0) {
+    s.abort_flag = 0;
+    mbar_init(&s.a_full, 1);
+    mbar_init(&s.a_empty, 1);
+    for (int i = 0; i < S::kStages; ++i) {
+      mbar_init(&s.b_full[i], 1);
+      mbar_init(&s.b_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s.acc_full[i], 1);
+      mbar_init(&s.acc_empty[i], 4);
+    }
+    mbar_init(&s.drained, 1);
+    fence_barrier_init();
+  }
+  if (warp == 1) tmem_alloc(&s.tmem_base, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = __shfl_sync(0xffffffffu, s.tmem_base, 0);
+  int tile = (int)(u0 / heads), head = (int)(u0 % heads);
+  const int n_units = (int)(u1 - u0);
+
+  if (warp == 0) {
+    if (elect_one()) {
+      int sent = 0, na = 0;
+      bool ok = true;
+      for (int i = 0; ok && i < n_units; ++i) {
+        if (i == 0 || head == 0) {
+          if (na > 0 && !(ok = wait_or_abort(s, &s.a_empty, (na - 1) & 1, err, 97))) break;
+          const int32_t* si = seq_info + 5 * work[2 * tile];
+          const int r0 = work[2 * tile + 1], ctx = si[2];
+          const int32_t* bt = block_tables + (int64_t)si[3] * max_blocks;
+          mbar_arrive_expect_tx(&s.a_full, S::kChunks * 128 * 128);
+          for (int r = 0; r < 128; r += page) {
+            const int y = (int)(r0 + r < ctx ? page_row(bt, r0 + r, page, num_blocks, err) : num_blocks * page);
+#pragma unroll
+            for (int c = 0; c < S::kChunks; ++c) tma_load_2d(s.a[c] + r * 128, &c_map, &s.a_full, c * 64, y);
+          }
+          ++na;
+        }
+        for (int ks = 0; ks < S::kChunks; ++ks, ++sent) {
+          const int st = sent % S::kStages;
+          if (sent >= S::kStages && !(ok = wait_or_abort(s, &s.b_empty[st], (sent / S::kStages - 1) & 1, err, 97))) break;
+          mbar_arrive_expect_tx(&s.b_full[st], 256 * 128);
+          tma_load_2d(s.b[st], &w_map, &s.b_full[st], ks * 64, head * 256);
+        }
+        if (++head == heads) head = 0, ++tile;
+      }
+      // the copies in flight end before the CTA does, on the way out of a time-out too
+      if (na > 0) mbar_wait_sleep(&s.a_full, (na - 1) & 1);
+      for (int i = max(0, sent - S::kStages); i < sent; ++i)
+        mbar_wait_sleep(&s.b_full[i % S::kStages], (i / S::kStages) & 1);
+    }
+  } else if (warp == 1) {
+    if (elect_one()) {
+      constexpr uint32_t idesc = idesc_bf16<128, 256>();
+      const uint64_t a_desc = smem_desc_sw128(smem_u32(s.a[0])), b_desc = smem_desc_sw128(smem_u32(s.b[0]));
+      int seen = 0, na = 0;
+      bool ok = true;
+      for (int i = 0; ok && i < n_units; ++i) {
+        if (i == 0 || head == 0) ok = wait_or_abort(s, &s.a_full, na++ & 1, err, 98);
+        if (i >= 2) ok = ok && wait_or_abort(s, &s.acc_empty[i & 1], ((i >> 1) - 1) & 1, err, 98);
+        const uint32_t d = tmem + (i & 1) * 256;
+        for (int ks = 0; ok && ks < S::kChunks; ++ks, ++seen) {
+          const int st = seen % S::kStages;
+          ok = wait_or_abort(s, &s.b_full[st], (seen / S::kStages) & 1, err, 98);
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t a = a_desc + ks * 1024, b = b_desc + st * 2048;
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk) mma_bf16(d, a + kk * 2, b + kk * 2, idesc, ks + kk > 0);
+          mma_commit(&s.b_empty[st]);
+        }
+        if (!ok) break;
+        mma_commit(&s.acc_full[i & 1]);
+        if (++head == heads) {
+          head = 0;
+          mma_commit(&s.a_empty);
+        }
+      }
+      mma_commit(&s.drained);
+      mbar_wait_sleep(&s.drained, 0);
+    }
+  } else {
+    const int quad = warp & 3;
+    uint8_t* slab = s.slab[quad];
+    const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
+    for (int i = 0; i < n_units; ++i) {
+      const int32_t* si = seq_info + 5 * work[2 * tile];
+      const int r0 = work[2 * tile + 1] + quad * 32, ctx = si[2];  // this warp's 32 rows
+      const int64_t row0 = (int64_t)si[4] + r0;
+      const int valid = ctx - r0, padded = min(32, (ctx + 15) / 16 * 16 - r0);
+      if (head == 0 && k_rope != nullptr) {
+        const int32_t* bt = block_tables + (int64_t)si[3] * max_blocks;
+#pragma unroll 2
+        for (int k = 0; k < 8; ++k) {  // 4 rows x 8 lanes
+          const int r = 4 * k + (lane >> 3), seg = lane & 7;
+          if (r < padded) {
+            uint4 x = make_uint4(0, 0, 0, 0);
+            if (r < valid) {
+              const int64_t at = page_row(bt, r0 + r, page, num_blocks, err) + (r0 + r) % page;
+              if (at < num_blocks * page)
+                x = *reinterpret_cast<const uint4*>(cache + at * (R + kRot) + R + seg * 8);
+            }
+            *reinterpret_cast<uint4*>(k_rope + (row0 + r) * kRot + seg * 8) = x;
+          }
+        }
+      }
+      const bool ok = wait_or_abort(s, &s.acc_full[i & 1], (i >> 1) & 1, err, 99);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      tc_fence_after();
+      bf16* dst = kv + row0 * kv_stride + head * 256;
+#pragma unroll 1
+      for (int c = 0; c < 256; c += 64) {
+        uint4* mine = reinterpret_cast<uint4*>(slab + lane * kSlabPitch);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          float v[32];
+          tmem_ld32w(tmem + lane_off + (i & 1) * 256 + c + half * 32, v);
+          if (lane >= valid) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) v[e] = 0.f;
+          }
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            mine[half * 4 + q] = make_uint4(pack_bf16(v[8 * q], v[8 * q + 1]), pack_bf16(v[8 * q + 2], v[8 * q + 3]),
+                                            pack_bf16(v[8 * q + 4], v[8 * q + 5]), pack_bf16(v[8 * q + 6], v[8 * q + 7]));
+        }
+        __syncwarp();
+        if (c == 192) {  // the accumulator has been read
+          tc_fence_before();
+          if (lane == 0) mbar_arrive(&s.acc_empty[i & 1]);
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int r = 4 * k + (lane >> 3), seg = lane & 7;
+          if (r < padded)
+            *reinterpret_cast<uint4*>(dst + r * kv_stride + c + seg * 8) =
+                *reinterpret_cast<const uint4*>(slab + r * kSlabPitch + seg * 16);
+        }
+        __syncwarp();
+      }
+      if (++head == heads) head = 0, ++tile;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
 }
 
 // ------------------------------------------------------------------ attention
@@ -79,23 +275,6 @@ struct alignas(1024) PrefillSmem {
   uint32_t tmem_base;
   volatile int abort_flag;
 };
-
-__device__ __forceinline__ bool wait_or_abort(PrefillSmem& s, uint64_t* bar, uint32_t parity, int* err, int code) {
-  uint64_t t0 = 0;
-  for (uint32_t spin = 1;; ++spin) {  // the clock is read rarely: it is slow
-    if (mbar_test_wait(bar, parity)) return true;
-    if ((spin & 1023) == 0) {
-      const uint64_t now = globaltimer_ns();
-      if (t0 == 0) t0 = now;
-      if (s.abort_flag) return false;
-      if (now - t0 > 2000000000ull) {
-        atomicCAS(err, 0, code);
-        s.abort_flag = 1;
-        return false;
-      }
-    }
-  }
-}
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -166,7 +345,7 @@ __device__ __forceinline__ float row_pass(uint32_t s_tmem, float scale_log2, flo
 __global__ void __launch_bounds__(kThreads, 1)
     latent_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap kv_map,
                           const __grid_constant__ CUtensorMap rope_map, const int32_t* work,
-                          const int32_t* seq_info, int64_t q_rows, int R, float scale_log2,
+                          const int32_t* seq_info, int64_t q_rows, float scale_log2,
                           bf16* out, int64_t out_stride, int* err) {
   griddep_entry();
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -223,7 +402,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_arrive_expect_tx(bar, 3 * kSlotBytes);
         tma_load_2d(s.ring[(5 * j) % kSlots], &kv_map, bar, h * 256, kv0 + j * 128);
         tma_load_2d(s.ring[(5 * j + 1) % kSlots], &kv_map, bar, h * 256 + 64, kv0 + j * 128);
-        tma_load_2d(s.ring[(5 * j + 2) % kSlots], &rope_map, bar, R, kv0 + j * 128);
+        tma_load_2d(s.ring[(5 * j + 2) % kSlots], &rope_map, bar, 0, kv0 + j * 128);
         if (j >= 1 && !wait_or_abort(s, &s.s_full[last], (j - 1) & 1, err, 91)) { ok = false; break; }
         bar = &s.v_full[j & 1];
         mbar_arrive_expect_tx(bar, 2 * kSlotBytes);
@@ -405,14 +584,27 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 }  // namespace
 
-void launch_latent_gather(const bf16* cache, int64_t num_blocks, int page, int R, const int32_t* seq_info, int nseq,
-                          const int32_t* block_tables, int max_blocks, bf16* rows, int64_t total, int* err,
-                          cudaStream_t st) {
-  if (total == 0 || nseq == 0) return;
-  launch_k(latent_gather_kernel, dim3((unsigned)((total + 7) / 8)), 256, 0, st, cache, num_blocks, page, R + kRot,
-           seq_info, nseq, block_tables, max_blocks, rows, total, err);
-  KAPSL_LAUNCH_CHECK();
-  note_launch();
+void launch_latent_expand(const LatentExpand& a, cudaStream_t st) {
+  if (a.nwork == 0 || a.heads == 0) return;
+  auto go = [&](auto kern, size_t smem, std::atomic<uint64_t>& attr_devs) {
+    ensure_smem_attr(attr_devs, kern, smem);
+    const CUtensorMap tc = make_tmap_2d_bf16(a.cache, (uint64_t)a.num_blocks * a.page, a.R + kRot, a.R + kRot, a.page, 64, true);
+    const CUtensorMap tw = make_tmap_2d_bf16(a.w, (uint64_t)a.heads * 256, a.R, a.R, 256, 64, true);
+    const int grid = (int)std::min<int64_t>(a.num_sms, (int64_t)a.nwork * a.heads);
+    launch_k(kern, dim3(grid), kExpandThreads, smem, st, tc, tw, a.cache, a.num_blocks, a.page, a.work, a.nwork,
+             a.seq_info, a.block_tables, a.max_blocks, a.heads, a.kv, a.kv_stride, a.k_rope, a.err);
+    KAPSL_LAUNCH_CHECK();
+    note_launch();
+  };
+  static_assert(sizeof(ExpandSmem<512>) <= 232448 && sizeof(ExpandSmem<256>) <= 232448, "shared memory of one CTA");
+  static std::atomic<uint64_t> attr512{0}, attr256{0};
+  if (a.R == 512) {
+    go(latent_expand_kernel<512>, sizeof(ExpandSmem<512>), attr512);
+  } else if (a.R == 256) {
+    go(latent_expand_kernel<256>, sizeof(ExpandSmem<256>), attr256);
+  } else {
+    throw std::runtime_error("latent prefill: the latent must have 256 or 512 values");
+  }
 }
 
 void launch_latent_prefill(const LatentPrefill& a, cudaStream_t st) {
@@ -423,8 +615,8 @@ void launch_latent_prefill(const LatentPrefill& a, cudaStream_t st) {
   ensure_smem_attr(attr_devs, latent_prefill_kernel, smem);
   const CUtensorMap tq = make_tmap_2d_bf16(a.q, a.T, (uint64_t)a.heads * (kNope + kRot), a.q_stride, 128, 64, true);
   const CUtensorMap tkv = make_tmap_2d_bf16(a.kv, a.kv_rows, (uint64_t)a.heads * (kNope + kVal), a.kv_stride, 128, 64, true);
-  const CUtensorMap tr = make_tmap_2d_bf16(a.rows, a.kv_rows, a.R + kRot, a.R + kRot, 128, 64, true);
-  launch_k(latent_prefill_kernel, dim3(a.nwork, a.heads), kThreads, smem, st, tq, tkv, tr, a.work, a.seq_info, a.T, a.R,
+  const CUtensorMap tr = make_tmap_2d_bf16(a.k_rope, a.kv_rows, kRot, kRot, 128, 64, true);
+  launch_k(latent_prefill_kernel, dim3(a.nwork, a.heads), kThreads, smem, st, tq, tkv, tr, a.work, a.seq_info, a.T,
            a.scale * kLog2e, a.out, a.out_stride, a.err);
   KAPSL_LAUNCH_CHECK();
   note_launch();

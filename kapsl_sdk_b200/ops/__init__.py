@@ -61,6 +61,7 @@ DEVICE_ERRORS = {
     **{c: "latent decode attention pipeline wait ran out" for c in range(84, 90)},
     90: "latent prefill attention: the plan's rows lie outside q, or shared memory is not 1 KiB aligned",
     **{c: "latent prefill attention pipeline wait ran out" for c in range(91, 97)},
+    **{c: "latent expansion pipeline wait ran out" for c in range(97, 100)},
 }
 
 
@@ -375,7 +376,8 @@ LATENT_KV_BYTES = 2 << 30  # expanded keys and values held at once; more heads g
 @dataclass
 class LatentPrefillPlan:
     """Tile list and sequence table of one :func:`latent_prefill_attention` call."""
-    work: torch.Tensor      # int32 [n, 2]: (sequence, first token of the tile)
+    work: torch.Tensor      # int32 [n, 2]: (sequence, first new token) of every tile of query rows
+    kv_work: torch.Tensor   # int32 [m, 2]: (sequence, first context row) of every 128 context rows
     seq_info: torch.Tensor  # int32 [S, 5]: (first q row, tokens, context, block-table row, first kv row)
     rows: int               # q rows up to the last sequence's end
     tables: int             # block-table rows read
@@ -408,8 +410,11 @@ def latent_prefill_plan(q_lens: Sequence[int], ctx_lens: Sequence[int], device, 
         raise ValueError("latent_prefill_plan: too many rows")
     work.sort(key=lambda w: -w[0])  # the tiles with the most keys start first
     dev = torch.device(device)
-    t = torch.tensor([v for w in work for v in w[1:]] + [v for i in info for v in i], dtype=torch.int32).to(dev)
-    return LatentPrefillPlan(work=t[:2 * len(work)].view(-1, 2), seq_info=t[2 * len(work):].view(-1, 5), rows=row,
+    kv_work = [(s, r) for s, i in enumerate(info) for r in range(0, i[2], 128)]
+    t = torch.tensor([v for w in work for v in w[1:]] + [v for w in kv_work for v in w] + [v for i in info for v in i],
+                     dtype=torch.int32).to(dev)
+    a, b = 2 * len(work), 2 * (len(work) + len(kv_work))
+    return LatentPrefillPlan(work=t[:a].view(-1, 2), kv_work=t[a:b].view(-1, 2), seq_info=t[b:].view(-1, 5), rows=row,
                              tables=bt_start + len(info) if info else 0, max_ctx=max([i[2] for i in info], default=0),
                              kv_rows=kv)
 
@@ -421,8 +426,8 @@ def latent_prefill_attention(q: torch.Tensor, cache: torch.Tensor, w_kv_b: torch
 
     The new tokens' rows are in ``cache`` already; arguments as in
     :func:`latent_decode_attention`, with ``plan`` from :func:`latent_prefill_plan`.  The
-    context's latents are gathered from their pages and expanded by ``w_kv_b`` to keys and
-    values (at most ``LATENT_KV_BYTES`` of them at a time, in passes over the heads).
+    context's latents are expanded out of their pages by ``w_kv_b`` to keys and values (at
+    most ``LATENT_KV_BYTES`` of them at a time, in passes over the heads).
     ``out`` rows outside the plan's sequences keep what they held (zeros when ``out`` is
     allocated here)."""
     if scale is None:
@@ -434,17 +439,16 @@ def latent_prefill_attention(q: torch.Tensor, cache: torch.Tensor, w_kv_b: torch
     if plan.work.shape[0] == 0:
         return out
     err = error_buffer(q.device)
-    R = cache.shape[2] - 64
-    rows = torch.empty(plan.kv_rows, R + 64, dtype=torch.bfloat16, device=q.device)
-    c.latent_gather(cache, plan.seq_info, block_tables, rows, err)
-    w = w_kv_b.view(num_heads * 256, R)
+    w = w_kv_b.view(num_heads * 256, -1)
     step = max(1, min(num_heads, LATENT_KV_BYTES // (plan.kv_rows * 512)))
+    k_rope = torch.empty(plan.kv_rows, 64, dtype=torch.bfloat16, device=q.device)
     kv_buf = torch.empty(plan.kv_rows * step * 256, dtype=torch.bfloat16, device=q.device)
     for h0 in range(0, num_heads, step):
         n = min(step, num_heads - h0)
         kv = kv_buf[:plan.kv_rows * n * 256].view(plan.kv_rows, n * 256)
-        c.gemm(rows[:, :R], w[h0 * 256:(h0 + n) * 256], kv, EPI_PLAIN, None, None, None, err, 0, 0)
-        c.latent_prefill(q[:, h0 * 192:(h0 + n) * 192], kv, rows, plan.work, plan.seq_info,
+        c.latent_expand(cache, w[h0 * 256:(h0 + n) * 256], plan.kv_work, plan.seq_info, block_tables, kv,
+                        k_rope if h0 == 0 else None, err)
+        c.latent_prefill(q[:, h0 * 192:(h0 + n) * 192], kv, k_rope, plan.work, plan.seq_info,
                          out[:, h0 * 128:(h0 + n) * 128], n, float(scale), err)
     return out
 
