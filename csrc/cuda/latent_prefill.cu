@@ -43,8 +43,11 @@ __device__ __forceinline__ bool wait_or_abort(Smem& s, uint64_t* bar, uint32_t p
 // ------------------------------------------------------------------ expansion
 //
 // kv[row, head] = w_head (256 x R) . c_row for every context row: a GEMM whose A rows come straight
-// out of the pages.  A unit is (128 context rows of one sequence, head): M = 128, N = 256,
-// K = R.  The units, rows outermost, are cut into equal stretches, one a CTA; the rows stay in
+// out of the pages.  A CTA pair (cluster of 2) works on units of (256 context rows, head) with
+// cta_group::2 MMAs (M = 256, N = 256): each CTA holds 128 rows of one sequence and half of the
+// head's weights, so a CTA loads 16 KB of weights for 512 cycles of products (one CTA alone needs
+// 32 KB, and beside 128 KB of rows only two such stages fit: 1.7 x the time at 20k rows x 128
+// heads).  The units, rows outermost, are cut into equal stretches, one a pair; the rows stay in
 // shared memory while the heads' weights stream past them, and two accumulators of 256 TMEM
 // columns let one unit's epilogue run beside the next one's products.
 // The epilogue turns 32-row slabs in shared memory so that every global store instruction
@@ -57,9 +60,9 @@ constexpr int kSlabPitch = 144;      // 64 bf16 and 16 bytes against bank confli
 template <int R>
 struct alignas(1024) ExpandSmem {
   static constexpr int kChunks = R / 64;
-  static constexpr int kStages = R == 512 ? 2 : 4;
+  static constexpr int kStages = R == 512 ? 5 : 8;
   uint8_t a[kChunks][128 * 128];
-  uint8_t b[kStages][256 * 128];
+  uint8_t b[kStages][128 * 128];
   uint8_t slab[4][32 * kSlabPitch];
   uint64_t a_full, a_empty, b_full[kStages], b_empty[kStages], acc_full[2], acc_empty[2], drained;
   uint32_t tmem_base;
@@ -74,8 +77,46 @@ __device__ __forceinline__ int64_t page_row(const int32_t* bt, int j, int page, 
   return num_blocks * page;
 }
 
+__device__ __forceinline__ uint32_t cta_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// arrives on the leader CTA's copy of a barrier
+__device__ __forceinline__ void arrive_leader(uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %0, 0;\n\t"
+      "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [a];\n\t}" ::"r"(smem_u32(bar))
+      : "memory");
+}
+// a load of this CTA whose bytes count on the leader's barrier (peer bit of the address cleared)
+__device__ __forceinline__ void tma_load_pair(void* dst, const CUtensorMap* m, uint64_t* bar, int32_t x, int32_t y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar) & 0xFEFFFFFFu), "r"(x), "r"(y)
+      : "memory");
+}
+__device__ __forceinline__ void mma_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void commit_pair(uint64_t* bar) {  // arrives on both CTAs' barrier
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          smem_u32(bar)),
+      "h"((uint16_t)3)
+      : "memory");
+}
+
 template <int R>
-__global__ void __launch_bounds__(kExpandThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kExpandThreads, 1)
     latent_expand_kernel(const __grid_constant__ CUtensorMap c_map, const __grid_constant__ CUtensorMap w_map,
                          const bf16* cache, int64_t num_blocks, int page, const int32_t* work, int nwork,
                          const int32_t* seq_info, const int32_t* block_tables, int max_blocks, int heads,
@@ -85,8 +126,10 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   S& s = *reinterpret_cast<S*>(smem_raw);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
-  const int64_t units = (int64_t)nwork * heads;
-  const int64_t u0 = units * blockIdx.x / gridDim.x, u1 = units * (blockIdx.x + 1) / gridDim.x;
+  const int rank = (int)cta_rank();
+  const int pairs = gridDim.x / 2, me = blockIdx.x / 2;
+  const int64_t units = (int64_t)((nwork + 1) / 2) * heads;
+  const int64_t u0 = units * me / pairs, u1 = units * (me + 1) / pairs;
   if (u0 >= u1) return;
   if (smem_u32(smem_raw) & 1023) {
     if (threadIdx.x == 0) atomicCAS(err, 0, 90);
@@ -102,17 +145,22 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s.acc_full[i], 1);
-      mbar_init(&s.acc_empty[i], 4);
+      mbar_init(&s.acc_empty[i], 8);  // 4 warps x 2 CTAs
     }
     mbar_init(&s.drained, 1);
     fence_barrier_init();
   }
-  if (warp == 1) tmem_alloc(&s.tmem_base, 512);
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s.tmem_base)),
+                 "r"(512)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
   tc_fence_before();
-  __syncthreads();
+  cluster_sync();  // both CTAs' barriers stand before the other uses them
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, s.tmem_base, 0);
-  int tile = (int)(u0 / heads), head = (int)(u0 % heads);
+  int tile = (int)(u0 / heads) * 2 + rank, head = (int)(u0 % heads);  // an odd last tile has no partner
   const int n_units = (int)(u1 - u0);
 
   if (warp == 0) {
@@ -122,33 +170,36 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
       for (int i = 0; ok && i < n_units; ++i) {
         if (i == 0 || head == 0) {
           if (na > 0 && !(ok = wait_or_abort(s, &s.a_empty, (na - 1) & 1, err, 97))) break;
-          const int32_t* si = seq_info + 5 * work[2 * tile];
-          const int r0 = work[2 * tile + 1], ctx = si[2];
+          const bool real = tile < nwork;
+          const int32_t* si = seq_info + 5 * (real ? work[2 * tile] : 0);
+          const int r0 = real ? work[2 * tile + 1] : 0, ctx = real ? si[2] : 0;
           const int32_t* bt = block_tables + (int64_t)si[3] * max_blocks;
-          mbar_arrive_expect_tx(&s.a_full, S::kChunks * 128 * 128);
+          if (rank == 0) mbar_arrive_expect_tx(&s.a_full, 2 * S::kChunks * 128 * 128);
           for (int r = 0; r < 128; r += page) {
             const int y = (int)(r0 + r < ctx ? page_row(bt, r0 + r, page, num_blocks, err) : num_blocks * page);
 #pragma unroll
-            for (int c = 0; c < S::kChunks; ++c) tma_load_2d(s.a[c] + r * 128, &c_map, &s.a_full, c * 64, y);
+            for (int c = 0; c < S::kChunks; ++c) tma_load_pair(s.a[c] + r * 128, &c_map, &s.a_full, c * 64, y);
           }
           ++na;
         }
         for (int ks = 0; ks < S::kChunks; ++ks, ++sent) {
           const int st = sent % S::kStages;
           if (sent >= S::kStages && !(ok = wait_or_abort(s, &s.b_empty[st], (sent / S::kStages - 1) & 1, err, 97))) break;
-          mbar_arrive_expect_tx(&s.b_full[st], 256 * 128);
-          tma_load_2d(s.b[st], &w_map, &s.b_full[st], ks * 64, head * 256);
+          if (rank == 0) mbar_arrive_expect_tx(&s.b_full[st], 2 * 128 * 128);
+          tma_load_pair(s.b[st], &w_map, &s.b_full[st], ks * 64, head * 256 + rank * 128);
         }
-        if (++head == heads) head = 0, ++tile;
+        if (++head == heads) head = 0, tile += 2;
       }
-      // the copies in flight end before the CTA does, on the way out of a time-out too
-      if (na > 0) mbar_wait_sleep(&s.a_full, (na - 1) & 1);
-      for (int i = max(0, sent - S::kStages); i < sent; ++i)
-        mbar_wait_sleep(&s.b_full[i % S::kStages], (i / S::kStages) & 1);
+      // both CTAs' copies in flight end before the pair does, on the way out of a time-out too
+      if (rank == 0) {
+        if (na > 0) mbar_wait_sleep(&s.a_full, (na - 1) & 1);
+        for (int i = max(0, sent - S::kStages); i < sent; ++i)
+          mbar_wait_sleep(&s.b_full[i % S::kStages], (i / S::kStages) & 1);
+      }
     }
   } else if (warp == 1) {
-    if (elect_one()) {
-      constexpr uint32_t idesc = idesc_bf16<128, 256>();
+    if (rank == 0 && elect_one()) {
+      constexpr uint32_t idesc = idesc_bf16<256, 256>();
       const uint64_t a_desc = smem_desc_sw128(smem_u32(s.a[0])), b_desc = smem_desc_sw128(smem_u32(s.b[0]));
       int seen = 0, na = 0;
       bool ok = true;
@@ -161,28 +212,28 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
           ok = wait_or_abort(s, &s.b_full[st], (seen / S::kStages) & 1, err, 98);
           if (!ok) break;
           tc_fence_after();
-          const uint64_t a = a_desc + ks * 1024, b = b_desc + st * 2048;
+          const uint64_t a = a_desc + ks * 1024, b = b_desc + st * 1024;
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk) mma_bf16(d, a + kk * 2, b + kk * 2, idesc, ks + kk > 0);
-          mma_commit(&s.b_empty[st]);
+          for (int kk = 0; kk < 4; ++kk) mma_pair(d, a + kk * 2, b + kk * 2, idesc, ks + kk > 0);
+          commit_pair(&s.b_empty[st]);
         }
         if (!ok) break;
-        mma_commit(&s.acc_full[i & 1]);
+        commit_pair(&s.acc_full[i & 1]);
         if (++head == heads) {
           head = 0;
-          mma_commit(&s.a_empty);
+          commit_pair(&s.a_empty);
         }
       }
-      mma_commit(&s.drained);
-      mbar_wait_sleep(&s.drained, 0);
+      commit_pair(&s.drained);
     }
   } else {
     const int quad = warp & 3;
     uint8_t* slab = s.slab[quad];
     const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
     for (int i = 0; i < n_units; ++i) {
-      const int32_t* si = seq_info + 5 * work[2 * tile];
-      const int r0 = work[2 * tile + 1] + quad * 32, ctx = si[2];  // this warp's 32 rows
+      const bool real = tile < nwork;
+      const int32_t* si = seq_info + 5 * (real ? work[2 * tile] : 0);
+      const int r0 = real ? work[2 * tile + 1] + quad * 32 : 0, ctx = real ? si[2] : 0;  // this warp's 32 rows
       const int64_t row0 = (int64_t)si[4] + r0;
       const int valid = ctx - r0, padded = min(32, (ctx + 15) / 16 * 16 - r0);
       if (head == 0 && k_rope != nullptr) {
@@ -224,7 +275,7 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
         __syncwarp();
         if (c == 192) {  // the accumulator has been read
           tc_fence_before();
-          if (lane == 0) mbar_arrive(&s.acc_empty[i & 1]);
+          if (lane == 0) arrive_leader(&s.acc_empty[i & 1]);
         }
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
@@ -235,15 +286,17 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
         }
         __syncwarp();
       }
-      if (++head == heads) head = 0, ++tile;
+      if (++head == heads) head = 0, tile += 2;
     }
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 1) {
-    tc_fence_after();
-    tmem_dealloc(tmem, 512);
-  }
+  if (threadIdx.x == 32) mbar_wait_sleep(&s.drained, 0);  // every MMA has finished before tensor memory is freed
+  __syncthreads();
+  cluster_sync();  // no CTA leaves while its peer may still signal it
+  tc_fence_after();
+  if (warp == 1)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
 // ------------------------------------------------------------------ attention
@@ -589,8 +642,8 @@ void launch_latent_expand(const LatentExpand& a, cudaStream_t st) {
   auto go = [&](auto kern, size_t smem, std::atomic<uint64_t>& attr_devs) {
     ensure_smem_attr(attr_devs, kern, smem);
     const CUtensorMap tc = make_tmap_2d_bf16(a.cache, (uint64_t)a.num_blocks * a.page, a.R + kRot, a.R + kRot, a.page, 64, true);
-    const CUtensorMap tw = make_tmap_2d_bf16(a.w, (uint64_t)a.heads * 256, a.R, a.R, 256, 64, true);
-    const int grid = (int)std::min<int64_t>(a.num_sms, (int64_t)a.nwork * a.heads);
+    const CUtensorMap tw = make_tmap_2d_bf16(a.w, (uint64_t)a.heads * 256, a.R, a.R, 128, 64, true);
+    const int grid = 2 * (int)std::max<int64_t>(1, std::min<int64_t>(a.num_sms / 2, (int64_t)((a.nwork + 1) / 2) * a.heads));
     launch_k(kern, dim3(grid), kExpandThreads, smem, st, tc, tw, a.cache, a.num_blocks, a.page, a.work, a.nwork,
              a.seq_info, a.block_tables, a.max_blocks, a.heads, a.kv, a.kv_stride, a.k_rope, a.err);
     KAPSL_LAUNCH_CHECK();
