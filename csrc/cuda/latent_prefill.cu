@@ -175,11 +175,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kExpandThreads, 1)
           const int r0 = real ? work[2 * tile + 1] : 0, ctx = real ? si[2] : 0;
           const int32_t* bt = block_tables + (int64_t)si[3] * max_blocks;
           if (rank == 0) mbar_arrive_expect_tx(&s.a_full, 2 * S::kChunks * 128 * 128);
-          for (int r = 0; r < 128; r += page) {
-            const int y = (int)(r0 + r < ctx ? page_row(bt, r0 + r, page, num_blocks, err) : num_blocks * page);
+          int y[8];  // the block ids first: their loads are independent of each other
 #pragma unroll
-            for (int c = 0; c < S::kChunks; ++c) tma_load_pair(s.a[c] + r * 128, &c_map, &s.a_full, c * 64, y);
+          for (int g = 0; g < 8; ++g) {
+            const int r = g * page;
+            y[g] = (int)(r < 128 && r0 + r < ctx ? page_row(bt, r0 + r, page, num_blocks, err) : num_blocks * page);
           }
+#pragma unroll
+          for (int g = 0; g < 8; ++g)
+            if (g * page < 128)
+#pragma unroll
+              for (int c = 0; c < S::kChunks; ++c)
+                tma_load_pair(s.a[c] + g * page * 128, &c_map, &s.a_full, c * 64, y[g]);
           ++na;
         }
         for (int ks = 0; ks < S::kChunks; ++ks, ++sent) {
@@ -238,7 +245,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kExpandThreads, 1)
       const int valid = ctx - r0, padded = min(32, (ctx + 15) / 16 * 16 - r0);
       if (head == 0 && k_rope != nullptr) {
         const int32_t* bt = block_tables + (int64_t)si[3] * max_blocks;
-#pragma unroll 2
+#pragma unroll
         for (int k = 0; k < 8; ++k) {  // 4 rows x 8 lanes
           const int r = 4 * k + (lane >> 3), seg = lane & 7;
           if (r < padded) {
