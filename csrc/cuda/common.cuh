@@ -94,6 +94,10 @@ __device__ __forceinline__ void griddep_entry() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }
+// The two halves of griddep_entry, for kernels that set up shared and tensor memory between them
+// (nothing that an earlier kernel writes is read before the wait).
+__device__ __forceinline__ void griddep_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void griddep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 // Entry of a kernel that does not let the next one launch early (it launches when
 // this grid completes): waits for the previous grid only.  The sampler uses it:
 // with the early trigger, back-to-back 256 x 152064 samplings measured 4x slower

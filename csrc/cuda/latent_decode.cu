@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(kAttnThreads<R>, 1)
                        const int32_t* ctx_lens, const int32_t* table,
                        float* part_o, float* part_lse, int B, int H, int heads_per_cta,
                        int head_tiles, float scale_log2, int* err) {
-  griddep_entry();
+  griddep_launch();
   using S = Shape<R, NT>;
   constexpr int kMma = S::kGroups;  // warps: producers, MMA issuer, softmax
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -248,8 +248,6 @@ __global__ void __launch_bounds__(kAttnThreads<R>, 1)
   const int ht = blockIdx.x % head_tiles, c = blockIdx.x / head_tiles;
   const int ctas = gridDim.x / head_tiles;
   const int h0 = ht * heads_per_cta, nheads = min(heads_per_cta, H - h0);
-  Pieces pc(table, B, c);
-  if (!pc.more()) return;
   if (smem_u32(smem_raw) & 1023) {  // the swizzled tiles need it
     if (threadIdx.x == 0) atomicCAS(err, 0, 83);
     return;
@@ -279,6 +277,8 @@ __global__ void __launch_bounds__(kAttnThreads<R>, 1)
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, s.tmem_base, 0);
   const uint32_t tmem_o = tmem + 2 * NT;
+  griddep_wait();
+  Pieces pc(table, B, c);  // without pieces, every role falls through its loop
 
   if (warp < S::kGroups) {
     // ------------------------------------------- TMA producer of dims [128 g, 128 g + 128)
@@ -373,10 +373,10 @@ __global__ void __launch_bounds__(kAttnThreads<R>, 1)
       const uint64_t p_desc = smem_desc_mn_sw128(smem_u32(s.p), 1024, 1024);
       // two cursors over the same tiles: scores (sc) and second products (pv)
       Pieces sp = pc;
-      int sc = 0, grp = 0, left_s = sp.tiles(), nq = 0;
+      int sc = 0, grp = 0, left_s = sp.more() ? sp.tiles() : 0, nq = 0;
       bool s_open = true, q_open = false;
       const int total = pc.end - pc.at;
-      int left_p = pc.tiles();
+      int left_p = left_s;
       bool first_p = true;
       uint64_t t_last = 0;
       uint32_t idle = 0;
@@ -626,9 +626,11 @@ __global__ void __launch_bounds__(kAttnThreads<R>, 1)
 
 // -------------------------------------------------------------- head products
 //
-// y[b, h, n] = sum_k x[b, h, k] w_h[k, n], small matrices per head: bound by the weights
-// (64 KB + 64 KB a head at R = 512) until hundreds of rows share them, which mma.sync
-// serves at the speed of the loads; a 128-row tcgen05 tile would be mostly padding.
+// y[b, h, n] = sum_k x[b, h, k] w_h[k, n], small matrices per head, bound by the weights (128 KB +
+// 128 KB a head at R = 512) and the rows' traffic.  Up to 16 rows: mma.sync on 16-row tiles,
+// many small CTAs, since latency is all that counts.  Above: tcgen05 on 128-row tiles fed by
+// TMA; at 64 rows x 128 heads the mma.sync form took ABS_OLD for both products where this
+// one takes ABS_NEW, held back by its shared-memory loads and stores.
 
 __device__ __forceinline__ void cp16(void* dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
@@ -637,67 +639,75 @@ __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_grou
 template <int N>
 __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
+// qa[b, h, R:] = q[b, h, 128:] for ROWS rows, by 128 threads: all loads before the first store (the
+// compiler cannot tell that they do not overlap).
+template <int R, int ROWS>
+__device__ __forceinline__ void copy_rotary(const bf16* q, int64_t q_stride, bf16* qa, int rows, int H, int h) {
+  constexpr int N = ROWS * 8 / 128;
+  uint4 v[N];
+  const int seg = threadIdx.x & 7;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int b = (i * 128 + threadIdx.x) >> 3;
+    if (b < rows)
+      v[i] = *reinterpret_cast<const uint4*>(q + (int64_t)b * q_stride + (int64_t)h * (kNope + kRot) + kNope + seg * 8);
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int b = (i * 128 + threadIdx.x) >> 3;
+    if (b < rows) *reinterpret_cast<uint4*>(qa + ((int64_t)b * H + h) * (R + kRot) + R + seg * 8) = v[i];
+  }
+}
+
 // qa[b, h, :R] = q[b, h, :128] . w[h, :128, :], qa[b, h, R:] = q[b, h, 128:].
-// One CTA per (64 columns, head, MROWS rows); qa is bf16, the tensor cores' operand type.
-template <int R, int MROWS>
+// One CTA per (64 columns, head); qa is bf16, the tensor cores' operand type.
+template <int R>
 __global__ void __launch_bounds__(128) latent_absorb_kernel(const bf16* q, int64_t q_stride,
                                                             const bf16* w, bf16* qa, int B,
                                                             int H, const int32_t* ctx_lens, int limit,
                                                             int ctas, int32_t* table) {
   griddep_entry();
-  if (blockIdx.x == gridDim.x - 1 && blockIdx.y == 0 && blockIdx.z == 0)
+  constexpr int MROWS = 16;
+  if (blockIdx.x == gridDim.x - 1 && blockIdx.y == 0)
     write_schedule(ctx_lens, B, limit, ctas, table);
   constexpr int kPitchW = 64 + 8, kPitchX = kNope + 8;  // 16 bytes of padding: conflict-free ldmatrix
   __shared__ __align__(16) bf16 ws[kNope * kPitchW];
   __shared__ __align__(16) bf16 xs[MROWS * kPitchX];
-  const int n0 = blockIdx.x * 64, h = blockIdx.y, b0 = blockIdx.z * MROWS;
+  const int n0 = blockIdx.x * 64, h = blockIdx.y;
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
   const bf16* wk = w + (int64_t)h * (kNope + kVal) * R + n0;
   for (int i = t; i < kNope * 8; i += 128) cp16(ws + (i >> 3) * kPitchW + (i & 7) * 8, wk + (int64_t)(i >> 3) * R + (i & 7) * 8);
   for (int i = t; i < MROWS * 16; i += 128) {
     const int r = i >> 4;
-    if (b0 + r < B)
-      cp16(xs + r * kPitchX + (i & 15) * 8, q + (int64_t)(b0 + r) * q_stride + (int64_t)h * (kNope + kRot) + (i & 15) * 8);
+    if (r < B)
+      cp16(xs + r * kPitchX + (i & 15) * 8, q + (int64_t)r * q_stride + (int64_t)h * (kNope + kRot) + (i & 15) * 8);
   }
   cp_commit();
   if (blockIdx.x == 0) {  // the rotary part
-    for (int i = t; i < MROWS * 8; i += 128) {
-      const int b = b0 + (i >> 3);
-      if (b < B)
-        *reinterpret_cast<uint4*>(qa + ((int64_t)b * H + h) * (R + kRot) + R + (i & 7) * 8) =
-            *reinterpret_cast<const uint4*>(q + (int64_t)b * q_stride + (int64_t)h * (kNope + kRot) + kNope + (i & 7) * 8);
-    }
+    copy_rotary<R, MROWS>(q, q_stride, qa, B, H, h);
   }
   cp_wait<0>();
   __syncthreads();
-  // MROWS = 64: a warp per 16 rows, 64 columns; 16: a warp per 16 columns
-  constexpr int NP = MROWS == 64 ? 4 : 1;  // 16-column pairs of n-tiles a warp
-  const int r0 = MROWS == 64 ? warp * 16 : 0, c0 = MROWS == 64 ? 0 : warp * 16;
-  float acc[NP][2][4] = {};
+  const int c0 = warp * 16;  // a warp's columns
+  float acc[2][4] = {};
 #pragma unroll
   for (int ks = 0; ks < kNope / 16; ++ks) {
-    uint32_t a[4];
-    ldmatrix_x4(a, smem_u32(xs + (r0 + (lane & 15)) * kPitchX + ks * 16 + (lane >> 4) * 8));
-#pragma unroll
-    for (int p = 0; p < NP; ++p) {
-      uint32_t bb[4];
-      ldmatrix_x4_trans(bb, smem_u32(ws + (ks * 16 + (lane & 15)) * kPitchW + c0 + p * 16 + (lane >> 4) * 8));
-      mma_bf16_16816(acc[p][0], a, {bb[0], bb[1]});
-      mma_bf16_16816(acc[p][1], a, {bb[2], bb[3]});
-    }
+    uint32_t a[4], bb[4];
+    ldmatrix_x4(a, smem_u32(xs + (lane & 15) * kPitchX + ks * 16 + (lane >> 4) * 8));
+    ldmatrix_x4_trans(bb, smem_u32(ws + (ks * 16 + (lane & 15)) * kPitchW + c0 + (lane >> 4) * 8));
+    mma_bf16_16816(acc[0], a, {bb[0], bb[1]});
+    mma_bf16_16816(acc[1], a, {bb[2], bb[3]});
   }
   __syncthreads();  // the result takes the queries' place, then leaves in whole 128-byte rows
 #pragma unroll
-  for (int p = 0; p < NP; ++p)
+  for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
-    for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-        *reinterpret_cast<uint32_t*>(xs + (r0 + (lane >> 2) + e * 8) * kPitchX + c0 + p * 16 + nt * 8 + (lane & 3) * 2) =
-            pack_bf16(acc[p][nt][2 * e], acc[p][nt][2 * e + 1]);
+    for (int e = 0; e < 2; ++e)
+      *reinterpret_cast<uint32_t*>(xs + ((lane >> 2) + e * 8) * kPitchX + c0 + nt * 8 + (lane & 3) * 2) =
+          pack_bf16(acc[nt][2 * e], acc[nt][2 * e + 1]);
   __syncthreads();
   for (int i = t; i < MROWS * 8; i += 128) {
-    const int b = b0 + (i >> 3);
+    const int b = i >> 3;
     if (b < B)
       *reinterpret_cast<uint4*>(qa + ((int64_t)b * H + h) * (R + kRot) + n0 + (i & 7) * 8) =
           *reinterpret_cast<const uint4*>(xs + (i >> 3) * kPitchX + (i & 7) * 8);
@@ -727,19 +737,27 @@ __global__ void __launch_bounds__(128)
   const int64_t step = (int64_t)heads_per_cta * R;
   const float a0 = lane < n ? part_lse[slot + (int64_t)lane * heads_per_cta] : -INFINITY;
   const float a1 = lane + 32 < n ? part_lse[slot + (int64_t)(lane + 32) * heads_per_cta] : -INFINITY;
+  float4 y[4][2];
+  auto load = [&](int p0) {
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      if (p0 + p < n) {
+        const float4* at = reinterpret_cast<const float4*>(src + (p0 + p) * step);
+        y[p][0] = at[0];
+        y[p][1] = at[1];
+      } else {  // its weight is 0
+        y[p][0] = y[p][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+    }
+  };
+  load(0);  // under way with the weights
   float M = warp_max(fmaxf(a0, a1));
   if (M == -INFINITY) M = 0.f;  // no finite score in the row: weights 0 (or NaN, which reaches the row)
   const float e0 = ex2(a0 - M), e1 = ex2(a1 - M);
   const float L = warp_sum(e0 + e1);
   float x[8] = {};
   for (int p0 = 0; p0 < n; p0 += 4) {
-    float4 y[4][2];
-#pragma unroll
-    for (int p = 0; p < 4; ++p) {
-      const float4* at = reinterpret_cast<const float4*>(src + min(p0 + p, n - 1) * step);  // weight 0 past the last
-      y[p][0] = at[0];
-      y[p][1] = at[1];
-    }
+    if (p0 > 0) load(p0);
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
       const float f = __shfl_sync(0xffffffffu, p0 < 32 ? e0 : e1, (p0 + p) & 31);
@@ -760,19 +778,20 @@ __global__ void __launch_bounds__(128)
   *reinterpret_cast<uint4*>(lo + row * R + k) = make_uint4(low[0], low[1], low[2], low[3]);
 }
 
-// out[b, h, n] = sum_r (hi + lo)[b, h, r] w[h, 128 + n, r].  One CTA per (NCOLS columns, head,
-// MROWS rows); K in chunks of 128 through STAGES shared-memory stages.
-template <int R, int MROWS, int NCOLS, int THREADS, int STAGES>
-__global__ void __launch_bounds__(THREADS)
+// out[b, h, n] = sum_r (hi + lo)[b, h, r] w[h, 128 + n, r] for up to 16 rows: one CTA per (32 columns,
+// head), everything it needs requested at once.
+template <int R>
+__global__ void __launch_bounds__(128)
     latent_out_kernel(const bf16* hi, const bf16* lo, const bf16* w,
                       bf16* out, int64_t out_stride, int B, int H) {
   griddep_entry();
+  constexpr int MROWS = 16, NCOLS = 32, THREADS = 128;
   constexpr int kPitch = 128 + 8;
-  constexpr int kSteps = R / 128;
+  constexpr int kSteps = R / 128, STAGES = kSteps + 1;
   constexpr int kStage = (NCOLS + 2 * MROWS) * kPitch;
   extern __shared__ __align__(16) uint8_t raw[];
   bf16* sm = reinterpret_cast<bf16*>(raw);  // a stage: [NCOLS] w, [MROWS] hi, [MROWS] lo rows
-  const int n0 = blockIdx.x * NCOLS, h = blockIdx.y, b0 = blockIdx.z * MROWS;
+  const int n0 = blockIdx.x * NCOLS, h = blockIdx.y;
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
   const bf16* wv = w + ((int64_t)h * (kNope + kVal) + kNope + n0) * R;
   auto load = [&](int c) {
@@ -782,19 +801,17 @@ __global__ void __launch_bounds__(THREADS)
         cp16(st + (i >> 4) * kPitch + (i & 15) * 8, wv + (int64_t)(i >> 4) * R + c * 128 + (i & 15) * 8);
       for (int i = t; i < 2 * MROWS * 16; i += THREADS) {
         const int r = (i >> 4) % MROWS;
-        if (b0 + r < B)
+        if (r < B)
           cp16(st + (NCOLS + (i >> 4)) * kPitch + (i & 15) * 8,
-               (i >= MROWS * 16 ? lo : hi) + ((int64_t)(b0 + r) * H + h) * R + c * 128 + (i & 15) * 8);
+               (i >= MROWS * 16 ? lo : hi) + ((int64_t)r * H + h) * R + c * 128 + (i & 15) * 8);
       }
     }
     cp_commit();
   };
 #pragma unroll
   for (int c = 0; c < STAGES - 1; ++c) load(c);
-  constexpr int MW = MROWS / 16, NW = THREADS / 32 / MW;  // warps along rows and columns
-  constexpr int NT8 = NCOLS / NW / 8;
-  const int r0 = (warp % MW) * 16, c0 = (warp / MW) * (NCOLS / NW);
-  float acc[NT8][4] = {};
+  const int c0 = warp * 8;  // a warp's columns
+  float acc[4] = {};
   for (int c = 0; c < kSteps; ++c) {
     cp_wait<STAGES - 2>();
     __syncthreads();  // the chunk is here, and the stage loaded next has been read
@@ -804,30 +821,218 @@ __global__ void __launch_bounds__(THREADS)
 #pragma unroll
     for (int ks = 0; ks < 8; ++ks) {
       uint32_t ah[4], al[4];
-      const int at = (r0 + (lane & 15)) * kPitch + ks * 16 + (lane >> 4) * 8;
+      const int at = (lane & 15) * kPitch + ks * 16 + (lane >> 4) * 8;
       ldmatrix_x4(ah, smem_u32(xh + at));
       ldmatrix_x4(al, smem_u32(xh + MROWS * kPitch + at));
-#pragma unroll
-      for (int n = 0; n < NT8; ++n) {
-        uint32_t bb[2];
-        // rows n, 16 bytes at k and k + 8
-        asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0,%1}, [%2];"
-                     : "=r"(bb[0]), "=r"(bb[1])
-                     : "r"(smem_u32(wc + (c0 + n * 8 + (lane & 7)) * kPitch + ks * 16 + ((lane >> 3) & 1) * 8)));
-        mma_bf16_16816(acc[n], ah, bb);
-        mma_bf16_16816(acc[n], al, bb);
-      }
+      uint32_t bb[2];  // rows n, 16 bytes at k and k + 8
+      asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0,%1}, [%2];"
+                   : "=r"(bb[0]), "=r"(bb[1])
+                   : "r"(smem_u32(wc + (c0 + (lane & 7)) * kPitch + ks * 16 + ((lane >> 3) & 1) * 8)));
+      mma_bf16_16816(acc, ah, bb);
+      mma_bf16_16816(acc, al, bb);
     }
   }
 #pragma unroll
-  for (int n = 0; n < NT8; ++n)
+  for (int e = 0; e < 2; ++e) {
+    const int b = (lane >> 2) + e * 8;
+    if (b < B)
+      *reinterpret_cast<uint32_t*>(out + (int64_t)b * out_stride + (int64_t)h * kVal + n0 + c0 + (lane & 3) * 2) =
+          pack_bf16(acc[2 * e], acc[2 * e + 1]);
+  }
+}
+
+// ---- the same on tcgen05: 128-row tiles, thread = row of the accumulator's quadrant
+
+// Stores 32 rows x 64 columns of an accumulator (this warp's lanes, columns from taddr) as bf16
+// rows of 128 bytes: through a shared-memory slab, so that a store instruction writes whole lines.
+constexpr int kSlabPitch = 144;  // 64 bf16 and 16 bytes against bank conflicts
+__device__ __forceinline__ void store_slab(uint32_t taddr, uint8_t* slab, bf16* dst, int64_t pitch, int rows) {
+  const int lane = threadIdx.x & 31;
+  uint4* mine = reinterpret_cast<uint4*>(slab + lane * kSlabPitch);
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int b = b0 + r0 + (lane >> 2) + e * 8;
-      if (b < B)
-        *reinterpret_cast<uint32_t*>(out + (int64_t)b * out_stride + (int64_t)h * kVal + n0 + c0 + n * 8 + (lane & 3) * 2) =
-            pack_bf16(acc[n][2 * e], acc[n][2 * e + 1]);
+  for (int half = 0; half < 2; ++half) {
+    float v[32];
+    tmem_ld32w(taddr + half * 32, v);
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      mine[half * 4 + q] = make_uint4(pack_bf16(v[8 * q], v[8 * q + 1]), pack_bf16(v[8 * q + 2], v[8 * q + 3]),
+                                      pack_bf16(v[8 * q + 4], v[8 * q + 5]), pack_bf16(v[8 * q + 6], v[8 * q + 7]));
+  }
+  __syncwarp();
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const int r = 4 * k + (lane >> 3), seg = lane & 7;
+    if (r < rows)
+      *reinterpret_cast<uint4*>(dst + r * pitch + seg * 8) = *reinterpret_cast<const uint4*>(slab + r * kSlabPitch + seg * 16);
+  }
+  __syncwarp();
+}
+
+struct AbsorbSmem {
+  alignas(1024) uint8_t x[2][128 * 128];  // 128 rows x 64 of k
+  alignas(1024) uint8_t w[4][128 * 128];  // 128 of k x 64 columns
+  uint64_t full, done;
+  uint32_t tmem_base;
+  volatile int abort_flag;
+};
+
+// One CTA per (256 columns, head, 128 rows); w is read MN-major, as it lies in memory.
+template <int R>
+__global__ void __launch_bounds__(128) latent_absorb_tc_kernel(const __grid_constant__ CUtensorMap q_map,
+                                                               const __grid_constant__ CUtensorMap w_map, const bf16* q,
+                                                               int64_t q_stride, bf16* qa, int B, int H,
+                                                               const int32_t* ctx_lens, int limit, int ctas,
+                                                               int32_t* table, int* err) {
+  griddep_launch();
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  AbsorbSmem& s = *reinterpret_cast<AbsorbSmem*>(smem_raw);
+  const int n0 = blockIdx.x * 256, h = blockIdx.y, b0 = blockIdx.z * 128;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
+  if (smem_u32(smem_raw) & 1023) {
+    if (threadIdx.x == 0) atomicCAS(err, 0, 83);
+    return;
+  }
+  if (threadIdx.x == 0) {
+    s.abort_flag = 0;
+    mbar_init(&s.full, 1);
+    mbar_init(&s.done, 1);
+    fence_barrier_init();
+  }
+  if (warp == 0) tmem_alloc(&s.tmem_base, 256);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  griddep_wait();
+  const uint32_t tmem = __shfl_sync(0xffffffffu, s.tmem_base, 0);
+  if (warp == 0 && elect_one()) {
+    mbar_arrive_expect_tx(&s.full, 6 * 128 * 128);
+#pragma unroll
+    for (int c = 0; c < 2; ++c) tma_load_2d(s.x[c], &q_map, &s.full, h * (kNope + kRot) + c * 64, b0);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) tma_load_2d(s.w[c], &w_map, &s.full, n0 + c * 64, h * (kNope + kVal));
+    if (wait_or_abort(s, &s.full, 0, err, 84)) {
+      tc_fence_after();
+      constexpr uint32_t idesc = idesc_bf16<128, 256>() | kIdescBMn;
+      const uint64_t a = smem_desc_sw128(smem_u32(s.x[0])), b = smem_desc_mn_sw128(smem_u32(s.w[0]), 128 * 128, 1024);
+#pragma unroll
+      for (int kk = 0; kk < 8; ++kk) mma_bf16(tmem, a + (kk >> 2) * 1024 + (kk & 3) * 2, b + kk * 128, idesc, kk > 0);
     }
+    mma_commit(&s.done);
+  }
+  __syncwarp();
+  if (blockIdx.x == 0) {  // the rotary part
+    copy_rotary<R, 128>(q + (int64_t)b0 * q_stride, q_stride, qa + (int64_t)b0 * H * (R + kRot), B - b0, H, h);
+  }
+  if (blockIdx.x == gridDim.x - 1 && blockIdx.y == 0 && blockIdx.z == 0)
+    write_schedule(ctx_lens, B, limit, ctas, table);
+  wait_or_abort(s, &s.done, 0, err, 85);
+  __syncwarp();
+  tc_fence_after();
+  // the operands have been read: their place serves as the slabs
+  uint8_t* slab = s.x[0] + warp * 32 * kSlabPitch;
+  const int r0 = b0 + warp * 32;
+  bf16* dst = qa + ((int64_t)r0 * H + h) * (R + kRot) + n0;
+#pragma unroll 1
+  for (int c = 0; c < 256; c += 64)
+    store_slab(tmem + ((uint32_t)(warp * 32) << 16) + c, slab, dst + c, (int64_t)H * (R + kRot), B - r0);
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 256);
+  }
+}
+
+constexpr int kOutStages = 4;
+struct OutSmem {
+  alignas(1024) uint8_t st[kOutStages][3][128 * 128];  // hi, lo rows and value weights, 64 of k
+  uint64_t full[kOutStages], empty[kOutStages], done;
+  uint32_t tmem_base;
+  volatile int abort_flag;
+};
+
+// out[b, h, n] = sum_r (hi + lo)[b, h, r] w[h, 128 + n, r]: one CTA per (head, 128 rows).
+template <int R>
+__global__ void __launch_bounds__(128, 1) latent_out_tc_kernel(const __grid_constant__ CUtensorMap hi_map,
+                                                            const __grid_constant__ CUtensorMap lo_map,
+                                                            const __grid_constant__ CUtensorMap w_map, bf16* out,
+                                                            int64_t out_stride, int B, int* err) {
+  griddep_launch();
+  constexpr int kSteps = R / 64;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  OutSmem& s = *reinterpret_cast<OutSmem*>(smem_raw);
+  const int h = blockIdx.x, b0 = blockIdx.y * 128;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0);
+  if (smem_u32(smem_raw) & 1023) {
+    if (threadIdx.x == 0) atomicCAS(err, 0, 83);
+    return;
+  }
+  if (threadIdx.x == 0) {
+    s.abort_flag = 0;
+    for (int i = 0; i < kOutStages; ++i) {
+      mbar_init(&s.full[i], 1);
+      mbar_init(&s.empty[i], 1);
+    }
+    mbar_init(&s.done, 1);
+    fence_barrier_init();
+  }
+  if (warp == 0) tmem_alloc(&s.tmem_base, 128);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  griddep_wait();
+  const uint32_t tmem = __shfl_sync(0xffffffffu, s.tmem_base, 0);
+  if (warp == 0) {
+    if (elect_one()) {
+      bool ok = true;
+      int k = 0;
+      for (; k < kSteps; ++k) {
+        const int st = k % kOutStages;
+        if (k >= kOutStages && !(ok = wait_or_abort(s, &s.empty[st], (k / kOutStages - 1) & 1, err, 84))) break;
+        mbar_arrive_expect_tx(&s.full[st], 3 * 128 * 128);
+        tma_load_2d(s.st[st][2], &w_map, &s.full[st], k * 64, h * (kNope + kVal) + kNope);
+        tma_load_2d(s.st[st][0], &hi_map, &s.full[st], h * R + k * 64, b0);
+        tma_load_2d(s.st[st][1], &lo_map, &s.full[st], h * R + k * 64, b0);
+      }
+      if (!ok)  // the copies in flight end before the CTA does
+        for (int i = max(0, k - kOutStages); i < k; ++i) mbar_wait_sleep(&s.full[i % kOutStages], (i / kOutStages) & 1);
+    }
+  } else if (warp == 1) {
+    if (elect_one()) {
+      constexpr uint32_t idesc = idesc_bf16<128, 128>();
+      const uint64_t d0 = smem_desc_sw128(smem_u32(s.st[0][0]));
+      for (int k = 0; k < kSteps; ++k) {
+        const int st = k % kOutStages;
+        if (!wait_or_abort(s, &s.full[st], (k / kOutStages) & 1, err, 85)) break;
+        tc_fence_after();
+        const uint64_t a = d0 + st * 3 * 1024, b = a + 2 * 1024;
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+          mma_bf16(tmem, a + kk * 2, b + kk * 2, idesc, k + kk > 0);
+          mma_bf16(tmem, a + 1024 + kk * 2, b + kk * 2, idesc, 1);
+        }
+        mma_commit(&s.empty[st]);
+      }
+      mma_commit(&s.done);
+    }
+  }
+  __syncwarp();
+  wait_or_abort(s, &s.done, 0, err, 86);
+  __syncwarp();
+  tc_fence_after();
+  // every operand has been read: the stages' place serves as the slabs
+  uint8_t* slab = s.st[0][0] + warp * 32 * kSlabPitch;
+  const int r0 = b0 + warp * 32;
+  bf16* dst = out + (int64_t)r0 * out_stride + (int64_t)h * kVal;
+#pragma unroll 1
+  for (int c = 0; c < 128; c += 64)
+    store_slab(tmem + ((uint32_t)(warp * 32) << 16) + c, slab, dst + c, out_stride, B - r0);
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 128);
+  }
 }
 
 // Heads are cut into equal tiles of at most 64; each gets an equal share of the SMs, and
@@ -855,14 +1060,10 @@ struct Layout {
   }
 };
 
-template <int R, int MROWS, int NCOLS, int THREADS, int STAGES>
-void run_out(const LatentDecode& a, const bf16* hi, const bf16* lo, cudaStream_t st) {
-  auto kern = latent_out_kernel<R, MROWS, NCOLS, THREADS, STAGES>;
-  constexpr size_t smem = (size_t)STAGES * (NCOLS + 2 * MROWS) * 136 * 2;
-  static std::atomic<uint64_t> attr_devs{0};
+template <class Kernel, class... Args>
+void run_smem(Kernel kern, std::atomic<uint64_t>& attr_devs, dim3 grid, size_t smem, cudaStream_t st, Args... args) {
   ensure_smem_attr(attr_devs, kern, smem);
-  launch_k(kern, dim3(kVal / NCOLS, a.H, (a.B + MROWS - 1) / MROWS), THREADS, smem, st, hi, lo, a.w, a.out,
-           a.out_stride, a.B, a.H);
+  launch_k(kern, grid, 128, smem, st, args...);
   KAPSL_LAUNCH_CHECK();
 }
 
@@ -893,14 +1094,18 @@ void run(const LatentDecode& a, cudaStream_t st) {
   float* part_lse = reinterpret_cast<float*>(ws + l.lse);
   float* part_o = reinterpret_cast<float*>(ws + l.part);
   const int limit = a.max_blocks * a.page;
-  if (a.B <= 16) {
-    launch_k(latent_absorb_kernel<R, 16>, dim3(R / 64, a.H, 1), 128, 0, st, a.q, a.q_stride, a.w, qa, a.B, a.H,
-             a.ctx_lens, limit, p.ctas, table);
+  const bool small = a.B <= 16;
+  const CUtensorMap tw = make_tmap_2d_bf16(a.w, (uint64_t)a.H * (kNope + kVal), R, R, 128, 64, true);
+  if (small) {
+    launch_k(latent_absorb_kernel<R>, dim3(R / 64, a.H), 128, 0, st, a.q, a.q_stride, a.w, qa, a.B, a.H, a.ctx_lens,
+             limit, p.ctas, table);
+    KAPSL_LAUNCH_CHECK();
   } else {
-    launch_k(latent_absorb_kernel<R, 64>, dim3(R / 64, a.H, (a.B + 63) / 64), 128, 0, st, a.q, a.q_stride, a.w, qa,
-             a.B, a.H, a.ctx_lens, limit, p.ctas, table);
+    const CUtensorMap tq = make_tmap_2d_bf16(a.q, a.B, (uint64_t)a.H * (kNope + kRot), a.q_stride, 128, 64, true);
+    static std::atomic<uint64_t> devs{0};
+    run_smem(latent_absorb_tc_kernel<R>, devs, dim3(R / 256, a.H, (a.B + 127) / 128), sizeof(AbsorbSmem), st, tq, tw, a.q,
+             a.q_stride, qa, a.B, a.H, a.ctx_lens, limit, p.ctas, table, a.err);
   }
-  KAPSL_LAUNCH_CHECK();
   if (p.heads_per_cta <= 16) {
     run_attn<R, 16>(a, p, qa, part_o, part_lse, table, st);
   } else if (p.heads_per_cta <= 32) {
@@ -914,10 +1119,16 @@ void run(const LatentDecode& a, cudaStream_t st) {
   launch_k(latent_join_kernel<R>, dim3((unsigned)((rows + per - 1) / per)), 128, 0, st, part_o, part_lse, table, qa,
            lo, a.B, a.H, p.heads_per_cta, p.ctas);
   KAPSL_LAUNCH_CHECK();
-  if (a.B <= 16) {
-    run_out<R, 16, 32, 128, R / 128 + 1>(a, qa, lo, st);
+  static std::atomic<uint64_t> devs{0}, devs_tc{0};
+  if (small) {
+    constexpr size_t smem = (size_t)(R / 128 + 1) * (32 + 2 * 16) * 136 * 2;
+    run_smem(latent_out_kernel<R>, devs, dim3(kVal / 32, a.H), smem, st, qa, lo, a.w, a.out, a.out_stride, a.B, a.H);
   } else {
-    run_out<R, 32, 128, 256, 2>(a, qa, lo, st);
+    const uint64_t width = (uint64_t)a.H * R;
+    const CUtensorMap th = make_tmap_2d_bf16(qa, a.B, width, width, 128, 64, true);
+    const CUtensorMap tl = make_tmap_2d_bf16(lo, a.B, width, width, 128, 64, true);
+    run_smem(latent_out_tc_kernel<R>, devs_tc, dim3(a.H, (a.B + 127) / 128), sizeof(OutSmem), st, th, tl, tw, a.out,
+             a.out_stride, a.B, a.err);
   }
   note_launch(4);
 }
