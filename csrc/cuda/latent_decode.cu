@@ -716,66 +716,89 @@ __global__ void __launch_bounds__(128) latent_absorb_kernel(const bf16* q, int64
 
 // Joins a row's pieces: o[b, h] = sum_c 2^(lse_c - M) o_c / sum_c 2^(lse_c - M), written as hi + lo,
 // two bf16 whose sum keeps 16 bits of it: the product below then rounds nothing else.  One
-// thread per 8 dims, whole warps a row: the pieces' weights are spread over the lanes, four
-// pieces' loads are in flight at once.
-template <int R>
+// thread per 8 dims of ROWS rows, whole warps a row: the pieces' weights are spread over the
+// lanes, and P pieces of every row are requested at once (few rows have many pieces: P = 8;
+// many rows have one or two: P = 2, and two rows a thread).
+template <int R, int P, int ROWS>
 __global__ void __launch_bounds__(128)
-    latent_join_kernel(const float* part_o, const float* part_lse,
-                       const int32_t* table, bf16* hi, bf16* lo, int B, int H,
-                       int heads_per_cta, int ctas) {
+    latent_join_kernel(const float* part_o, const float* part_lse, const int32_t* table, bf16* hi, bf16* lo, int B,
+                       int H, int heads_per_cta, int ctas) {
   griddep_entry();
   constexpr int kRowThreads = R / 8;
   const int lane = threadIdx.x & 31;
-  const int64_t row = (int64_t)blockIdx.x * (128 / kRowThreads) + threadIdx.x / kRowThreads;  // b * H + h
-  if (row >= (int64_t)B * H) return;
+  const int64_t rows = (int64_t)B * H;
+  const int64_t row0 = ((int64_t)blockIdx.x * (128 / kRowThreads) + threadIdx.x / kRowThreads) * ROWS;  // b * H + h
   const int k = threadIdx.x % kRowThreads * 8;
-  const int b = (int)(row / H), h = (int)(row % H), ht = h / heads_per_cta;
-  const int quota = table[0], s0 = table[1 + b], s1 = table[2 + b];
-  const int c0 = s0 / quota, n = s1 > s0 ? (s1 - 1) / quota - c0 + 1 : 0;
-  const int64_t slot = ((int64_t)ht * (B + ctas) + b + c0) * heads_per_cta + h % heads_per_cta;
-  const float* src = part_o + slot * R + k;
   const int64_t step = (int64_t)heads_per_cta * R;
-  const float a0 = lane < n ? part_lse[slot + (int64_t)lane * heads_per_cta] : -INFINITY;
-  const float a1 = lane + 32 < n ? part_lse[slot + (int64_t)(lane + 32) * heads_per_cta] : -INFINITY;
-  float4 y[4][2];
+  const int quota = table[0];
+  int n[ROWS], most = 0;
+  const float* src[ROWS];
+  float e0[ROWS], e1[ROWS], inv[ROWS], x[ROWS][8] = {};
+  float4 y[ROWS][P][2];
   auto load = [&](int p0) {
 #pragma unroll
-    for (int p = 0; p < 4; ++p) {
-      if (p0 + p < n) {
-        const float4* at = reinterpret_cast<const float4*>(src + (p0 + p) * step);
-        y[p][0] = at[0];
-        y[p][1] = at[1];
-      } else {  // its weight is 0
-        y[p][0] = y[p][1] = make_float4(0.f, 0.f, 0.f, 0.f);
-      }
-    }
+    for (int i = 0; i < ROWS; ++i)
+#pragma unroll
+      for (int p = 0; p < P; ++p)
+        if (p0 + p < n[i]) {
+          const float4* at = reinterpret_cast<const float4*>(src[i] + (p0 + p) * step);
+          y[i][p][0] = at[0];
+          y[i][p][1] = at[1];
+        } else {  // its weight is 0
+          y[i][p][0] = y[i][p][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+        }
   };
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    n[i] = 0;
+    src[i] = part_o;
+    e0[i] = e1[i] = -INFINITY;
+    if (row0 + i < rows) {
+      const int b = (int)((row0 + i) / H), h = (int)((row0 + i) % H);
+      const int s0 = table[1 + b], s1 = table[2 + b], c0 = s0 / quota;
+      n[i] = s1 > s0 ? (s1 - 1) / quota - c0 + 1 : 0;
+      const int64_t slot = ((int64_t)(h / heads_per_cta) * (B + ctas) + b + c0) * heads_per_cta + h % heads_per_cta;
+      src[i] = part_o + slot * R + k;
+      if (lane < n[i]) e0[i] = part_lse[slot + (int64_t)lane * heads_per_cta];
+      if (lane + 32 < n[i]) e1[i] = part_lse[slot + (int64_t)(lane + 32) * heads_per_cta];
+    }
+    most = max(most, n[i]);
+  }
   load(0);  // under way with the weights
-  float M = warp_max(fmaxf(a0, a1));
-  if (M == -INFINITY) M = 0.f;  // no finite score in the row: weights 0 (or NaN, which reaches the row)
-  const float e0 = ex2(a0 - M), e1 = ex2(a1 - M);
-  const float L = warp_sum(e0 + e1);
-  float x[8] = {};
-  for (int p0 = 0; p0 < n; p0 += 4) {
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    float M = warp_max(fmaxf(e0[i], e1[i]));
+    if (M == -INFINITY) M = 0.f;  // no finite score in the row: weights 0 (or NaN, which reaches the row)
+    e0[i] = ex2(e0[i] - M), e1[i] = ex2(e1[i] - M);
+    const float L = warp_sum(e0[i] + e1[i]);
+    inv[i] = L == 0.f ? 0.f : 1.f / L;
+  }
+  for (int p0 = 0; p0 < most; p0 += P) {
     if (p0 > 0) load(p0);
 #pragma unroll
-    for (int p = 0; p < 4; ++p) {
-      const float f = __shfl_sync(0xffffffffu, p0 < 32 ? e0 : e1, (p0 + p) & 31);
-      x[0] += f * y[p][0].x, x[1] += f * y[p][0].y, x[2] += f * y[p][0].z, x[3] += f * y[p][0].w;
-      x[4] += f * y[p][1].x, x[5] += f * y[p][1].y, x[6] += f * y[p][1].z, x[7] += f * y[p][1].w;
-    }
-  }
-  const float inv = L == 0.f ? 0.f : 1.f / L;
-  uint32_t top[4], low[4];
+    for (int i = 0; i < ROWS; ++i)
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float u = x[2 * i] * inv, v = x[2 * i + 1] * inv;
-    top[i] = pack_bf16(u, v);
-    const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&top[i]));
-    low[i] = pack_bf16(u - f.x, v - f.y);
+      for (int p = 0; p < P; ++p) {
+        const float f = __shfl_sync(0xffffffffu, p0 < 32 ? e0[i] : e1[i], (p0 + p) & 31);
+        const float4 u = y[i][p][0], v = y[i][p][1];
+        x[i][0] += f * u.x, x[i][1] += f * u.y, x[i][2] += f * u.z, x[i][3] += f * u.w;
+        x[i][4] += f * v.x, x[i][5] += f * v.y, x[i][6] += f * v.z, x[i][7] += f * v.w;
+      }
   }
-  *reinterpret_cast<uint4*>(hi + row * R + k) = make_uint4(top[0], top[1], top[2], top[3]);
-  *reinterpret_cast<uint4*>(lo + row * R + k) = make_uint4(low[0], low[1], low[2], low[3]);
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    if (row0 + i >= rows) return;
+    uint32_t top[4], low[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float u = x[i][2 * j] * inv[i], v = x[i][2 * j + 1] * inv[i];
+      top[j] = pack_bf16(u, v);
+      const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&top[j]));
+      low[j] = pack_bf16(u - f.x, v - f.y);
+    }
+    *reinterpret_cast<uint4*>(hi + (row0 + i) * R + k) = make_uint4(top[0], top[1], top[2], top[3]);
+    *reinterpret_cast<uint4*>(lo + (row0 + i) * R + k) = make_uint4(low[0], low[1], low[2], low[3]);
+  }
 }
 
 // out[b, h, n] = sum_r (hi + lo)[b, h, r] w[h, 128 + n, r] for up to 16 rows: one CTA per (32 columns,
@@ -1115,9 +1138,9 @@ void run(const LatentDecode& a, cudaStream_t st) {
   }
   // qa has been read: the high halves take its place
   bf16* lo = reinterpret_cast<bf16*>(ws + l.low);
-  const int64_t rows = (int64_t)a.B * a.H, per = 1024 / R;
-  launch_k(latent_join_kernel<R>, dim3((unsigned)((rows + per - 1) / per)), 128, 0, st, part_o, part_lse, table, qa,
-           lo, a.B, a.H, p.heads_per_cta, p.ctas);
+  const int64_t rows = (int64_t)a.B * a.H, per = 1024 / R * (small ? 1 : 2);
+  launch_k(small ? latent_join_kernel<R, 8, 1> : latent_join_kernel<R, 2, 2>, dim3((unsigned)((rows + per - 1) / per)),
+           128, 0, st, part_o, part_lse, table, qa, lo, a.B, a.H, p.heads_per_cta, p.ctas);
   KAPSL_LAUNCH_CHECK();
   static std::atomic<uint64_t> devs{0}, devs_tc{0};
   if (small) {
