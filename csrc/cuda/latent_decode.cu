@@ -207,28 +207,46 @@ __device__ __forceinline__ void columns16(const float (&v)[V], int c, float (&ou
     out[n] = __shfl_sync(0xffffffffu, v[((c + n) >> 3) * 2 + (n & 1)], (n & 7) >> 1);
 }
 
-// A CTA's stretch of the line, piece by piece.
+// A CTA's stretch of the line, piece by piece.  The next sequence's place and length are loaded
+// while the present one is worked on.
 struct Pieces {
-  const int32_t* start;  // table + 1
-  int at, end, b;
-  __device__ Pieces(const int32_t* table, int B, int c) : start(table + 1) {
-    const int quota = table[0], all = table[1 + B];
-    at = min((int64_t)c * quota, (int64_t)all);
+  const int32_t *start, *ctx_lens;  // start = table + 1
+  int B, limit, at, end, b, s0, s1, s2, len, len1;
+  __device__ Pieces(const int32_t* table, const int32_t* lens, int B_, int limit_, int c)
+      : start(table + 1), ctx_lens(lens), B(B_), limit(limit_) {  // called by whole warps
+    const int quota = table[0], all = table[1 + B], lane = threadIdx.x & 31;
+    at = (int)min((int64_t)c * quota, (int64_t)all);
     end = min(at + quota, all);
-    int lo = 0, hi = B - 1;  // last sequence that starts at or before `at`
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) / 2;
-      if (start[mid] <= at) lo = mid;
-      else hi = mid - 1;
+    b = 0;  // last sequence that starts at or before `at`, 32 candidates at a time
+    for (int n = B; n > 1;) {
+      const int step = (n + 31) / 32, i = lane * step;
+      const bool le = i < n && start[b + i] <= at;
+      const int k = __popc(__ballot_sync(0xffffffffu, le)) - 1;
+      b += k * step;
+      n = min(step, n - k * step);
     }
-    b = lo;
+    s0 = start[b];
+    s1 = start[b + 1];
+    len = ctx_lens[b];
+    ahead();
+  }
+  __device__ void ahead() {
+    s2 = start[min(b + 2, B)];
+    len1 = ctx_lens[min(b + 1, B - 1)];
   }
   __device__ bool more() const { return at < end; }
-  __device__ int first() const { return at - start[b]; }             // tile within the sequence
-  __device__ int tiles() const { return min(end, start[b + 1]) - at; }
+  __device__ int first() const { return at - s0; }  // tile within the sequence
+  __device__ int tiles() const { return min(end, s1) - at; }
+  __device__ int keys() const { return min(len, limit); }
   __device__ void next() {
-    at = min(end, start[b + 1]);
-    while (at < end && start[b + 1] <= at) ++b;  // sequences without keys take no tiles
+    at = min(end, s1);
+    while (at < end && s1 <= at) {  // sequences without keys take no tiles
+      ++b;
+      s0 = s1;
+      s1 = s2;
+      len = len1;
+      ahead();
+    }
   }
 };
 
@@ -278,7 +296,7 @@ __global__ void __launch_bounds__(kAttnThreads<R>, 1)
   const uint32_t tmem = __shfl_sync(0xffffffffu, s.tmem_base, 0);
   const uint32_t tmem_o = tmem + 2 * NT;
   griddep_wait();
-  Pieces pc(table, B, c);  // without pieces, every role falls through its loop
+  Pieces pc(table, ctx_lens, B, max_blocks * page, c);  // without pieces, every role falls through its loop
 
   if (warp < S::kGroups) {
     // ------------------------------------------- TMA producer of dims [128 g, 128 g + 128)
@@ -288,18 +306,17 @@ __global__ void __launch_bounds__(kAttnThreads<R>, 1)
     int sent = 0, nq = 0;
     bool ok = true;
     // lane l < pages: first row of page l of a tile
-    auto page_row = [&](int b, int tile) {
+    auto page_row = [&](int tile) {
       const int j = tile * pages + lane;
-      const int nblk = (min(ctx_lens[b], max_blocks * page) + page - 1) / page;
-      if (lane >= pages || j >= nblk) return oob;
-      const int blk = block_tables[(int64_t)b * max_blocks + j];
+      if (lane >= pages || j >= (pc.keys() + page - 1) / page) return oob;
+      const int blk = block_tables[(int64_t)pc.b * max_blocks + j];
       if (blk >= 0 && blk < num_blocks) return blk * page;
       atomicCAS(err, 0, 82);
       return oob;
     };
     for (; ok && pc.more(); pc.next()) {
       const int b = pc.b, t0 = pc.first(), n = pc.tiles();
-      int y = page_row(b, t0), y1 = n > 1 ? page_row(b, t0 + 1) : oob;
+      int y = page_row(t0), y1 = n > 1 ? page_row(t0 + 1) : oob;
       if (g == 0) {
         if (nq > 0) ok = wait_or_abort(s, &s.q_empty, (nq - 1) & 1, err, 84);
         if (!__all_sync(0xffffffffu, ok)) break;
@@ -313,7 +330,7 @@ __global__ void __launch_bounds__(kAttnThreads<R>, 1)
       }
       for (int i = 0; i < n; ++i, ++sent) {
         const int st = sent % S::kStages;
-        const int y2 = i + 2 < n ? page_row(b, t0 + i + 2) : oob;
+        const int y2 = i + 2 < n ? page_row(t0 + i + 2) : oob;
         int yy[4], zz[4];
 #pragma unroll
         for (int pg = 0; pg < 4; ++pg) {
@@ -467,7 +484,7 @@ __global__ void __launch_bounds__(kAttnThreads<R>, 1)
     int tile = 0;  // of the CTA
     for (; pc.more(); pc.next()) {
       const int b = pc.b, n_tiles = pc.tiles();
-      const int left = min(ctx_lens[b], max_blocks * page) - pc.first() * kKeys;  // keys from the piece's first on
+      const int left = pc.keys() - pc.first() * kKeys;  // keys from the piece's first on
       float m_ref[V], l[V];
 #pragma unroll
       for (int n = 0; n < V; ++n) m_ref[n] = 0.f, l[n] = 0.f;
@@ -597,20 +614,24 @@ __global__ void __launch_bounds__(kAttnThreads<R>, 1)
         if (sw == 0 && lane < 4 && col < nheads) part_lse[slot + col] = sum == 0.f ? -INFINITY : m_ref[n] + log2f(sum);
       }
       soft_barrier();  // the sums have been read: the next piece may write here
+      constexpr int NC = NT < 32 ? NT : 32;  // heads at a time
 #pragma unroll
-      for (int col = 0; col < NT; col += 16) {
-        if (col >= nheads) break;
-        float f[16];
-        columns16(l, col, f);
-#pragma unroll 1
+      for (int col = 0; col < NT; col += NC) {
+        float f[NC];
+#pragma unroll
+        for (int n = 0; n < NC; ++n)
+          f[n] = __shfl_sync(0xffffffffu, l[((col + n) >> 3) * 2 + (n & 1)], (n & 7) >> 1);
+        uint32_t o[2][NC];
+        tmem_ld_start(tmem_o + lane_off + col, o[0]);
+#pragma unroll
         for (int m = 0; m < S::kGroups; ++m) {
-          float o[16];
-          tmem_ld16(tmem_o + lane_off + m * NT + col, o);
+          tmem_ld_wait(o[m & 1]);
+          if (m + 1 < S::kGroups) tmem_ld_start(tmem_o + lane_off + (m + 1) * NT + col, o[(m + 1) & 1]);
           // a warp writes 32 consecutive dims of one head at a time
           float* dst = part_o + (slot + col) * R + m * 128 + quad * 32 + lane;
 #pragma unroll
-          for (int n = 0; n < 16; ++n)
-            if (col + n < nheads) dst[n * R] = o[n] * f[n];
+          for (int n = 0; n < NC; ++n)
+            if (col + n < nheads) dst[n * R] = __uint_as_float(o[m & 1][n]) * f[n];
         }
       }
       tc_fence_before();  // O^T has been read: ordered before the next p_full

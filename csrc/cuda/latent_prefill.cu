@@ -377,11 +377,11 @@ __device__ __forceinline__ float row_pass(uint32_t s_tmem, float scale_log2, flo
   float top = -INFINITY;
   uint64_t acc = pair(0.f, 0.f);
   uint32_t v[2][32];
-  tmem_ld32_start(s_tmem, v[0]);
+  tmem_ld_start(s_tmem, v[0]);
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
     tmem_ld_wait(v[c & 1]);
-    if (c < 3) tmem_ld32_start(s_tmem + (c + 1) * 32, v[(c + 1) & 1]);
+    if (c < 3) tmem_ld_start(s_tmem + (c + 1) * 32, v[(c + 1) & 1]);
 #pragma unroll
     for (int i = 0; i < 32; i += 2) {
       float x0, x1;
