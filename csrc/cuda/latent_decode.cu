@@ -126,7 +126,8 @@ struct DecodeSmem {
   alignas(1024) uint8_t k[S::kStages][S::kTileBytes];
   alignas(1024) uint8_t q[S::kQBytes];
   alignas(1024) uint8_t p[S::kP];
-  float red[kSoft][NT];  // per warp column maxima, or sums
+  float red[kSoft][NT];      // per warp column maxima, or sums
+  float mcol[NT], fac[NT];   // the columns' running maxima; factors on O^T
   uint64_t q_full, q_empty, kv_full[S::kStages][S::kGroups], kv_empty[S::kStages][S::kGroups], s_full[2], s_free[2],
       p_full, pv_done, drained;
   uint32_t tmem_base;
@@ -197,15 +198,6 @@ __device__ __forceinline__ int reduce_columns(float (&v)[V], F f) {
 
 // column of a thread's n-th column value (pairs of adjacent columns, 8 apart)
 __device__ __forceinline__ int frag_col(int n) { return (n >> 1) * 8 + (threadIdx.x & 3) * 2 + (n & 1); }
-
-// The values of columns c .. c + 15 in every lane, from the lanes that hold them (v indexed as
-// frag_col).
-template <int V>
-__device__ __forceinline__ void columns16(const float (&v)[V], int c, float (&out)[16]) {
-#pragma unroll
-  for (int n = 0; n < 16; ++n)
-    out[n] = __shfl_sync(0xffffffffu, v[((c + n) >> 3) * 2 + (n & 1)], (n & 7) >> 1);
-}
 
 // A CTA's stretch of the line, piece by piece.  The next sequence's place and length are loaded
 // while the present one is worked on.
@@ -476,7 +468,7 @@ __global__ void __launch_bounds__(kAttnThreads<R>, 1)
   } else {
     // ------------------------------------------------------- softmax, epilogue
     const int quad = warp & 3;  // TMEM lane quadrant
-    const int sw = warp - kMma - 1;
+    const int sw = warp - kMma - 1, tid = sw * 32 + lane;
     constexpr int V = NT / 4;  // columns a thread holds
     constexpr int VF = V >= 8 ? V / 8 : 1;
     const int row = quad * 16 + (lane >> 2);  // keys row and row + 8 of the tile
@@ -534,32 +526,31 @@ __global__ void __launch_bounds__(kAttnThreads<R>, 1)
 #pragma unroll
           for (int n = 0; n < VF; ++n) s.red[sw][frag_col(first + n)] = mx[n];
           soft_barrier();
-          float f[V];
+          if (tid < NT) {  // one thread a column
+            float mn = fmaxf(fmaxf(s.red[0][tid], s.red[1][tid]), fmaxf(s.red[2][tid], s.red[3][tid]));
+            const float old = i == 0 ? 0.f : s.mcol[tid];
+            mn = i == 0 ? (mn == -INFINITY ? 0.f : mn) : fmaxf(mn, old);  // no finite score yet: any reference
+            s.mcol[tid] = mn;
+            s.fac[tid] = ex2(old - mn);
+          }
+          soft_barrier();
 #pragma unroll
           for (int n = 0; n < V; ++n) {
-            const int col = frag_col(n);
-            float mn = fmaxf(fmaxf(s.red[0][col], s.red[1][col]), fmaxf(s.red[2][col], s.red[3][col]));
-            mn = i == 0 ? (mn == -INFINITY ? 0.f : mn) : fmaxf(mn, m_ref[n]);  // no finite score yet: any reference
-            f[n] = ex2(m_ref[n] - mn);
-            m_ref[n] = mn;
-            l[n] *= f[n];
+            m_ref[n] = s.mcol[frag_col(n)];
+            l[n] *= s.fac[frag_col(n)];
           }
           if (i > 0) {
             tc_fence_after();
-#pragma unroll
-            for (int col = 0; col < NT; col += 16) {
-              float fc[16];
-              columns16(f, col, fc);
 #pragma unroll 1
-              for (int m = 0; m < S::kGroups; ++m) {
-                float o[16];
-                uint32_t u[16];
-                const uint32_t at = tmem_o + lane_off + m * NT + col;
-                tmem_ld16(at, o);
+            for (int k = 0; k < S::kGroups * (NT / 16); ++k) {  // 16 columns of 128 dims at a time
+              const int col = k % (NT / 16) * 16;
+              const uint32_t at = tmem_o + lane_off + k / (NT / 16) * NT + col;
+              float o[16];
+              uint32_t u[16];
+              tmem_ld16(at, o);
 #pragma unroll
-                for (int n = 0; n < 16; ++n) u[n] = __float_as_uint(o[n] * fc[n]);
-                tmem_st16(at, u);
-              }
+              for (int n = 0; n < 16; ++n) u[n] = __float_as_uint(o[n] * s.fac[col + n]);
+              tmem_st16(at, u);
             }
             tmem_wait_st();
           }
@@ -581,8 +572,8 @@ __global__ void __launch_bounds__(kAttnThreads<R>, 1)
           const int st = tile % S::kStages;
           for (int g = 0; g < S::kGroups; ++g)
             wait_or_abort(s, &s.kv_full[st][g], (tile / S::kStages) & 1, err, 88);
-          const int t = sw * 32 + lane, per_row = R / 8;  // 16-byte vectors of a row's latent
-          for (int e = t; e < (kKeys - valid) * per_row; e += kSoft * 32) {
+          const int per_row = R / 8;  // 16-byte vectors of a row's latent
+          for (int e = tid; e < (kKeys - valid) * per_row; e += kSoft * 32) {
             const int r = valid + e / per_row, x = e % per_row;
             *reinterpret_cast<uint4*>(s.k[st] + (x >> 3) * S::kChunkBytes + r * 128 + (x & 7) * 16) = make_uint4(0, 0, 0, 0);
           }
@@ -606,33 +597,22 @@ __global__ void __launch_bounds__(kAttnThreads<R>, 1)
         for (int n = 0; n < VF; ++n) s.red[sw][frag_col(first + n)] = part[n];
       }
       soft_barrier();
-#pragma unroll
-      for (int n = 0; n < V; ++n) {
-        const int col = frag_col(n);
-        const float sum = s.red[0][col] + s.red[1][col] + s.red[2][col] + s.red[3][col];
-        l[n] = sum == 0.f ? 0.f : 1.f / sum;
-        if (sw == 0 && lane < 4 && col < nheads) part_lse[slot + col] = sum == 0.f ? -INFINITY : m_ref[n] + log2f(sum);
+      if (tid < NT) {
+        const float sum = s.red[0][tid] + s.red[1][tid] + s.red[2][tid] + s.red[3][tid];
+        s.fac[tid] = sum == 0.f ? 0.f : __fdividef(1.f, sum);
+        if (tid < nheads) part_lse[slot + tid] = sum == 0.f ? -INFINITY : s.mcol[tid] + __log2f(sum);
       }
-      soft_barrier();  // the sums have been read: the next piece may write here
-      constexpr int NC = NT < 32 ? NT : 32;  // heads at a time
+      soft_barrier();
+#pragma unroll 1
+      for (int k = 0; k < S::kGroups * (NT / 16); ++k) {
+        const int col = k % (NT / 16) * 16, m = k / (NT / 16);
+        float o[16];
+        tmem_ld16(tmem_o + lane_off + m * NT + col, o);
+        // a warp writes 32 consecutive dims of one head at a time
+        float* dst = part_o + (slot + col) * R + m * 128 + quad * 32 + lane;
 #pragma unroll
-      for (int col = 0; col < NT; col += NC) {
-        float f[NC];
-#pragma unroll
-        for (int n = 0; n < NC; ++n)
-          f[n] = __shfl_sync(0xffffffffu, l[((col + n) >> 3) * 2 + (n & 1)], (n & 7) >> 1);
-        uint32_t o[2][NC];
-        tmem_ld_start(tmem_o + lane_off + col, o[0]);
-#pragma unroll
-        for (int m = 0; m < S::kGroups; ++m) {
-          tmem_ld_wait(o[m & 1]);
-          if (m + 1 < S::kGroups) tmem_ld_start(tmem_o + lane_off + (m + 1) * NT + col, o[(m + 1) & 1]);
-          // a warp writes 32 consecutive dims of one head at a time
-          float* dst = part_o + (slot + col) * R + m * 128 + quad * 32 + lane;
-#pragma unroll
-          for (int n = 0; n < NC; ++n)
-            if (col + n < nheads) dst[n * R] = __uint_as_float(o[m & 1][n]) * f[n];
-        }
+        for (int n = 0; n < 16; ++n)
+          if (col + n < nheads) dst[n * R] = o[n] * s.fac[col + n];
       }
       tc_fence_before();  // O^T has been read: ordered before the next p_full
     }
