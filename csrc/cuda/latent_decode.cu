@@ -414,7 +414,7 @@ __global__ void __launch_bounds__(kAttnThreads<R>, 1)
           }
           moved = true;
         }
-        if (sc < total) {
+        if (sc < total && sc < pv + 2) {  // two score tiles ahead, only the second product can go on
           if (!q_open) q_open = mbar_test_wait(&s.q_full, nq & 1);
           if (!s_open) s_open = mbar_test_wait(&s.s_free[sc & 1], ((sc >> 1) - 1) & 1);
           const int st = sc % S::kStages;
