@@ -65,61 +65,57 @@ __device__ __forceinline__ void load_cs(const float* p, float (&o)[N]) {
   }
 }
 
-// Rotates one unit of a head: N elements at a (interleaved: N/2 pairs), or N pairs
-// (a[k], b[k]) in the half layout.  `i` is the unit's first angle index.
-template <class T, int N, bool IL>
-__device__ __forceinline__ void rotate_unit(const float* cs, int half, int i, Vec<T, N>& a, Vec<T, N>& b) {
-  if constexpr (IL) {
-    float c[N / 2], s[N / 2];
-    load_cs<N / 2>(cs + i, c);
-    load_cs<N / 2>(cs + half + i, s);
+// The angles of one unit of a head: N elements (interleaved: N/2 pairs), or N pairs (a[k], b[k])
+// in the half layout; `i` is the unit's first angle index.
+template <int N, bool IL>
+struct Angles {
+  static constexpr int M = IL ? N / 2 : N;
+  float c[M], s[M];
+  __device__ __forceinline__ Angles(const float* cs, int half, int i) {
+    load_cs<M>(cs + i, c);
+    load_cs<M>(cs + half + i, s);
+  }
+  template <class T>
+  __device__ __forceinline__ void rotate(Vec<T, N>& a, Vec<T, N>& b) const {
 #pragma unroll
-    for (int k = 0; k < N / 2; ++k) {
-      const float x = to_f(a.v[2 * k]), y = to_f(a.v[2 * k + 1]);
-      a.v[2 * k] = from_f<T>(x * c[k] - y * s[k]);
-      a.v[2 * k + 1] = from_f<T>(y * c[k] + x * s[k]);
-    }
-  } else {
-    float c[N], s[N];
-    load_cs<N>(cs + i, c);
-    load_cs<N>(cs + half + i, s);
-#pragma unroll
-    for (int k = 0; k < N; ++k) {
-      const float x = to_f(a.v[k]), y = to_f(b.v[k]);
-      a.v[k] = from_f<T>(x * c[k] - y * s[k]);
-      b.v[k] = from_f<T>(y * c[k] + x * s[k]);
+    for (int k = 0; k < M; ++k) {
+      T& p = IL ? a.v[2 * k] : a.v[k];
+      T& q = IL ? a.v[(2 * k + 1) % N] : b.v[k % N];
+      const float x = to_f(p), y = to_f(q);
+      p = from_f<T>(x * c[k] - y * s[k]);
+      q = from_f<T>(y * c[k] + x * s[k]);
     }
   }
-}
+};
 
 // One thread column (threadIdx.x) per unit of a head, one thread row per (token, head)
-// row, kRopeRows rows a thread so that several independent 16-byte loads are in
+// row, several rows a thread so that several independent 16-byte loads are in
 // flight.  Units [0, nrot) rotate, the rest (out of place only) copy elements of the
 // dims outside the rotated part (one element on the narrow path).
-constexpr int kRopeRows = 4;
+template <class T, bool IL>
+constexpr int kRopeRows = sizeof(T) == 2 && !IL ? 2 : 4;
 
 template <class T, int N, bool IL>
-__global__ void __launch_bounds__(256) rope_kernel(const T* x, int64_t xs_t, int64_t xs_h, T* y, int64_t ys_t,
-                                                   int64_t ys_h, const int32_t* positions,
-                                                   const float* __restrict__ cos_sin, int max_pos, int64_t rows,
-                                                   int H, int D, int P, int offset, bool in_place,
-                                                   int* err) {
-  griddep_entry();
+__device__ __forceinline__ void rope_rows(int64_t block, const T* x, int64_t xs_t, int64_t xs_h, T* y, int64_t ys_t,
+                                          int64_t ys_h, const int32_t* positions, const float* __restrict__ cos_sin,
+                                          int max_pos, int64_t rows, int H, int D, int P, int offset, bool in_place,
+                                          int* err) {
+  constexpr int kRows = kRopeRows<T, IL>;
   const int half = P >> 1;
   const int nrot = IL ? P / N : half / N;
   constexpr int NC = sizeof(T) * N == 16 ? N : 1;  // elements a copying unit moves
   const int nunit = nrot + (in_place ? 0 : (D - P) / NC);
-  const int64_t r0 = (int64_t)blockIdx.x * blockDim.y * kRopeRows + threadIdx.y;
+  const int64_t r0 = block * blockDim.y * kRows + threadIdx.y;
   for (int u = threadIdx.x; u < nunit; u += blockDim.x) {
     const bool rot = u < nrot;
     // element offsets inside the head
     const int c = (u - nrot) * NC;
     const int e0 = rot ? offset + u * N : (c < offset ? c : c + P);
-    Vec<T, N> a[kRopeRows], b[kRopeRows];
-    int pos[kRopeRows];
-    T* dst[kRopeRows];
+    Vec<T, N> a[kRows], b[kRows];
+    int pos[kRows];
+    T* dst[kRows];
 #pragma unroll
-    for (int k = 0; k < kRopeRows; ++k) {
+    for (int k = 0; k < kRows; ++k) {
       const int64_t r = r0 + (int64_t)k * blockDim.y;
       dst[k] = nullptr;
       if (r < rows) {
@@ -137,11 +133,11 @@ __global__ void __launch_bounds__(256) rope_kernel(const T* x, int64_t xs_t, int
       }
     }
 #pragma unroll
-    for (int k = 0; k < kRopeRows; ++k) {
+    for (int k = 0; k < kRows; ++k) {
       if (dst[k] == nullptr) continue;
       if (rot) {
         if (pos[k] >= 0 && pos[k] < max_pos) {
-          rotate_unit<T, N, IL>(cos_sin + (int64_t)pos[k] * P, half, IL ? u * N / 2 : u * N, a[k], b[k]);
+          Angles<N, IL>(cos_sin + (int64_t)pos[k] * P, half, IL ? u * N / 2 : u * N).rotate(a[k], b[k]);
         } else {
           atomicCAS(err, 0, 80);  // no such table row: the head keeps its values
         }
@@ -157,6 +153,16 @@ __global__ void __launch_bounds__(256) rope_kernel(const T* x, int64_t xs_t, int
 }
 
 template <class T, int N, bool IL>
+__global__ void __launch_bounds__(256) rope_kernel(const T* x, int64_t xs_t, int64_t xs_h, T* y, int64_t ys_t,
+                                                   int64_t ys_h, const int32_t* positions,
+                                                   const float* __restrict__ cos_sin, int max_pos, int64_t rows, int H,
+                                                   int D, int P, int offset, bool in_place, int* err) {
+  griddep_entry();
+  rope_rows<T, N, IL>(blockIdx.x, x, xs_t, xs_h, y, ys_t, ys_h, positions, cos_sin, max_pos, rows, H, D, P, offset,
+                      in_place, err);
+}
+
+template <class T, int N, bool IL>
 void rope_launch(const RopeArgs& a, cudaStream_t st) {
   const int nrot = IL ? a.P / N : a.P / 2 / N;
   constexpr int NC = sizeof(T) * N == 16 ? N : 1;
@@ -164,7 +170,7 @@ void rope_launch(const RopeArgs& a, cudaStream_t st) {
   const int bx = std::min(nunit, 256);
   const int by = std::max(1, 256 / bx);
   const int64_t rows = a.T * a.H;
-  const int64_t grid = (rows + (int64_t)by * kRopeRows - 1) / ((int64_t)by * kRopeRows);
+  const int64_t grid = (rows + (int64_t)by * kRopeRows<T, IL> - 1) / ((int64_t)by * kRopeRows<T, IL>);
   if (grid > 0x7fffffff) throw std::runtime_error("rope: too many rows");
   launch_k(rope_kernel<T, N, IL>, dim3((unsigned)grid), dim3(bx, by), 0, st, static_cast<const T*>(a.x), a.xs_t,
            a.xs_h, static_cast<T*>(a.y), a.ys_t, a.ys_h, a.positions, a.cos_sin, a.max_pos, rows, a.H, a.D, a.P,
@@ -193,68 +199,84 @@ void rope_dispatch(const RopeArgs& a, cudaStream_t st) {
 }
 
 // ------------------------------------------------------- latent cache write
-// One CTA per token.  Warp 0 normalises the latent (R / 256 16-byte vectors a lane,
-// sum of squares by shuffles: no block barrier) and rotates the shared key; all warps
-// rotate the query heads.
+// The first blocks take a token a warp: the latent is normalised (R / 256 16-byte vectors a
+// lane, sum of squares by shuffles) and the shared key rotated.  The others take a token each
+// and rotate its query heads: a thread keeps the angles of its unit for all its heads, two
+// heads' loads in flight.  8191 tokens x 128 heads, out of place: 67 us, 4.3 TB/s of the bytes it
+// needs (of q that is every third 128 bytes); one block a token for both parts took 67 us too,
+// and rope_kernel's row order, which loads the angles again for every head, 70-87 us.
 template <int R, bool IL>
 __global__ void __launch_bounds__(256) rope_latent_write_kernel(
-    const bf16* q, int64_t qs_t, int64_t qs_h, bf16* qo, int64_t qo_t, int64_t qo_h, const bf16* kv,
-    int64_t kv_stride, const int32_t* positions, const int64_t* slots,
-    const float* __restrict__ cos_sin, int max_pos, const bf16* __restrict__ w, float eps, bf16* cache,
-    int64_t num_slots, int H, int* err) {
+    const bf16* q, int64_t qs_t, int64_t qs_h, bf16* qo, int64_t qo_t, int64_t qo_h, const bf16* kv, int64_t kv_stride,
+    const int32_t* positions, const int64_t* slots, const float* __restrict__ cos_sin, int max_pos,
+    const bf16* __restrict__ w, float eps, bf16* cache, int64_t num_slots, int T, int H, int latent_blocks, int* err) {
   griddep_entry();
   constexpr int P = 64, N = 8, half = P / 2;
   constexpr int NU = IL ? P / N : half / N;  // rotating units a head
-  const int t = blockIdx.x;
-  const int pos = positions[t];
-  const bool ok = pos >= 0 && pos < max_pos;
-  const float* cs = cos_sin + (int64_t)(ok ? pos : 0) * P;
-  if (threadIdx.x < 32) {
-    const int lane = threadIdx.x;
-    const int64_t slot = slots[t];
-    if (!ok && lane == 0) atomicCAS(err, 0, 80);
-    if (slot >= num_slots && lane == 0) atomicCAS(err, 0, 81);
-    if (slot >= 0 && slot < num_slots) {
-      const bf16* src = kv + (int64_t)t * kv_stride;
-      bf16* dst = cache + slot * (R + P);
-      Vec<bf16, N> v[R / 256];
-      Vec<bf16, N> a, b;
+  if (blockIdx.x >= latent_blocks) {
+    const int t = blockIdx.x - latent_blocks, u = threadIdx.x % NU, step = blockDim.x / NU;
+    const int pos = positions[t];
+    const bool ok = pos >= 0 && pos < max_pos;
+    const bf16* src = q + t * qs_t + (int64_t)u * N;
+    bf16* dst = qo + t * qo_t + (int64_t)u * N;
+    const Angles<N, IL> angles(cos_sin + (int64_t)(ok ? pos : 0) * P, half, IL ? u * N / 2 : u * N);
+    for (int h = threadIdx.x / NU; h < H; h += 2 * step) {
+      Vec<bf16, N> a[2], b[2];
 #pragma unroll
-      for (int i = 0; i < R / 256; ++i) v[i] = *reinterpret_cast<const Vec<bf16, N>*>(src + (i * 32 + lane) * N);
-      if (lane < NU) {
-        a = *reinterpret_cast<const Vec<bf16, N>*>(src + R + lane * N);
-        if (!IL) b = *reinterpret_cast<const Vec<bf16, N>*>(src + R + half + lane * N);
+      for (int k = 0; k < 2; ++k) {
+        if (h + k * step < H) {
+          const bf16* at = src + (h + k * step) * qs_h;
+          a[k] = *reinterpret_cast<const Vec<bf16, N>*>(at);
+          if (!IL) b[k] = *reinterpret_cast<const Vec<bf16, N>*>(at + half);
+        }
       }
-      float ss = 0.f;
 #pragma unroll
-      for (int i = 0; i < R / 256; ++i)
-#pragma unroll
-        for (int k = 0; k < N; ++k) ss += to_f(v[i].v[k]) * to_f(v[i].v[k]);
-      const float inv = rsqrtf(warp_sum(ss) / (float)R + eps);
-#pragma unroll
-      for (int i = 0; i < R / 256; ++i) {
-        const Vec<bf16, N> ww = *reinterpret_cast<const Vec<bf16, N>*>(w + (i * 32 + lane) * N);
-#pragma unroll
-        for (int k = 0; k < N; ++k) v[i].v[k] = from_f<bf16>(to_f(v[i].v[k]) * inv * to_f(ww.v[k]));
-        *reinterpret_cast<Vec<bf16, N>*>(dst + (i * 32 + lane) * N) = v[i];
-      }
-      if (lane < NU) {
-        if (ok) rotate_unit<bf16, N, IL>(cs, half, IL ? lane * N / 2 : lane * N, a, b);
-        *reinterpret_cast<Vec<bf16, N>*>(dst + R + lane * N) = a;
-        if (!IL) *reinterpret_cast<Vec<bf16, N>*>(dst + R + half + lane * N) = b;
+      for (int k = 0; k < 2; ++k) {
+        if (h + k * step < H) {
+          bf16* at = dst + (h + k * step) * qo_h;
+          if (ok) angles.rotate(a[k], b[k]);
+          *reinterpret_cast<Vec<bf16, N>*>(at) = a[k];
+          if (!IL) *reinterpret_cast<Vec<bf16, N>*>(at + half) = b[k];
+        }
       }
     }
+    return;
   }
-  const bf16* qr = q + t * qs_t;
-  bf16* qd = qo + t * qo_t;
-  for (int i = threadIdx.x; i < H * NU; i += blockDim.x) {
-    const int h = i / NU, u = i % NU;
-    Vec<bf16, N> a, b;
-    a = *reinterpret_cast<const Vec<bf16, N>*>(qr + h * qs_h + u * N);
-    if (!IL) b = *reinterpret_cast<const Vec<bf16, N>*>(qr + h * qs_h + half + u * N);
-    if (ok) rotate_unit<bf16, N, IL>(cs, half, IL ? u * N / 2 : u * N, a, b);
-    *reinterpret_cast<Vec<bf16, N>*>(qd + h * qo_h + u * N) = a;
-    if (!IL) *reinterpret_cast<Vec<bf16, N>*>(qd + h * qo_h + half + u * N) = b;
+  const int lane = threadIdx.x & 31, t = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  if (t >= T) return;
+  const int pos = positions[t];
+  const int64_t slot = slots[t];
+  const bool ok = pos >= 0 && pos < max_pos;
+  if (!ok && lane == 0) atomicCAS(err, 0, 80);
+  if (slot >= num_slots && lane == 0) atomicCAS(err, 0, 81);
+  if (slot < 0 || slot >= num_slots) return;
+  const bf16* src = kv + (int64_t)t * kv_stride;
+  bf16* dst = cache + slot * (R + P);
+  Vec<bf16, N> v[R / 256];
+  Vec<bf16, N> a, b;
+#pragma unroll
+  for (int i = 0; i < R / 256; ++i) v[i] = *reinterpret_cast<const Vec<bf16, N>*>(src + (i * 32 + lane) * N);
+  if (lane < NU) {
+    a = *reinterpret_cast<const Vec<bf16, N>*>(src + R + lane * N);
+    if (!IL) b = *reinterpret_cast<const Vec<bf16, N>*>(src + R + half + lane * N);
+  }
+  float ss = 0.f;
+#pragma unroll
+  for (int i = 0; i < R / 256; ++i)
+#pragma unroll
+    for (int k = 0; k < N; ++k) ss += to_f(v[i].v[k]) * to_f(v[i].v[k]);
+  const float inv = rsqrtf(warp_sum(ss) / (float)R + eps);
+#pragma unroll
+  for (int i = 0; i < R / 256; ++i) {
+    const Vec<bf16, N> ww = *reinterpret_cast<const Vec<bf16, N>*>(w + (i * 32 + lane) * N);
+#pragma unroll
+    for (int k = 0; k < N; ++k) v[i].v[k] = from_f<bf16>(to_f(v[i].v[k]) * inv * to_f(ww.v[k]));
+    *reinterpret_cast<Vec<bf16, N>*>(dst + (i * 32 + lane) * N) = v[i];
+  }
+  if (lane < NU) {
+    if (ok) Angles<N, IL>(cos_sin + (int64_t)pos * P, half, IL ? lane * N / 2 : lane * N).rotate(a, b);
+    *reinterpret_cast<Vec<bf16, N>*>(dst + R + lane * N) = a;
+    if (!IL) *reinterpret_cast<Vec<bf16, N>*>(dst + R + half + lane * N) = b;
   }
 }
 
@@ -274,10 +296,15 @@ void launch_rope(const RopeArgs& a, int dtype, cudaStream_t st) {
 void launch_rope_latent_write(const RopeArgs& a, const bf16* kv, int64_t kv_stride, const int64_t* slots,
                               const bf16* w, float eps, bf16* cache, int64_t num_slots, int R, cudaStream_t st) {
   if (a.T == 0) return;
+  const int units = a.H * (a.interleaved ? 8 : 4);  // of 16 bytes (half layout: a pair of them) a token
+  const int threads = std::min(256, std::max(32, (units + 31) / 32 * 32));
+  const int latent_blocks = (int)((a.T * 32 + threads - 1) / threads);
+  const int64_t q_blocks = a.H > 0 ? a.T : 0;
+  if (latent_blocks + q_blocks > 0x7fffffff) throw std::runtime_error("rope_latent_write: too many rows");
   auto go = [&](auto kern) {
-    launch_k(kern, dim3((unsigned)a.T), dim3(256), 0, st, static_cast<const bf16*>(a.x), a.xs_t, a.xs_h,
-             static_cast<bf16*>(a.y), a.ys_t, a.ys_h, kv, kv_stride, a.positions, slots, a.cos_sin, a.max_pos, w, eps,
-             cache, num_slots, a.H, a.err);
+    launch_k(kern, dim3((unsigned)(latent_blocks + q_blocks)), dim3(threads), 0, st,
+             static_cast<const bf16*>(a.x), a.xs_t, a.xs_h, static_cast<bf16*>(a.y), a.ys_t, a.ys_h, kv, kv_stride,
+             a.positions, slots, a.cos_sin, a.max_pos, w, eps, cache, num_slots, (int)a.T, a.H, latent_blocks, a.err);
   };
   if (R == 512) {
     a.interleaved ? go(rope_latent_write_kernel<512, true>) : go(rope_latent_write_kernel<512, false>);
