@@ -321,6 +321,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kExpandThreads, 1)
 // S_t(j + 1) is issued after PV_t(j) by the same thread, so once its scores are complete O_t is at
 // rest: the softmax warps themselves rescale it, and only when a score exceeds the running
 // maximum by 8 (in log2; p <= 256 loses nothing in bf16 or fp32).
+// A CTA with 128 rows or fewer gives its two halves the even and the odd key tiles of the same
+// rows instead (and the second half's m, l and O join the first's at the end): the chain of
+// scores, softmax and product that bounds a lone row tile is half as long.
+//
 // Keys past a row's position have p = 0.  PV stops at the row tile's last key, rounded up
 // to 16; the rows there are the gather's zeros, so nothing behind a sequence is read.
 constexpr int kThreads = 384;  // warp 0 TMA, warp 1 MMA, warps 4-7 and 8-11 softmax of row tile 0 and 1
@@ -415,9 +419,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int32_t* si = seq_info + 5 * work[2 * blockIdx.x];
   const int t0 = work[2 * blockIdx.x + 1];
   const int row0 = si[0] + t0, n = si[1] - t0, pos0 = si[2] - si[1] + t0, kv0 = si[4];  // n: rows from t0 on
-  // keys and key tiles of the two row tiles
-  const int keys0 = pos0 + min(n, 128), keys1 = n > 128 ? pos0 + min(n, 256) : 0;
-  const int nt0 = (keys0 + 127) / 128, nt1 = (keys1 + 127) / 128, nt = max(nt0, nt1);
+  // keys of the two halves, key tiles of the CTA and of each half
+  const bool split = n <= 128;
+  const int keys0 = pos0 + min(n, 128), keys1 = split ? keys0 : pos0 + min(n, 256);
+  const int nt = (keys1 + 127) / 128;
+  const int nt0 = split ? (nt + 1) / 2 : (keys0 + 127) / 128, nt1 = split ? nt / 2 : nt;
   if ((smem_u32(smem_raw) & 1023) || row0 < 0 || row0 + min(n, 256) > q_rows || n <= 0) {
     if (threadIdx.x == 0) atomicCAS(err, 0, 90);
     return;
@@ -446,14 +452,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer
     if (elect_one()) {
-      const int tiles_q = nt1 > 0 ? 2 : 1;
+      const int tiles_q = split ? 1 : 2;
       mbar_arrive_expect_tx(&s.q_full, tiles_q * 3 * kSlotBytes);
       for (int t = 0; t < tiles_q; ++t)
         for (int c = 0; c < 3; ++c) tma_load_2d(s.q[t][c], &q_map, &s.q_full, h * 192 + c * 64, row0 + t * 128);
       // Slots of tile j: keys 5j .. 5j + 2, values 5j + 3, 5j + 4 (mod 8).  Those of K_j were
-      // last used by K_{j-2} and V_{j-2}, those of V_j by K_{j-1}, which is free once the last row
-      // tile's scores of tile j - 1 are complete.
-      const int last = tiles_q - 1;
+      // last used by K_{j-2} and V_{j-2}, those of V_j by K_{j-1}, which is free once the last
+      // scores of tile j - 1 are complete.
       bool ok = true;
       int j = 0;
       for (; j < nt; ++j) {
@@ -463,7 +468,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         tma_load_2d(s.ring[(5 * j) % kSlots], &kv_map, bar, h * 256, kv0 + j * 128);
         tma_load_2d(s.ring[(5 * j + 1) % kSlots], &kv_map, bar, h * 256 + 64, kv0 + j * 128);
         tma_load_2d(s.ring[(5 * j + 2) % kSlots], &rope_map, bar, 0, kv0 + j * 128);
-        if (j >= 1 && !wait_or_abort(s, &s.s_full[last], (j - 1) & 1, err, 91)) { ok = false; break; }
+        const int h_last = split ? (j - 1) & 1 : 1, phase = split ? (j - 1) >> 1 : j - 1;
+        if (j >= 1 && !wait_or_abort(s, &s.s_full[h_last], phase & 1, err, 91)) { ok = false; break; }
         bar = &s.v_full[j & 1];
         mbar_arrive_expect_tx(bar, 2 * kSlotBytes);
         tma_load_2d(s.ring[(5 * j + 3) % kSlots], &kv_map, bar, h * 256 + 128, kv0 + j * 128);
@@ -486,21 +492,22 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint64_t q_desc = smem_desc_sw128(smem_u32(s.q[0][0])), k_desc = smem_desc_sw128(smem_u32(s.ring[0]));
       const uint64_t v_desc = smem_desc_mn_sw128(smem_u32(s.ring[0]), kSlotBytes, 1024);
       bool ok = wait_or_abort(s, &s.q_full, 0, err, 92);
-      auto issue_s = [&](int t, int j) {  // scores of row tile t
+      auto issue_s = [&](int t, int j) {  // scores of half t
         ok = ok && wait_or_abort(s, &s.k_full[j & 1], (j >> 1) & 1, err, 93);
         if (!ok) return;
         tc_fence_after();
 #pragma unroll
         for (int c = 0; c < 3; ++c) {
-          const uint64_t a = q_desc + (t * 3 + c) * kSlotStep, b = k_desc + ((5 * j + c) % kSlots) * kSlotStep;
+          const uint64_t a = q_desc + (split ? c : t * 3 + c) * kSlotStep, b = k_desc + ((5 * j + c) % kSlots) * kSlotStep;
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk) mma_bf16(tmem + t * 128, a + kk * 2, b + kk * 2, idesc_s, c + kk > 0);
         }
         mma_commit(&s.s_full[t]);
       };
       auto issue_pv = [&](int t, int j, int keys, bool last) {
+        const int i = split ? j >> 1 : j;  // the half's own count of tiles
         ok = ok && wait_or_abort(s, &s.v_full[j & 1], (j >> 1) & 1, err, 93);
-        ok = ok && wait_or_abort(s, &s.p_full[t], j & 1, err, 94);
+        ok = ok && wait_or_abort(s, &s.p_full[t], i & 1, err, 94);
         if (!ok) return;
         tc_fence_after();
         // the two value chunks may wrap around the ring's end: one descriptor step between them
@@ -510,35 +517,42 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (s1 > s0 && steps == 8) {
 #pragma unroll
           for (int kk = 0; kk < 8; ++kk)
-            mma_bf16_tmem_a(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, v + kk * 128, idesc_o, j + kk > 0);
+            mma_bf16_tmem_a(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, v + kk * 128, idesc_o, i + kk > 0);
         } else {
           constexpr uint32_t idesc_h = idesc_bf16<128, 64>() | kIdescBMn;
           for (int c = 0; c < 2; ++c)
             for (int kk = 0; kk < steps; ++kk)
               mma_bf16_tmem_a(tmem + 256 + t * 128 + c * 64, tmem + t * 128 + kk * 8,
-                              v_desc + (c ? s1 : s0) * kSlotStep + kk * 128, idesc_h, j + kk > 0);
+                              v_desc + (c ? s1 : s0) * kSlotStep + kk * 128, idesc_h, i + kk > 0);
         }
         if (last) mma_commit(&s.v_empty[j & 1]);
       };
-      const bool two = nt1 > 0;
       issue_s(0, 0);
-      if (two) issue_s(1, 0);
+      if (!split || nt > 1) issue_s(1, split ? 1 : 0);
       for (int j = 0; ok && j < nt; ++j) {
+        if (split) {
+          const int t = j & 1;
+          issue_pv(t, j, keys0, true);
+          if (j + 2 < nt) {
+            issue_s(t, j + 2);
+          } else if (ok) {
+            mma_commit(&s.o_full[t]);
+          }
+          continue;
+        }
         if (j < nt0) {
-          issue_pv(0, j, keys0, !two);
-          if (j + 1 == nt0) {
-            if (ok) mma_commit(&s.o_full[0]);
-          } else {
+          issue_pv(0, j, keys0, false);
+          if (j + 1 < nt0) {
             issue_s(0, j + 1);
+          } else if (ok) {
+            mma_commit(&s.o_full[0]);
           }
         }
-        if (j < nt1) {
-          issue_pv(1, j, keys1, true);
-          if (j + 1 == nt1) {
-            if (ok) mma_commit(&s.o_full[1]);
-          } else {
-            issue_s(1, j + 1);
-          }
+        issue_pv(1, j, keys1, true);
+        if (j + 1 < nt) {
+          issue_s(1, j + 1);
+        } else if (ok) {
+          mma_commit(&s.o_full[1]);
         }
       }
       // every MMA issued has finished before the tensor memory is freed
@@ -548,57 +562,52 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp >= 4) {
     // ------------------------------------------------------- softmax, epilogue
     const int t = (warp - 4) / 4, quad = warp & 3;
-    const int r = quad * 32 + lane;  // row of the tile
+    const int row = quad * 32 + lane + (split ? 0 : t * 128);
     const int keys = t ? keys1 : keys0, tiles = t ? nt1 : nt0;
-    const int last_key = min(pos0 + t * 128 + r, keys - 1);  // this row's; rows past the chunk see the tile's keys
+    const int last_key = min(pos0 + row, keys - 1);  // this row's; rows past the chunk see the tile's keys
     const uint32_t s_tmem = tmem + t * 128 + ((uint32_t)(quad * 32) << 16);
     const uint32_t o_tmem = s_tmem + 256;
     float m = 0.f, l = 0.f;
     bool ok = true;
-    for (int j = 0; j < tiles; ++j) {
-      ok = wait_or_abort(s, &s.s_full[t], j & 1, err, 95);
+    for (int i = 0; i < tiles; ++i) {
+      ok = wait_or_abort(s, &s.s_full[t], i & 1, err, 95);
       if (!__all_sync(0xffffffffu, ok)) {
         ok = false;
         break;
       }
       tc_fence_after();
-      const int limit = last_key - j * 128;  // columns up to this one count
+      const int limit = last_key - (split ? 2 * i + t : i) * 128;  // columns up to this one count
       const bool masked = __any_sync(0xffffffffu, limit < 127);
       uint32_t p[64];
       float sum = 0.f;
-      auto pass = [&]() {
-        return masked ? row_pass<true>(s_tmem, scale_log2, m, limit, p, sum)
-                      : row_pass<false>(s_tmem, scale_log2, m, limit, p, sum);
-      };
-      float top;
-      if (j == 0) {  // nothing to be relative to yet
-        top = -INFINITY;
+      if (i == 0) {  // no running maximum yet
+        float top = -INFINITY;
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
           float v[32];
           tmem_ld32w(s_tmem + c * 32, v);
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            top = fmaxf(top, c * 32 + i > limit ? -INFINITY : v[i] * scale_log2);
+          for (int e = 0; e < 32; ++e) top = fmaxf(top, c * 32 + e > limit ? -INFINITY : v[e] * scale_log2);
         }
         m = top == -INFINITY ? 0.f : top;
-        pass();
-      } else {
-        top = pass();
-        if (__any_sync(0xffffffffu, top > kRaise)) {
-          const float up = fmaxf(top, 0.f), f = ex2(-up);
-          m += up;
-          l *= f;
+      }
+      // one place for the pass (its code is long, and fetched anew by every CTA): a second
+      // round where a score passed the running maximum too far
+      while (true) {
+        const float top = masked ? row_pass<true>(s_tmem, scale_log2, m, limit, p, sum)
+                                 : row_pass<false>(s_tmem, scale_log2, m, limit, p, sum);
+        if (i == 0 || !__any_sync(0xffffffffu, top > kRaise)) break;
+        const float up = fmaxf(top, 0.f), f = ex2(-up);
+        m += up;
+        l *= f;
 #pragma unroll 1
-          for (int c = 0; c < 8; ++c) {
-            float o[16];
-            uint32_t u[16];
-            tmem_ld16(o_tmem + c * 16, o);
+        for (int c = 0; c < 8; ++c) {
+          float o[16];
+          uint32_t u[16];
+          tmem_ld16(o_tmem + c * 16, o);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) u[i] = __float_as_uint(o[i] * f);
-            tmem_st16(o_tmem + c * 16, u);
-          }
-          pass();
+          for (int e = 0; e < 16; ++e) u[e] = __float_as_uint(o[e] * f);
+          tmem_st16(o_tmem + c * 16, u);
         }
       }
       l += sum;
@@ -615,21 +624,57 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) mbar_arrive(&s.p_full[t]);
     }
     if (ok && tiles > 0) ok = wait_or_abort(s, &s.o_full[t], 0, err, 96);
-    if (__all_sync(0xffffffffu, ok && tiles > 0)) {
-      tc_fence_after();
+    ok = __all_sync(0xffffffffu, ok && tiles > 0);
+    tc_fence_after();
+    float f0 = 1.f, f1 = 0.f;  // factors of the halves' O
+    // the second half's O [dim][row], m and l go through the ring: every tile of it has been used
+    float* other = reinterpret_cast<float*>(s.ring[0]);
+    const int at = quad * 32 + lane;
+    if (split) {
+      if (t == 1) {
+        if (!ok) l = 0.f;
+        wait_or_abort(s, &s.o_full[0], 0, err, 96);  // the first half's tiles are in the ring too
+        __syncwarp();
+        if (ok) {
+#pragma unroll 1
+          for (int c = 0; c < 8; ++c) {
+            float o[16];
+            tmem_ld16(o_tmem + c * 16, o);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) other[(c * 16 + e) * 128 + at] = o[e];
+          }
+        }
+        other[128 * 128 + at] = m;
+        other[129 * 128 + at] = l;
+      }
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      if (t == 0) {
+        const float m1 = other[128 * 128 + at], l1 = other[129 * 128 + at];
+        if (l1 != 0.f) {  // a row without keys in the second half, or a half without tiles: 0
+          const float top = fmaxf(m, m1);
+          f0 = ex2(m - top), f1 = ex2(m1 - top);
+          l = l * f0 + l1 * f1;
+        }
+      }
+    }
+    if (ok && !(split && t == 1)) {
       const float inv = 1.f / l;
-      bf16* dst = out + (int64_t)(row0 + t * 128 + r) * out_stride + (int64_t)h * kVal;
-      const bool write = t * 128 + r < n;
+      bf16* dst = out + (int64_t)(row0 + row) * out_stride + (int64_t)h * kVal;
 #pragma unroll 1
       for (int c = 0; c < 8; ++c) {
         float o[16];
         tmem_ld16(o_tmem + c * 16, o);
-        if (write) {
+        if (__any_sync(0xffffffffu, f1 != 0.f)) {
 #pragma unroll
-          for (int i = 0; i < 2; ++i)
-            *reinterpret_cast<uint4*>(dst + c * 16 + i * 8) =
-                make_uint4(pack_bf16(o[8 * i] * inv, o[8 * i + 1] * inv), pack_bf16(o[8 * i + 2] * inv, o[8 * i + 3] * inv),
-                           pack_bf16(o[8 * i + 4] * inv, o[8 * i + 5] * inv), pack_bf16(o[8 * i + 6] * inv, o[8 * i + 7] * inv));
+          for (int e = 0; e < 16; ++e)
+            o[e] = o[e] * f0 + (f1 != 0.f ? other[(c * 16 + e) * 128 + at] * f1 : 0.f);
+        }
+        if (row < n) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            *reinterpret_cast<uint4*>(dst + c * 16 + e * 8) =
+                make_uint4(pack_bf16(o[8 * e] * inv, o[8 * e + 1] * inv), pack_bf16(o[8 * e + 2] * inv, o[8 * e + 3] * inv),
+                           pack_bf16(o[8 * e + 4] * inv, o[8 * e + 5] * inv), pack_bf16(o[8 * e + 6] * inv, o[8 * e + 7] * inv));
         }
       }
     }

@@ -412,7 +412,7 @@ def test_decode_refuses(dev):
 
 
 PREFILLS = [([1], [1]), ([17], [17]), ([130], [130]), ([128, 256], [128, 300]), ([300, 0, 1, 64], [557, 9, 900, 64]),
-            ([257, 129, 5, 385], [257, 513, 1000, 400])]
+            ([257, 129, 5, 385], [257, 513, 1000, 400]), ([128, 3, 100, 1, 64], [128, 129, 640, 2500, 385])]
 
 
 @pytest.mark.parametrize("q_lens,ctx_lens", PREFILLS)
