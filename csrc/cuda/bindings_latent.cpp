@@ -173,7 +173,8 @@ void check_heads(const char* op, const Tensor& q, const Tensor& w, const Tensor&
 }
 
 void latent_decode_attention(Tensor q, Tensor cache, Tensor w, Tensor block_tables, Tensor ctx_lens, Tensor out,
-                             int64_t H, double scale, int64_t max_ctx, Tensor workspace, Tensor err) {
+                             int64_t H, double scale, int64_t max_ctx, Tensor workspace,
+                             c10::optional<Tensor> table_rows, Tensor err) {
   const char* op = "latent_decode_attention";
   TORCH_CHECK(q.is_cuda(), op, ": q must be a CUDA tensor");
   check(q, at::kBFloat16, q, op, "q");
@@ -181,8 +182,8 @@ void latent_decode_attention(Tensor q, Tensor cache, Tensor w, Tensor block_tabl
   check_heads(op, q, w, out, H, R);
   const int64_t B = q.size(0);
   check(block_tables, at::kInt, q, op, "block_tables");
-  TORCH_CHECK(block_tables.dim() == 2 && block_tables.is_contiguous() && block_tables.size(0) >= B &&
-                  (block_tables.size(1) >= 1 || B == 0),
+  TORCH_CHECK(block_tables.dim() == 2 && block_tables.is_contiguous() &&
+                  (table_rows.has_value() || block_tables.size(0) >= B) && (block_tables.size(1) >= 1 || B == 0),
               op, ": block_tables must be [B, max_blocks] contiguous");
   TORCH_CHECK(block_tables.size(1) * cache.size(1) <= INT32_MAX, op, ": block_tables too wide");
   check(ctx_lens, at::kInt, q, op, "ctx_lens");
@@ -196,6 +197,13 @@ void latent_decode_attention(Tensor q, Tensor cache, Tensor w, Tensor block_tabl
   check(err, at::kInt, q, op, "err");
   const c10::cuda::CUDAGuard g(q.device());
   kapsl::LatentDecode a;
+  if (table_rows.has_value()) {
+    check(*table_rows, at::kInt, q, op, "table_rows");
+    TORCH_CHECK(table_rows->dim() == 1 && table_rows->is_contiguous() && table_rows->size(0) >= B, op,
+                ": table_rows must hold an int32 per row");
+    a.table_rows = table_rows->data_ptr<int32_t>();
+  }
+  a.num_tables = (int)block_tables.size(0);
   a.q = bf(q);
   a.q_stride = q.stride(0);
   a.cache = bf(cache);

@@ -50,8 +50,9 @@ struct LatentDecode {
   int64_t num_blocks = 0;
   int page = 0, R = 0;
   const __nv_bfloat16* w = nullptr;
-  const int32_t* block_tables = nullptr;
-  int max_blocks = 0;
+  const int32_t* block_tables = nullptr;  // [num_tables, max_blocks]
+  int max_blocks = 0, num_tables = 0;
+  const int32_t* table_rows = nullptr;    // table of each row (null: its own index)
   const int32_t* ctx_lens = nullptr;
   __nv_bfloat16* out = nullptr;  // [B, H * 128], pitch out_stride
   int64_t out_stride = 0;

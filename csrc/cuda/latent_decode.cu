@@ -246,6 +246,7 @@ template <int R, int NT>
 __global__ void __launch_bounds__(kAttnThreads<R>, 1)
     latent_attn_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap c_map,
                        int64_t num_blocks, int page, const int32_t* block_tables, int max_blocks,
+                       const int32_t* table_rows, int num_tables,
                        const int32_t* ctx_lens, const int32_t* table,
                        float* part_o, float* part_lse, int B, int H, int heads_per_cta,
                        int head_tiles, float scale_log2, int* err) {
@@ -298,17 +299,18 @@ __global__ void __launch_bounds__(kAttnThreads<R>, 1)
     int sent = 0, nq = 0;
     bool ok = true;
     // lane l < pages: first row of page l of a tile
-    auto page_row = [&](int tile) {
+    auto page_row = [&](int trow, int tile) {
       const int j = tile * pages + lane;
       if (lane >= pages || j >= (pc.keys() + page - 1) / page) return oob;
-      const int blk = block_tables[(int64_t)pc.b * max_blocks + j];
+      const int blk = trow >= 0 && trow < num_tables ? block_tables[(int64_t)trow * max_blocks + j] : -1;
       if (blk >= 0 && blk < num_blocks) return blk * page;
       atomicCAS(err, 0, 82);
       return oob;
     };
     for (; ok && pc.more(); pc.next()) {
       const int b = pc.b, t0 = pc.first(), n = pc.tiles();
-      int y = page_row(t0), y1 = n > 1 ? page_row(t0 + 1) : oob;
+      const int trow = table_rows != nullptr ? table_rows[b] : b;
+      int y = page_row(trow, t0), y1 = n > 1 ? page_row(trow, t0 + 1) : oob;
       if (g == 0) {
         if (nq > 0) ok = wait_or_abort(s, &s.q_empty, (nq - 1) & 1, err, 84);
         if (!__all_sync(0xffffffffu, ok)) break;
@@ -322,7 +324,7 @@ __global__ void __launch_bounds__(kAttnThreads<R>, 1)
       }
       for (int i = 0; i < n; ++i, ++sent) {
         const int st = sent % S::kStages;
-        const int y2 = i + 2 < n ? page_row(t0 + i + 2) : oob;
+        const int y2 = i + 2 < n ? page_row(trow, t0 + i + 2) : oob;
         int yy[4], zz[4];
 #pragma unroll
         for (int pg = 0; pg < 4; ++pg) {
@@ -628,8 +630,8 @@ __global__ void __launch_bounds__(kAttnThreads<R>, 1)
 // -------------------------------------------------------------- head products
 //
 // y[b, h, n] = sum_k x[b, h, k] w_h[k, n], small matrices per head, bound by the weights (128 KB +
-// 128 KB a head at R = 512) and the rows' traffic.  Up to 16 rows: mma.sync on 16-row tiles,
-// many small CTAs, since latency is all that counts.  Above: tcgen05 on 128-row tiles fed by
+// 128 KB a head at R = 512) and the rows' traffic.  Few rows: mma.sync on 16-row tiles, many
+// small CTAs, since latency is all that counts.  Else: tcgen05 on 128-row tiles fed by
 // TMA; at 64 rows x 128 heads the mma.sync form took 13 us for either product, held back by its
 // shared-memory loads, where this one takes 10 (absorb, which writes 9 MB) and 7 us.
 
@@ -661,7 +663,7 @@ __device__ __forceinline__ void copy_rotary(const bf16* q, int64_t q_stride, bf1
 }
 
 // qa[b, h, :R] = q[b, h, :128] . w[h, :128, :], qa[b, h, R:] = q[b, h, 128:].
-// One CTA per (64 columns, head); qa is bf16, the tensor cores' operand type.
+// One CTA per (64 columns, head, 16 rows); qa is bf16, the tensor cores' operand type.
 template <int R>
 __global__ void __launch_bounds__(128) latent_absorb_kernel(const bf16* q, int64_t q_stride,
                                                             const bf16* w, bf16* qa, int B,
@@ -669,23 +671,26 @@ __global__ void __launch_bounds__(128) latent_absorb_kernel(const bf16* q, int64
                                                             int ctas, int32_t* table) {
   griddep_entry();
   constexpr int MROWS = 16;
-  if (blockIdx.x == gridDim.x - 1 && blockIdx.y == 0)
+  if (blockIdx.x == gridDim.x - 1 && blockIdx.y == 0 && blockIdx.z == 0)
     write_schedule(ctx_lens, B, limit, ctas, table);
   constexpr int kPitchW = 64 + 8, kPitchX = kNope + 8;  // 16 bytes of padding: conflict-free ldmatrix
   __shared__ __align__(16) bf16 ws[kNope * kPitchW];
   __shared__ __align__(16) bf16 xs[MROWS * kPitchX];
-  const int n0 = blockIdx.x * 64, h = blockIdx.y;
+  const int n0 = blockIdx.x * 64, h = blockIdx.y, b0 = blockIdx.z * MROWS;
+  const int rows = min(MROWS, B - b0);
+  q += (int64_t)b0 * q_stride;
+  qa += (int64_t)b0 * H * (R + kRot);
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
   const bf16* wk = w + (int64_t)h * (kNope + kVal) * R + n0;
   for (int i = t; i < kNope * 8; i += 128) cp16(ws + (i >> 3) * kPitchW + (i & 7) * 8, wk + (int64_t)(i >> 3) * R + (i & 7) * 8);
   for (int i = t; i < MROWS * 16; i += 128) {
     const int r = i >> 4;
-    if (r < B)
+    if (r < rows)
       cp16(xs + r * kPitchX + (i & 15) * 8, q + (int64_t)r * q_stride + (int64_t)h * (kNope + kRot) + (i & 15) * 8);
   }
   cp_commit();
   if (blockIdx.x == 0) {  // the rotary part
-    copy_rotary<R, MROWS>(q, q_stride, qa, B, H, h);
+    copy_rotary<R, MROWS>(q, q_stride, qa, rows, H, h);
   }
   cp_wait<0>();
   __syncthreads();
@@ -709,7 +714,7 @@ __global__ void __launch_bounds__(128) latent_absorb_kernel(const bf16* q, int64
   __syncthreads();
   for (int i = t; i < MROWS * 8; i += 128) {
     const int b = i >> 3;
-    if (b < B)
+    if (b < rows)
       *reinterpret_cast<uint4*>(qa + ((int64_t)b * H + h) * (R + kRot) + n0 + (i & 7) * 8) =
           *reinterpret_cast<const uint4*>(xs + (i >> 3) * kPitchX + (i & 7) * 8);
   }
@@ -802,8 +807,8 @@ __global__ void __launch_bounds__(128)
   }
 }
 
-// out[b, h, n] = sum_r (hi + lo)[b, h, r] w[h, 128 + n, r] for up to 16 rows: one CTA per (32 columns,
-// head), everything it needs requested at once.
+// out[b, h, n] = sum_r (hi + lo)[b, h, r] w[h, 128 + n, r]: one CTA per (32 columns, head, 16 rows),
+// everything it needs requested at once.
 template <int R>
 __global__ void __launch_bounds__(128)
     latent_out_kernel(const bf16* hi, const bf16* lo, const bf16* w,
@@ -815,7 +820,7 @@ __global__ void __launch_bounds__(128)
   constexpr int kStage = (NCOLS + 2 * MROWS) * kPitch;
   extern __shared__ __align__(16) uint8_t raw[];
   bf16* sm = reinterpret_cast<bf16*>(raw);  // a stage: [NCOLS] w, [MROWS] hi, [MROWS] lo rows
-  const int n0 = blockIdx.x * NCOLS, h = blockIdx.y;
+  const int n0 = blockIdx.x * NCOLS, h = blockIdx.y, b0 = blockIdx.z * MROWS, rows = min(MROWS, B - b0);
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
   const bf16* wv = w + ((int64_t)h * (kNope + kVal) + kNope + n0) * R;
   auto load = [&](int c) {
@@ -825,9 +830,9 @@ __global__ void __launch_bounds__(128)
         cp16(st + (i >> 4) * kPitch + (i & 15) * 8, wv + (int64_t)(i >> 4) * R + c * 128 + (i & 15) * 8);
       for (int i = t; i < 2 * MROWS * 16; i += THREADS) {
         const int r = (i >> 4) % MROWS;
-        if (r < B)
+        if (r < rows)
           cp16(st + (NCOLS + (i >> 4)) * kPitch + (i & 15) * 8,
-               (i >= MROWS * 16 ? lo : hi) + ((int64_t)r * H + h) * R + c * 128 + (i & 15) * 8);
+               (i >= MROWS * 16 ? lo : hi) + ((int64_t)(b0 + r) * H + h) * R + c * 128 + (i & 15) * 8);
       }
     }
     cp_commit();
@@ -859,8 +864,8 @@ __global__ void __launch_bounds__(128)
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
     const int b = (lane >> 2) + e * 8;
-    if (b < B)
-      *reinterpret_cast<uint32_t*>(out + (int64_t)b * out_stride + (int64_t)h * kVal + n0 + c0 + (lane & 3) * 2) =
+    if (b < rows)
+      *reinterpret_cast<uint32_t*>(out + (int64_t)(b0 + b) * out_stride + (int64_t)h * kVal + n0 + c0 + (lane & 3) * 2) =
           pack_bf16(acc[2 * e], acc[2 * e + 1]);
   }
 }
@@ -1103,7 +1108,7 @@ void run_attn(const LatentDecode& a, const Plan& p, const bf16* qa, float* part_
   const CUtensorMap tq = make_tmap_2d_bf16(qa, (uint64_t)a.B * a.H, S::W, S::W, NT, 64, true);
   const CUtensorMap tc = make_tmap_2d_bf16(a.cache, (uint64_t)a.num_blocks * a.page, S::W, S::W, a.page, 64, true);
   launch_k(kern, dim3(p.ctas * p.head_tiles), kAttnThreads<R>, smem, st, tq, tc, a.num_blocks, a.page, a.block_tables,
-           a.max_blocks, a.ctx_lens, table, part_o, part_lse, a.B, a.H, p.heads_per_cta, p.head_tiles,
+           a.max_blocks, a.table_rows, a.num_tables, a.ctx_lens, table, part_o, part_lse, a.B, a.H, p.heads_per_cta, p.head_tiles,
            a.scale * kLog2e, a.err);
   KAPSL_LAUNCH_CHECK();
 }
@@ -1118,10 +1123,13 @@ void run(const LatentDecode& a, cudaStream_t st) {
   float* part_lse = reinterpret_cast<float*>(ws + l.lse);
   float* part_o = reinterpret_cast<float*>(ws + l.part);
   const int limit = a.max_blocks * a.page;
-  const bool small = a.B <= 16;
+  // Tiles of 16 rows while their CTAs are few (33 rows x 20 heads: SMALL_T, with the 128-row tiles
+  // BIG_T; 64 rows x 128 heads 120 and 101 us).
+  const bool small = (a.B + 15) / 16 * a.H <= 256;
+  const unsigned tiles16 = (a.B + 15) / 16;
   const CUtensorMap tw = make_tmap_2d_bf16(a.w, (uint64_t)a.H * (kNope + kVal), R, R, 128, 64, true);
   if (small) {
-    launch_k(latent_absorb_kernel<R>, dim3(R / 64, a.H), 128, 0, st, a.q, a.q_stride, a.w, qa, a.B, a.H, a.ctx_lens,
+    launch_k(latent_absorb_kernel<R>, dim3(R / 64, a.H, tiles16), 128, 0, st, a.q, a.q_stride, a.w, qa, a.B, a.H, a.ctx_lens,
              limit, p.ctas, table);
     KAPSL_LAUNCH_CHECK();
   } else {
@@ -1146,7 +1154,7 @@ void run(const LatentDecode& a, cudaStream_t st) {
   static std::atomic<uint64_t> devs{0}, devs_tc{0};
   if (small) {
     constexpr size_t smem = (size_t)(R / 128 + 1) * (32 + 2 * 16) * 136 * 2;
-    run_smem(latent_out_kernel<R>, devs, dim3(kVal / 32, a.H), smem, st, qa, lo, a.w, a.out, a.out_stride, a.B, a.H);
+    run_smem(latent_out_kernel<R>, devs, dim3(kVal / 32, a.H, tiles16), smem, st, qa, lo, a.w, a.out, a.out_stride, a.B, a.H);
   } else {
     const uint64_t width = (uint64_t)a.H * R;
     const CUtensorMap th = make_tmap_2d_bf16(qa, a.B, width, width, 128, 64, true);

@@ -365,7 +365,7 @@ def latent_decode_attention(q: torch.Tensor, cache: torch.Tensor, w_kv_b: torch.
     ws = torch.empty(c.latent_workspace_bytes(q, num_heads, cache.shape[-1] - 64, max_ctx), dtype=torch.uint8,
                      device=q.device)
     c.latent_decode_attention(q, cache, w_kv_b, block_tables, ctx_lens, out, num_heads, float(scale), max_ctx, ws,
-                              error_buffer(q.device))
+                              None, error_buffer(q.device))
     return out
 
 
@@ -383,6 +383,27 @@ class LatentPrefillPlan:
     tables: int             # block-table rows read
     max_ctx: int
     kv_rows: int            # context rows of all sequences, each padded to a multiple of 16
+    q_start: int
+    row_ctx: torch.Tensor   # int32 [rows - q_start]: context of every new token (itself included)
+    row_table: torch.Tensor  # int32 [rows - q_start]: its block-table row
+    single_tiles: int       # 64-key tiles of all new tokens taken one by one
+    row_tiles: int          # 128-key tiles of all 256-row tiles of new tokens
+    chain_us: float         # the longest of those row tiles by itself (microseconds)
+
+    def absorbed_is_shorter(self, num_heads: int, rank: int = 512) -> bool:
+        """Whether taking every new token by itself in the absorbed form is estimated to take less time
+        than expanding the contexts.  In microseconds, fitted to both forms' times on B200 (148
+        SMs) over 34 ragged batches: absorbed, a 64-key tile of up to 64 heads 3.0 (rank 256: 1.4) of
+        an SM and 2 for a thousand rows x heads of head products; expanded, 256 context rows of a head
+        4.5 (2.3) of an SM pair, a 128-key tile of 256 new tokens 1.9 of an SM, or the longest row
+        tile by itself.  20 new tokens over 4020, 8 heads: 42 and 80; five prompts of 17 to 300
+        tokens, 28 heads: 98 and 58."""
+        rows, wide = self.rows - self.q_start, rank > 256
+        absorbed = ((19 if -(-rows // 16) * num_heads <= 256 else 26) + (3.0 if wide else 1.4) * self.single_tiles * -(-num_heads // 64) / 148 +
+                    0.002 * rows * num_heads)
+        expanded = 20 + 1.2 * ((4.5 if wide else 2.3) * -(-self.kv_work.shape[0] // 2) * num_heads / 74 +
+                               max(self.chain_us, 1.9 * self.row_tiles * num_heads / 148))
+        return absorbed < expanded and rows <= 4096
 
 
 def latent_prefill_plan(q_lens: Sequence[int], ctx_lens: Sequence[int], device, q_start: int = 0,
@@ -397,13 +418,20 @@ def latent_prefill_plan(q_lens: Sequence[int], ctx_lens: Sequence[int], device, 
     if q_start < 0 or bt_start < 0:
         raise ValueError("latent_prefill_plan: negative start")
     info, work, row, kv = [], [], int(q_start), 0
+    row_ctx, row_table, single, chain = [], [], 0, 0.0
     for s, (n, ctx) in enumerate(zip(q_lens, ctx_lens)):
         if n < 0 or n > ctx:
             raise ValueError(f"latent_prefill_plan: sequence {s} has {n} new tokens in a context of {ctx}")
         if n == 0:  # nothing asks for its context
             ctx = 0
         info.append((row, n, ctx, bt_start + s, kv))
-        work += [(ctx - n + min(n, t0 + LATENT_PREFILL_TILE), s, t0) for t0 in range(0, n, LATENT_PREFILL_TILE)]
+        for t0 in range(0, n, LATENT_PREFILL_TILE):
+            keys = ctx - n + min(n, t0 + LATENT_PREFILL_TILE)
+            work.append((keys, s, t0))
+            chain = max(chain, -(-keys // 128) * (1.35 if n - t0 <= 128 else 1.9))
+        row_ctx += range(ctx - n + 1, ctx + 1)
+        row_table += [bt_start + s] * n
+        single += sum(-(-c // 64) for c in range(ctx - n + 1, ctx + 1))
         row += n
         kv += -(-ctx // 16) * 16
     if row >= 2 ** 31 or kv >= 2 ** 31:
@@ -411,23 +439,27 @@ def latent_prefill_plan(q_lens: Sequence[int], ctx_lens: Sequence[int], device, 
     work.sort(key=lambda w: -w[0])  # the tiles with the most keys start first
     dev = torch.device(device)
     kv_work = [(s, r) for s, i in enumerate(info) for r in range(0, i[2], 128)]
-    t = torch.tensor([v for w in work for v in w[1:]] + [v for w in kv_work for v in w] + [v for i in info for v in i],
-                     dtype=torch.int32).to(dev)
-    a, b = 2 * len(work), 2 * (len(work) + len(kv_work))
-    return LatentPrefillPlan(work=t[:a].view(-1, 2), kv_work=t[a:b].view(-1, 2), seq_info=t[b:].view(-1, 5), rows=row,
+    parts = [[v for w in work for v in w[1:]], [v for w in kv_work for v in w], [v for i in info for v in i], row_ctx,
+             row_table]
+    t = torch.tensor([v for p in parts for v in p], dtype=torch.int32).to(dev).split([len(p) for p in parts])
+    return LatentPrefillPlan(work=t[0].view(-1, 2), kv_work=t[1].view(-1, 2), seq_info=t[2].view(-1, 5), rows=row,
                              tables=bt_start + len(info) if info else 0, max_ctx=max([i[2] for i in info], default=0),
-                             kv_rows=kv)
+                             kv_rows=kv, q_start=int(q_start), row_ctx=t[3], row_table=t[4], single_tiles=single,
+                             row_tiles=sum(-(-w[0] // 128) for w in work), chain_us=chain)
 
 
 def latent_prefill_attention(q: torch.Tensor, cache: torch.Tensor, w_kv_b: torch.Tensor, plan: LatentPrefillPlan,
                              block_tables: torch.Tensor, num_heads: int, scale: Optional[float] = None,
-                             out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """Causal latent attention of chunks of new tokens over the paged latent cache, expanded form.
+                             out: Optional[torch.Tensor] = None, form: Optional[str] = None) -> torch.Tensor:
+    """Causal latent attention of chunks of new tokens over the paged latent cache.
 
     The new tokens' rows are in ``cache`` already; arguments as in
-    :func:`latent_decode_attention`, with ``plan`` from :func:`latent_prefill_plan`.  The
-    context's latents are expanded out of their pages by ``w_kv_b`` to keys and values (at
-    most ``LATENT_KV_BYTES`` of them at a time, in passes over the heads).
+    :func:`latent_decode_attention`, with ``plan`` from :func:`latent_prefill_plan`.  In the
+    expanded form the context's latents are expanded out of their pages by ``w_kv_b`` to keys
+    and values (at most ``LATENT_KV_BYTES`` of them at a time, in passes over the heads); in
+    the absorbed form every new token is a row of :func:`latent_decode_attention`, which is
+    shorter for few of them.  ``form`` ("expanded" or "absorbed") overrides
+    :meth:`LatentPrefillPlan.absorbed_is_shorter`; the two round differently.
     ``out`` rows outside the plan's sequences keep what they held (zeros when ``out`` is
     allocated here)."""
     if scale is None:
@@ -439,6 +471,15 @@ def latent_prefill_attention(q: torch.Tensor, cache: torch.Tensor, w_kv_b: torch
     if plan.work.shape[0] == 0:
         return out
     err = error_buffer(q.device)
+    if form not in (None, "expanded", "absorbed"):
+        raise ValueError(f"latent_prefill_attention: form {form!r}")
+    if form == "absorbed" or (form is None and plan.absorbed_is_shorter(num_heads, cache.shape[2] - 64)):
+        rows = slice(plan.q_start, plan.rows)
+        ws = torch.empty(c.latent_workspace_bytes(q[rows], num_heads, cache.shape[2] - 64, plan.max_ctx),
+                         dtype=torch.uint8, device=q.device)
+        c.latent_decode_attention(q[rows], cache, w_kv_b, block_tables, plan.row_ctx, out[rows], num_heads,
+                                  float(scale), plan.max_ctx, ws, plan.row_table, err)
+        return out
     w = w_kv_b.view(num_heads * 256, -1)
     step = max(1, min(num_heads, LATENT_KV_BYTES // (plan.kv_rows * 512)))
     k_rope = torch.empty(plan.kv_rows, 64, dtype=torch.bfloat16, device=q.device)

@@ -17,6 +17,12 @@ def test_plan_rows_and_tiles():
     # every query row in exactly one tile, most keys first
     got = [(s, t) for s, t in p.work.tolist()]
     assert got == [(2, 0), (0, 256), (0, 0), (3, 0)]
+    # every 128 context rows once
+    assert p.kv_work.tolist() == [[0, r] for r in range(0, 557, 128)] + [[2, r] for r in range(0, 900, 128)] + [[3, 0]]
+    # every new token by itself
+    assert p.row_ctx.tolist() == list(range(258, 558)) + [900] + list(range(1, 18))
+    assert p.row_table.tolist() == [2] * 300 + [4] + [5] * 17
+    assert p.single_tiles == sum(-(-c // 64) for c in p.row_ctx.tolist())
 
 
 def test_plan_of_nothing():

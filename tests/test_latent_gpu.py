@@ -416,8 +416,9 @@ PREFILLS = [([1], [1]), ([17], [17]), ([130], [130]), ([128, 256], [128, 300]), 
 
 
 @pytest.mark.parametrize("q_lens,ctx_lens", PREFILLS)
+@pytest.mark.parametrize("form", ["expanded", "absorbed"])
 @pytest.mark.parametrize("H,R,page", [(1, 512, 16), (5, 256, 64), (28, 512, 32)])
-def test_prefill(dev, q_lens, ctx_lens, H, R, page):
+def test_prefill(dev, form, q_lens, ctx_lens, H, R, page):
     from kapsl_sdk_b200 import ops
 
     k = Cache(dev, ctx_lens, R, page, H + len(q_lens))
@@ -428,11 +429,16 @@ def test_prefill(dev, q_lens, ctx_lens, H, R, page):
     out = torch.full((T, H * 128 + 8), 3.0, device=dev, dtype=torch.bfloat16)
     bt = torch.cat([k.bt.new_full((2, k.bt.shape[1]), -1), k.bt])
     plan = ops.latent_prefill_plan(q_lens, ctx_lens, dev, q_start=q0, bt_start=2)
-    ops.latent_prefill_attention(q, k.cache, w, plan, bt, H, out=out[:, :H * 128])
+    ops.latent_prefill_attention(q, k.cache, w, plan, bt, H, out=out[:, :H * 128], form=form)
     no_error(dev)
     at = q0
     for i, n in enumerate(q_lens):
-        if n:
+        if n and form == "absorbed":  # a few tokens of each sequence, the ends among them
+            for t in sorted({0, n - 1, n // 2, n // 3}):
+                exp, tol = decode64(q[at + t].view(H, 192), k.rows[i][:ctx_lens[i] - n + t + 1], w.view(H, 256, R),
+                                    1 / math.sqrt(192))
+                within(out[at + t, :H * 128].view(H, 128), exp, tol)
+        elif n:
             exp, tol = prefill64(q[at:at + n].view(n, H, 192), k.rows[i], w.view(H, 256, R), 1 / math.sqrt(192))
             within(out[at:at + n, :H * 128].view(n, H, 128), exp, tol)
         at += n
@@ -447,9 +453,26 @@ def test_prefill_passes_over_heads(dev, monkeypatch):
     H = 7
     q, w = k.randn(200, H * 192), k.randn(H * 256, 512, std=0.05)
     plan = ops.latent_prefill_plan([110, 90], [200, 90], dev)
-    one = ops.latent_prefill_attention(q, k.cache, w, plan, k.bt, H)
+    one = ops.latent_prefill_attention(q, k.cache, w, plan, k.bt, H, form="expanded")
     monkeypatch.setattr(ops, "LATENT_KV_BYTES", plan.kv_rows * 512 * 3)
-    assert torch.equal(one, ops.latent_prefill_attention(q, k.cache, w, plan, k.bt, H))
+    assert torch.equal(one, ops.latent_prefill_attention(q, k.cache, w, plan, k.bt, H, form="expanded"))
+    no_error(dev)
+
+
+def test_prefill_picks_a_form(dev):
+    """Few tokens over a long context go by themselves, a long chunk is expanded; the result is that of the
+    form named."""
+    from kapsl_sdk_b200 import ops
+
+    for q_lens, ctx_lens, H, form in (([3, 1], [900, 300], 8, "absorbed"), ([600], [700], 30, "expanded")):
+        k = Cache(dev, ctx_lens, 512, 16, 2)
+        q, w = k.randn(sum(q_lens), H * 192), k.randn(H * 256, 512, std=0.05)
+        plan = ops.latent_prefill_plan(q_lens, ctx_lens, dev)
+        assert plan.absorbed_is_shorter(H) == (form == "absorbed")
+        assert torch.equal(ops.latent_prefill_attention(q, k.cache, w, plan, k.bt, H),
+                           ops.latent_prefill_attention(q, k.cache, w, plan, k.bt, H, form=form))
+    with pytest.raises(ValueError):
+        ops.latent_prefill_attention(q, k.cache, w, plan, k.bt, H, form="folded")
     no_error(dev)
 
 
@@ -464,24 +487,25 @@ def test_prefill_large_logits(dev):
     j = torch.arange(n, device=dev)
     k.cache.view(-1, R + 64)[k.bt[0, j // 16].long() * 16 + j % 16] = rows
     q, w = k.randn(n, H * 192), k.randn(H * 256, R, std=1 / math.sqrt(R))
-    out = ops.latent_prefill_attention(q, k.cache, w, ops.latent_prefill_plan([n], [n], dev), k.bt, H)
+    out = ops.latent_prefill_attention(q, k.cache, w, ops.latent_prefill_plan([n], [n], dev), k.bt, H, form="expanded")
     no_error(dev)
     exp, tol = prefill64(q.view(n, H, 192), rows, w.view(H, 256, R), 1 / math.sqrt(192))
     within(out.view(n, H, 128), exp, tol)
 
 
-def test_prefill_pages_outside_and_refusals(dev):
+@pytest.mark.parametrize("form", ["expanded", "absorbed"])
+def test_prefill_pages_outside_and_refusals(dev, form):
     from kapsl_sdk_b200 import ops
 
     k = Cache(dev, [40, 50], 512, 16, 3)
     q, w = k.randn(50, 5 * 192), k.randn(5, 256, 512, std=0.04)
     plan = ops.latent_prefill_plan([20, 30], [40, 50], dev)
-    good = ops.latent_prefill_attention(q, k.cache, w, plan, k.bt, 5)
+    good = ops.latent_prefill_attention(q, k.cache, w, plan, k.bt, 5, form=form)
     no_error(dev)
     for bad in (-1, k.cache.shape[0], 2 ** 31 - 1):
         bt = k.bt.clone()
         bt[0, 1] = bad
-        out = ops.latent_prefill_attention(q, k.cache, w, plan, bt, 5)
+        out = ops.latent_prefill_attention(q, k.cache, w, plan, bt, 5, form=form)
         torch.cuda.synchronize()
         assert ops.check_errors(dev) == 82
         assert torch.equal(out[20:], good[20:]) and torch.isfinite(out.float()).all()
@@ -515,7 +539,7 @@ def test_graphs_streams_and_repeats(dev):
         return ops.latent_decode_attention(qd, k.cache, w, k.bt, k.ctx, H, max_ctx=1000)
 
     def prefill():
-        return ops.latent_prefill_attention(qp, k.cache, w, plan, k.bt, H)
+        return ops.latent_prefill_attention(qp, k.cache, w, plan, k.bt, H, form="expanded")
 
     decode(), prefill()
     torch.cuda.synchronize()
@@ -582,7 +606,7 @@ def test_layer_run_together(dev):
             done[s] += n
         if prefill:
             plan = ops.latent_prefill_plan(news, done, dev)
-            o = ops.latent_prefill_attention(q, cache, w, plan, bt, H, scale=scale)
+            o = ops.latent_prefill_attention(q, cache, w, plan, bt, H, scale=scale, form="expanded")
         else:
             ctx = torch.tensor(done, dtype=torch.int32, device=dev)
             o = ops.latent_decode_attention(q, cache, w, bt, ctx, H, scale=scale, max_ctx=max(done))
