@@ -155,7 +155,8 @@ int64_t latent_workspace_bytes(Tensor q, int64_t H, int64_t R, int64_t max_ctx) 
 }
 
 // q / out [rows, heads * width] and w [H, 256, R]
-void check_heads(const char* op, const Tensor& q, const Tensor& w, const Tensor& out, int64_t H, int64_t R) {
+void check_heads(const char* op, const Tensor& q, const Tensor& cache, const Tensor& w, const Tensor& out, int64_t H,
+                 int64_t R) {
   TORCH_CHECK(H >= 1 && H <= 1024, op, ": num_heads out of range");
   TORCH_CHECK(q.dim() == 2 && q.size(1) == H * (kNope + kRot) && (q.size(1) == 0 || q.stride(1) == 1), op, ": q must be [T, ",
               num(H * (kNope + kRot)), "] (128 + 64 dims a head)");
@@ -165,11 +166,12 @@ void check_heads(const char* op, const Tensor& q, const Tensor& w, const Tensor&
               ": out must be [T, ", num(H * kVal), "]");
   check_rows16(op, out, "out");
   TORCH_CHECK(out.size(0) <= 1 || out.stride(0) > 0, op, ": out must not be expanded");
-  TORCH_CHECK(!ranges_meet(q, out), op, ": out must not overlap q");
   check(w, at::kBFloat16, q, op, "w_kv_b");
   TORCH_CHECK(w.numel() == H * (kNope + kVal) * R && w.size(-1) == R && w.is_contiguous(), op, ": w_kv_b must be [", num(H),
               " * 256, ", num(R), "] contiguous");
   TORCH_CHECK((reinterpret_cast<uintptr_t>(w.data_ptr()) & 15) == 0, op, ": w_kv_b must be 16-byte aligned");
+  TORCH_CHECK(!ranges_meet(q, out) && !ranges_meet(cache, out) && !ranges_meet(w, out), op,
+              ": out must not overlap q, the cache or w_kv_b");
 }
 
 void latent_decode_attention(Tensor q, Tensor cache, Tensor w, Tensor block_tables, Tensor ctx_lens, Tensor out,
@@ -179,7 +181,7 @@ void latent_decode_attention(Tensor q, Tensor cache, Tensor w, Tensor block_tabl
   TORCH_CHECK(q.is_cuda(), op, ": q must be a CUDA tensor");
   check(q, at::kBFloat16, q, op, "q");
   const int64_t R = check_cache(op, cache, q);
-  check_heads(op, q, w, out, H, R);
+  check_heads(op, q, cache, w, out, H, R);
   const int64_t B = q.size(0);
   check(block_tables, at::kInt, q, op, "block_tables");
   TORCH_CHECK(block_tables.dim() == 2 && block_tables.is_contiguous() &&
@@ -280,7 +282,7 @@ void check_latent_prefill(Tensor q, Tensor cache, Tensor w, Tensor block_tables,
   TORCH_CHECK(q.is_cuda(), op, ": q must be a CUDA tensor");
   check(q, at::kBFloat16, q, op, "q");
   const int64_t R = check_cache(op, cache, q);
-  check_heads(op, q, w, out, H, R);
+  check_heads(op, q, cache, w, out, H, R);
   check(block_tables, at::kInt, q, op, "block_tables");
   TORCH_CHECK(block_tables.dim() == 2 && block_tables.is_contiguous(), op, ": block_tables must be contiguous");
   TORCH_CHECK(q.size(0) >= rows, op, ": the plan covers ", num(rows), " rows of q, which has ",

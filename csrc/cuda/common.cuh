@@ -94,8 +94,9 @@ __device__ __forceinline__ void griddep_entry() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }
-// The two halves of griddep_entry, for kernels that set up shared and tensor memory between them
-// (nothing that an earlier kernel writes is read before the wait).
+// The two halves of griddep_entry, for kernels that set up shared memory between them.  Nothing that
+// an earlier kernel writes is read before the wait, and no tensor memory is taken: a CTA of
+// the grid waited for may still be about to allocate it on the same SM.
 __device__ __forceinline__ void griddep_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void griddep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 // Entry of a kernel that does not let the next one launch early (it launches when

@@ -282,13 +282,13 @@ __global__ void __launch_bounds__(kAttnThreads<R>, 1)
     mbar_init(&s.drained, 1);
     fence_barrier_init();
   }
+  griddep_wait();  // before the allocation: a CTA of the grid waited for may still need its own
   if (warp == kMma) tmem_alloc(&s.tmem_base, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, s.tmem_base, 0);
   const uint32_t tmem_o = tmem + 2 * NT;
-  griddep_wait();
   Pieces pc(table, ctx_lens, B, max_blocks * page, c);  // without pieces, every role falls through its loop
 
   if (warp < S::kGroups) {
@@ -577,7 +577,8 @@ __global__ void __launch_bounds__(kAttnThreads<R>, 1)
           const int per_row = R / 8;  // 16-byte vectors of a row's latent
           for (int e = tid; e < (kKeys - valid) * per_row; e += kSoft * 32) {
             const int r = valid + e / per_row, x = e % per_row;
-            *reinterpret_cast<uint4*>(s.k[st] + (x >> 3) * S::kChunkBytes + r * 128 + (x & 7) * 16) = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4*>(s.k[st] + (x >> 3) * S::kChunkBytes + r * 128 + (x & 7) * 16) =
+                make_uint4(0, 0, 0, 0);
           }
         }
         fence_proxy_async_smem();
@@ -682,7 +683,8 @@ __global__ void __launch_bounds__(128) latent_absorb_kernel(const bf16* q, int64
   qa += (int64_t)b0 * H * (R + kRot);
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
   const bf16* wk = w + (int64_t)h * (kNope + kVal) * R + n0;
-  for (int i = t; i < kNope * 8; i += 128) cp16(ws + (i >> 3) * kPitchW + (i & 7) * 8, wk + (int64_t)(i >> 3) * R + (i & 7) * 8);
+  for (int i = t; i < kNope * 8; i += 128)
+    cp16(ws + (i >> 3) * kPitchW + (i & 7) * 8, wk + (int64_t)(i >> 3) * R + (i & 7) * 8);
   for (int i = t; i < MROWS * 16; i += 128) {
     const int r = i >> 4;
     if (r < rows)
@@ -892,7 +894,8 @@ __device__ __forceinline__ void store_slab(uint32_t taddr, uint8_t* slab, bf16* 
   for (int k = 0; k < 8; ++k) {
     const int r = 4 * k + (lane >> 3), seg = lane & 7;
     if (r < rows)
-      *reinterpret_cast<uint4*>(dst + r * pitch + seg * 8) = *reinterpret_cast<const uint4*>(slab + r * kSlabPitch + seg * 16);
+      *reinterpret_cast<uint4*>(dst + r * pitch + seg * 8) =
+          *reinterpret_cast<const uint4*>(slab + r * kSlabPitch + seg * 16);
   }
   __syncwarp();
 }
@@ -927,11 +930,11 @@ __global__ void __launch_bounds__(128) latent_absorb_tc_kernel(const __grid_cons
     mbar_init(&s.done, 1);
     fence_barrier_init();
   }
+  griddep_wait();  // before the allocation: a CTA of the grid waited for may still need its own
   if (warp == 0) tmem_alloc(&s.tmem_base, 256);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  griddep_wait();
   const uint32_t tmem = __shfl_sync(0xffffffffu, s.tmem_base, 0);
   if (warp == 0 && elect_one()) {
     mbar_arrive_expect_tx(&s.full, 6 * 128 * 128);
@@ -1005,11 +1008,11 @@ __global__ void __launch_bounds__(128, 1) latent_out_tc_kernel(const __grid_cons
     mbar_init(&s.done, 1);
     fence_barrier_init();
   }
+  griddep_wait();  // before the allocation: a CTA of the grid waited for may still need its own
   if (warp == 0) tmem_alloc(&s.tmem_base, 128);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  griddep_wait();
   const uint32_t tmem = __shfl_sync(0xffffffffu, s.tmem_base, 0);
   if (warp == 0) {
     if (elect_one()) {
@@ -1108,8 +1111,8 @@ void run_attn(const LatentDecode& a, const Plan& p, const bf16* qa, float* part_
   const CUtensorMap tq = make_tmap_2d_bf16(qa, (uint64_t)a.B * a.H, S::W, S::W, NT, 64, true);
   const CUtensorMap tc = make_tmap_2d_bf16(a.cache, (uint64_t)a.num_blocks * a.page, S::W, S::W, a.page, 64, true);
   launch_k(kern, dim3(p.ctas * p.head_tiles), kAttnThreads<R>, smem, st, tq, tc, a.num_blocks, a.page, a.block_tables,
-           a.max_blocks, a.table_rows, a.num_tables, a.ctx_lens, table, part_o, part_lse, a.B, a.H, p.heads_per_cta, p.head_tiles,
-           a.scale * kLog2e, a.err);
+           a.max_blocks, a.table_rows, a.num_tables, a.ctx_lens, table, part_o, part_lse, a.B, a.H, p.heads_per_cta,
+           p.head_tiles, a.scale * kLog2e, a.err);
   KAPSL_LAUNCH_CHECK();
 }
 
@@ -1123,8 +1126,8 @@ void run(const LatentDecode& a, cudaStream_t st) {
   float* part_lse = reinterpret_cast<float*>(ws + l.lse);
   float* part_o = reinterpret_cast<float*>(ws + l.part);
   const int limit = a.max_blocks * a.page;
-  // Tiles of 16 rows while their CTAs are few (33 rows x 20 heads: SMALL_T, with the 128-row tiles
-  // BIG_T; 64 rows x 128 heads 120 and 101 us).
+  // Tiles of 16 rows while their CTAs are few (a whole call of 33 rows x 20 heads 27 us, with the 128-row
+  // tiles 32; of 64 rows x 128 heads 118 and 101 us).
   const bool small = (a.B + 15) / 16 * a.H <= 256;
   const unsigned tiles16 = (a.B + 15) / 16;
   const CUtensorMap tw = make_tmap_2d_bf16(a.w, (uint64_t)a.H * (kNope + kVal), R, R, 128, 64, true);
@@ -1135,8 +1138,8 @@ void run(const LatentDecode& a, cudaStream_t st) {
   } else {
     const CUtensorMap tq = make_tmap_2d_bf16(a.q, a.B, (uint64_t)a.H * (kNope + kRot), a.q_stride, 128, 64, true);
     static std::atomic<uint64_t> devs{0};
-    run_smem(latent_absorb_tc_kernel<R>, devs, dim3(R / 256, a.H, (a.B + 127) / 128), sizeof(AbsorbSmem), st, tq, tw, a.q,
-             a.q_stride, qa, a.B, a.H, a.ctx_lens, limit, p.ctas, table, a.err);
+    run_smem(latent_absorb_tc_kernel<R>, devs, dim3(R / 256, a.H, (a.B + 127) / 128), sizeof(AbsorbSmem), st, tq, tw,
+             a.q, a.q_stride, qa, a.B, a.H, a.ctx_lens, limit, p.ctas, table, a.err);
   }
   if (p.heads_per_cta <= 16) {
     run_attn<R, 16>(a, p, qa, part_o, part_lse, table, st);

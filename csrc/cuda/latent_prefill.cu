@@ -191,7 +191,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kExpandThreads, 1)
         }
         for (int ks = 0; ks < S::kChunks; ++ks, ++sent) {
           const int st = sent % S::kStages;
-          if (sent >= S::kStages && !(ok = wait_or_abort(s, &s.b_empty[st], (sent / S::kStages - 1) & 1, err, 97))) break;
+          if (sent >= S::kStages) ok = wait_or_abort(s, &s.b_empty[st], (sent / S::kStages - 1) & 1, err, 97);
+          if (!ok) break;
           if (rank == 0) mbar_arrive_expect_tx(&s.b_full[st], 2 * 128 * 128);
           tma_load_pair(s.b[st], &w_map, &s.b_full[st], ks * 64, head * 256 + rank * 128);
         }
@@ -276,8 +277,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kExpandThreads, 1)
           }
 #pragma unroll
           for (int q = 0; q < 4; ++q)
-            mine[half * 4 + q] = make_uint4(pack_bf16(v[8 * q], v[8 * q + 1]), pack_bf16(v[8 * q + 2], v[8 * q + 3]),
-                                            pack_bf16(v[8 * q + 4], v[8 * q + 5]), pack_bf16(v[8 * q + 6], v[8 * q + 7]));
+            mine[half * 4 + q] =
+                make_uint4(pack_bf16(v[8 * q], v[8 * q + 1]), pack_bf16(v[8 * q + 2], v[8 * q + 3]),
+                           pack_bf16(v[8 * q + 4], v[8 * q + 5]), pack_bf16(v[8 * q + 6], v[8 * q + 7]));
         }
         __syncwarp();
         if (c == 192) {  // the accumulator has been read
@@ -498,7 +500,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_after();
 #pragma unroll
         for (int c = 0; c < 3; ++c) {
-          const uint64_t a = q_desc + (split ? c : t * 3 + c) * kSlotStep, b = k_desc + ((5 * j + c) % kSlots) * kSlotStep;
+          const uint64_t a = q_desc + (split ? c : t * 3 + c) * kSlotStep;
+          const uint64_t b = k_desc + ((5 * j + c) % kSlots) * kSlotStep;
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk) mma_bf16(tmem + t * 128, a + kk * 2, b + kk * 2, idesc_s, c + kk > 0);
         }
@@ -671,10 +674,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (row < n) {
 #pragma unroll
-          for (int e = 0; e < 2; ++e)
-            *reinterpret_cast<uint4*>(dst + c * 16 + e * 8) =
-                make_uint4(pack_bf16(o[8 * e] * inv, o[8 * e + 1] * inv), pack_bf16(o[8 * e + 2] * inv, o[8 * e + 3] * inv),
-                           pack_bf16(o[8 * e + 4] * inv, o[8 * e + 5] * inv), pack_bf16(o[8 * e + 6] * inv, o[8 * e + 7] * inv));
+          for (int e = 0; e < 16; ++e) o[e] *= inv;
+#pragma unroll
+          for (int e = 0; e < 16; e += 8)
+            *reinterpret_cast<uint4*>(dst + c * 16 + e) =
+                make_uint4(pack_bf16(o[e], o[e + 1]), pack_bf16(o[e + 2], o[e + 3]), pack_bf16(o[e + 4], o[e + 5]),
+                           pack_bf16(o[e + 6], o[e + 7]));
         }
       }
     }

@@ -23,6 +23,8 @@ _err_bufs: dict[int, torch.Tensor] = {}
 def error_buffer(device: torch.device) -> torch.Tensor:
     """Per-device int32[16] status words written by kernels whose bounded
     waits time out (0 = ok).  Read with :func:`check_errors`."""
+    if device.type != "cuda":
+        raise RuntimeError(f"the kernels take CUDA tensors, got one on {device}")
     idx = device.index if device.index is not None else torch.cuda.current_device()
     buf = _err_bufs.get(idx)
     if buf is None:
@@ -396,10 +398,11 @@ class LatentPrefillPlan:
         SMs) over 34 ragged batches: absorbed, a 64-key tile of up to 64 heads 3.0 (rank 256: 1.4) of
         an SM and 2 for a thousand rows x heads of head products; expanded, 256 context rows of a head
         4.5 (2.3) of an SM pair, a 128-key tile of 256 new tokens 1.9 of an SM, or the longest row
-        tile by itself.  20 new tokens over 4020, 8 heads: 42 and 80; five prompts of 17 to 300
+        tile by itself.  20 new tokens over 4020, 8 heads: 35 and 80; five prompts of 17 to 300
         tokens, 28 heads: 98 and 58."""
         rows, wide = self.rows - self.q_start, rank > 256
-        absorbed = ((19 if -(-rows // 16) * num_heads <= 256 else 26) + (3.0 if wide else 1.4) * self.single_tiles * -(-num_heads // 64) / 148 +
+        start = 19 if -(-rows // 16) * num_heads <= 256 else 26
+        absorbed = (start + (3.0 if wide else 1.4) * self.single_tiles * -(-num_heads // 64) / 148 +
                     0.002 * rows * num_heads)
         expanded = 20 + 1.2 * ((4.5 if wide else 2.3) * -(-self.kv_work.shape[0] // 2) * num_heads / 74 +
                                max(self.chain_us, 1.9 * self.row_tiles * num_heads / 148))
@@ -459,7 +462,9 @@ def latent_prefill_attention(q: torch.Tensor, cache: torch.Tensor, w_kv_b: torch
     and values (at most ``LATENT_KV_BYTES`` of them at a time, in passes over the heads); in
     the absorbed form every new token is a row of :func:`latent_decode_attention`, which is
     shorter for few of them.  ``form`` ("expanded" or "absorbed") overrides
-    :meth:`LatentPrefillPlan.absorbed_is_shorter`; the two round differently.
+    :meth:`LatentPrefillPlan.absorbed_is_shorter`; the two round differently.  Page slots behind
+    a context may hold anything; its own rows have to be finite, since in the expanded form
+    a row that is not also reaches earlier new tokens (0 * NaN in the product with the values).
     ``out`` rows outside the plan's sequences keep what they held (zeros when ``out`` is
     allocated here)."""
     if scale is None:
