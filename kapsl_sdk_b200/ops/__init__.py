@@ -422,6 +422,11 @@ def latent_prefill_plan(q_lens: Sequence[int], ctx_lens: Sequence[int], device, 
         raise ValueError("latent_prefill_plan: negative start")
     info, work, row, kv = [], [], int(q_start), 0
     row_ctx, row_table, single, chain = [], [], 0, 0.0
+
+    def tiles64(c: int) -> int:  # 64-key tiles of contexts 1 .. c, summed
+        full = c // 64
+        return 32 * full * (full + 1) + (c % 64) * (full + 1)
+
     for s, (n, ctx) in enumerate(zip(q_lens, ctx_lens)):
         if n < 0 or n > ctx:
             raise ValueError(f"latent_prefill_plan: sequence {s} has {n} new tokens in a context of {ctx}")
@@ -432,9 +437,9 @@ def latent_prefill_plan(q_lens: Sequence[int], ctx_lens: Sequence[int], device, 
             keys = ctx - n + min(n, t0 + LATENT_PREFILL_TILE)
             work.append((keys, s, t0))
             chain = max(chain, -(-keys // 128) * (1.35 if n - t0 <= 128 else 1.9))
-        row_ctx += range(ctx - n + 1, ctx + 1)
-        row_table += [bt_start + s] * n
-        single += sum(-(-c // 64) for c in range(ctx - n + 1, ctx + 1))
+        row_ctx.append(torch.arange(ctx - n + 1, ctx + 1, dtype=torch.int32))
+        row_table.append(torch.full((n,), bt_start + s, dtype=torch.int32))
+        single += tiles64(ctx) - tiles64(ctx - n)
         row += n
         kv += -(-ctx // 16) * 16
     if row >= 2 ** 31 or kv >= 2 ** 31:
@@ -442,9 +447,11 @@ def latent_prefill_plan(q_lens: Sequence[int], ctx_lens: Sequence[int], device, 
     work.sort(key=lambda w: -w[0])  # the tiles with the most keys start first
     dev = torch.device(device)
     kv_work = [(s, r) for s, i in enumerate(info) for r in range(0, i[2], 128)]
-    parts = [[v for w in work for v in w[1:]], [v for w in kv_work for v in w], [v for i in info for v in i], row_ctx,
-             row_table]
-    t = torch.tensor([v for p in parts for v in p], dtype=torch.int32).to(dev).split([len(p) for p in parts])
+    parts = [torch.tensor(v, dtype=torch.int32) for v in (
+        [v for w in work for v in w[1:]], [v for w in kv_work for v in w], [v for i in info for v in i])]
+    none = torch.empty(0, dtype=torch.int32)
+    parts += [torch.cat(row_ctx or [none]), torch.cat(row_table or [none])]
+    t = torch.cat(parts).to(dev).split([p.numel() for p in parts])
     return LatentPrefillPlan(work=t[0].view(-1, 2), kv_work=t[1].view(-1, 2), seq_info=t[2].view(-1, 5), rows=row,
                              tables=bt_start + len(info) if info else 0, max_ctx=max([i[2] for i in info], default=0),
                              kv_rows=kv, q_start=int(q_start), row_ctx=t[3], row_table=t[4], single_tiles=single,

@@ -128,7 +128,8 @@ def test_rope_refuses(dev):
     x = torch.randn(4, 2, 64, device=dev, dtype=torch.bfloat16)
     pos = torch.zeros(4, dtype=torch.int32, device=dev)
     for bad in (lambda: ops.rope(x.cpu(), pos, cs), lambda: ops.rope(x.double(), pos, cs),
-                lambda: ops.rope(x, pos.long(), cs), lambda: ops.rope(x, pos[:3], cs), lambda: ops.rope(x, pos.cpu(), cs),
+                lambda: ops.rope(x, pos.long(), cs), lambda: ops.rope(x, pos[:3], cs),
+                lambda: ops.rope(x, pos.cpu(), cs),
                 lambda: ops.rope(x, pos, cs, offset=33), lambda: ops.rope(x, pos, cs, offset=-1),
                 lambda: ops.rope(x, pos, cs[:, :31]), lambda: ops.rope(x, pos, cs.half()),
                 lambda: ops.rope(x[0], pos, cs), lambda: ops.rope(x.transpose(1, 2), pos, cs),
@@ -522,6 +523,84 @@ def test_prefill_pages_outside_and_refusals(dev, form):
             bad()
     empty = ops.latent_prefill_plan([0], [0], dev)
     assert bool((ops.latent_prefill_attention(q, k.cache, w, empty, k.bt, 5) == 0).all())
+    no_error(dev)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.05, 1.0])
+def test_scales(dev, scale):
+    """Scale 0 weighs every key alike, a negative one prefers the least similar, a large one a single key."""
+    from kapsl_sdk_b200 import ops
+
+    H, R, n, ctx = 3, 512, 70, 200
+    k = Cache(dev, [ctx], R, 16, 12)
+    q, w = k.randn(n, H * 192), k.randn(H * 256, R, std=1 / math.sqrt(R))
+    plan = ops.latent_prefill_plan([n], [ctx], dev)
+    out = ops.latent_prefill_attention(q, k.cache, w, plan, k.bt, H, scale=scale, form="expanded")
+    exp, tol = prefill64(q.view(n, H, 192), k.rows[0], w.view(H, 256, R), scale)
+    within(out.view(n, H, 128), exp, tol)
+    one = ops.latent_decode_attention(q[-1:], k.cache, w, k.bt, k.ctx, H, scale=scale)
+    exp, tol = decode64(q[-1].view(H, 192), k.rows[0], w.view(H, 256, R), scale)
+    within(one.view(H, 128), exp, tol)
+    no_error(dev)
+
+
+def test_cache_past_32_bit_offsets(dev):
+    """Pages whose elements lie more than 2^31 from the cache's start: write, decode, both prefill forms."""
+    from kapsl_sdk_b200 import ops
+    from kapsl_sdk_b200.ops import reference as ref
+
+    page, R, H, n = 64, 512, 4, 150
+    blocks = 2 ** 31 // (page * (R + 64)) + 40
+    cache = torch.empty(blocks, page, R + 64, dtype=torch.bfloat16, device=dev)
+    g = torch.Generator(device=dev).manual_seed(8)
+
+    def rn(*s, std=1.0):
+        return (torch.randn(*s, generator=g, device=dev) * std).to(torch.bfloat16)
+
+    bt = torch.tensor([[blocks - 1, 3, blocks - 7]], dtype=torch.int32, device=dev)
+    pos = torch.arange(n, device=dev, dtype=torch.int32)
+    slots = bt[0].long()[pos.long() // page] * page + pos.long() % page
+    cs = ref.rope_cos_sin(n, 64, 1e4, device=dev)
+    kv, q, wn, w = rn(n, R + 64), rn(n, H, 192), 1 + rn(R, std=0.1), rn(H * 256, R, std=1 / math.sqrt(R))
+    ops.rope_latent_write(q[..., 128:], kv, pos, slots, cs, wn, 1e-5, cache)
+    rows = cache.view(-1, R + 64)[slots]
+    exp = ref.latent_row(kv, pos, cs, wn, 1e-5)
+    assert float((rows.float() - exp).abs().max()) < 2 * U * float(exp.abs().max())
+    plan = ops.latent_prefill_plan([40], [n], dev)
+    q2 = q[-40:].reshape(40, -1)
+    got = ops.latent_prefill_attention(q2, cache, w, plan, bt, H, form="expanded")
+    e, t = prefill64(q[-40:], rows, w.view(H, 256, R), 1 / math.sqrt(192))
+    within(got.view(40, H, 128), e, t)
+    got = ops.latent_prefill_attention(q2, cache, w, plan, bt, H, form="absorbed")
+    one = ops.latent_decode_attention(q2[-1:], cache, w, bt, torch.tensor([n], dtype=torch.int32, device=dev), H)
+    e, t = decode64(q[-1], rows, w.view(H, 256, R), 1 / math.sqrt(192))
+    within(got[-1].view(H, 128), e, t)
+    within(one[0].view(H, 128), e, t)
+    no_error(dev)
+
+
+def test_write_from_one_projection(dev):
+    """Queries and latents as views of one projection's rows, rotated in place: its other columns stay."""
+    from kapsl_sdk_b200 import ops
+    from kapsl_sdk_b200.ops import reference as ref
+
+    T, H, R = 9, 3, 256
+    g = torch.Generator(device=dev).manual_seed(2)
+    y = torch.randn(T, H * 192 + R + 64, generator=g, device=dev).to(torch.bfloat16)
+    before = y.clone()
+    q, kv = y[:, :H * 192].view(T, H, 192), y[:, H * 192:]
+    cs = ref.rope_cos_sin(50, 64, 1e4, device=dev)
+    pos = torch.randint(0, 50, (T,), generator=g, device=dev, dtype=torch.int32)
+    cache = torch.zeros(1, 16, R + 64, dtype=torch.bfloat16, device=dev)
+    w = torch.ones(R, dtype=torch.bfloat16, device=dev)
+    ops.rope_latent_write(q[..., 128:], kv, pos, torch.arange(T, device=dev), cs, w, 1e-6, cache, interleaved=True)
+    exp, mag = rope64(before[:, :H * 192].view(T, H, 192)[..., 128:], pos, cs, 0, True)
+    within(q[..., 128:], exp, U * exp.abs() + 2.0 ** -22 * mag)
+    assert torch.equal(q[..., :128], before[:, :H * 192].view(T, H, 192)[..., :128])
+    assert torch.equal(kv, before[:, H * 192:])
+    c = before[:, H * 192:H * 192 + R].double()
+    lat = c / (c.pow(2).mean(1, keepdim=True) + 1e-6).sqrt()
+    within(cache[0, :T, :R], lat, lat.abs() * (U + 2.0 ** -18))
     no_error(dev)
 
 
