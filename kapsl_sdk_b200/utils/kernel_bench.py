@@ -5,6 +5,8 @@
     python -m kapsl_sdk_b200.utils.kernel_bench moe T E D F [--time]
     python -m kapsl_sdk_b200.utils.kernel_bench decode B CTX HQ HKV [--time]
     python -m kapsl_sdk_b200.utils.kernel_bench prefill S CHUNK HQ HKV [--time]
+    python -m kapsl_sdk_b200.utils.kernel_bench latent_decode B CTX H [--time]
+    python -m kapsl_sdk_b200.utils.kernel_bench latent_prefill S CHUNK CTX H [--time]
     python -m kapsl_sdk_b200.utils.kernel_bench sample B V [--time]
 
 Without ``--time`` each command launches the kernel 3 times (a capture target
@@ -116,6 +118,41 @@ def bench_prefill(S, chunk, hq, hkv, timed):
     ms = _time(fn)
     flops = S * hq * 128 * 4 * chunk * chunk / 2
     return {"kernel": name, "S": S, "chunk": chunk, "ms": ms, "tflops": flops / ms / 1e9}
+
+
+def bench_latent(S, chunk, ctx, H, timed, decode):
+    """Latent attention (rank 512) of S sequences of ctx tokens: one new token each (decode), or the
+    last ``chunk`` of them."""
+    from .. import ops
+
+    dev = torch.device("cuda", 0)
+    n = 1 if decode else chunk
+    nb = (ctx + 15) // 16
+    cache = torch.randn(S * nb, 16, 576, device=dev).to(torch.bfloat16)
+    bt = torch.randperm(S * nb, device=dev).to(torch.int32).view(S, nb)
+    q = torch.randn(S * n, H * 192, device=dev).to(torch.bfloat16)
+    w = (torch.randn(H * 256, 512, device=dev) / math.sqrt(512)).to(torch.bfloat16)
+    out = torch.empty(S * n, H * 128, device=dev, dtype=torch.bfloat16)
+    lens = torch.full((S,), ctx, dtype=torch.int32, device=dev)
+    plan = ops.latent_prefill_plan([n] * S, [ctx] * S, dev)
+    if decode:
+        fn = lambda: ops.latent_decode_attention(q, cache, w, bt, lens, H, out=out, max_ctx=ctx)
+    else:
+        fn = lambda: ops.latent_prefill_attention(q, cache, w, plan, bt, H, out=out)
+    r = {"kernel": "latent_decode" if decode else "latent_prefill", "S": S, "chunk": n, "ctx": ctx, "heads": H}
+    if not timed:
+        for _ in range(3):
+            fn()
+        torch.cuda.synchronize()
+        return r
+    r["ms"] = _time(fn)
+    if decode:
+        r["tflops"] = S * H * 2 * (ctx * 1088 + 256 * 512) / r["ms"] / 1e9
+        r["GBps"] = (S * ctx * 1152 + H * 256 * 512 * 2) / r["ms"] / 1e6
+    else:
+        pairs = n * ctx - n * (n - 1) // 2
+        r["tflops"] = S * H * 2 * (ctx * 256 * 512 + pairs * 320) / r["ms"] / 1e9
+    return r
 
 
 def bench_sample(B, V, timed):
@@ -243,7 +280,8 @@ def bench_gemm_issue(M, N, K, units=3):
 
 def main(argv=None):
     p = argparse.ArgumentParser()
-    p.add_argument("what", choices=["gemm", "gemm_q4k", "gemm_issue", "moe", "decode", "prefill", "sample"])
+    p.add_argument("what", choices=["gemm", "gemm_q4k", "gemm_issue", "moe", "decode", "prefill", "latent_decode",
+                                    "latent_prefill", "sample"])
     p.add_argument("dims", nargs="+", type=int)
     p.add_argument("--epi", default="plain", choices=["plain", "bias", "residual", "swiglu"])
     p.add_argument("--time", action="store_true")
@@ -262,6 +300,10 @@ def main(argv=None):
         r = bench_decode(*a.dims[:4], a.time)
     elif a.what == "prefill":
         r = bench_prefill(*a.dims[:4], a.time)
+    elif a.what == "latent_decode":
+        r = bench_latent(a.dims[0], 1, a.dims[1], a.dims[2], a.time, True)
+    elif a.what == "latent_prefill":
+        r = bench_latent(*a.dims[:4], a.time, False)
     else:
         r = bench_sample(*a.dims[:2], a.time)
     print(json.dumps(r))
