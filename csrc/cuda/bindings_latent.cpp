@@ -295,7 +295,7 @@ void check_latent_prefill(Tensor q, Tensor cache, Tensor w, Tensor block_tables,
 
 // attention of `heads` heads: q / out already narrowed to them
 void latent_prefill(Tensor q, Tensor kv, Tensor k_rope, Tensor work, Tensor seq_info, Tensor out, int64_t heads,
-                    double scale, Tensor err) {
+                    double scale, int64_t ranges, c10::optional<Tensor> parts, Tensor err) {
   const char* op = "latent_prefill";
   TORCH_CHECK(q.is_cuda(), op, ": q must be a CUDA tensor");
   check(q, at::kBFloat16, q, op, "q");
@@ -326,6 +326,16 @@ void latent_prefill(Tensor q, Tensor kv, Tensor k_rope, Tensor work, Tensor seq_
   a.kv = bf(kv);
   a.kv_stride = kv.stride(0);
   a.kv_rows = kv.size(0);
+  TORCH_CHECK(ranges >= 1 && ranges <= 32, op, ": 1 to 32 key ranges");
+  if (ranges > 1) {
+    const int64_t rows = ranges * heads * work.size(0) * 256;
+    TORCH_CHECK(parts.has_value(), op, ": key ranges need room for partial results");
+    check(*parts, at::kFloat, q, op, "parts");
+    TORCH_CHECK(parts->is_contiguous() && parts->numel() >= rows * (kVal + 1), op, ": parts too small");
+    a.ranges = (int)ranges;
+    a.part_o = parts->data_ptr<float>();
+    a.part_lse = a.part_o + rows * kVal;
+  }
   a.k_rope = bf(k_rope);
   a.work = work.data_ptr<int32_t>();
   a.nwork = (int)work.size(0);

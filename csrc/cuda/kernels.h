@@ -98,6 +98,9 @@ struct LatentPrefill {
   int64_t out_stride = 0;
   int heads = 0;
   float scale = 0.f;
+  int ranges = 1;             // parts of the key tiles (at most 32), joined from
+  float* part_o = nullptr;    // [ranges, heads, nwork, 256, 128]
+  float* part_lse = nullptr;  // [ranges, heads, nwork, 256]
   int* err = nullptr;
 };
 void launch_latent_prefill(const LatentPrefill& a, cudaStream_t st);

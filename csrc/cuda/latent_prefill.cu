@@ -46,8 +46,8 @@ __device__ __forceinline__ bool wait_or_abort(Smem& s, uint64_t* bar, uint32_t p
 // out of the pages.  A CTA pair (cluster of 2) works on units of (256 context rows, head) with
 // cta_group::2 MMAs (M = 256, N = 256): each CTA holds 128 rows of one sequence and half of the
 // head's weights, so a CTA loads 16 KB of weights for 512 cycles of products (one CTA alone needs
-// 32 KB, and beside 128 KB of rows only two such stages fit: 1.7 x the time at 20k rows x 128
-// heads).  The units, rows outermost, are cut into equal stretches, one a pair; the rows stay in
+// 32 KB, and beside 128 KB of rows only two such stages fit: 1.45 x the time at 20k rows x
+// 128 heads).  The units, rows outermost, are cut into equal stretches, one a pair; the rows stay in
 // shared memory while the heads' weights stream past them, and two accumulators of 256 TMEM
 // columns let one unit's epilogue run beside the next one's products.
 // The epilogue turns 32-row slabs in shared memory so that every global store instruction
@@ -327,6 +327,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kExpandThreads, 1)
 // rows instead (and the second half's m, l and O join the first's at the end): the chain of
 // scores, softmax and product that bounds a lone row tile is half as long.
 //
+// Where the CTAs are too few for the GPU, gridDim.z ranges of key tiles give fp32 partial results
+// per row, which latent_prefill_join_kernel joins.
+//
 // Keys past a row's position have p = 0.  PV stops at the row tile's last key, rounded up
 // to 16; the rows there are the gather's zeros, so nothing behind a sequence is read.
 constexpr int kThreads = 384;  // warp 0 TMA, warp 1 MMA, warps 4-7 and 8-11 softmax of row tile 0 and 1
@@ -412,7 +415,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     latent_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap kv_map,
                           const __grid_constant__ CUtensorMap rope_map, const int32_t* work,
                           const int32_t* seq_info, int64_t q_rows, float scale_log2,
-                          bf16* out, int64_t out_stride, int* err) {
+                          bf16* out, int64_t out_stride, float* part_o, float* part_lse,
+                          int* err) {
   griddep_entry();
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   PrefillSmem& s = *reinterpret_cast<PrefillSmem*>(smem_raw);
@@ -420,14 +424,24 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int h = blockIdx.y;
   const int32_t* si = seq_info + 5 * work[2 * blockIdx.x];
   const int t0 = work[2 * blockIdx.x + 1];
-  const int row0 = si[0] + t0, n = si[1] - t0, pos0 = si[2] - si[1] + t0, kv0 = si[4];  // n: rows from t0 on
+  const int row0 = si[0] + t0, n = si[1] - t0;  // n: rows from t0 on
+  // this CTA's range of key tiles; keys and positions count from its first key
+  const int all_keys = si[2] - si[1] + t0 + min(n, 256);
+  const int range = ((all_keys + 127) / 128 + gridDim.z - 1) / gridDim.z * 128, key0 = blockIdx.z * range;
+  const int pos0 = si[2] - si[1] + t0 - key0, kv0 = si[4] + key0;
   // keys of the two halves, key tiles of the CTA and of each half
   const bool split = n <= 128;
-  const int keys0 = pos0 + min(n, 128), keys1 = split ? keys0 : pos0 + min(n, 256);
+  const int keys0 = max(0, min(range, pos0 + min(n, 128)));
+  const int keys1 = split ? keys0 : max(0, min(range, pos0 + min(n, 256)));
   const int nt = (keys1 + 127) / 128;
   const int nt0 = split ? (nt + 1) / 2 : (keys0 + 127) / 128, nt1 = split ? nt / 2 : nt;
+  const int64_t part_row = ((int64_t)(blockIdx.z * gridDim.y + h) * gridDim.x + blockIdx.x) * 256;
   if ((smem_u32(smem_raw) & 1023) || row0 < 0 || row0 + min(n, 256) > q_rows || n <= 0) {
     if (threadIdx.x == 0) atomicCAS(err, 0, 90);
+    return;
+  }
+  if (nt == 0) {  // no keys in this range
+    if (threadIdx.x < 256) part_lse[part_row + threadIdx.x] = -INFINITY;
     return;
   }
 
@@ -530,7 +544,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (last) mma_commit(&s.v_empty[j & 1]);
       };
-      issue_s(0, 0);
+      if (nt0 > 0) issue_s(0, 0);
       if (!split || nt > 1) issue_s(1, split ? 1 : 0);
       for (int j = 0; ok && j < nt; ++j) {
         if (split) {
@@ -629,7 +643,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (ok && tiles > 0) ok = wait_or_abort(s, &s.o_full[t], 0, err, 96);
     ok = __all_sync(0xffffffffu, ok && tiles > 0);
     tc_fence_after();
-    float f0 = 1.f, f1 = 0.f;  // factors of the halves' O
+    float f0 = 1.f, f1 = 0.f, m_out = m;  // factors of the halves' O, the maximum they count from
     // the second half's O [dim][row], m and l go through the ring: every tile of it has been used
     float* other = reinterpret_cast<float*>(s.ring[0]);
     const int at = quad * 32 + lane;
@@ -654,13 +668,34 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (t == 0) {
         const float m1 = other[128 * 128 + at], l1 = other[129 * 128 + at];
         if (l1 != 0.f) {  // a row without keys in the second half, or a half without tiles: 0
-          const float top = fmaxf(m, m1);
-          f0 = ex2(m - top), f1 = ex2(m1 - top);
+          const float top = l == 0.f ? m1 : fmaxf(m, m1);
+          f0 = l == 0.f ? 0.f : ex2(m - top), f1 = ex2(m1 - top);
           l = l * f0 + l1 * f1;
+          m_out = top;
         }
       }
     }
-    if (ok && !(split && t == 1)) {
+    if (part_o != nullptr) {
+      if (!(split && t == 1)) {
+        const float inv = !ok || l == 0.f ? 0.f : 1.f / l;
+        part_lse[part_row + row] = !ok || l == 0.f ? -INFINITY : m_out + __log2f(l);
+        if (split) part_lse[part_row + row + 128] = -INFINITY;
+        float* dst = part_o + (part_row + row) * kVal;
+        for (int c = 0; ok && c < 8; ++c) {
+          float o[16];
+          tmem_ld16(o_tmem + c * 16, o);
+          if (__any_sync(0xffffffffu, f1 != 0.f)) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              o[e] = o[e] * f0 + (f1 != 0.f ? other[(c * 16 + e) * 128 + at] * f1 : 0.f);
+          }
+#pragma unroll
+          for (int e = 0; e < 16; e += 4)
+            *reinterpret_cast<float4*>(dst + c * 16 + e) =
+                make_float4(o[e] * inv, o[e + 1] * inv, o[e + 2] * inv, o[e + 3] * inv);
+        }
+      }
+    } else if (ok && !(split && t == 1)) {
       const float inv = 1.f / l;
       bf16* dst = out + (int64_t)(row0 + row) * out_stride + (int64_t)h * kVal;
 #pragma unroll 1
@@ -690,6 +725,35 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
+}
+
+// out = sum_z 2^(lse_z - M) o_z / sum_z 2^(lse_z - M) over the key ranges z: one warp per (row of a row
+// tile, head), 4 dims a lane.
+__global__ void __launch_bounds__(256) latent_prefill_join_kernel(const float* part_o, const float* part_lse, int ranges,
+                                                                  const int32_t* work, const int32_t* seq_info,
+                                                                  bf16* out, int64_t out_stride) {
+  griddep_entry();
+  const int row = blockIdx.z * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31, h = blockIdx.y;
+  const int32_t* si = seq_info + 5 * work[2 * blockIdx.x];
+  const int t0 = work[2 * blockIdx.x + 1];
+  if (t0 + row >= si[1]) return;
+  const int64_t first = ((int64_t)h * gridDim.x + blockIdx.x) * 256 + row, step = (int64_t)gridDim.y * gridDim.x * 256;
+  const float lse = lane < ranges ? part_lse[first + lane * step] : -INFINITY;
+  float M = warp_max(lse);
+  if (M == -INFINITY) M = 0.f;
+  const float e = ex2(lse - M), L = warp_sum(e);
+  const float w = L == 0.f ? 0.f : e / L;
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int z = 0; z < ranges; ++z) {
+    const float f = __shfl_sync(0xffffffffu, w, z);
+    if (f != 0.f) {  // a range without keys wrote no partial result
+      const float4 y = *reinterpret_cast<const float4*>(part_o + (first + z * step) * kVal + lane * 4);
+      x.x += f * y.x, x.y += f * y.y, x.z += f * y.z, x.w += f * y.w;
+    }
+  }
+  *reinterpret_cast<uint2*>(out + (int64_t)(si[0] + t0 + row) * out_stride + h * kVal + lane * 4) =
+      make_uint2(pack_bf16(x.x, x.y), pack_bf16(x.z, x.w));
 }
 
 }  // namespace
@@ -726,8 +790,14 @@ void launch_latent_prefill(const LatentPrefill& a, cudaStream_t st) {
   const CUtensorMap tq = make_tmap_2d_bf16(a.q, a.T, (uint64_t)a.heads * (kNope + kRot), a.q_stride, 128, 64, true);
   const CUtensorMap tkv = make_tmap_2d_bf16(a.kv, a.kv_rows, (uint64_t)a.heads * (kNope + kVal), a.kv_stride, 128, 64, true);
   const CUtensorMap tr = make_tmap_2d_bf16(a.k_rope, a.kv_rows, kRot, kRot, 128, 64, true);
-  launch_k(latent_prefill_kernel, dim3(a.nwork, a.heads), kThreads, smem, st, tq, tkv, tr, a.work, a.seq_info, a.T,
-           a.scale * kLog2e, a.out, a.out_stride, a.err);
+  const bool ranges = a.ranges > 1;
+  launch_k(latent_prefill_kernel, dim3(a.nwork, a.heads, a.ranges), kThreads, smem, st, tq, tkv, tr, a.work, a.seq_info,
+           a.T, a.scale * kLog2e, a.out, a.out_stride, ranges ? a.part_o : nullptr, a.part_lse, a.err);
+  KAPSL_LAUNCH_CHECK();
+  note_launch();
+  if (!ranges) return;
+  launch_k(latent_prefill_join_kernel, dim3(a.nwork, a.heads, 32), 256, 0, st, a.part_o, a.part_lse, a.ranges, a.work,
+           a.seq_info, a.out, a.out_stride);
   KAPSL_LAUNCH_CHECK();
   note_launch();
 }

@@ -392,20 +392,29 @@ class LatentPrefillPlan:
     row_tiles: int          # 128-key tiles of all 256-row tiles of new tokens
     chain_us: float         # the longest of those row tiles by itself (microseconds)
 
+    def key_ranges(self, num_heads: int) -> int:
+        """Parts into which the expanded form cuts every row tile's keys: as often as the longest row tile
+        by itself takes what all of them take spread over the 148 SMs, parts of 4 key tiles or
+        more.  512 new tokens over 16384, 20 heads: 331 us whole, 187 in three parts; row tiles that
+        fill the GPU stay whole, since parts cost fp32 partial results and a joining kernel."""
+        spread = max(4.0, 1.9 * self.row_tiles * num_heads / 148)
+        return max(1, min(32, -(-self.max_ctx // 128) // 4, int(self.chain_us / spread)))
+
     def absorbed_is_shorter(self, num_heads: int, rank: int = 512) -> bool:
         """Whether taking every new token by itself in the absorbed form is estimated to take less time
         than expanding the contexts.  In microseconds, fitted to both forms' times on B200 (148
         SMs) over 34 ragged batches: absorbed, a 64-key tile of up to 64 heads 3.0 (rank 256: 1.4) of
         an SM and 2 for a thousand rows x heads of head products; expanded, 256 context rows of a head
         4.5 (2.3) of an SM pair, a 128-key tile of 256 new tokens 1.9 of an SM, or the longest row
-        tile by itself.  20 new tokens over 4020, 8 heads: 35 and 80; five prompts of 17 to 300
-        tokens, 28 heads: 98 and 58."""
-        rows, wide = self.rows - self.q_start, rank > 256
+        tile by itself, or a key range of it and 9 for the join.  20 new tokens over 4020, 8
+        heads: 37 and 46; five prompts of 17 to 300 tokens, 28 heads: 98 and 59."""
+        rows, wide, ranges = self.rows - self.q_start, rank > 256, self.key_ranges(num_heads)
         start = 19 if -(-rows // 16) * num_heads <= 256 else 26
         absorbed = (start + (3.0 if wide else 1.4) * self.single_tiles * -(-num_heads // 64) / 148 +
                     0.002 * rows * num_heads)
         expanded = 20 + 1.2 * ((4.5 if wide else 2.3) * -(-self.kv_work.shape[0] // 2) * num_heads / 74 +
-                               max(self.chain_us, 1.9 * self.row_tiles * num_heads / 148))
+                               max(self.chain_us / ranges, 1.9 * self.row_tiles * num_heads / 148) +
+                               9 * (ranges > 1))
         return absorbed < expanded and rows <= 4096
 
 
@@ -460,7 +469,8 @@ def latent_prefill_plan(q_lens: Sequence[int], ctx_lens: Sequence[int], device, 
 
 def latent_prefill_attention(q: torch.Tensor, cache: torch.Tensor, w_kv_b: torch.Tensor, plan: LatentPrefillPlan,
                              block_tables: torch.Tensor, num_heads: int, scale: Optional[float] = None,
-                             out: Optional[torch.Tensor] = None, form: Optional[str] = None) -> torch.Tensor:
+                             out: Optional[torch.Tensor] = None, form: Optional[str] = None,
+                             key_ranges: int = 0) -> torch.Tensor:
     """Causal latent attention of chunks of new tokens over the paged latent cache.
 
     The new tokens' rows are in ``cache`` already; arguments as in
@@ -469,7 +479,8 @@ def latent_prefill_attention(q: torch.Tensor, cache: torch.Tensor, w_kv_b: torch
     and values (at most ``LATENT_KV_BYTES`` of them at a time, in passes over the heads); in
     the absorbed form every new token is a row of :func:`latent_decode_attention`, which is
     shorter for few of them.  ``form`` ("expanded" or "absorbed") overrides
-    :meth:`LatentPrefillPlan.absorbed_is_shorter`; the two round differently.  Page slots behind
+    :meth:`LatentPrefillPlan.absorbed_is_shorter`, ``key_ranges`` (1 to 32, expanded form)
+    :meth:`LatentPrefillPlan.key_ranges`; the two forms round differently.  Page slots behind
     a context may hold anything; its own rows have to be finite, since in the expanded form
     a row that is not also reaches earlier new tokens (0 * NaN in the product with the values).
     ``out`` rows outside the plan's sequences keep what they held (zeros when ``out`` is
@@ -496,13 +507,17 @@ def latent_prefill_attention(q: torch.Tensor, cache: torch.Tensor, w_kv_b: torch
     step = max(1, min(num_heads, LATENT_KV_BYTES // (plan.kv_rows * 512)))
     k_rope = torch.empty(plan.kv_rows, 64, dtype=torch.bfloat16, device=q.device)
     kv_buf = torch.empty(plan.kv_rows * step * 256, dtype=torch.bfloat16, device=q.device)
+    ranges = key_ranges if key_ranges > 0 else plan.key_ranges(min(step, num_heads))
+    parts = None
+    if ranges > 1:
+        parts = torch.empty(ranges * step * plan.work.shape[0] * 256 * 129, dtype=torch.float32, device=q.device)
     for h0 in range(0, num_heads, step):
         n = min(step, num_heads - h0)
         kv = kv_buf[:plan.kv_rows * n * 256].view(plan.kv_rows, n * 256)
         c.latent_expand(cache, w[h0 * 256:(h0 + n) * 256], plan.kv_work, plan.seq_info, block_tables, kv,
                         k_rope if h0 == 0 else None, err)
         c.latent_prefill(q[:, h0 * 192:(h0 + n) * 192], kv, k_rope, plan.work, plan.seq_info,
-                         out[:, h0 * 128:(h0 + n) * 128], n, float(scale), err)
+                         out[:, h0 * 128:(h0 + n) * 128], n, float(scale), ranges, parts, err)
     return out
 
 

@@ -25,6 +25,17 @@ def test_plan_rows_and_tiles():
     assert p.single_tiles == sum(-(-c // 64) for c in p.row_ctx.tolist())
 
 
+def test_plan_key_ranges():
+    def ranges(q_lens, ctx_lens, heads):
+        return ops.latent_prefill_plan(q_lens, ctx_lens, device="cpu").key_ranges(heads)
+
+    assert ranges([512], [16384], 20) == 3      # few row tiles over a long context
+    assert ranges([20], [4020], 8) == 8         # never under 4 key tiles a part
+    assert ranges([2048] * 4, [8192] * 4, 128) == 1  # a full GPU
+    assert ranges([17, 1], [17, 300], 4) == 1   # short contexts
+    assert ranges([256], [200000], 1) == 32     # what the join takes
+
+
 def test_plan_of_nothing():
     p = ops.latent_prefill_plan([], [], device="cpu")
     assert p.work.shape == (0, 2) and p.seq_info.shape == (0, 5) and p.kv_rows == 0 and p.tables == 0

@@ -460,6 +460,26 @@ def test_prefill_passes_over_heads(dev, monkeypatch):
     no_error(dev)
 
 
+@pytest.mark.parametrize("key_ranges", [2, 3, 7, 32])
+def test_prefill_key_ranges(dev, key_ranges):
+    """The keys in parts: parts that end inside a row's keys, that only later rows see, that hold nothing."""
+    from kapsl_sdk_b200 import ops
+
+    q_lens, ctx_lens, H, R = [300, 20, 129, 1], [1100, 2000, 129, 7], 3, 512
+    k = Cache(dev, ctx_lens, R, 16, 21)
+    q, w = k.randn(sum(q_lens), H * 192, std=1.5), k.randn(H * 256, R, std=1 / math.sqrt(R))
+    plan = ops.latent_prefill_plan(q_lens, ctx_lens, dev)
+    out = ops.latent_prefill_attention(q, k.cache, w, plan, k.bt, H, form="expanded", key_ranges=key_ranges)
+    no_error(dev)
+    at = 0
+    for i, n in enumerate(q_lens):
+        exp, tol = prefill64(q[at:at + n].view(n, H, 192), k.rows[i], w.view(H, 256, R), 1 / math.sqrt(192))
+        within(out[at:at + n].view(n, H, 128), exp, tol)
+        at += n
+    with pytest.raises(RuntimeError):
+        ops.latent_prefill_attention(q, k.cache, w, plan, k.bt, H, form="expanded", key_ranges=33)
+
+
 def test_prefill_picks_a_form(dev):
     """Few tokens over a long context go by themselves, a long chunk is expanded; the result is that of the
     form named."""
