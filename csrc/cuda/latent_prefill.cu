@@ -4,6 +4,12 @@
 // and value rows (kv = w_h c, [128 | 128] a head), and the attention runs with keys
 // [k_h (128) | k_r (64, shared)] and values of 128:
 //   out_i = sum_j softmax_j(scale q_i . k_j) v_j  over j <= position of i.
+//
+// Roundings: the expanded keys and values are bf16, the type of the query's rows that the first
+// product takes and half the bytes of fp32, and so is P, the second product's operand (sums
+// are fp32).  fp16 would keep 3 bits more, but not every model's values are within its range.  With the
+// output's own, three roundings of 2^-9 at most: an output is 0.0029 from 64-bit arithmetic
+// in the mean square, where one rounded once at the end is 0.0017.
 #include <algorithm>
 
 #include "common.cuh"
