@@ -46,18 +46,18 @@ constexpr int kMaxPieces = 33;
 
 __host__ __device__ constexpr int table_ints(int B) { return (B + 2 + 31) / 32 * 32; }
 
-__device__ __forceinline__ int seq_tiles(const int32_t* ctx_lens, int b, int limit) {
-  return (max(0, min(ctx_lens[b], limit)) + kKeys - 1) / kKeys;
+__device__ __forceinline__ int seq_tiles(const int32_t* ctx_lens, int b, int limit, int keys) {
+  return (max(0, min(ctx_lens[b], limit)) + keys - 1) / keys;
 }
 
 // One block writes the table (`limit`: tokens the block tables hold).
-__device__ void write_schedule(const int32_t* ctx_lens, int B, int limit, int ctas, int32_t* table) {
+__device__ void write_schedule(const int32_t* ctx_lens, int B, int limit, int keys, int ctas, int32_t* table) {
   __shared__ int sums[33], longest;
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5, nw = blockDim.x >> 5;
   if (t == 0) longest = 0;
   int base = 0;
   for (int b0 = 0; b0 < B; b0 += blockDim.x) {
-    const int n = b0 + t < B ? seq_tiles(ctx_lens, b0 + t, limit) : 0;
+    const int n = b0 + t < B ? seq_tiles(ctx_lens, b0 + t, limit, keys) : 0;
     int x = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -634,6 +634,526 @@ __global__ void __launch_bounds__(kAttnThreads<R>, 1)
   }
 }
 
+// ------------------------------------------------------------- attention, CTA pairs
+//
+// Up to 128 heads of a rank-512 latent.  Here the heads are the MMA's M:
+//   S [128 heads, 64 keys] = qa . K^T     O [128 heads, 256 dims] += P . c
+// A cluster of two CTAs takes tiles of 128 keys.  Each computes the scores of its own 64 and
+// the output's own 256 dims over all 128, so the scores' operand qa may come from tensor memory
+// (O takes 256 columns, two thirds of qa 192, S 64) and no product is done twice: an MMA reads
+// its 2 KB of keys for 32 cycles of work, where the 64-head form reads 4 KB of operands.
+// The two CTAs exchange the rows' maxima (st.async, one float a row and tile) and P (4 KB a
+// warp, copied from shared memory to shared memory): both scale a row by the same maximum.
+// The values of the other CTA's keys come from L2 a second time (13 chunks of 64 keys x 64 dims
+// a tile instead of 9).
+//
+// S(t + 1) is issued before the second product of t: the softmax warps (one thread a head) take
+// S(t) into registers at once, so one S tile in tensor memory is enough, and maxima, exponentials
+// and the exchange of P run behind S(t + 1).  The chunks live in three rings, each in the order
+// in which it is freed: a: the 5 that only the scores read, b: the 4 of the own keys and dims,
+// which both products read (two tiles), c: the 4 of the other's keys.
+//
+// Whole calls, 64-head tiles and pairs: 192 x 8192 tokens x 128 heads 674 and 531 us, 64 x 4096 x 128 145
+// and 121, 64 x 500 x 128 56 and 51, 16 x 1000 x 80 31 and 30; at 64 heads and fewer, where half
+// of the MMA's rows would be empty, 151 and 189 (64 x 8192 x 64).
+constexpr int kPairThreads = 256;  // warps 0-2 TMA (a, b, c), 3 MMA, 4-7 softmax
+constexpr int kPairKeys = 128;
+constexpr int kPairHeads = 64;  // more heads than this take pairs
+constexpr uint32_t kChunk = 64 * 128;  // 64 keys x 64 dims
+
+struct alignas(1024) PairSmem {
+  uint8_t a[6][kChunk];
+  uint8_t b[2][4][kChunk];
+  uint8_t c[4][kChunk];
+  uint8_t q[3][128 * 128];
+  uint8_t p[2][128 * 128];  // by the CTA whose keys they are of
+  float other[2][128];      // the other CTA's maxima (or sums)
+  uint64_t a_full[6], a_empty[6], b_full[2], b_empty[2], c_full, c_empty, q_full, q_empty, s_full, s_free, p_full,
+      p_free, other_full[2][4], drained;
+  uint32_t tmem_base;
+  volatile int abort_flag;
+};
+
+__device__ __forceinline__ uint32_t pair_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void pair_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t in_cta(const void* p, uint32_t rank) {  // the same place in a CTA of the cluster
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  return a;
+}
+// wait_or_abort that polls: the clock and the abort flag are read rarely (both are slow beside a poll)
+__device__ __forceinline__ bool poll_or_abort(PairSmem& s, uint64_t* bar, uint32_t parity, int* err, int code) {
+  uint64_t t0 = 0;
+  for (uint32_t spin = 1;; ++spin) {
+    if (mbar_test_wait(bar, parity)) return true;
+    if ((spin & 1023) == 0) {
+      const uint64_t now = globaltimer_ns();
+      if (t0 == 0) t0 = now;
+      if (s.abort_flag) return false;
+      if (now - t0 > 2000000000ull) {
+        atomicCAS(err, 0, code);
+        s.abort_flag = 1;
+        return false;
+      }
+    }
+  }
+}
+__device__ __forceinline__ bool try_wait_cluster(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+    latent_attn_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap c_map,
+                            const bf16* qa, int64_t num_blocks, int page, const int32_t* block_tables,
+                            int max_blocks, const int32_t* table_rows, int num_tables, const int32_t* ctx_lens,
+                            const int32_t* table, float* part_o, float* part_lse, int B, int H,
+                            int heads_per_cta, int head_tiles, float scale_log2, int* err) {
+  griddep_launch();
+  constexpr int R = 512, W = R + kRot;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  PairSmem& s = *reinterpret_cast<PairSmem*>(smem_raw);
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
+  const int rank = (int)pair_rank(), pair = blockIdx.x / 2;
+  const int ht = pair % head_tiles, c = pair / head_tiles;
+  const int pairs = gridDim.x / 2 / head_tiles;
+  const int h0 = ht * heads_per_cta, nheads = min(heads_per_cta, H - h0);
+  if (smem_u32(smem_raw) & 1023) {  // the same in both CTAs
+    if (threadIdx.x == 0) atomicCAS(err, 0, 83);
+    return;
+  }
+  if (threadIdx.x == 0) {
+    s.abort_flag = 0;
+    for (int i = 0; i < 6; ++i) {
+      mbar_init(&s.a_full[i], 1);
+      mbar_init(&s.a_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s.b_full[i], 1);
+      mbar_init(&s.b_empty[i], 1);
+      for (int w = 0; w < 4; ++w) mbar_init(&s.other_full[i][w], 1);
+    }
+    mbar_init(&s.c_full, 1);
+    mbar_init(&s.c_empty, 1);
+    mbar_init(&s.q_full, 5);  // the copies, and four warps' part in tensor memory
+    mbar_init(&s.q_empty, 1);
+    mbar_init(&s.s_full, 1);
+    mbar_init(&s.s_free, 4);
+    mbar_init(&s.p_full, 4);  // and the bytes of the other CTA's P
+    mbar_init(&s.p_free, 2);  // both CTAs' second product
+    mbar_init(&s.drained, 1);
+    fence_barrier_init();
+  }
+  griddep_wait();  // before the allocation: a CTA of the grid waited for may still need its own
+  if (warp == 3) tmem_alloc(&s.tmem_base, 512);
+  tc_fence_before();
+  pair_sync();  // both CTAs' barriers stand before the other uses them
+  tc_fence_after();
+  const uint32_t tmem = __shfl_sync(0xffffffffu, s.tmem_base, 0);
+  const uint32_t tmem_q = tmem + 64, tmem_o = tmem + 256;
+  Pieces pc(table, ctx_lens, B, max_blocks * page, c);
+  // The chunk of 64 dims that is the i-th in the scores' product: the rotary dims, the other CTA's
+  // 256 dims, the own.  The first three of qa are in shared memory, the rest in tensor memory.
+  auto dims = [&](int i) { return i == 0 ? R : i < 5 ? 256 * (1 - rank) + 64 * (i - 1) : 256 * rank + 64 * (i - 5); };
+
+  if (warp < 3) {
+    // ------------------------------------------------------------ TMA producers
+    const int half = warp == 2 ? 1 - rank : rank;  // whose keys of the tile
+    const int pages = kKeys / page;
+    const int oob = (int)(num_blocks * page);  // a row past the cache reads as zeros
+    int sent = 0, chunks = 0, nq = 0;
+    bool ok = true;
+    auto page_row = [&](int trow, int tile) {  // lane l < pages: first row of page l of the 64 keys
+      const int j = (2 * tile + half) * pages + lane;
+      if (lane >= pages || j >= (pc.keys() + page - 1) / page) return oob;
+      const int blk = trow >= 0 && trow < num_tables ? block_tables[(int64_t)trow * max_blocks + j] : -1;
+      if (blk >= 0 && blk < num_blocks) return blk * page;
+      atomicCAS(err, 0, 82);
+      return oob;
+    };
+    for (; ok && pc.more(); pc.next()) {
+      const int b = pc.b, t0 = pc.first(), n = pc.tiles();
+      const int trow = table_rows != nullptr ? table_rows[b] : b;
+      int y = page_row(trow, t0), y1 = n > 1 ? page_row(trow, t0 + 1) : oob;
+      if (warp == 0) {
+        if (nq > 0) ok = poll_or_abort(s, &s.q_empty, (nq - 1) & 1, err, 84);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        if (elect_one()) {
+          mbar_arrive_expect_tx(&s.q_full, sizeof(s.q));
+          for (int i = 0; i < 3; ++i) tma_load_2d(s.q[i], &q_map, &s.q_full, dims(i), b * H + h0);
+        }
+        ++nq;
+      }
+      for (int i = 0; i < n; ++i, ++sent) {
+        const int y2 = i + 2 < n ? page_row(trow, t0 + i + 2) : oob;
+        int yy[4], zz[4];
+#pragma unroll
+        for (int pg = 0; pg < 4; ++pg) {
+          yy[pg] = __shfl_sync(0xffffffffu, y, pg);
+          zz[pg] = __shfl_sync(0xffffffffu, y1, pg);
+        }
+        if (warp < 2 && elect_one()) {  // the next tile comes into L2 while its slots are still in use
+          const int first = warp == 0 ? 0 : 5, last = warp == 0 ? 5 : 9;
+#pragma unroll
+          for (int pg = 0; pg < 4; ++pg)
+            if (pg < pages && zz[pg] < oob)
+              for (int k = first; k < last; ++k) tma_prefetch_2d(&c_map, dims(k), zz[pg]);
+        }
+        __syncwarp();
+        auto load = [&](uint8_t* dst, uint64_t* bar, int x) {
+#pragma unroll
+          for (int pg = 0; pg < 4; ++pg)
+            if (pg < pages) tma_load_2d(dst + pg * page * 128, &c_map, bar, x, yy[pg]);
+        };
+        if (warp == 0) {
+          for (int k = 0; ok && k < 5; ++k) {
+            const int st = chunks % 6;
+            if (chunks >= 6) ok = poll_or_abort(s, &s.a_empty[st], (chunks / 6 - 1) & 1, err, 84);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            if (elect_one()) {
+              mbar_arrive_expect_tx(&s.a_full[st], kChunk);
+              load(s.a[st], &s.a_full[st], dims(k));
+            }
+            __syncwarp();
+            ++chunks;
+          }
+          if (!ok) break;
+        } else {
+          const int st = warp == 1 ? sent & 1 : 0;
+          uint64_t* full = warp == 1 ? &s.b_full[st] : &s.c_full;
+          if (warp == 1 && sent >= 2) ok = poll_or_abort(s, &s.b_empty[st], ((sent >> 1) - 1) & 1, err, 84);
+          if (warp == 2 && sent >= 1) ok = poll_or_abort(s, &s.c_empty, (sent - 1) & 1, err, 84);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          if (elect_one()) {
+            mbar_arrive_expect_tx(full, 4 * kChunk);
+            for (int k = 0; k < 4; ++k) load(warp == 1 ? s.b[st][k] : s.c[k], full, 256 * rank + 64 * k);
+          }
+          __syncwarp();
+        }
+        y = y1;
+        y1 = y2;
+      }
+    }
+    // the copies in flight end before the CTA does, on the way out of a time-out too
+    if (lane == 0) {
+      if (warp == 0) {
+        if (nq > 0) {  // the other arrivals of q_full may be missing after a time-out: chunks alone tell
+          for (int i = max(0, chunks - 6); i < chunks; ++i) mbar_wait_sleep(&s.a_full[i % 6], (i / 6) & 1);
+          mbar_wait_sleep(&s.q_full, (nq - 1) & 1);
+        }
+      } else if (warp == 1) {
+        for (int i = max(0, sent - 2); i < sent; ++i) mbar_wait_sleep(&s.b_full[i & 1], (i >> 1) & 1);
+      } else if (sent > 0) {
+        mbar_wait_sleep(&s.c_full, (sent - 1) & 1);
+      }
+    }
+  } else if (warp == 3) {
+    // -------------------------------------------------------------- MMA issuer
+    if (elect_one()) {
+      constexpr uint32_t idesc_s = idesc_bf16<128, 64>();
+      constexpr uint32_t idesc_o = idesc_bf16<128, 256>() | kIdescBMn;
+      constexpr uint64_t kStep = kChunk >> 4;
+      const uint64_t a_desc = smem_desc_sw128(smem_u32(s.a[0])), b_desc = smem_desc_sw128(smem_u32(s.b[0][0]));
+      const uint64_t q_desc = smem_desc_sw128(smem_u32(s.q[0]));
+      const uint64_t p_own = smem_desc_sw128(smem_u32(s.p[rank])), p_other = smem_desc_sw128(smem_u32(s.p[1 - rank]));
+      const uint64_t v_own = smem_desc_mn_sw128(smem_u32(s.b[0][0]), kChunk, 1024);
+      const uint64_t v_other = smem_desc_mn_sw128(smem_u32(s.c[0]), kChunk, 1024);
+      const int total = pc.end - pc.at;
+      Pieces sp = pc;
+      int left_s = sp.more() ? sp.tiles() : 0, left_p = left_s, nq = 0, chunks = 0;
+      bool ok = true, first_s = true, first_p = true;
+      for (int t = 0; ok && t <= total; ++t) {
+        if (t < total) {
+          if (first_s) ok = poll_or_abort(s, &s.q_full, nq & 1, err, 86);
+          if (t > 0) ok = ok && poll_or_abort(s, &s.s_free, (t - 1) & 1, err, 86);
+          for (int k = 0; ok && k < 5; ++k, ++chunks) {
+            const int st = chunks % 6;
+            ok = poll_or_abort(s, &s.a_full[st], (chunks / 6) & 1, err, 86);
+            if (!ok) break;
+            tc_fence_after();
+            if (k < 3) {
+#pragma unroll
+              for (int kk = 0; kk < 4; ++kk)
+                mma_bf16(tmem, q_desc + k * 1024 + kk * 2, a_desc + st * kStep + kk * 2, idesc_s, k + kk > 0);
+            } else {
+#pragma unroll
+              for (int kk = 0; kk < 4; ++kk)
+                mma_bf16_tmem_a(tmem, tmem_q + (k - 3) * 32 + kk * 8, a_desc + st * kStep + kk * 2, idesc_s, 1);
+            }
+            mma_commit(&s.a_empty[st]);
+          }
+          ok = ok && poll_or_abort(s, &s.b_full[t & 1], (t >> 1) & 1, err, 86);
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              mma_bf16_tmem_a(tmem, tmem_q + (k + 2) * 32 + kk * 8, b_desc + ((t & 1) * 4 + k) * kStep + kk * 2,
+                              idesc_s, 1);
+          mma_commit(&s.s_full);
+          first_s = false;
+          if (--left_s == 0) {  // the piece's last scores: its queries are free
+            mma_commit(&s.q_empty);
+            ++nq;
+            first_s = true;
+            sp.next();
+            left_s = sp.more() ? sp.tiles() : 0;
+          }
+        }
+        if (t > 0) {
+          const int u = t - 1;
+          ok = poll_or_abort(s, &s.p_full, u & 1, err, 86) && poll_or_abort(s, &s.c_full, u & 1, err, 86);
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            mma_bf16(tmem_o, p_own + kk * 2, v_own + (u & 1) * 4 * kStep + kk * 128, idesc_o, !(first_p && kk == 0));
+          mma_commit(&s.b_empty[u & 1]);
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk) mma_bf16(tmem_o, p_other + kk * 2, v_other + kk * 128, idesc_o, 1);
+          mma_commit(&s.c_empty);
+          asm volatile(  // on both CTAs' barrier
+              "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+                  smem_u32(&s.p_free)),
+              "h"((uint16_t)3)
+              : "memory");
+          first_p = false;
+          if (--left_p == 0) {
+            pc.next();
+            left_p = pc.more() ? pc.tiles() : 0;
+            first_p = true;
+          }
+        }
+      }
+      // every MMA issued has finished before the tensor memory is freed
+      mma_commit(&s.drained);
+      mbar_wait_sleep(&s.drained, 0);
+    }
+  } else {
+    // ------------------------------------------------------- softmax, epilogue
+    const int quad = warp & 3, row = quad * 32 + lane;  // head h0 + row
+    const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
+    const uint32_t peer_val = in_cta(&s.other[0][row], 1 - rank), peer_bar = in_cta(&s.other_full[0][quad], 1 - rank);
+    const uint32_t peer_p = in_cta(s.p[rank] + quad * 4096, 1 - rank), peer_p_full = in_cta(&s.p_full, 1 - rank);
+    int xch = 0;  // exchanges with the other CTA
+    // A thread sends x + 1 after it has read x: two places are enough.
+    auto send = [&](float v) {
+      const int at = xch & 1;
+      if (lane == 0) mbar_arrive_expect_tx(&s.other_full[at][quad], 128);
+      asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(
+                       peer_val + at * 512),
+                   "r"(__float_as_uint(v)), "r"(peer_bar + at * 32)
+                   : "memory");
+    };
+    auto receive = [&]() {
+      const int at = xch & 1;
+      uint64_t* bar = &s.other_full[at][quad];
+      const uint64_t t0 = globaltimer_ns();
+      while (!try_wait_cluster(bar, (xch >> 1) & 1) && !s.abort_flag) {
+        if (globaltimer_ns() - t0 > 2000000000ull) {
+          atomicCAS(err, 0, 87);
+          s.abort_flag = 1;
+        }
+      }
+      __syncwarp();
+      ++xch;
+      return s.other[at][row];
+    };
+    auto load_q = [&](int b) {  // qa's later six chunks of this thread's head -> tensor memory
+      const bf16* src = qa + ((int64_t)b * H + h0 + row) * W;
+#pragma unroll 1
+      for (int g = 0; g < 3; ++g) {
+        uint4 v[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k)
+          v[k] = row < nheads ? *reinterpret_cast<const uint4*>(src + dims(3 + 2 * g + k / 8) + k % 8 * 8)
+                              : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          uint32_t u[16];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            u[4 * e] = v[4 * k + e].x, u[4 * e + 1] = v[4 * k + e].y;
+            u[4 * e + 2] = v[4 * k + e].z, u[4 * e + 3] = v[4 * k + e].w;
+          }
+          tmem_st16(tmem_q + lane_off + g * 64 + k * 16, u);
+        }
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s.q_full);
+    };
+    if (pc.more()) load_q(pc.b);
+    int tile = 0;  // of the pair
+    bool live = true;  // false after a time-out
+    while (pc.more()) {
+      const int b = pc.b, n_tiles = pc.tiles();
+      const int left = pc.keys() - pc.first() * kPairKeys;  // keys from the piece's first on
+      float m = -INFINITY, l = 0.f;
+      for (int i = 0; i < n_tiles; ++i, ++tile) {
+        live = __all_sync(0xffffffffu, poll_or_abort(s, &s.s_full, tile & 1, err, 88) && !s.abort_flag);
+        if (!live) break;
+        tc_fence_after();
+        float v[2][32];
+        {
+          uint32_t r0[32], r1[32];
+          tmem_ld_start(tmem + lane_off, r0);
+          tmem_ld_start(tmem + lane_off + 32, r1);
+          tmem_ld_wait(r0);
+          tmem_ld_wait(r1);
+#pragma unroll
+          for (int n = 0; n < 32; ++n) {
+            v[0][n] = __uint_as_float(r0[n]) * scale_log2;
+            v[1][n] = __uint_as_float(r1[n]) * scale_log2;
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s.s_free);
+        const int valid = left - i * kPairKeys - rank * 64;  // of this CTA's keys
+        if (valid < 64) {
+#pragma unroll
+          for (int n = 0; n < 64; ++n)
+            if (n >= valid) v[n >> 5][n & 31] = -INFINITY;
+        }
+        float top4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int n = 0; n < 64; ++n) top4[n & 3] = fmaxf(top4[n & 3], v[n >> 5][n & 31]);
+        const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3]));
+        send(top);
+        uint32_t p[32];
+        float sum;
+        auto exps = [&]() {
+          const float ref = m == -INFINITY ? 0.f : m;  // no finite score yet: every p is 0 or NaN
+          float add[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int n = 0; n < 64; n += 2) {
+            const float e0 = ex2(v[n >> 5][n & 31] - ref), e1 = ex2(v[n >> 5][(n & 31) + 1] - ref);
+            add[n & 2] += e0;
+            add[(n & 2) + 1] += e1;
+            p[n >> 1] = pack_bf16(e0, e1);
+          }
+          sum = (add[0] + add[1]) + (add[2] + add[3]);
+        };
+        if (i > 0) exps();  // with the present maximum, while the other CTA's is under way
+        const float M = fmaxf(top, receive());
+        const bool up = M > m + kRaise;
+        const bool raise = __any_sync(0xffffffffu, up);
+        if (tile > 0) poll_or_abort(s, &s.p_free, (tile - 1) & 1, err, 89);  // P is free, O at rest
+        __syncwarp();
+        if (raise && i > 0) {
+          const float fac = up ? ex2(m - M) : 1.f;
+          l *= fac;
+          tc_fence_after();
+#pragma unroll 1
+          for (int k = 0; k < 16; ++k) {
+            float o[16];
+            uint32_t u[16];
+            tmem_ld16(tmem_o + lane_off + k * 16, o);
+#pragma unroll
+            for (int n = 0; n < 16; ++n) u[n] = __float_as_uint(o[n] * fac);
+            tmem_st16(tmem_o + lane_off + k * 16, u);
+          }
+          tmem_wait_st();
+        }
+        if (up) m = M;
+        if (raise || i == 0) exps();
+        l += sum;
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          *reinterpret_cast<uint4*>(s.p[rank] + sw128_offset(row, k)) =
+              make_uint4(p[4 * k], p[4 * k + 1], p[4 * k + 2], p[4 * k + 3]);
+        if (left - i * kPairKeys < kPairKeys) {  // the sequence's last tile: value rows past the context
+          poll_or_abort(s, &s.b_full[tile & 1], (tile >> 1) & 1, err, 88);
+          poll_or_abort(s, &s.c_full, tile & 1, err, 88);
+#pragma unroll 1
+          for (int own = 0; own < 2; ++own) {
+            const int first = max(0, left - i * kPairKeys - (own ? rank : 1 - rank) * 64);
+            uint8_t* at = own ? s.b[tile & 1][0] : s.c[0];
+            for (int e = row; e < (64 - first) * 32; e += 128)  // 16-byte vectors of a row's 256 dims
+              *reinterpret_cast<uint4*>(at + (e & 31) / 8 * kChunk + (first + (e >> 5)) * 128 + (e & 7) * 16) =
+                  make_uint4(0, 0, 0, 0);
+          }
+        }
+        fence_proxy_async_smem();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          asm volatile(
+              "cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                  peer_p),
+              "r"(smem_u32(s.p[rank] + quad * 4096)), "r"(4096), "r"(peer_p_full)
+              : "memory");
+          if (quad == 0) {
+            mbar_arrive_expect_tx(&s.p_full, 128 * 128);
+          } else {
+            mbar_arrive(&s.p_full);
+          }
+        }
+      }
+      if (!live) break;
+      // ---- the piece's partial result; the next piece's queries first
+      send(l);
+      pc.next();
+      if (pc.more()) load_q(pc.b);
+      l += receive();
+      poll_or_abort(s, &s.p_free, (tile - 1) & 1, err, 89);
+      __syncwarp();
+      tc_fence_after();
+      const int64_t slot = ((int64_t)ht * (B + pairs) + b + c) * heads_per_cta;
+      if (rank == 0 && row < nheads) part_lse[slot + row] = l == 0.f ? -INFINITY : m + __log2f(l);
+      const float inv = l == 0.f ? 0.f : __fdividef(1.f, l);
+      uint8_t* turn = s.p[rank] + quad * 4096;  // 32 rows x 32 dims, turned for whole-line stores
+#pragma unroll 1
+      for (int k = 0; k < 8; ++k) {
+        float o[32];
+        tmem_ld32w(tmem_o + lane_off + k * 32, o);
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+          *reinterpret_cast<float4*>(turn + lane * 128 + ((q ^ (lane & 7)) * 16)) =
+              make_float4(o[4 * q] * inv, o[4 * q + 1] * inv, o[4 * q + 2] * inv, o[4 * q + 3] * inv);
+        __syncwarp();
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          const int r = 4 * q + (lane >> 3), seg = lane & 7;
+          if (quad * 32 + r < nheads)
+            *reinterpret_cast<float4*>(part_o + (slot + quad * 32 + r) * R + rank * 256 + k * 32 + seg * 4) =
+                *reinterpret_cast<const float4*>(turn + r * 128 + ((seg ^ (r & 7)) * 16));
+        }
+        __syncwarp();
+      }
+      tc_fence_before();  // O has been read: ordered before the next p_full
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (s.abort_flag && threadIdx.x == 0)  // after a time-out: copies to the other CTA have long landed
+    for (const uint64_t t0 = globaltimer_ns(); globaltimer_ns() - t0 < 100000;) {
+    }
+  pair_sync();  // no CTA leaves while its peer may still write to it
+  if (warp == 3) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
 // -------------------------------------------------------------- head products
 //
 // y[b, h, n] = sum_k x[b, h, k] w_h[k, n], small matrices per head, bound by the weights (128 KB +
@@ -674,12 +1194,12 @@ __device__ __forceinline__ void copy_rotary(const bf16* q, int64_t q_stride, bf1
 template <int R>
 __global__ void __launch_bounds__(128) latent_absorb_kernel(const bf16* q, int64_t q_stride,
                                                             const bf16* w, bf16* qa, int B,
-                                                            int H, const int32_t* ctx_lens, int limit,
+                                                            int H, const int32_t* ctx_lens, int limit, int keys,
                                                             int ctas, int32_t* table) {
   griddep_entry();
   constexpr int MROWS = 16;
   if (blockIdx.x == gridDim.x - 1 && blockIdx.y == 0 && blockIdx.z == 0)
-    write_schedule(ctx_lens, B, limit, ctas, table);
+    write_schedule(ctx_lens, B, limit, keys, ctas, table);
   constexpr int kPitchW = 64 + 8, kPitchX = kNope + 8;  // 16 bytes of padding: conflict-free ldmatrix
   __shared__ __align__(16) bf16 ws[kNope * kPitchW];
   __shared__ __align__(16) bf16 xs[MROWS * kPitchX];
@@ -919,7 +1439,7 @@ template <int R>
 __global__ void __launch_bounds__(128) latent_absorb_tc_kernel(const __grid_constant__ CUtensorMap q_map,
                                                                const __grid_constant__ CUtensorMap w_map, const bf16* q,
                                                                int64_t q_stride, bf16* qa, int B, int H,
-                                                               const int32_t* ctx_lens, int limit, int ctas,
+                                                               const int32_t* ctx_lens, int limit, int keys, int ctas,
                                                                int32_t* table, int* err) {
   griddep_launch();
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -962,7 +1482,7 @@ __global__ void __launch_bounds__(128) latent_absorb_tc_kernel(const __grid_cons
     copy_rotary<R, 128>(q + (int64_t)b0 * q_stride, q_stride, qa + (int64_t)b0 * H * (R + kRot), B - b0, H, h);
   }
   if (blockIdx.x == gridDim.x - 1 && blockIdx.y == 0 && blockIdx.z == 0)
-    write_schedule(ctx_lens, B, limit, ctas, table);
+    write_schedule(ctx_lens, B, limit, keys, ctas, table);
   wait_or_abort(s, &s.done, 0, err, 85);
   __syncwarp();
   tc_fence_after();
@@ -1073,14 +1593,18 @@ __global__ void __launch_bounds__(128, 1) latent_out_tc_kernel(const __grid_cons
   }
 }
 
-// Heads are cut into equal tiles of at most 64; each gets an equal share of the SMs, and
-// no more CTAs than B contexts of max_ctx tokens have tiles.
+// Heads are cut into equal tiles of at most 64, or 128 where CTA pairs do the attention; each gets an
+// equal share of the SMs (or pairs), and no more CTAs than B contexts of max_ctx tokens have tiles.
 struct Plan {
-  int head_tiles, heads_per_cta, ctas;
-  Plan(int B, int H, int max_ctx, int num_sms)
-      : head_tiles((H + 63) / 64), heads_per_cta((H + head_tiles - 1) / head_tiles) {
-    const int64_t tiles = (int64_t)B * std::max(1, max_ctx / kKeys + (max_ctx % kKeys != 0));
-    ctas = (int)std::max<int64_t>(1, std::min<int64_t>(num_sms / head_tiles, tiles));
+  bool pairs;
+  int keys, head_tiles, heads_per_cta, ctas;
+  Plan(int B, int H, int R, int max_ctx, int num_sms)
+      : pairs(R == 512 && H > kPairHeads && num_sms >= 2),
+        keys(pairs ? kPairKeys : kKeys),
+        head_tiles(pairs ? (H + 127) / 128 : (H + 63) / 64),
+        heads_per_cta((H + head_tiles - 1) / head_tiles) {
+    const int64_t tiles = (int64_t)B * std::max(1, max_ctx / keys + (max_ctx % keys != 0));
+    ctas = (int)std::max<int64_t>(1, std::min<int64_t>(num_sms / (pairs ? 2 : 1) / head_tiles, tiles));
   }
 };
 
@@ -1122,9 +1646,23 @@ void run_attn(const LatentDecode& a, const Plan& p, const bf16* qa, float* part_
   KAPSL_LAUNCH_CHECK();
 }
 
+void run_pairs(const LatentDecode& a, const Plan& p, const bf16* qa, float* part_o, float* part_lse,
+               const int32_t* table, cudaStream_t st) {
+  static_assert(sizeof(PairSmem) <= 232448, "shared memory of one CTA");
+  static std::atomic<uint64_t> attr_devs{0};
+  ensure_smem_attr(attr_devs, latent_attn_pair_kernel, sizeof(PairSmem));
+  const int W = a.R + kRot;
+  const CUtensorMap tq = make_tmap_2d_bf16(qa, (uint64_t)a.B * a.H, W, W, 128, 64, true);
+  const CUtensorMap tc = make_tmap_2d_bf16(a.cache, (uint64_t)a.num_blocks * a.page, W, W, a.page, 64, true);
+  launch_k(latent_attn_pair_kernel, dim3(2 * p.ctas * p.head_tiles), kPairThreads, sizeof(PairSmem), st, tq, tc, qa,
+           a.num_blocks, a.page, a.block_tables, a.max_blocks, a.table_rows, a.num_tables, a.ctx_lens, table, part_o,
+           part_lse, a.B, a.H, p.heads_per_cta, p.head_tiles, a.scale * kLog2e, a.err);
+  KAPSL_LAUNCH_CHECK();
+}
+
 template <int R>
 void run(const LatentDecode& a, cudaStream_t st) {
-  const Plan p(a.B, a.H, a.max_ctx, a.num_sms);
+  const Plan p(a.B, a.H, R, a.max_ctx, a.num_sms);
   const Layout l(a.B, a.H, R, p);
   uint8_t* ws = static_cast<uint8_t*>(a.workspace);
   bf16* qa = reinterpret_cast<bf16*>(ws);
@@ -1138,16 +1676,18 @@ void run(const LatentDecode& a, cudaStream_t st) {
   const unsigned tiles16 = (a.B + 15) / 16;
   const CUtensorMap tw = make_tmap_2d_bf16(a.w, (uint64_t)a.H * (kNope + kVal), R, R, 128, 64, true);
   if (small) {
-    launch_k(latent_absorb_kernel<R>, dim3(R / 64, a.H, tiles16), 128, 0, st, a.q, a.q_stride, a.w, qa, a.B, a.H, a.ctx_lens,
-             limit, p.ctas, table);
+    launch_k(latent_absorb_kernel<R>, dim3(R / 64, a.H, tiles16), 128, 0, st, a.q, a.q_stride, a.w, qa, a.B, a.H,
+             a.ctx_lens, limit, p.keys, p.ctas, table);
     KAPSL_LAUNCH_CHECK();
   } else {
     const CUtensorMap tq = make_tmap_2d_bf16(a.q, a.B, (uint64_t)a.H * (kNope + kRot), a.q_stride, 128, 64, true);
     static std::atomic<uint64_t> devs{0};
     run_smem(latent_absorb_tc_kernel<R>, devs, dim3(R / 256, a.H, (a.B + 127) / 128), sizeof(AbsorbSmem), st, tq, tw,
-             a.q, a.q_stride, qa, a.B, a.H, a.ctx_lens, limit, p.ctas, table, a.err);
+             a.q, a.q_stride, qa, a.B, a.H, a.ctx_lens, limit, p.keys, p.ctas, table, a.err);
   }
-  if (p.heads_per_cta <= 16) {
+  if (p.pairs) {
+    run_pairs(a, p, qa, part_o, part_lse, table, st);
+  } else if (p.heads_per_cta <= 16) {
     run_attn<R, 16>(a, p, qa, part_o, part_lse, table, st);
   } else if (p.heads_per_cta <= 32) {
     run_attn<R, 32>(a, p, qa, part_o, part_lse, table, st);
@@ -1177,7 +1717,7 @@ void run(const LatentDecode& a, cudaStream_t st) {
 }  // namespace
 
 size_t latent_decode_workspace_bytes(int B, int H, int R, int max_ctx, int num_sms) {
-  return Layout(B, H, R, Plan(B, H, max_ctx, num_sms)).bytes;
+  return Layout(B, H, R, Plan(B, H, R, max_ctx, num_sms)).bytes;
 }
 
 void launch_latent_decode(const LatentDecode& a, cudaStream_t st) {
