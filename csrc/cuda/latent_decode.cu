@@ -653,9 +653,13 @@ __global__ void __launch_bounds__(kAttnThreads<R>, 1)
 // in which it is freed: a: the 5 that only the scores read, b: the 4 of the own keys and dims,
 // which both products read (two tiles), c: the 4 of the other's keys.
 //
-// Whole calls, 64-head tiles and pairs: 192 x 8192 tokens x 128 heads 674 and 531 us, 64 x 4096 x 128 145
-// and 121, 64 x 500 x 128 56 and 51, 16 x 1000 x 80 31 and 30; at 64 heads and fewer, where half
-// of the MMA's rows would be empty, 151 and 189 (64 x 8192 x 64).
+// Whole calls, 64-head tiles and pairs: 192 x 8192 tokens x 128 heads 674 and 508 us, 64 x 4096 x 128 145
+// and 119, 64 x 500 x 128 56 and 51, 16 x 1000 x 80 31 and 30; at 64 heads and fewer, where half
+// of the MMA's rows would be empty, 151 and 189 (64 x 8192 x 64).  A tile takes 4,100 cycles where its
+// MMAs alone would take 2,500 (S 1,460, second product 1,050): operands, arriving chunks and P
+// share the shared memory, and loads from L2 run at 5.9 TB/s over the GPU.  The end of a piece
+// (queries to tensor memory, partial result) takes 19,000 cycles; a form that turned the queries in
+// shared memory and overlapped more of it took as long over whole calls.
 constexpr int kPairThreads = 256;  // warps 0-2 TMA (a, b, c), 3 MMA, 4-7 softmax
 constexpr int kPairKeys = 128;
 constexpr int kPairHeads = 64;  // more heads than this take pairs
@@ -718,8 +722,8 @@ __device__ __forceinline__ bool try_wait_cluster(uint64_t* bar, uint32_t parity)
 
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     latent_attn_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap c_map,
-                            const bf16* qa, int64_t num_blocks, int page, const int32_t* block_tables,
-                            int max_blocks, const int32_t* table_rows, int num_tables, const int32_t* ctx_lens,
+                            const bf16* qa, const bf16* cache, int64_t num_blocks, int page,
+                            const int32_t* block_tables, int max_blocks, const int32_t* table_rows, int num_tables, const int32_t* ctx_lens,
                             const int32_t* table, float* part_o, float* part_lse, int B, int H,
                             int heads_per_cta, int head_tiles, float scale_log2, int* err) {
   griddep_launch();
@@ -789,7 +793,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       const int trow = table_rows != nullptr ? table_rows[b] : b;
       int y = page_row(trow, t0), y1 = n > 1 ? page_row(trow, t0 + 1) : oob;
       if (warp == 0) {
-        if (nq > 0) ok = poll_or_abort(s, &s.q_empty, (nq - 1) & 1, err, 84);
+        if (nq > 0) ok = wait_or_abort(s, &s.q_empty, (nq - 1) & 1, err, 84);
         if (!__all_sync(0xffffffffu, ok)) break;
         if (elect_one()) {
           mbar_arrive_expect_tx(&s.q_full, sizeof(s.q));
@@ -799,20 +803,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       }
       for (int i = 0; i < n; ++i, ++sent) {
         const int y2 = i + 2 < n ? page_row(trow, t0 + i + 2) : oob;
-        int yy[4], zz[4];
+        int yy[4];
 #pragma unroll
-        for (int pg = 0; pg < 4; ++pg) {
-          yy[pg] = __shfl_sync(0xffffffffu, y, pg);
-          zz[pg] = __shfl_sync(0xffffffffu, y1, pg);
-        }
-        if (warp < 2 && elect_one()) {  // the next tile comes into L2 while its slots are still in use
-          const int first = warp == 0 ? 0 : 5, last = warp == 0 ? 5 : 9;
-#pragma unroll
-          for (int pg = 0; pg < 4; ++pg)
-            if (pg < pages && zz[pg] < oob)
-              for (int k = first; k < last; ++k) tma_prefetch_2d(&c_map, dims(k), zz[pg]);
-        }
-        __syncwarp();
+        for (int pg = 0; pg < 4; ++pg) yy[pg] = __shfl_sync(0xffffffffu, y, pg);
+        if (warp == 1 && y2 < oob)  // whole pages come into L2 two tiles ahead, a lane each
+          asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(cache + (int64_t)y2 * W), "r"(page * W * 2)
+                       : "memory");
         auto load = [&](uint8_t* dst, uint64_t* bar, int x) {
 #pragma unroll
           for (int pg = 0; pg < 4; ++pg)
@@ -821,7 +817,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         if (warp == 0) {
           for (int k = 0; ok && k < 5; ++k) {
             const int st = chunks % 6;
-            if (chunks >= 6) ok = poll_or_abort(s, &s.a_empty[st], (chunks / 6 - 1) & 1, err, 84);
+            if (chunks >= 6) ok = wait_or_abort(s, &s.a_empty[st], (chunks / 6 - 1) & 1, err, 84);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             if (elect_one()) {
@@ -835,8 +831,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         } else {
           const int st = warp == 1 ? sent & 1 : 0;
           uint64_t* full = warp == 1 ? &s.b_full[st] : &s.c_full;
-          if (warp == 1 && sent >= 2) ok = poll_or_abort(s, &s.b_empty[st], ((sent >> 1) - 1) & 1, err, 84);
-          if (warp == 2 && sent >= 1) ok = poll_or_abort(s, &s.c_empty, (sent - 1) & 1, err, 84);
+          if (warp == 1 && sent >= 2) ok = wait_or_abort(s, &s.b_empty[st], ((sent >> 1) - 1) & 1, err, 84);
+          if (warp == 2 && sent >= 1) ok = wait_or_abort(s, &s.c_empty, (sent - 1) & 1, err, 84);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           if (elect_one()) {
@@ -1008,7 +1004,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       const int left = pc.keys() - pc.first() * kPairKeys;  // keys from the piece's first on
       float m = -INFINITY, l = 0.f;
       for (int i = 0; i < n_tiles; ++i, ++tile) {
-        live = __all_sync(0xffffffffu, poll_or_abort(s, &s.s_full, tile & 1, err, 88) && !s.abort_flag);
+        live = __all_sync(0xffffffffu, wait_or_abort(s, &s.s_full, tile & 1, err, 88) && !s.abort_flag);
         if (!live) break;
         tc_fence_after();
         float v[2][32];
@@ -1056,7 +1052,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         const float M = fmaxf(top, receive());
         const bool up = M > m + kRaise;
         const bool raise = __any_sync(0xffffffffu, up);
-        if (tile > 0) poll_or_abort(s, &s.p_free, (tile - 1) & 1, err, 89);  // P is free, O at rest
+        if (tile > 0) wait_or_abort(s, &s.p_free, (tile - 1) & 1, err, 89);  // P is free, O at rest
         __syncwarp();
         if (raise && i > 0) {
           const float fac = up ? ex2(m - M) : 1.f;
@@ -1081,8 +1077,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
           *reinterpret_cast<uint4*>(s.p[rank] + sw128_offset(row, k)) =
               make_uint4(p[4 * k], p[4 * k + 1], p[4 * k + 2], p[4 * k + 3]);
         if (left - i * kPairKeys < kPairKeys) {  // the sequence's last tile: value rows past the context
-          poll_or_abort(s, &s.b_full[tile & 1], (tile >> 1) & 1, err, 88);
-          poll_or_abort(s, &s.c_full, tile & 1, err, 88);
+          wait_or_abort(s, &s.b_full[tile & 1], (tile >> 1) & 1, err, 88);
+          wait_or_abort(s, &s.c_full, tile & 1, err, 88);
 #pragma unroll 1
           for (int own = 0; own < 2; ++own) {
             const int first = max(0, left - i * kPairKeys - (own ? rank : 1 - rank) * 64);
@@ -1114,7 +1110,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       pc.next();
       if (pc.more()) load_q(pc.b);
       l += receive();
-      poll_or_abort(s, &s.p_free, (tile - 1) & 1, err, 89);
+      wait_or_abort(s, &s.p_free, (tile - 1) & 1, err, 89);
       __syncwarp();
       tc_fence_after();
       const int64_t slot = ((int64_t)ht * (B + pairs) + b + c) * heads_per_cta;
@@ -1655,7 +1651,7 @@ void run_pairs(const LatentDecode& a, const Plan& p, const bf16* qa, float* part
   const CUtensorMap tq = make_tmap_2d_bf16(qa, (uint64_t)a.B * a.H, W, W, 128, 64, true);
   const CUtensorMap tc = make_tmap_2d_bf16(a.cache, (uint64_t)a.num_blocks * a.page, W, W, a.page, 64, true);
   launch_k(latent_attn_pair_kernel, dim3(2 * p.ctas * p.head_tiles), kPairThreads, sizeof(PairSmem), st, tq, tc, qa,
-           a.num_blocks, a.page, a.block_tables, a.max_blocks, a.table_rows, a.num_tables, a.ctx_lens, table, part_o,
+           static_cast<const bf16*>(a.cache), a.num_blocks, a.page, a.block_tables, a.max_blocks, a.table_rows, a.num_tables, a.ctx_lens, table, part_o,
            part_lse, a.B, a.H, p.heads_per_cta, p.head_tiles, a.scale * kLog2e, a.err);
   KAPSL_LAUNCH_CHECK();
 }

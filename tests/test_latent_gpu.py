@@ -369,6 +369,108 @@ def test_decode_large_logits(dev):
             within(out[b].view(H, 128), exp, tol)
 
 
+@pytest.mark.parametrize("H,page,max_ctx", [(65, 16, None), (72, 32, 64), (128, 64, 300), (128, 16, 1000), (129, 16, None),
+                                            (200, 32, 130), (257, 64, None)])
+def test_decode_many_heads(dev, H, page, max_ctx):
+    """CTA pairs: tiles of 128 keys whose second half is empty, begins or ends within; heads that fill
+    no tile of 128, one, or several; no, one and many pieces a row."""
+    from kapsl_sdk_b200 import ops
+
+    lens = [128, 1, 0, 63, 64, 65, 127, 129, 191, 192, 193, 255, 256, 257, 900, 0]
+    k = Cache(dev, lens, 512, page, H + page)
+    qw, w = k.randn(len(lens), H * 192 + 8, std=1.5), k.randn(H, 256, 512, std=1 / math.sqrt(512))
+    out = torch.full((len(lens) + 1, H * 128 + 8), 3.0, device=dev, dtype=torch.bfloat16)
+    q = qw[:, :H * 192]
+    ops.latent_decode_attention(q, k.cache, w, k.bt, k.ctx, H, out=out[:-1, :H * 128], max_ctx=max_ctx)
+    no_error(dev)
+    assert bool((out[:, H * 128:] == 3.0).all()) and bool((out[-1] == 3.0).all())
+    for b in range(len(lens)):
+        exp, tol = decode64(q[b].view(H, 192), k.rows[b], w, 1 / math.sqrt(192))
+        within(out[b, :H * 128].view(H, 128), exp, tol)
+
+
+def test_decode_many_heads_maxima_and_pages(dev):
+    """Maxima that grow, shrink or jump along a context, in either CTA's keys; block table entries outside."""
+    from kapsl_sdk_b200 import ops
+
+    H, lens = 70, [700, 640, 330, 330]
+    k = Cache(dev, lens, 512, 16, 8)
+    q, w = k.randn(4, H * 192), k.randn(H, 256, 512, std=1 / math.sqrt(512))
+    flat = k.cache.view(-1, 576)
+    for b, n in enumerate(lens):
+        f = torch.linspace(0.1, 6.0, n, device=dev) if b == 0 else torch.linspace(6.0, 0.1, n, device=dev)
+        if b >= 2:
+            f = torch.full((n,), 0.2, device=dev)
+            f[140 if b == 2 else 200] = 8.0
+        rows = (k.rows[b].float() * f[:, None]).to(torch.bfloat16)
+        j = torch.arange(n, device=dev)
+        flat[k.bt[b, j // 16].long() * 16 + j % 16] = rows
+        k.rows[b] = rows
+    for max_ctx in (None, 64, 256):
+        good = ops.latent_decode_attention(q, k.cache, w, k.bt, k.ctx, H, max_ctx=max_ctx)
+        no_error(dev)
+        for b in range(4):
+            exp, tol = decode64(q[b].view(H, 192), k.rows[b], w, 1 / math.sqrt(192))
+            within(good[b].view(H, 128), exp, tol)
+    for bad in (-1, k.cache.shape[0], 2 ** 31 - 1):
+        bt = k.bt.clone()
+        bt[1, 6] = bad
+        out = ops.latent_decode_attention(q, k.cache, w, bt, k.ctx, H, max_ctx=256)
+        torch.cuda.synchronize()
+        assert ops.check_errors(dev) == 82
+        assert torch.equal(out[[0, 2, 3]], good[[0, 2, 3]])
+
+
+def test_decode_many_heads_graphs_and_streams(dev):
+    """Captured, replayed and run on two streams at once: the eager results, bit for bit."""
+    from kapsl_sdk_b200 import ops
+
+    H = 128
+    k = Cache(dev, [300, 77, 0, 1000] * 9, 512, 16, 10)
+    w, q = k.randn(H * 256, 512, std=1 / math.sqrt(512)), k.randn(36, H * 192)
+
+    def run():
+        return ops.latent_decode_attention(q, k.cache, w, k.bt, k.ctx, H, max_ctx=1000)
+
+    run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o = run()
+    for _ in range(3):
+        q.copy_(k.randn(36, H * 192))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(o, run())
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], []
+    for _ in range(3):
+        for st in streams:
+            st.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(st):
+                got.append(run())
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, o) for g in got)
+    no_error(dev)
+
+
+def test_prefill_absorbed_many_heads(dev):
+    """New tokens one by one through the CTA pairs: neighbours in the batch share a block table."""
+    from kapsl_sdk_b200 import ops
+
+    q_lens, ctx_lens, H = [5, 1, 3], [300, 64, 3], 66
+    k = Cache(dev, ctx_lens, 512, 32, 14)
+    q, w = k.randn(9, H * 192, std=1.5), k.randn(H, 256, 512, std=1 / math.sqrt(512))
+    plan = ops.latent_prefill_plan(q_lens, ctx_lens, dev)
+    out = ops.latent_prefill_attention(q, k.cache, w, plan, k.bt, H, form="absorbed")
+    no_error(dev)
+    at = 0
+    for s, (n, c) in enumerate(zip(q_lens, ctx_lens)):
+        for i in range(n):
+            exp, tol = decode64(q[at].view(H, 192), k.rows[s][:c - n + i + 1], w, 1 / math.sqrt(192))
+            within(out[at].view(H, 128), exp, tol)
+            at += 1
+
+
 def test_decode_pages_outside(dev):
     """A table entry outside the cache records an error; other rows are untouched by it."""
     from kapsl_sdk_b200 import ops
