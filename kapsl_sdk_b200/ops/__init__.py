@@ -403,15 +403,16 @@ class LatentPrefillPlan:
     def absorbed_is_shorter(self, num_heads: int, rank: int = 512) -> bool:
         """Whether taking every new token by itself in the absorbed form is estimated to take less time
         than expanding the contexts.  In microseconds, fitted to both forms' times on B200 (148
-        SMs) over 34 ragged batches: absorbed, a 64-key tile of up to 64 heads 3.0 (rank 256: 1.4) of
-        an SM and 2 for a thousand rows x heads of head products; expanded, 256 context rows of a head
+        SMs) over some 40 ragged batches: absorbed, a 64-key tile of up to 64 heads 3.0 (rank 256: 1.4) of
+        an SM, of 65 - 128 heads 2.6 (rank 256: 2.8), and 2 for a thousand rows x heads of head products; expanded, 256 context rows of a head
         4.5 (2.3) of an SM pair, a 128-key tile of 256 new tokens 1.9 of an SM, or the longest row
         tile by itself, or a key range of it and 9 for the join.  20 new tokens over 4020, 8
         heads: 37 and 46; five prompts of 17 to 300 tokens, 28 heads: 98 and 59."""
         rows, wide, ranges = self.rows - self.q_start, rank > 256, self.key_ranges(num_heads)
         start = 19 if -(-rows // 16) * num_heads <= 256 else 26
-        absorbed = (start + (3.0 if wide else 1.4) * self.single_tiles * -(-num_heads // 64) / 148 +
-                    0.002 * rows * num_heads)
+        tile = (2.6 * -(-num_heads // 128) if wide and num_heads > 64 else
+                (3.0 if wide else 1.4) * -(-num_heads // 64))
+        absorbed = start + tile * self.single_tiles / 148 + 0.002 * rows * num_heads
         expanded = 20 + 1.2 * ((4.5 if wide else 2.3) * -(-self.kv_work.shape[0] // 2) * num_heads / 74 +
                                max(self.chain_us / ranges, 1.9 * self.row_tiles * num_heads / 148) +
                                9 * (ranges > 1))
