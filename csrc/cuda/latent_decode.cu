@@ -112,6 +112,7 @@ constexpr int kSoft = 4;  // softmax warps
 template <int R>
 constexpr int kAttnThreads = (R / 128 + 1 + kSoft) * 32;
 constexpr float kRaise = 8.f;
+constexpr float kNoMax = -1e30f;
 
 template <int R, int NT>
 struct Shape {
@@ -537,9 +538,10 @@ __global__ void __launch_bounds__(kAttnThreads<R>, 1)
           if (tid < NT) {  // one thread a column
             float mn = fmaxf(fmaxf(s.red[0][tid], s.red[1][tid]), fmaxf(s.red[2][tid], s.red[3][tid]));
             const float old = i == 0 ? 0.f : s.mcol[tid];
-            mn = i == 0 ? (mn == -INFINITY ? 0.f : mn) : fmaxf(mn, old);  // no finite score yet: any reference
+            // no finite score yet: a reference that the first one passes
+            mn = i == 0 ? (mn == -INFINITY ? kNoMax : mn) : fmaxf(mn, old);
             s.mcol[tid] = mn;
-            s.fac[tid] = ex2(old - mn);
+            s.fac[tid] = i == 0 ? 1.f : ex2(old - mn);  // (2^-mn may be infinite, and l is 0 yet)
           }
           soft_barrier();
 #pragma unroll

@@ -342,6 +342,7 @@ constexpr int kThreads = 384;  // warp 0 TMA, warp 1 MMA, warps 4-7 and 8-11 sof
 constexpr int kSlots = 8;
 constexpr uint32_t kSlotBytes = 128 * 128;
 constexpr float kRaise = 8.f;
+constexpr float kNoMax = -1e30f;
 
 struct alignas(1024) PrefillSmem {
   uint8_t q[2][3][kSlotBytes];
@@ -591,6 +592,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t s_tmem = tmem + t * 128 + ((uint32_t)(quad * 32) << 16);
     const uint32_t o_tmem = s_tmem + 256;
     float m = 0.f, l = 0.f;
+    bool fresh = true;
     bool ok = true;
     for (int i = 0; i < tiles; ++i) {
       ok = wait_or_abort(s, &s.s_full[t], i & 1, err, 95);
@@ -603,7 +605,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool masked = __any_sync(0xffffffffu, limit < 127);
       uint32_t p[64];
       float sum = 0.f;
-      if (i == 0) {  // no running maximum yet
+      if (fresh) {  // rows without a running maximum: the first tile, or later where its scores are all -inf
+        if (i == 0) m = kNoMax;
         float top = -INFINITY;
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
@@ -612,7 +615,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int e = 0; e < 32; ++e) top = fmaxf(top, c * 32 + e > limit ? -INFINITY : v[e] * scale_log2);
         }
-        m = top == -INFINITY ? 0.f : top;
+        // a row without keys in the tile has none later: any reference
+        if (m == kNoMax && (top != -INFINITY || limit < 0)) m = limit < 0 ? 0.f : top;
+        fresh = __any_sync(0xffffffffu, m == kNoMax);
       }
       // one place for the pass (its code is long, and fetched anew by every CTA): a second
       // round where a score passed the running maximum too far

@@ -471,6 +471,46 @@ def test_prefill_absorbed_many_heads(dev):
             at += 1
 
 
+@pytest.mark.parametrize("form", ["single", "expanded", "absorbed"])
+@pytest.mark.parametrize("H", [3, 66])
+def test_first_keys_weigh_nothing(dev, form, H):
+    """The first two tiles' scores are -inf (an infinite rotary value), the others far below zero: the
+    result is the softmax over those."""
+    from kapsl_sdk_b200 import ops
+
+    ctx, n, scale = 400, 3, 1 / math.sqrt(192)
+    k = Cache(dev, [ctx], 512, 16, 30)
+    q, w = k.randn(n, H, 192), k.randn(H, 256, 512, std=1 / math.sqrt(512))
+    q[..., 128] = 8.0
+    rows = k.rows[0].clone()
+    rows[:, 512] = -500.0
+    j = torch.arange(ctx, device=dev)
+    flat = k.cache.view(-1, 576)
+    flat[k.bt[0, j // 16].long() * 16 + j % 16] = rows
+    flat[k.bt[0, j[:256] // 16].long() * 16 + j[:256] % 16, 512] = -math.inf
+    if form == "single":
+        n = 1
+        out = ops.latent_decode_attention(q[-1:].reshape(1, H * 192), k.cache, w, k.bt, k.ctx, H, max_ctx=64)
+        q = q[-1:]
+    else:
+        plan = ops.latent_prefill_plan([n], [ctx], dev)
+        out = ops.latent_prefill_attention(q.reshape(n, H * 192), k.cache, w, plan, k.bt, H, form=form)
+    no_error(dev)
+    for i in range(n):
+        exp, tol = decode64(q[i], rows[256:ctx - n + i + 1], w, scale)
+        kn = rows[256:ctx - n + i + 1, :512].double() @ w[:, :128].double().transpose(1, 2)  # keys, rounded to bf16
+        vh = rows[256:ctx - n + i + 1, :512].double() @ w[:, 128:].double().transpose(1, 2)
+        s = (torch.einsum("hd,hkd->hk", q[i, :, :128].double(), kn) +
+             q[i, :, 128:].double() @ rows[256:ctx - n + i + 1, 512:].double().T) * scale
+        p = torch.softmax(s, -1)
+        ds2 = torch.einsum("hd,hkd->hk", q[i, :, :128].double() ** 2, kn ** 2) * scale ** 2
+        var = torch.einsum("hk,hkv->hv", p ** 2 * ds2, (vh - exp[:, None]) ** 2)
+        var += torch.einsum("hk,hkv->hv", p ** 2, vh ** 2)
+        # scores of some -290: fp32 sums of 576 products err by 2^-24 * 24 * 290 in the exponent
+        slop = 2.0 ** -24 * 24 * 290 * torch.einsum("hk,hkv->hv", p, vh.abs())
+        within(out[i].view(H, 128), exp, tol + 8 * U / math.sqrt(3) * var.sqrt() + slop)
+
+
 def test_decode_pages_outside(dev):
     """A table entry outside the cache records an error; other rows are untouched by it."""
     from kapsl_sdk_b200 import ops
