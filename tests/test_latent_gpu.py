@@ -369,8 +369,8 @@ def test_decode_large_logits(dev):
             within(out[b].view(H, 128), exp, tol)
 
 
-@pytest.mark.parametrize("H,page,max_ctx", [(65, 16, None), (72, 32, 64), (128, 64, 300), (128, 16, 1000), (129, 16, None),
-                                            (200, 32, 130), (257, 64, None)])
+@pytest.mark.parametrize("H,page,max_ctx", [(65, 16, None), (72, 32, 64), (128, 64, 300), (128, 16, 1000),
+                                            (129, 16, None), (200, 32, 130), (257, 64, None)])
 def test_decode_many_heads(dev, H, page, max_ctx):
     """CTA pairs: tiles of 128 keys whose second half is empty, begins or ends within; heads that fill
     no tile of 128, one, or several; no, one and many pieces a row."""
