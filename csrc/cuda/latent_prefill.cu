@@ -385,11 +385,14 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 
 // P of one row of a key tile relative to the running maximum m: 128 scores from TMEM, 64
 // packed bf16 pairs, their fp32 sum, and the largest relative score.  The load of the
-// next 32 columns is under way while 32 are worked on.
+// next 32 columns is under way while 32 are worked on.  The scaled scores are rounded before m is
+// taken off, as m's own was, so that the largest is 0 at any size: scale * s - m in one
+// rounding is up to half of m's last place there, from 2^28 on more than kRaise whatever m is.  (A packed
+// product by itself was seen to be contracted with the packed sum; an fma is not.)
 template <bool MASKED>
 __device__ __forceinline__ float row_pass(uint32_t s_tmem, float scale_log2, float m, int limit, uint32_t (&p)[64],
                                           float& sum) {
-  const uint64_t sc = pair(scale_log2, scale_log2), off = pair(-m, -m);
+  const uint64_t sc = pair(scale_log2, scale_log2), off = pair(-m, -m), zero = pair(0.f, 0.f);
   float top = -INFINITY;
   uint64_t acc = pair(0.f, 0.f);
   uint32_t v[2][32];
@@ -401,7 +404,7 @@ __device__ __forceinline__ float row_pass(uint32_t s_tmem, float scale_log2, flo
 #pragma unroll
     for (int i = 0; i < 32; i += 2) {
       float x0, x1;
-      unpair(fma2(pair(__uint_as_float(v[c & 1][i]), __uint_as_float(v[c & 1][i + 1])), sc, off), x0, x1);
+      unpair(add2(fma2(pair(__uint_as_float(v[c & 1][i]), __uint_as_float(v[c & 1][i + 1])), sc, zero), off), x0, x1);
       if (MASKED) {
         if (c * 32 + i > limit) x0 = -INFINITY;
         if (c * 32 + i + 1 > limit) x1 = -INFINITY;
@@ -591,8 +594,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int last_key = min(pos0 + row, keys - 1);  // this row's; rows past the chunk see the tile's keys
     const uint32_t s_tmem = tmem + t * 128 + ((uint32_t)(quad * 32) << 16);
     const uint32_t o_tmem = s_tmem + 256;
-    float m = 0.f, l = 0.f;
-    bool fresh = true;
+    float m = kNoMax, l = 0.f;
+    bool fresh = true;  // any row of the warp without a maximum
     bool ok = true;
     for (int i = 0; i < tiles; ++i) {
       ok = wait_or_abort(s, &s.s_full[t], i & 1, err, 95);
@@ -605,38 +608,44 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool masked = __any_sync(0xffffffffu, limit < 127);
       uint32_t p[64];
       float sum = 0.f;
-      if (fresh) {  // rows without a running maximum: the first tile, or later where its scores are all -inf
-        if (i == 0) m = kNoMax;
-        float top = -INFINITY;
+      // The maximum is looked for where a row has none (the first tile, or later where its scores are all
+      // -inf) and where a score passed the running one too far.  No score is above it then, and
+      // the pass after it is the last.  One place for the pass: its code is long, and fetched
+      // anew by every CTA.
+      bool look = fresh;
 #pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-          float v[32];
-          tmem_ld32w(s_tmem + c * 32, v);
-#pragma unroll
-          for (int e = 0; e < 32; ++e) top = fmaxf(top, c * 32 + e > limit ? -INFINITY : v[e] * scale_log2);
-        }
-        // a row without keys in the tile has none later: any reference
-        if (m == kNoMax && (top != -INFINITY || limit < 0)) m = limit < 0 ? 0.f : top;
-        fresh = __any_sync(0xffffffffu, m == kNoMax);
-      }
-      // one place for the pass (its code is long, and fetched anew by every CTA): a second
-      // round where a score passed the running maximum too far
       while (true) {
+        if (look) {
+          float top = -INFINITY;
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            float v[32];
+            tmem_ld32w(s_tmem + c * 32, v);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) top = fmaxf(top, c * 32 + e > limit ? -INFINITY : v[e] * scale_log2);
+          }
+          float mn = fmaxf(m, top), f = ex2(m - mn);
+          // a row without keys in the tile has none later: any reference
+          if (m == kNoMax) mn = limit < 0 ? 0.f : top == -INFINITY ? kNoMax : top, f = 1.f;
+          m = mn;
+          fresh = __any_sync(0xffffffffu, m == kNoMax);
+          if (i > 0 && __any_sync(0xffffffffu, f != 1.f)) {
+            l *= f;
+#pragma unroll 1
+            for (int c = 0; c < 8; ++c) {
+              float o[16];
+              uint32_t u[16];
+              tmem_ld16(o_tmem + c * 16, o);
+#pragma unroll
+              for (int e = 0; e < 16; ++e) u[e] = __float_as_uint(o[e] * f);
+              tmem_st16(o_tmem + c * 16, u);
+            }
+          }
+        }
         const float top = masked ? row_pass<true>(s_tmem, scale_log2, m, limit, p, sum)
                                  : row_pass<false>(s_tmem, scale_log2, m, limit, p, sum);
-        if (i == 0 || !__any_sync(0xffffffffu, top > kRaise)) break;
-        const float up = fmaxf(top, 0.f), f = ex2(-up);
-        m += up;
-        l *= f;
-#pragma unroll 1
-        for (int c = 0; c < 8; ++c) {
-          float o[16];
-          uint32_t u[16];
-          tmem_ld16(o_tmem + c * 16, o);
-#pragma unroll
-          for (int e = 0; e < 16; ++e) u[e] = __float_as_uint(o[e] * f);
-          tmem_st16(o_tmem + c * 16, u);
-        }
+        if (look || !__any_sync(0xffffffffu, top > kRaise)) break;
+        look = true;
       }
       l += sum;
 #pragma unroll

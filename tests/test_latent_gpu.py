@@ -656,6 +656,39 @@ def test_prefill_large_logits(dev):
     within(out.view(n, H, 128), exp, tol)
 
 
+def far_scores(dev, n, H, ctx, mag, kind, R=512):
+    """Scores of mag times small numbers, exact in fp32 (a product of two short rotary values): the largest
+    are equal, all others far below, so the result is the mean over the equal ones, however
+    large mag is.  Every other query prefers the smallest rotary values."""
+    k = Cache(dev, [ctx], R, 16, n + ctx)
+    q, w = torch.zeros(n, H, 192, device=dev, dtype=torch.bfloat16), k.randn(H * 256, R, std=1 / math.sqrt(R))
+    q[:, :, 128] = 2.0 ** (mag // 2)
+    q[::2, :, 128] *= -1
+    j = torch.arange(ctx, device=dev)
+    f = {"mixed": 0.5 + j * 7 % 5, "growing": 1.0 + j // 100, "above zero": 4.0 + j * 3 % 2}[kind]
+    rows = k.rows[0]
+    rows[:, R:] = 0
+    rows[:, R] = f * 2.0 ** (mag - mag // 2) * (1 if kind == "above zero" else -1)
+    k.cache.view(-1, R + 64)[k.bt[0, j // 16].long() * 16 + j % 16] = rows
+    return k, q, w, rows
+
+
+@pytest.mark.parametrize("kind", ["mixed", "growing", "above zero"])
+@pytest.mark.parametrize("mag", [20, 26, 31, 36, 60, 110])
+@pytest.mark.parametrize("n,ctx", [(3, 700), (300, 700)])
+def test_prefill_far_scores(dev, n, ctx, mag, kind):
+    """Scores whose last place in fp32 is worth more than the steps in which the running maximum is raised."""
+    from kapsl_sdk_b200 import ops
+
+    H = 2
+    k, q, w, rows = far_scores(dev, n, H, ctx, mag, kind)
+    plan = ops.latent_prefill_plan([n], [ctx], dev)
+    out = ops.latent_prefill_attention(q.view(n, -1), k.cache, w, plan, k.bt, H, form="expanded", key_ranges=1)
+    no_error(dev)
+    exp, tol = prefill64(q, rows, w.view(H, 256, 512), 1 / math.sqrt(192))
+    within(out.view(n, H, 128), exp, tol)
+
+
 @pytest.mark.parametrize("form", ["expanded", "absorbed"])
 def test_prefill_pages_outside_and_refusals(dev, form):
     from kapsl_sdk_b200 import ops
