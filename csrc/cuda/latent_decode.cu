@@ -104,8 +104,10 @@ __device__ void write_schedule(const int32_t* ctx_lens, int B, int limit, int ke
 // Softmax: scores (times log2 e) are compared with the running maximum; only when one
 // exceeds it by 8 (a vote over the four warps) is the maximum raised - column maxima by
 // register and shared-memory exchange - and O^T rescaled in TMEM.  p <= 256 loses nothing in bf16 or
-// fp32, and the final division uses the same maximum.  P is rounded to bf16, the operand
-// type of the second product; the row sums are of the fp32 values.  Keys past the context
+// fp32, and the final division uses the same maximum.  The scaled scores are rounded before the
+// maximum, one of them, is taken off: in one rounding scale * s - m would be up to half of m's
+// last place at the maximum, and 2^ of that infinite from 2^31 on.  P is rounded to bf16, the
+// operand type of the second product; the row sums are of the fp32 values.  Keys past the context
 // have p = 0 and their cache rows are cleared in shared memory, since 0 * NaN of a
 // stale row would count.
 constexpr int kSoft = 4;  // softmax warps
@@ -506,7 +508,7 @@ __global__ void __launch_bounds__(kAttnThreads<R>, 1)
           for (int g = 0; g < NT / 8; ++g)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              x[g][e] = fmaf(v[g][e], scale_log2, relative ? -m_ref[2 * g + (e & 1)] : 0.f);
+              x[g][e] = __fadd_rn(__fmul_rn(v[g][e], scale_log2), relative ? -m_ref[2 * g + (e & 1)] : 0.f);
           if (valid < kKeys) {
 #pragma unroll
             for (int g = 0; g < NT / 8; ++g)

@@ -689,6 +689,21 @@ def test_prefill_far_scores(dev, n, ctx, mag, kind):
     within(out.view(n, H, 128), exp, tol)
 
 
+@pytest.mark.parametrize("kind", ["mixed", "growing", "above zero"])
+@pytest.mark.parametrize("mag", [20, 26, 31, 36, 60, 110])
+@pytest.mark.parametrize("H", [2, 66])
+def test_decode_far_scores(dev, H, mag, kind):
+    """The same for single tokens, each context one piece."""
+    from kapsl_sdk_b200 import ops
+
+    k, q, w, rows = far_scores(dev, 2, H, 700, mag, kind)
+    for i in range(2):
+        out = ops.latent_decode_attention(q[i:i + 1].view(1, -1), k.cache, w, k.bt, k.ctx, H, max_ctx=1)
+        no_error(dev)
+        exp, tol = decode64(q[i], rows, w.view(H, 256, 512), 1 / math.sqrt(192))
+        within(out.view(H, 128), exp, tol)
+
+
 @pytest.mark.parametrize("form", ["expanded", "absorbed"])
 def test_prefill_pages_outside_and_refusals(dev, form):
     from kapsl_sdk_b200 import ops
