@@ -331,10 +331,10 @@ void latent_prefill(Tensor q, Tensor kv, Tensor k_rope, Tensor work, Tensor seq_
     const int64_t rows = ranges * heads * work.size(0) * 256;
     TORCH_CHECK(parts.has_value(), op, ": key ranges need room for partial results");
     check(*parts, at::kFloat, q, op, "parts");
-    TORCH_CHECK(parts->is_contiguous() && parts->numel() >= rows * (kVal + 1), op, ": parts too small");
+    TORCH_CHECK(parts->is_contiguous() && parts->numel() >= rows * (kVal + 2), op, ": parts too small");
     a.ranges = (int)ranges;
     a.part_o = parts->data_ptr<float>();
-    a.part_lse = a.part_o + rows * kVal;
+    a.part_ml = reinterpret_cast<float2*>(a.part_o + rows * kVal);
   }
   a.k_rope = bf(k_rope);
   a.work = work.data_ptr<int32_t>();

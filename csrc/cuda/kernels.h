@@ -100,7 +100,7 @@ struct LatentPrefill {
   float scale = 0.f;
   int ranges = 1;             // parts of the key tiles (at most 32), joined from
   float* part_o = nullptr;    // [ranges, heads, nwork, 256, 128]
-  float* part_lse = nullptr;  // [ranges, heads, nwork, 256]
+  float2* part_ml = nullptr;  // [ranges, heads, nwork, 256]: a part's maximum (log2) and sum
   int* err = nullptr;
 };
 void launch_latent_prefill(const LatentPrefill& a, cudaStream_t st);

@@ -257,7 +257,7 @@ __global__ void __launch_bounds__(kAttnThreads<R>, 1)
                        int64_t num_blocks, int page, const int32_t* block_tables, int max_blocks,
                        const int32_t* table_rows, int num_tables,
                        const int32_t* ctx_lens, const int32_t* table,
-                       float* part_o, float* part_lse, int B, int H, int heads_per_cta,
+                       float* part_o, float2* part_ml, int B, int H, int heads_per_cta,
                        int head_tiles, float scale_log2, int* err) {
   griddep_launch();
   using S = Shape<R, NT>;
@@ -613,7 +613,7 @@ __global__ void __launch_bounds__(kAttnThreads<R>, 1)
       if (tid < NT) {
         const float sum = s.red[0][tid] + s.red[1][tid] + s.red[2][tid] + s.red[3][tid];
         s.fac[tid] = sum == 0.f ? 0.f : __fdividef(1.f, sum);
-        if (tid < nheads) part_lse[slot + tid] = sum == 0.f ? -INFINITY : s.mcol[tid] + __log2f(sum);
+        if (tid < nheads) part_ml[slot + tid] = make_float2(sum == 0.f ? -INFINITY : s.mcol[tid], sum);
       }
       soft_barrier();
 #pragma unroll 1
@@ -728,7 +728,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     latent_attn_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap c_map,
                             const bf16* qa, const bf16* cache, int64_t num_blocks, int page,
                             const int32_t* block_tables, int max_blocks, const int32_t* table_rows, int num_tables, const int32_t* ctx_lens,
-                            const int32_t* table, float* part_o, float* part_lse, int B, int H,
+                            const int32_t* table, float* part_o, float2* part_ml, int B, int H,
                             int heads_per_cta, int head_tiles, float scale_log2, int* err) {
   griddep_launch();
   constexpr int R = 512, W = R + kRot;
@@ -1118,7 +1118,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       __syncwarp();
       tc_fence_after();
       const int64_t slot = ((int64_t)ht * (B + pairs) + b + c) * heads_per_cta;
-      if (rank == 0 && row < nheads) part_lse[slot + row] = l == 0.f ? -INFINITY : m + __log2f(l);
+      if (rank == 0 && row < nheads) part_ml[slot + row] = make_float2(l == 0.f ? -INFINITY : m, l);
       const float inv = l == 0.f ? 0.f : __fdividef(1.f, l);
       uint8_t* turn = s.p[rank] + quad * 4096;  // 32 rows x 32 dims, turned for whole-line stores
 #pragma unroll 1
@@ -1248,14 +1248,16 @@ __global__ void __launch_bounds__(128) latent_absorb_kernel(const bf16* q, int64
   }
 }
 
-// Joins a row's pieces: o[b, h] = sum_c 2^(lse_c - M) o_c / sum_c 2^(lse_c - M), written as hi + lo,
-// two bf16 whose sum keeps 16 bits of it: the product below then rounds nothing else.  One
+// Joins a row's pieces: o[b, h] = sum_c w_c o_c / sum_c w_c, w_c = l_c 2^(m_c - M), written as hi + lo,
+// two bf16 whose sum keeps 16 bits of it: the product below then rounds nothing else.  A piece
+// brings its maximum m_c and sum l_c apart: the sum of m_c and log2 l_c would round l_c to m_c's
+// last place, 2^-6 at scores of 2^17.  One
 // thread per 8 dims of ROWS rows, whole warps a row: the pieces' weights are spread over the
 // lanes, and P pieces of every row are requested at once (few rows have many pieces: P = 8;
 // many rows have one or two: P = 2, and two rows a thread).
 template <int R, int P, int ROWS>
 __global__ void __launch_bounds__(128)
-    latent_join_kernel(const float* part_o, const float* part_lse, const int32_t* table, bf16* hi, bf16* lo, int B,
+    latent_join_kernel(const float* part_o, const float2* part_ml, const int32_t* table, bf16* hi, bf16* lo, int B,
                        int H, int heads_per_cta, int ctas) {
   griddep_entry();
   constexpr int kRowThreads = R / 8;
@@ -1267,7 +1269,7 @@ __global__ void __launch_bounds__(128)
   const int quota = table[0];
   int n[ROWS], most = 0;
   const float* src[ROWS];
-  float e0[ROWS], e1[ROWS], inv[ROWS], x[ROWS][8] = {};
+  float e0[ROWS], e1[ROWS], l0[ROWS], l1[ROWS], inv[ROWS], x[ROWS][8] = {};
   float4 y[ROWS][P][2];
   auto load = [&](int p0) {
 #pragma unroll
@@ -1287,14 +1289,21 @@ __global__ void __launch_bounds__(128)
     n[i] = 0;
     src[i] = part_o;
     e0[i] = e1[i] = -INFINITY;
+    l0[i] = l1[i] = 0.f;
     if (row0 + i < rows) {
       const int b = (int)((row0 + i) / H), h = (int)((row0 + i) % H);
       const int s0 = table[1 + b], s1 = table[2 + b], c0 = s0 / quota;
       n[i] = s1 > s0 ? (s1 - 1) / quota - c0 + 1 : 0;
       const int64_t slot = ((int64_t)(h / heads_per_cta) * (B + ctas) + b + c0) * heads_per_cta + h % heads_per_cta;
       src[i] = part_o + slot * R + k;
-      if (lane < n[i]) e0[i] = part_lse[slot + (int64_t)lane * heads_per_cta];
-      if (lane + 32 < n[i]) e1[i] = part_lse[slot + (int64_t)(lane + 32) * heads_per_cta];
+      if (lane < n[i]) {
+        const float2 ml = part_ml[slot + (int64_t)lane * heads_per_cta];
+        e0[i] = ml.x, l0[i] = ml.y;
+      }
+      if (lane + 32 < n[i]) {
+        const float2 ml = part_ml[slot + (int64_t)(lane + 32) * heads_per_cta];
+        e1[i] = ml.x, l1[i] = ml.y;
+      }
     }
     most = max(most, n[i]);
   }
@@ -1303,7 +1312,7 @@ __global__ void __launch_bounds__(128)
   for (int i = 0; i < ROWS; ++i) {
     float M = warp_max(fmaxf(e0[i], e1[i]));
     if (M == -INFINITY) M = 0.f;  // no finite score in the row: weights 0 (or NaN, which reaches the row)
-    e0[i] = ex2(e0[i] - M), e1[i] = ex2(e1[i] - M);
+    e0[i] = l0[i] * ex2(e0[i] - M), e1[i] = l1[i] * ex2(e1[i] - M);
     const float L = warp_sum(e0[i] + e1[i]);
     inv[i] = L == 0.f ? 0.f : 1.f / L;
   }
@@ -1608,16 +1617,16 @@ struct Plan {
   }
 };
 
-// Workspace: qa, the schedule, the joined rows' low halves, the pieces' lse and o (each part 128-byte aligned).
+// Workspace: qa, the schedule, the joined rows' low halves, the pieces' (m, l) and o (each part 128-byte aligned).
 struct Layout {
-  size_t table, low, lse, part, bytes;
+  size_t table, low, ml, part, bytes;
   Layout(int B, int H, int R, const Plan& p) {
     const size_t slots = (size_t)p.head_tiles * (B + p.ctas) * p.heads_per_cta;
     auto up = [](size_t n) { return (n + 127) / 128 * 128; };
     table = up((size_t)B * H * (R + kRot) * 2);
     low = table + up((size_t)table_ints(B) * 4);
-    lse = low + up((size_t)B * H * R * 2);
-    part = lse + up(slots * 4);
+    ml = low + up((size_t)B * H * R * 2);
+    part = ml + up(slots * 8);
     bytes = part + slots * R * 4;
   }
 };
@@ -1630,7 +1639,7 @@ void run_smem(Kernel kern, std::atomic<uint64_t>& attr_devs, dim3 grid, size_t s
 }
 
 template <int R, int NT>
-void run_attn(const LatentDecode& a, const Plan& p, const bf16* qa, float* part_o, float* part_lse,
+void run_attn(const LatentDecode& a, const Plan& p, const bf16* qa, float* part_o, float2* part_ml,
               const int32_t* table, cudaStream_t st) {
   using S = Shape<R, NT>;
   auto kern = latent_attn_kernel<R, NT>;
@@ -1641,12 +1650,12 @@ void run_attn(const LatentDecode& a, const Plan& p, const bf16* qa, float* part_
   const CUtensorMap tq = make_tmap_2d_bf16(qa, (uint64_t)a.B * a.H, S::W, S::W, NT, 64, true);
   const CUtensorMap tc = make_tmap_2d_bf16(a.cache, (uint64_t)a.num_blocks * a.page, S::W, S::W, a.page, 64, true);
   launch_k(kern, dim3(p.ctas * p.head_tiles), kAttnThreads<R>, smem, st, tq, tc, a.num_blocks, a.page, a.block_tables,
-           a.max_blocks, a.table_rows, a.num_tables, a.ctx_lens, table, part_o, part_lse, a.B, a.H, p.heads_per_cta,
+           a.max_blocks, a.table_rows, a.num_tables, a.ctx_lens, table, part_o, part_ml, a.B, a.H, p.heads_per_cta,
            p.head_tiles, a.scale * kLog2e, a.err);
   KAPSL_LAUNCH_CHECK();
 }
 
-void run_pairs(const LatentDecode& a, const Plan& p, const bf16* qa, float* part_o, float* part_lse,
+void run_pairs(const LatentDecode& a, const Plan& p, const bf16* qa, float* part_o, float2* part_ml,
                const int32_t* table, cudaStream_t st) {
   static_assert(sizeof(PairSmem) <= 232448, "shared memory of one CTA");
   static std::atomic<uint64_t> attr_devs{0};
@@ -1656,7 +1665,7 @@ void run_pairs(const LatentDecode& a, const Plan& p, const bf16* qa, float* part
   const CUtensorMap tc = make_tmap_2d_bf16(a.cache, (uint64_t)a.num_blocks * a.page, W, W, a.page, 64, true);
   launch_k(latent_attn_pair_kernel, dim3(2 * p.ctas * p.head_tiles), kPairThreads, sizeof(PairSmem), st, tq, tc, qa,
            static_cast<const bf16*>(a.cache), a.num_blocks, a.page, a.block_tables, a.max_blocks, a.table_rows, a.num_tables, a.ctx_lens, table, part_o,
-           part_lse, a.B, a.H, p.heads_per_cta, p.head_tiles, a.scale * kLog2e, a.err);
+           part_ml, a.B, a.H, p.heads_per_cta, p.head_tiles, a.scale * kLog2e, a.err);
   KAPSL_LAUNCH_CHECK();
 }
 
@@ -1667,7 +1676,7 @@ void run(const LatentDecode& a, cudaStream_t st) {
   uint8_t* ws = static_cast<uint8_t*>(a.workspace);
   bf16* qa = reinterpret_cast<bf16*>(ws);
   int32_t* table = reinterpret_cast<int32_t*>(ws + l.table);
-  float* part_lse = reinterpret_cast<float*>(ws + l.lse);
+  float2* part_ml = reinterpret_cast<float2*>(ws + l.ml);
   float* part_o = reinterpret_cast<float*>(ws + l.part);
   const int limit = a.max_blocks * a.page;
   // Tiles of 16 rows while their CTAs are few (a whole call of 33 rows x 20 heads 27 us, with the 128-row
@@ -1686,19 +1695,19 @@ void run(const LatentDecode& a, cudaStream_t st) {
              a.q, a.q_stride, qa, a.B, a.H, a.ctx_lens, limit, p.keys, p.ctas, table, a.err);
   }
   if (p.pairs) {
-    run_pairs(a, p, qa, part_o, part_lse, table, st);
+    run_pairs(a, p, qa, part_o, part_ml, table, st);
   } else if (p.heads_per_cta <= 16) {
-    run_attn<R, 16>(a, p, qa, part_o, part_lse, table, st);
+    run_attn<R, 16>(a, p, qa, part_o, part_ml, table, st);
   } else if (p.heads_per_cta <= 32) {
-    run_attn<R, 32>(a, p, qa, part_o, part_lse, table, st);
+    run_attn<R, 32>(a, p, qa, part_o, part_ml, table, st);
   } else {
-    run_attn<R, 64>(a, p, qa, part_o, part_lse, table, st);
+    run_attn<R, 64>(a, p, qa, part_o, part_ml, table, st);
   }
   // qa has been read: the high halves take its place
   bf16* lo = reinterpret_cast<bf16*>(ws + l.low);
   const int64_t rows = (int64_t)a.B * a.H, per = 1024 / R * (small ? 1 : 2);
   launch_k(small ? latent_join_kernel<R, 8, 1> : latent_join_kernel<R, 2, 2>, dim3((unsigned)((rows + per - 1) / per)),
-           128, 0, st, part_o, part_lse, table, qa, lo, a.B, a.H, p.heads_per_cta, p.ctas);
+           128, 0, st, part_o, part_ml, table, qa, lo, a.B, a.H, p.heads_per_cta, p.ctas);
   KAPSL_LAUNCH_CHECK();
   static std::atomic<uint64_t> devs{0}, devs_tc{0};
   if (small) {

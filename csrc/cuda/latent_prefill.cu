@@ -425,7 +425,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     latent_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap kv_map,
                           const __grid_constant__ CUtensorMap rope_map, const int32_t* work,
                           const int32_t* seq_info, int64_t q_rows, float scale_log2,
-                          bf16* out, int64_t out_stride, float* part_o, float* part_lse,
+                          bf16* out, int64_t out_stride, float* part_o, float2* part_ml,
                           int* err) {
   griddep_entry();
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -451,7 +451,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     return;
   }
   if (nt == 0) {  // no keys in this range
-    if (threadIdx.x < 256) part_lse[part_row + threadIdx.x] = -INFINITY;
+    if (threadIdx.x < 256) part_ml[part_row + threadIdx.x] = make_float2(-INFINITY, 0.f);
     return;
   }
 
@@ -698,8 +698,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (part_o != nullptr) {
       if (!(split && t == 1)) {
         const float inv = !ok || l == 0.f ? 0.f : 1.f / l;
-        part_lse[part_row + row] = !ok || l == 0.f ? -INFINITY : m_out + __log2f(l);
-        if (split) part_lse[part_row + row + 128] = -INFINITY;
+        part_ml[part_row + row] = !ok || l == 0.f ? make_float2(-INFINITY, 0.f) : make_float2(m_out, l);
+        if (split) part_ml[part_row + row + 128] = make_float2(-INFINITY, 0.f);
         float* dst = part_o + (part_row + row) * kVal;
         for (int c = 0; ok && c < 8; ++c) {
           float o[16];
@@ -747,9 +747,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// out = sum_z 2^(lse_z - M) o_z / sum_z 2^(lse_z - M) over the key ranges z: one warp per (row of a row
-// tile, head), 4 dims a lane.
-__global__ void __launch_bounds__(256) latent_prefill_join_kernel(const float* part_o, const float* part_lse, int ranges,
+// out = sum_z w_z o_z / sum_z w_z over the key ranges z, w_z = l_z 2^(m_z - M) of their maxima and sums
+// (kept apart: m_z + log2 l_z would round l_z to m_z's last place): one warp per (row of a
+// row tile, head), 4 dims a lane.
+__global__ void __launch_bounds__(256) latent_prefill_join_kernel(const float* part_o, const float2* part_ml, int ranges,
                                                                   const int32_t* work, const int32_t* seq_info,
                                                                   bf16* out, int64_t out_stride) {
   griddep_entry();
@@ -758,10 +759,10 @@ __global__ void __launch_bounds__(256) latent_prefill_join_kernel(const float* p
   const int t0 = work[2 * blockIdx.x + 1];
   if (t0 + row >= si[1]) return;
   const int64_t first = ((int64_t)h * gridDim.x + blockIdx.x) * 256 + row, step = (int64_t)gridDim.y * gridDim.x * 256;
-  const float lse = lane < ranges ? part_lse[first + lane * step] : -INFINITY;
-  float M = warp_max(lse);
+  const float2 ml = lane < ranges ? part_ml[first + lane * step] : make_float2(-INFINITY, 0.f);
+  float M = warp_max(ml.x);
   if (M == -INFINITY) M = 0.f;
-  const float e = ex2(lse - M), L = warp_sum(e);
+  const float e = ml.y * ex2(ml.x - M), L = warp_sum(e);
   const float w = L == 0.f ? 0.f : e / L;
   float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
@@ -812,11 +813,11 @@ void launch_latent_prefill(const LatentPrefill& a, cudaStream_t st) {
   const CUtensorMap tr = make_tmap_2d_bf16(a.k_rope, a.kv_rows, kRot, kRot, 128, 64, true);
   const bool ranges = a.ranges > 1;
   launch_k(latent_prefill_kernel, dim3(a.nwork, a.heads, a.ranges), kThreads, smem, st, tq, tkv, tr, a.work, a.seq_info,
-           a.T, a.scale * kLog2e, a.out, a.out_stride, ranges ? a.part_o : nullptr, a.part_lse, a.err);
+           a.T, a.scale * kLog2e, a.out, a.out_stride, ranges ? a.part_o : nullptr, a.part_ml, a.err);
   KAPSL_LAUNCH_CHECK();
   note_launch();
   if (!ranges) return;
-  launch_k(latent_prefill_join_kernel, dim3(a.nwork, a.heads, 32), 256, 0, st, a.part_o, a.part_lse, a.ranges, a.work,
+  launch_k(latent_prefill_join_kernel, dim3(a.nwork, a.heads, 32), 256, 0, st, a.part_o, a.part_ml, a.ranges, a.work,
            a.seq_info, a.out, a.out_stride);
   KAPSL_LAUNCH_CHECK();
   note_launch();

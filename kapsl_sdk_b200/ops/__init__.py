@@ -511,7 +511,7 @@ def latent_prefill_attention(q: torch.Tensor, cache: torch.Tensor, w_kv_b: torch
     ranges = key_ranges if key_ranges > 0 else plan.key_ranges(min(step, num_heads))
     parts = None
     if ranges > 1:
-        parts = torch.empty(ranges * step * plan.work.shape[0] * 256 * 129, dtype=torch.float32, device=q.device)
+        parts = torch.empty(ranges * step * plan.work.shape[0] * 256 * 130, dtype=torch.float32, device=q.device)
     for h0 in range(0, num_heads, step):
         n = min(step, num_heads - h0)
         kv = kv_buf[:plan.kv_rows * n * 256].view(plan.kv_rows, n * 256)

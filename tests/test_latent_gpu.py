@@ -704,6 +704,30 @@ def test_decode_far_scores(dev, H, mag, kind):
         within(out.view(H, 128), exp, tol)
 
 
+@pytest.mark.parametrize("kind", ["mixed", "growing", "above zero"])
+@pytest.mark.parametrize("mag", [20, 26, 36, 110])
+@pytest.mark.parametrize("H", [2, 66])
+def test_pieces_of_far_scores(dev, H, mag, kind):
+    """Equal largest scores in several pieces of a context count one by one, not piece by piece."""
+    from kapsl_sdk_b200 import ops
+
+    n, ctx, scale = 4, 700, 1 / math.sqrt(192)
+    k, q, w, rows = far_scores(dev, n, H, ctx, mag, kind)
+    plan = ops.latent_prefill_plan([n], [ctx], dev)
+    flat = q.view(n, -1)
+    got = [ops.latent_prefill_attention(flat, k.cache, w, plan, k.bt, H, form="expanded", key_ranges=r) for r in (2, 5)]
+    exp, tol = prefill64(q, rows, w.view(H, 256, 512), scale)
+    one = ops.latent_decode_attention(flat[-1:], k.cache, w, k.bt, k.ctx, H)
+    rows_alone = ops.latent_prefill_attention(flat, k.cache, w, plan, k.bt, H, form="absorbed")
+    no_error(dev)
+    for out in got:
+        within(out.view(n, H, 128), exp, tol)
+    for i in range(n):
+        exp, tol = decode64(q[i], rows[:ctx - n + i + 1], w.view(H, 256, 512), scale)
+        within(rows_alone[i].view(H, 128), exp, tol)
+    within(one.view(H, 128), exp, tol)
+
+
 @pytest.mark.parametrize("form", ["expanded", "absorbed"])
 def test_prefill_pages_outside_and_refusals(dev, form):
     from kapsl_sdk_b200 import ops
