@@ -221,6 +221,28 @@ def test_rope_latent_write_bounds_and_refusals(dev):
     no_error(dev)
 
 
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_tables_without_rows(dev, interleaved):
+    """No position lies in an empty table: nothing is read from it, nothing is rotated, the error is recorded."""
+    from kapsl_sdk_b200 import ops
+
+    cs = torch.empty(0, 64, device=dev)
+    x = torch.randn(5, 3, 64, device=dev).to(torch.bfloat16)
+    pos = torch.tensor([0, 1, -1, 5, 7], dtype=torch.int32, device=dev)
+    assert torch.equal(ops.rope(x, pos, cs, interleaved=interleaved), x)
+    torch.cuda.synchronize()
+    assert ops.check_errors(dev) == 80
+    cache = torch.zeros(1, 16, 320, device=dev, dtype=torch.bfloat16)
+    kv, w = torch.randn(5, 320, device=dev).to(torch.bfloat16), torch.ones(256, device=dev, dtype=torch.bfloat16)
+    q = ops.rope_latent_write(x, kv, pos, torch.arange(5, device=dev), cs, w, 1e-6, cache, interleaved,
+                              q_out=torch.empty_like(x))
+    torch.cuda.synchronize()
+    assert ops.check_errors(dev) == 80
+    assert torch.equal(q, x) and torch.equal(cache[0, :5, 256:], kv[:, 256:])
+    ops.rope_latent_write(x[:0], kv[:0], pos[:0], torch.arange(0, device=dev), cs, w, 1e-6, cache, interleaved)
+    no_error(dev)
+
+
 # -------------------------------------------------------------------------- attention
 class Cache:
     """Ragged contexts in permuted pages; what no sequence owns is NaN."""
