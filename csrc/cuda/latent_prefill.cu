@@ -716,7 +716,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
     } else if (ok && !(split && t == 1)) {
-      const float inv = 1.f / l;
+      const float inv = l == 0.f ? 0.f : 1.f / l;  // a row without a finite score: zeros, as in the other forms
       bf16* dst = out + (int64_t)(row0 + row) * out_stride + (int64_t)h * kVal;
 #pragma unroll 1
       for (int c = 0; c < 8; ++c) {

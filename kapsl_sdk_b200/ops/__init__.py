@@ -354,8 +354,9 @@ def latent_decode_attention(q: torch.Tensor, cache: torch.Tensor, w_kv_b: torch.
     128 key and 128 value dims; here its key half moves to the query's side and its value
     half is applied to the attended latents, so nothing is expanded per cached token.
     ``q`` [B, H * 192] has 128 position-free and 64 rotated dims a head; ``out`` is
-    [B, H * 128].  Rows with ``ctx_lens`` 0 (a padded batch) give zeros.  ``max_ctx`` (a host
-    number, default the block tables' width) only bounds how many CTAs are launched.
+    [B, H * 128].  Rows with ``ctx_lens`` 0 (a padded batch) and rows whose scores are all -inf give
+    zeros.  ``max_ctx`` (a host number, default the block tables' width) only bounds how many
+    CTAs are launched.
     The keys of a block table entry outside the cache read as zeros, and device error 82 is recorded."""
     if scale is None:
         scale = 1.0 / math.sqrt(192)
@@ -482,10 +483,10 @@ def latent_prefill_attention(q: torch.Tensor, cache: torch.Tensor, w_kv_b: torch
     shorter for few of them.  ``form`` ("expanded" or "absorbed") overrides
     :meth:`LatentPrefillPlan.absorbed_is_shorter`, ``key_ranges`` (1 to 32, expanded form)
     :meth:`LatentPrefillPlan.key_ranges`; the two forms round differently.  Page slots behind
-    a context may hold anything; its own rows have to be finite, since in the expanded form
+    a context may hold anything; its own latents have to be finite, since in the expanded form
     a row that is not also reaches earlier new tokens (0 * NaN in the product with the values).
-    ``out`` rows outside the plan's sequences keep what they held (zeros when ``out`` is
-    allocated here)."""
+    Rows whose scores are all -inf give zeros.  ``out`` rows outside the plan's sequences keep
+    what they held (zeros when ``out`` is allocated here)."""
     if scale is None:
         scale = 1.0 / math.sqrt(192)
     if out is None:

@@ -137,14 +137,16 @@ def latent_row(kv: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor,
 
 def latent_attention(q: torch.Tensor, rows: torch.Tensor, w_kv_b: torch.Tensor, scale: float) -> torch.Tensor:
     """One sequence's latent attention, expanded form: q [n, H, 192] are the last n of the
-    tokens whose cache rows are rows [ctx, R + 64]; w_kv_b [H * 256, R].  -> [n, H, 128]"""
+    tokens whose cache rows are rows [ctx, R + 64]; w_kv_b [H * 256, R].  -> [n, H, 128]; a row
+    whose scores are all -inf gives zeros"""
     H, R = q.shape[1], rows.shape[1] - 64
     kv = torch.einsum("tr,hdr->thd", rows[:, :R].float(), w_kv_b.float().view(H, 256, R))
     k = torch.cat([kv[..., :128], rows[:, None, R:].float().expand(-1, H, -1)], -1)
     s = torch.einsum("qhd,khd->hqk", q.float(), k) * scale
     pos = torch.arange(rows.shape[0] - q.shape[0], rows.shape[0], device=q.device)
     s = s.masked_fill(torch.arange(rows.shape[0], device=q.device)[None, :] > pos[:, None], float("-inf"))
-    return torch.einsum("hqk,khd->qhd", torch.softmax(s, -1), kv[..., 128:])
+    p = torch.softmax(s, -1).masked_fill((s == float("-inf")).all(-1, keepdim=True), 0.0)
+    return torch.einsum("hqk,khd->qhd", p, kv[..., 128:])
 
 
 def silu_mul(x: torch.Tensor) -> torch.Tensor:

@@ -83,3 +83,17 @@ def test_reference_forms_agree():
         o = torch.softmax(qa @ c.T * 0.07, -1) @ c[:, :R]
         exp = torch.einsum("hr,hvr->hv", o, w[:, 128:])
         assert (got[i].double() - exp).abs().max() < 1e-4
+
+
+def test_reference_rows_without_a_finite_score():
+    g = torch.Generator().manual_seed(3)
+    H, R, ctx, n = 2, 256, 9, 7
+    q, rows = torch.randn(n, H, 192, generator=g), torch.randn(ctx, R + 64, generator=g)
+    w = torch.randn(H * 256, R, generator=g) / math.sqrt(R)
+    q[..., 128] = 1.0
+    rows[:5, R] = -math.inf  # new tokens 0 - 2 see keys up to 2 - 4
+    out = ref.latent_attention(q, rows, w, 0.07)
+    assert bool((out[:3] == 0).all()) and bool(torch.isfinite(out).all())
+    rest = ref.latent_attention(q[3:], rows[5:], w, 0.07)
+    # the same keys with weights of 0 between them: sums of at most 9 values
+    assert (out[3:] - rest).abs().max() <= 16 * 2.0 ** -24 * rest.abs().max() * 9

@@ -533,6 +533,43 @@ def test_first_keys_weigh_nothing(dev, form, H):
         within(out[i].view(H, 128), exp, tol + 8 * U / math.sqrt(3) * var.sqrt() + slop)
 
 
+@pytest.mark.parametrize("H", [3, 66])
+@pytest.mark.parametrize("n,first", [(3, 400), (200, 400), (400, 150)])
+def test_rows_without_a_finite_score(dev, H, n, first):
+    """The first keys' scores are -inf (an infinite rotary value).  A row that sees no others gives zeros in
+    every form, with one key range or several, whatever its neighbours in the batch are."""
+    from kapsl_sdk_b200 import ops
+
+    lens, scale = [400, 30], 1 / math.sqrt(192)
+    k = Cache(dev, lens, 512, 16, 31)
+    q, w = k.randn(n + 5, H, 192), k.randn(H, 256, 512, std=1 / math.sqrt(512))
+    q[:n, :, 128] = 8.0
+    j = torch.arange(lens[0], device=dev)
+    flat = k.cache.view(-1, 576)
+    k.rows[0][:first, 512] = -math.inf
+    flat[k.bt[0, j // 16].long() * 16 + j % 16] = k.rows[0]
+    plan = ops.latent_prefill_plan([n, 5], lens, dev)
+    outs = [ops.latent_prefill_attention(q.view(n + 5, -1), k.cache, w, plan, k.bt, H, form="expanded", key_ranges=r)
+            for r in (1, 2, 4)]
+    outs.append(ops.latent_prefill_attention(q.view(n + 5, -1), k.cache, w, plan, k.bt, H, form="absorbed"))
+    empty = max(0, first - (lens[0] - n))  # rows that see the first keys only
+    two = torch.stack([q[empty - 1], q[-1]]).view(2, -1)
+    for max_ctx in (1, None):  # one piece, several
+        ctx = torch.tensor([first, 30], dtype=torch.int32, device=dev)
+        one = ops.latent_decode_attention(two, k.cache, w, k.bt, ctx, H, max_ctx=max_ctx)
+        assert bool((one[0] == 0).all()) and bool(torch.isfinite(one[1].float()).all())
+    no_error(dev)
+    exp, tol = prefill64(q[n:], k.rows[1], w, scale)
+    for i, out in enumerate(outs):
+        assert bool((out[:empty] == 0).all())
+        assert bool(torch.isfinite(out[empty:].float()).all())
+        if i < 3:
+            within(out[n:].view(5, H, 128), exp, tol)
+            if empty < n:  # the others: softmax over the keys that count
+                e, t = prefill64(q[empty:n], k.rows[0][first:], w, scale)
+                within(out[empty:n].view(n - empty, H, 128), e, t)
+
+
 def test_decode_pages_outside(dev):
     """A table entry outside the cache records an error; other rows are untouched by it."""
     from kapsl_sdk_b200 import ops
