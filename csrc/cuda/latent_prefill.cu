@@ -347,7 +347,7 @@ constexpr float kNoMax = -1e30f;
 struct alignas(1024) PrefillSmem {
   uint8_t q[2][3][kSlotBytes];
   uint8_t ring[kSlots][kSlotBytes];
-  uint64_t q_full, k_full[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], drained;
+  uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], drained;
   uint32_t tmem_base;
   volatile int abort_flag;
 };
@@ -460,6 +460,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&s.q_full, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s.k_full[i], 1);
+      mbar_init(&s.k_empty[i], 1);
       mbar_init(&s.v_full[i], 1);
       mbar_init(&s.v_empty[i], 1);
       mbar_init(&s.s_full[i], 1);
@@ -484,7 +485,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int c = 0; c < 3; ++c) tma_load_2d(s.q[t][c], &q_map, &s.q_full, h * 192 + c * 64, row0 + t * 128);
       // Slots of tile j: keys 5j .. 5j + 2, values 5j + 3, 5j + 4 (mod 8).  Those of K_j were
       // last used by K_{j-2} and V_{j-2}, those of V_j by K_{j-1}, which is free once the last
-      // scores of tile j - 1 are complete.
+      // scores of tile j - 1 are complete.  The empty barriers go by the tile's parity: their
+      // next phase needs a tile that this thread has not sent yet, so none can be missed.
       bool ok = true;
       int j = 0;
       for (; j < nt; ++j) {
@@ -494,8 +496,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tma_load_2d(s.ring[(5 * j) % kSlots], &kv_map, bar, h * 256, kv0 + j * 128);
         tma_load_2d(s.ring[(5 * j + 1) % kSlots], &kv_map, bar, h * 256 + 64, kv0 + j * 128);
         tma_load_2d(s.ring[(5 * j + 2) % kSlots], &rope_map, bar, 0, kv0 + j * 128);
-        const int h_last = split ? (j - 1) & 1 : 1, phase = split ? (j - 1) >> 1 : j - 1;
-        if (j >= 1 && !wait_or_abort(s, &s.s_full[h_last], phase & 1, err, 91)) { ok = false; break; }
+        if (j >= 1 && !wait_or_abort(s, &s.k_empty[(j - 1) & 1], ((j - 1) >> 1) & 1, err, 91)) { ok = false; break; }
         bar = &s.v_full[j & 1];
         mbar_arrive_expect_tx(bar, 2 * kSlotBytes);
         tma_load_2d(s.ring[(5 * j + 3) % kSlots], &kv_map, bar, h * 256 + 128, kv0 + j * 128);
@@ -530,6 +531,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int kk = 0; kk < 4; ++kk) mma_bf16(tmem + t * 128, a + kk * 2, b + kk * 2, idesc_s, c + kk > 0);
         }
         mma_commit(&s.s_full[t]);
+        if (split || t == 1) mma_commit(&s.k_empty[j & 1]);  // the tile's last scores
       };
       auto issue_pv = [&](int t, int j, int keys, bool last) {
         const int i = split ? j >> 1 : j;  // the half's own count of tiles

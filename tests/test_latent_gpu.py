@@ -661,6 +661,24 @@ def test_prefill_passes_over_heads(dev, monkeypatch):
     no_error(dev)
 
 
+@pytest.mark.parametrize("n", [20, 200])
+def test_prefill_numbers_of_key_tiles(dev, n):
+    """One to eleven key tiles, in the order of two row tiles and in that of one (the ring's barriers turn
+    over at every second tile)."""
+    from kapsl_sdk_b200 import ops
+
+    H, R = 3, 512
+    lens = [c for c in range(100, 1401, 65) if c >= n]
+    k = Cache(dev, lens, R, 16, n)
+    q, w = k.randn(n * len(lens), H * 192, std=1.5), k.randn(H * 256, R, std=1 / math.sqrt(R))
+    plan = ops.latent_prefill_plan([n] * len(lens), lens, dev)
+    out = ops.latent_prefill_attention(q, k.cache, w, plan, k.bt, H, form="expanded", key_ranges=1)
+    no_error(dev)
+    for i in range(len(lens)):
+        exp, tol = prefill64(q[i * n:(i + 1) * n].view(n, H, 192), k.rows[i], w.view(H, 256, R), 1 / math.sqrt(192))
+        within(out[i * n:(i + 1) * n].view(n, H, 128), exp, tol)
+
+
 @pytest.mark.parametrize("key_ranges", [2, 3, 7, 32])
 def test_prefill_key_ranges(dev, key_ranges):
     """The keys in parts: parts that end inside a row's keys, that only later rows see, that hold nothing."""
