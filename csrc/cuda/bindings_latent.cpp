@@ -295,7 +295,7 @@ void check_latent_prefill(Tensor q, Tensor cache, Tensor w, Tensor block_tables,
 
 // attention of `heads` heads: q / out already narrowed to them
 void latent_prefill(Tensor q, Tensor kv, Tensor k_rope, Tensor work, Tensor seq_info, Tensor out, int64_t heads,
-                    double scale, int64_t ranges, c10::optional<Tensor> parts, Tensor err) {
+                    double scale, int64_t cut, int64_t part_tiles, int64_t slots, c10::optional<Tensor> parts, Tensor err) {
   const char* op = "latent_prefill";
   TORCH_CHECK(q.is_cuda(), op, ": q must be a CUDA tensor");
   check(q, at::kBFloat16, q, op, "q");
@@ -326,13 +326,16 @@ void latent_prefill(Tensor q, Tensor kv, Tensor k_rope, Tensor work, Tensor seq_
   a.kv = bf(kv);
   a.kv_stride = kv.stride(0);
   a.kv_rows = kv.size(0);
-  TORCH_CHECK(ranges >= 1 && ranges <= 32, op, ": 1 to 32 key ranges");
-  if (ranges > 1) {
-    const int64_t rows = ranges * heads * work.size(0) * 256;
+  if (cut > 0) {
+    TORCH_CHECK(cut <= work.size(0) && part_tiles >= 1 && part_tiles <= INT32_MAX && slots >= 1 && slots <= 32, op,
+                ": row tiles or parts out of range");
+    const int64_t rows = slots * heads * cut * 256;
     TORCH_CHECK(parts.has_value(), op, ": key ranges need room for partial results");
     check(*parts, at::kFloat, q, op, "parts");
     TORCH_CHECK(parts->is_contiguous() && parts->numel() >= rows * (kVal + 2), op, ": parts too small");
-    a.ranges = (int)ranges;
+    a.cut = (int)cut;
+    a.part_tiles = (int)part_tiles;
+    a.slots = (int)slots;
     a.part_o = parts->data_ptr<float>();
     a.part_ml = reinterpret_cast<float2*>(a.part_o + rows * kVal);
   }

@@ -98,9 +98,11 @@ struct LatentPrefill {
   int64_t out_stride = 0;
   int heads = 0;
   float scale = 0.f;
-  int ranges = 1;             // parts of the key tiles (at most 32), joined from
-  float* part_o = nullptr;    // [ranges, heads, nwork, 256, 128]
-  float2* part_ml = nullptr;  // [ranges, heads, nwork, 256]: a part's maximum (log2) and sum
+  // The first `cut` row tiles of work (the longest) have their keys cut into parts of part_tiles
+  // key tiles, no more than `slots` (at most 32) each, joined from
+  int cut = 0, part_tiles = 0, slots = 1;
+  float* part_o = nullptr;    // [slots, heads, cut, 256, 128]
+  float2* part_ml = nullptr;  // [slots, heads, cut, 256]: a part's maximum (log2) and sum
   int* err = nullptr;
 };
 void launch_latent_prefill(const LatentPrefill& a, cudaStream_t st);

@@ -333,11 +333,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kExpandThreads, 1)
 // rows instead (and the second half's m, l and O join the first's at the end): the chain of
 // scores, softmax and product that bounds a lone row tile is half as long.
 //
-// Where the CTAs are too few for the GPU, gridDim.z ranges of key tiles give fp32 partial results
-// per row, which latent_prefill_join_kernel joins.
+// Where the CTAs are too few for the GPU, the longest row tiles have their keys cut into parts of
+// part_tiles key tiles, a CTA each, that give fp32 partial results per row, which
+// latent_prefill_join_kernel joins.  Row tiles no longer than a part stay whole.
 //
 // Keys past a row's position have p = 0.  PV stops at the row tile's last key, rounded up
-// to 16; the rows there are the gather's zeros, so nothing behind a sequence is read.
+// to 16; the rows there are the expansion's zeros, so nothing behind a sequence is read.
 constexpr int kThreads = 384;  // warp 0 TMA, warp 1 MMA, warps 4-7 and 8-11 softmax of row tile 0 and 1
 constexpr int kSlots = 8;
 constexpr uint32_t kSlotBytes = 128 * 128;
@@ -425,19 +426,23 @@ __global__ void __launch_bounds__(kThreads, 1)
     latent_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap kv_map,
                           const __grid_constant__ CUtensorMap rope_map, const int32_t* work,
                           const int32_t* seq_info, int64_t q_rows, float scale_log2,
-                          bf16* out, int64_t out_stride, float* part_o, float2* part_ml,
-                          int* err) {
+                          bf16* out, int64_t out_stride, int cut, int part_tiles, int slots, float* part_o,
+                          float2* part_ml, int* err) {
   griddep_entry();
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   PrefillSmem& s = *reinterpret_cast<PrefillSmem*>(smem_raw);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
   const int h = blockIdx.y;
-  const int32_t* si = seq_info + 5 * work[2 * blockIdx.x];
-  const int t0 = work[2 * blockIdx.x + 1];
+  // `slots` CTAs a row tile that is cut, one for each of the others
+  const int cut_ctas = cut * slots, bx = blockIdx.x;
+  const bool parted = bx < cut_ctas;
+  const int tile = parted ? bx / slots : cut + bx - cut_ctas, part = parted ? bx - tile * slots : 0;
+  const int32_t* si = seq_info + 5 * work[2 * tile];
+  const int t0 = work[2 * tile + 1];
   const int row0 = si[0] + t0, n = si[1] - t0;  // n: rows from t0 on
-  // this CTA's range of key tiles; keys and positions count from its first key
-  const int all_keys = si[2] - si[1] + t0 + min(n, 256);
-  const int range = ((all_keys + 127) / 128 + gridDim.z - 1) / gridDim.z * 128, key0 = blockIdx.z * range;
+  // this CTA's key tiles; keys and positions count from its first key
+  const int all_keys = si[2] - si[1] + t0 + min(n, 256), all_tiles = (all_keys + 127) / 128;
+  const int range = 128 * (parted ? part_tiles : all_tiles), key0 = part * range;
   const int pos0 = si[2] - si[1] + t0 - key0, kv0 = si[4] + key0;
   // keys of the two halves, key tiles of the CTA and of each half
   const bool split = n <= 128;
@@ -445,15 +450,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int keys1 = split ? keys0 : max(0, min(range, pos0 + min(n, 256)));
   const int nt = (keys1 + 127) / 128;
   const int nt0 = split ? (nt + 1) / 2 : (keys0 + 127) / 128, nt1 = split ? nt / 2 : nt;
-  const int64_t part_row = ((int64_t)(blockIdx.z * gridDim.y + h) * gridDim.x + blockIdx.x) * 256;
+  const int64_t part_row = ((int64_t)(part * gridDim.y + h) * cut + tile) * 256;
   if ((smem_u32(smem_raw) & 1023) || row0 < 0 || row0 + min(n, 256) > q_rows || n <= 0) {
     if (threadIdx.x == 0) atomicCAS(err, 0, 90);
     return;
   }
-  if (nt == 0) {  // no keys in this range
-    if (threadIdx.x < 256) part_ml[part_row + threadIdx.x] = make_float2(-INFINITY, 0.f);
-    return;
-  }
+  if (key0 >= all_keys) return;  // this row tile has fewer parts than the longest
 
   if (threadIdx.x == 0) {
     s.abort_flag = 0;
@@ -697,7 +699,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
     }
-    if (part_o != nullptr) {
+    if (parted) {
       if (!(split && t == 1)) {
         const float inv = !ok || l == 0.f ? 0.f : 1.f / l;
         part_ml[part_row + row] = !ok || l == 0.f ? make_float2(-INFINITY, 0.f) : make_float2(m_out, l);
@@ -749,28 +751,32 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// out = sum_z w_z o_z / sum_z w_z over the key ranges z, w_z = l_z 2^(m_z - M) of their maxima and sums
+// out = sum_z w_z o_z / sum_z w_z over the parts z of a row tile's keys, w_z = l_z 2^(m_z - M) of their maxima and sums
 // (kept apart: m_z + log2 l_z would round l_z to m_z's last place): one warp per (row of a
 // row tile, head), 4 dims a lane.
-__global__ void __launch_bounds__(256) latent_prefill_join_kernel(const float* part_o, const float2* part_ml, int ranges,
-                                                                  const int32_t* work, const int32_t* seq_info,
-                                                                  bf16* out, int64_t out_stride) {
+__global__ void __launch_bounds__(256) latent_prefill_join_kernel(const float* part_o, const float2* part_ml,
+                                                                  int part_tiles, int slots, const int32_t* work,
+                                                                  const int32_t* seq_info, bf16* out,
+                                                                  int64_t out_stride) {
   griddep_entry();
   const int row = blockIdx.z * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31, h = blockIdx.y;
   const int32_t* si = seq_info + 5 * work[2 * blockIdx.x];
   const int t0 = work[2 * blockIdx.x + 1];
   if (t0 + row >= si[1]) return;
+  const int keys = si[2] - si[1] + t0 + min(si[1] - t0, 256);
+  const bool mine = lane < slots && lane * part_tiles * 128 < keys;  // lane z: part z
+  const int parts = __popc(__ballot_sync(0xffffffffu, mine));
   const int64_t first = ((int64_t)h * gridDim.x + blockIdx.x) * 256 + row, step = (int64_t)gridDim.y * gridDim.x * 256;
-  const float2 ml = lane < ranges ? part_ml[first + lane * step] : make_float2(-INFINITY, 0.f);
+  const float2 ml = mine ? part_ml[first + lane * step] : make_float2(-INFINITY, 0.f);
   float M = warp_max(ml.x);
   if (M == -INFINITY) M = 0.f;
   const float e = ml.y * ex2(ml.x - M), L = warp_sum(e);
   const float w = L == 0.f ? 0.f : e / L;
   float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-  for (int z = 0; z < ranges; ++z) {
+  for (int z = 0; z < parts; ++z) {
     const float f = __shfl_sync(0xffffffffu, w, z);
-    if (f != 0.f) {  // a range without keys wrote no partial result
+    if (f != 0.f) {  // a part without keys of this row may have written no result
       const float4 y = *reinterpret_cast<const float4*>(part_o + (first + z * step) * kVal + lane * 4);
       x.x += f * y.x, x.y += f * y.y, x.z += f * y.z, x.w += f * y.w;
     }
@@ -813,14 +819,14 @@ void launch_latent_prefill(const LatentPrefill& a, cudaStream_t st) {
   const CUtensorMap tq = make_tmap_2d_bf16(a.q, a.T, (uint64_t)a.heads * (kNope + kRot), a.q_stride, 128, 64, true);
   const CUtensorMap tkv = make_tmap_2d_bf16(a.kv, a.kv_rows, (uint64_t)a.heads * (kNope + kVal), a.kv_stride, 128, 64, true);
   const CUtensorMap tr = make_tmap_2d_bf16(a.k_rope, a.kv_rows, kRot, kRot, 128, 64, true);
-  const bool ranges = a.ranges > 1;
-  launch_k(latent_prefill_kernel, dim3(a.nwork, a.heads, a.ranges), kThreads, smem, st, tq, tkv, tr, a.work, a.seq_info,
-           a.T, a.scale * kLog2e, a.out, a.out_stride, ranges ? a.part_o : nullptr, a.part_ml, a.err);
+  launch_k(latent_prefill_kernel, dim3(a.cut * a.slots + a.nwork - a.cut, a.heads), kThreads, smem, st, tq, tkv, tr,
+           a.work, a.seq_info, a.T, a.scale * kLog2e, a.out, a.out_stride, a.cut, a.part_tiles, a.slots, a.part_o,
+           a.part_ml, a.err);
   KAPSL_LAUNCH_CHECK();
   note_launch();
-  if (!ranges) return;
-  launch_k(latent_prefill_join_kernel, dim3(a.nwork, a.heads, 32), 256, 0, st, a.part_o, a.part_ml, a.ranges, a.work,
-           a.seq_info, a.out, a.out_stride);
+  if (a.cut == 0) return;
+  launch_k(latent_prefill_join_kernel, dim3(a.cut, a.heads, 32), 256, 0, st, a.part_o, a.part_ml, a.part_tiles, a.slots,
+           a.work, a.seq_info, a.out, a.out_stride);
   KAPSL_LAUNCH_CHECK();
   note_launch();
 }

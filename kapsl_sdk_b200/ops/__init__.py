@@ -373,7 +373,8 @@ def latent_decode_attention(q: torch.Tensor, cache: torch.Tensor, w_kv_b: torch.
 
 
 LATENT_PREFILL_TILE = 256  # query tokens a CTA of the expanded-form attention handles
-LATENT_KV_BYTES = 2 << 30  # expanded keys and values held at once; more heads go in further passes
+LATENT_KV_BYTES = 2 << 30  # expanded keys, values and partial results held at once; more heads go in further passes
+LATENT_PART_BYTES = LATENT_PREFILL_TILE * 130 * 4  # partial result of one part of a row tile's keys and one head
 
 
 @dataclass
@@ -392,6 +393,7 @@ class LatentPrefillPlan:
     single_tiles: int       # 64-key tiles of all new tokens taken one by one
     row_tiles: int          # 128-key tiles of all 256-row tiles of new tokens
     chain_us: float         # the longest of those row tiles by itself (microseconds)
+    key_tiles: list[int]    # 128-key tiles of each row tile, in the order of work (most first)
 
     def key_ranges(self, num_heads: int) -> int:
         """Parts into which the expanded form cuts every row tile's keys: as often as the longest row tile
@@ -400,6 +402,23 @@ class LatentPrefillPlan:
         fill the GPU stay whole, since parts cost fp32 partial results and a joining kernel."""
         spread = max(4.0, 1.9 * self.row_tiles * num_heads / 148)
         return max(1, min(32, -(-self.max_ctx // 128) // 4, int(self.chain_us / spread)))
+
+    def passes(self, num_heads: int, key_ranges: int = 0) -> tuple[int, int, int, int]:
+        """The expanded form's (heads a pass, row tiles cut, key tiles a part, parts of the longest row tile)
+        under LATENT_KV_BYTES (one head may take more keys and values than that).  Only row tiles longer
+        than a part are cut: the others write no partial results.  One chunk of 256 tokens over 65,536 beside
+        500 single tokens, 8 heads: 10 MB of them for one row tile; cutting all 501 took 4.8 GB."""
+        kv = self.kv_rows * 512
+        step = max(1, min(num_heads, LATENT_KV_BYTES // kv))
+        ranges = key_ranges if key_ranges > 0 else self.key_ranges(step)
+        while ranges > 1:
+            part = -(-self.key_tiles[0] // ranges)
+            cut, slots = sum(n > part for n in self.key_tiles), -(-self.key_tiles[0] // part)
+            room = cut * slots * LATENT_PART_BYTES
+            if room <= LATENT_KV_BYTES:
+                return max(1, min(step, LATENT_KV_BYTES // (kv + room))), cut, part, slots
+            ranges //= 2
+        return step, 0, 0, 1
 
     def absorbed_is_shorter(self, num_heads: int, rank: int = 512) -> bool:
         """Whether taking every new token by itself in the absorbed form is estimated to take less time
@@ -466,7 +485,8 @@ def latent_prefill_plan(q_lens: Sequence[int], ctx_lens: Sequence[int], device, 
     return LatentPrefillPlan(work=t[0].view(-1, 2), kv_work=t[1].view(-1, 2), seq_info=t[2].view(-1, 5), rows=row,
                              tables=bt_start + len(info) if info else 0, max_ctx=max([i[2] for i in info], default=0),
                              kv_rows=kv, q_start=int(q_start), row_ctx=t[3], row_table=t[4], single_tiles=single,
-                             row_tiles=sum(-(-w[0] // 128) for w in work), chain_us=chain)
+                             row_tiles=sum(-(-w[0] // 128) for w in work), chain_us=chain,
+                             key_tiles=[-(-w[0] // 128) for w in work])
 
 
 def latent_prefill_attention(q: torch.Tensor, cache: torch.Tensor, w_kv_b: torch.Tensor, plan: LatentPrefillPlan,
@@ -478,7 +498,7 @@ def latent_prefill_attention(q: torch.Tensor, cache: torch.Tensor, w_kv_b: torch
     The new tokens' rows are in ``cache`` already; arguments as in
     :func:`latent_decode_attention`, with ``plan`` from :func:`latent_prefill_plan`.  In the
     expanded form the context's latents are expanded out of their pages by ``w_kv_b`` to keys
-    and values (at most ``LATENT_KV_BYTES`` of them at a time, in passes over the heads); in
+    and values (with partial results at most ``LATENT_KV_BYTES`` at a time, in passes over the heads); in
     the absorbed form every new token is a row of :func:`latent_decode_attention`, which is
     shorter for few of them.  ``form`` ("expanded" or "absorbed") overrides
     :meth:`LatentPrefillPlan.absorbed_is_shorter`, ``key_ranges`` (1 to 32, expanded form)
@@ -505,21 +525,22 @@ def latent_prefill_attention(q: torch.Tensor, cache: torch.Tensor, w_kv_b: torch
         c.latent_decode_attention(q[rows], cache, w_kv_b, block_tables, plan.row_ctx, out[rows], num_heads,
                                   float(scale), plan.max_ctx, ws, plan.row_table, err)
         return out
+    if key_ranges > 32:
+        raise RuntimeError("latent_prefill_attention: 1 to 32 key ranges")
     w = w_kv_b.view(num_heads * 256, -1)
-    step = max(1, min(num_heads, LATENT_KV_BYTES // (plan.kv_rows * 512)))
+    step, cut, part, slots = plan.passes(num_heads, key_ranges)
     k_rope = torch.empty(plan.kv_rows, 64, dtype=torch.bfloat16, device=q.device)
     kv_buf = torch.empty(plan.kv_rows * step * 256, dtype=torch.bfloat16, device=q.device)
-    ranges = key_ranges if key_ranges > 0 else plan.key_ranges(min(step, num_heads))
     parts = None
-    if ranges > 1:
-        parts = torch.empty(ranges * step * plan.work.shape[0] * 256 * 130, dtype=torch.float32, device=q.device)
+    if cut > 0:
+        parts = torch.empty(cut * slots * step * LATENT_PART_BYTES // 4, dtype=torch.float32, device=q.device)
     for h0 in range(0, num_heads, step):
         n = min(step, num_heads - h0)
         kv = kv_buf[:plan.kv_rows * n * 256].view(plan.kv_rows, n * 256)
         c.latent_expand(cache, w[h0 * 256:(h0 + n) * 256], plan.kv_work, plan.seq_info, block_tables, kv,
                         k_rope if h0 == 0 else None, err)
         c.latent_prefill(q[:, h0 * 192:(h0 + n) * 192], kv, k_rope, plan.work, plan.seq_info,
-                         out[:, h0 * 128:(h0 + n) * 128], n, float(scale), ranges, parts, err)
+                         out[:, h0 * 128:(h0 + n) * 128], n, float(scale), cut, part, slots, parts, err)
     return out
 
 

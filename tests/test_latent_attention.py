@@ -97,3 +97,32 @@ def test_reference_rows_without_a_finite_score():
     rest = ref.latent_attention(q[3:], rows[5:], w, 0.07)
     # the same keys with weights of 0 between them: sums of at most 9 values
     assert (out[3:] - rest).abs().max() <= 16 * 2.0 ** -24 * rest.abs().max() * 9
+
+
+@pytest.mark.parametrize("q_lens,ctx_lens,heads", [
+    ([256] + [1] * 500, [65536] + [64] * 500, 8), ([512] + [17] * 1000, [30000] + [40] * 1000, 4),
+    ([256] + [40] * 1000, [131072] + [40] * 1000, 8), ([256] + [80] * 100, [65536] + [80] * 100, 16)])
+def test_partial_results_of_mixed_batches(q_lens, ctx_lens, heads):
+    """Short sequences beside a long context are not cut with it, and need no partial results."""
+    p = ops.latent_prefill_plan(q_lens, ctx_lens, device="cpu")
+    step, cut, part, slots = p.passes(heads)
+    assert step == heads and cut == -(-q_lens[0] // 256) and part >= 4 and slots == p.key_ranges(heads) > 1
+    assert cut * slots * step * ops.LATENT_PART_BYTES < 80 << 20
+    # every tile in order, the parts cover the longest
+    assert p.key_tiles == sorted(p.key_tiles, reverse=True) and len(p.key_tiles) == p.work.shape[0]
+    assert slots * part >= p.key_tiles[0] and all(n <= part for n in p.key_tiles[cut:])
+
+
+@pytest.mark.parametrize("q_lens,ctx_lens,heads,ranges", [
+    ([4096] * 8, [20000] * 8, 128, 32), ([256] * 900, [2000] * 900, 16, 32), ([300] * 40, [9000] * 40, 20, 7),
+    ([64], [500], 5, 32), ([2048] * 300, [3000] * 300, 2, 32)])
+def test_scratch_of_prefill_is_bounded(q_lens, ctx_lens, heads, ranges):
+    """However many parts are asked for, what a pass holds stays within the bound while one head's keys and
+    values do."""
+    p = ops.latent_prefill_plan(q_lens, ctx_lens, device="cpu")
+    step, cut, part, slots = p.passes(heads, ranges)
+    assert 1 <= step <= heads and slots <= 32
+    room = cut * slots * ops.LATENT_PART_BYTES
+    assert room <= ops.LATENT_KV_BYTES
+    assert step == 1 or step * (p.kv_rows * 512 + room) <= ops.LATENT_KV_BYTES
+    assert p.passes(heads, 1)[1:] == (0, 0, 1)

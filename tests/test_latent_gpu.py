@@ -699,6 +699,38 @@ def test_prefill_key_ranges(dev, key_ranges):
         ops.latent_prefill_attention(q, k.cache, w, plan, k.bt, H, form="expanded", key_ranges=33)
 
 
+@pytest.mark.parametrize("key_ranges", [0, 2, 9])
+def test_prefill_ranges_and_passes(dev, key_ranges, monkeypatch):
+    """A long context cut into parts beside whole short ones, with the heads in several passes; rows between
+    and behind the sequences stay."""
+    from kapsl_sdk_b200 import ops
+
+    q_lens, ctx_lens, H, R = [140, 3, 257, 1, 30], [6000, 3, 3100, 129, 700], 5, 512
+    k = Cache(dev, ctx_lens, R, 16, 50)
+    T, q0 = sum(q_lens) + 4, 2
+    q, w = k.randn(T, H * 192, std=1.5), k.randn(H * 256, R, std=1 / math.sqrt(R))
+    plan = ops.latent_prefill_plan(q_lens, ctx_lens, dev, q_start=q0)
+    step, cut, part, slots = plan.passes(H, key_ranges)
+    assert step == H and 0 < cut < plan.work.shape[0] and slots > 1
+    outs = []
+    for room in (ops.LATENT_KV_BYTES, 2 * (plan.kv_rows * 512 + cut * slots * ops.LATENT_PART_BYTES)):
+        monkeypatch.setattr(ops, "LATENT_KV_BYTES", room)
+        if outs:
+            assert plan.passes(H, key_ranges or slots)[0] == 2  # heads 2, 2, 1
+        out = torch.full((T, H * 128), 3.0, device=dev, dtype=torch.bfloat16)
+        ops.latent_prefill_attention(q, k.cache, w, plan, k.bt, H, out=out, form="expanded",
+                                     key_ranges=key_ranges or slots)
+        outs.append(out)
+    no_error(dev)
+    assert torch.equal(*outs)
+    at = q0
+    for i, n in enumerate(q_lens):
+        exp, tol = prefill64(q[at:at + n].view(n, H, 192), k.rows[i], w.view(H, 256, R), 1 / math.sqrt(192))
+        within(out[at:at + n].view(n, H, 128), exp, tol)
+        at += n
+    assert bool((out[:q0] == 3.0).all()) and bool((out[at:] == 3.0).all())
+
+
 def test_prefill_picks_a_form(dev):
     """Few tokens over a long context go by themselves, a long chunk is expanded; the result is that of the
     form named."""
