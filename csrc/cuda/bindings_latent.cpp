@@ -45,6 +45,16 @@ bool same_view(const Tensor& a, const Tensor& b) {
 // Strides of dims of one index never step, whatever they say.
 int64_t step(const Tensor& t, int64_t d) { return t.size(d) > 1 ? t.stride(d) : 0; }
 
+// Row pitch of a [rows, width] view, for kernels and tensor maps: that of a lone row never counts.
+int64_t pitch(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
+
+// Rows that share memory (an expanded query) are copied: a tensor map's rows lie apart.
+Tensor rows_apart(const Tensor& t) {
+  if (t.size(0) <= 1 || t.stride(0) >= t.size(1)) return t;
+  const c10::cuda::CUDAGuard g(t.device());
+  return t.contiguous();
+}
+
 kapsl::RopeArgs rope_args(const char* op, const Tensor& x, const Tensor& y, const Tensor& positions,
                           const Tensor& cos_sin, int64_t offset, bool interleaved, const Tensor& err) {
   TORCH_CHECK(x.is_cuda(), op, ": x must be a CUDA tensor");
@@ -197,6 +207,7 @@ void latent_decode_attention(Tensor q, Tensor cache, Tensor w, Tensor block_tabl
                   (reinterpret_cast<uintptr_t>(workspace.data_ptr()) & 127) == 0,
               op, ": workspace too small or not 128-byte aligned");
   check(err, at::kInt, q, op, "err");
+  q = rows_apart(q);
   const c10::cuda::CUDAGuard g(q.device());
   kapsl::LatentDecode a;
   if (table_rows.has_value()) {
@@ -207,7 +218,7 @@ void latent_decode_attention(Tensor q, Tensor cache, Tensor w, Tensor block_tabl
   }
   a.num_tables = (int)block_tables.size(0);
   a.q = bf(q);
-  a.q_stride = q.stride(0);
+  a.q_stride = pitch(q);
   a.cache = bf(cache);
   a.num_blocks = cache.size(0);
   a.page = (int)cache.size(1);
@@ -217,7 +228,7 @@ void latent_decode_attention(Tensor q, Tensor cache, Tensor w, Tensor block_tabl
   a.max_blocks = (int)block_tables.size(1);
   a.ctx_lens = ctx_lens.data_ptr<int32_t>();
   a.out = bf(out);
-  a.out_stride = out.stride(0);
+  a.out_stride = pitch(out);
   a.B = (int)B;
   a.H = (int)H;
   a.max_ctx = (int)std::min<int64_t>(std::max<int64_t>(max_ctx, 0), INT32_MAX);
@@ -271,7 +282,7 @@ void latent_expand(Tensor cache, Tensor w, Tensor work, Tensor seq_info, Tensor 
   a.heads = (int)heads;
   a.num_sms = kapsl::gemm_num_sms();
   a.kv = bf(kv);
-  a.kv_stride = kv.stride(0);
+  a.kv_stride = pitch(kv);
   a.err = err.data_ptr<int>();
   kapsl::launch_latent_expand(a, cur_stream());
 }
@@ -318,13 +329,14 @@ void latent_prefill(Tensor q, Tensor kv, Tensor k_rope, Tensor work, Tensor seq_
   check_rows16(op, kv, "kv");
   check_rows16(op, k_rope, "k_rope");
   check_rows16(op, out, "out");
+  q = rows_apart(q);
   const c10::cuda::CUDAGuard g(q.device());
   kapsl::LatentPrefill a;
   a.q = bf(q);
-  a.q_stride = q.stride(0);
+  a.q_stride = pitch(q);
   a.T = q.size(0);
   a.kv = bf(kv);
-  a.kv_stride = kv.stride(0);
+  a.kv_stride = pitch(kv);
   a.kv_rows = kv.size(0);
   if (cut > 0) {
     TORCH_CHECK(cut <= work.size(0) && part_tiles >= 1 && part_tiles <= INT32_MAX && slots >= 1 && slots <= 32, op,
@@ -344,7 +356,7 @@ void latent_prefill(Tensor q, Tensor kv, Tensor k_rope, Tensor work, Tensor seq_
   a.nwork = (int)work.size(0);
   a.seq_info = seq_info.data_ptr<int32_t>();
   a.out = bf(out);
-  a.out_stride = out.stride(0);
+  a.out_stride = pitch(out);
   a.heads = (int)heads;
   a.scale = (float)scale;
   a.err = err.data_ptr<int>();

@@ -613,6 +613,40 @@ def test_decode_refuses(dev):
     no_error(dev)
 
 
+@pytest.mark.parametrize("H", [3, 66, 300])
+def test_one_row_of_any_pitch(dev, H):
+    """A single row may be a view whose row stride no tensor map could take (dims of one index never step),
+    and rows may share memory (an expanded query)."""
+    from kapsl_sdk_b200 import ops
+
+    k = Cache(dev, [70], 512, 16, 40)
+    w, scale = k.randn(H, 256, 512, std=1 / math.sqrt(512)), 1 / math.sqrt(192)
+    q = k.randn(1, H * 192 + 3)[:, :H * 192]
+    assert q.stride(0) % 8 != 0
+    plan = ops.latent_prefill_plan([1], [70], dev)
+    exp, tol = decode64(q.view(H, 192), k.rows[0], w, scale)
+    e2, t2 = prefill64(q.reshape(1, H, 192), k.rows[0], w, scale)
+    for form, e, t in (("decode", exp, tol), ("absorbed", exp, tol), ("expanded", e2[0], t2[0])):
+        out = torch.full((1, H * 128 + 3), 3.0, device=dev, dtype=torch.bfloat16)
+        if form == "decode":
+            ops.latent_decode_attention(q, k.cache, w, k.bt, k.ctx, H, out=out[:, :H * 128])
+        else:
+            ops.latent_prefill_attention(q, k.cache, w, plan, k.bt, H, out=out[:, :H * 128], form=form)
+        no_error(dev)
+        within(out[0, :H * 128].view(H, 128), e, t)
+        assert bool((out[:, H * 128:] == 3.0).all())
+    n = 5
+    many = q[0].expand(n, H * 192)
+    out = ops.latent_decode_attention(many, k.cache, w, k.bt.expand(n, -1).contiguous(), k.ctx.expand(n).contiguous(), H)
+    within(out.view(n, H, 128), exp.expand(n, H, 128), tol.expand(n, H, 128))
+    plan = ops.latent_prefill_plan([n], [70], dev)
+    for form in ("absorbed", "expanded"):
+        out = ops.latent_prefill_attention(many, k.cache, w, plan, k.bt, H, form=form)
+        no_error(dev)
+        e, t = (exp, tol) if form == "absorbed" else (e2[0], t2[0])
+        within(out[-1].view(H, 128), e, t)
+
+
 PREFILLS = [([1], [1]), ([17], [17]), ([130], [130]), ([128, 256], [128, 300]), ([300, 0, 1, 64], [557, 9, 900, 64]),
             ([257, 129, 5, 385], [257, 513, 1000, 400]), ([128, 3, 100, 1, 64], [128, 129, 640, 2500, 385])]
 
