@@ -249,9 +249,12 @@ __global__ void __launch_bounds__(256) rope_latent_write_kernel(
   const int pos = positions[t];
   const int64_t slot = slots[t];
   const bool ok = pos >= 0 && pos < max_pos;
+  if (slot < 0) return;  // a padded row, whatever its position
   if (!ok && lane == 0) atomicCAS(err, 0, 80);
-  if (slot >= num_slots && lane == 0) atomicCAS(err, 0, 81);
-  if (slot < 0 || slot >= num_slots) return;
+  if (slot >= num_slots) {
+    if (lane == 0) atomicCAS(err, 0, 81);
+    return;
+  }
   const bf16* src = kv + (int64_t)t * kv_stride;
   bf16* dst = cache + slot * (R + P);
   Vec<bf16, N> v[R / 256];

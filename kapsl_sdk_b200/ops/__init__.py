@@ -119,8 +119,10 @@ def rope_latent_write(q_rope: torch.Tensor, kv: torch.Tensor, positions: torch.T
 
     ``kv`` [T, R + 64] (R 256 or 512) is a token's compressed row: the first R values are RMS-normed
     with ``weight``, the last 64 rotated by ``positions``, and the row goes to
-    ``cache`` [blocks, page, R + 64] at ``slots[t]`` = block * page + offset (a negative slot
-    writes nothing; one past the cache is skipped and records device error 81).
+    ``cache`` [blocks, page, R + 64] at ``slots[t]`` = block * page + offset (a negative slot marks
+    a padded row: nothing is written, and its position is not looked at for errors; a slot past
+    the cache is skipped and records device error 81).  A position outside the table leaves its
+    key and queries unrotated and, unless the row is padded, records device error 80.
     ``q_rope`` [T, H, 64], the rotary part of the query heads (usually a view
     ``q.view(T, H, 192)[..., 128:]``), is rotated in place, or into ``q_out``.
     Two tokens of one call must not share a slot."""

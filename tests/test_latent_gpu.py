@@ -243,6 +243,28 @@ def test_tables_without_rows(dev, interleaved):
     no_error(dev)
 
 
+def test_write_padded_rows_need_no_position(dev):
+    """A row whose slot is negative writes nothing and records nothing, whatever its position says; its query
+    heads stay as they were."""
+    from kapsl_sdk_b200 import ops
+    from kapsl_sdk_b200.ops import reference as ref
+
+    cs = ref.rope_cos_sin(10, 64, 1e4, device=dev)
+    cache = torch.full((1, 16, 576), 3.0, device=dev, dtype=torch.bfloat16)
+    q = torch.randn(4, 2, 64, device=dev).to(torch.bfloat16)
+    kv, w = torch.randn(4, 576, device=dev).to(torch.bfloat16), torch.ones(512, device=dev, dtype=torch.bfloat16)
+    pos = torch.tensor([5, -1, 10, 2 ** 31 - 1], dtype=torch.int32, device=dev)
+    slots = torch.tensor([0, -1, -1, -7], device=dev)
+    out = ops.rope_latent_write(q, kv, pos, slots, cs, w, 1e-6, cache, q_out=torch.empty_like(q))
+    no_error(dev)
+    assert torch.equal(out[1:], q[1:]) and not torch.equal(out[0], q[0])
+    assert bool((cache[0, 1:] == 3.0).all()) and not bool((cache[0, 0] == 3.0).any())
+    slots[1] = 1  # a row that is written has to have one
+    ops.rope_latent_write(q, kv, pos, slots, cs, w, 1e-6, cache, q_out=out)
+    torch.cuda.synchronize()
+    assert ops.check_errors(dev) == 80
+
+
 # -------------------------------------------------------------------------- attention
 class Cache:
     """Ragged contexts in permuted pages; what no sequence owns is NaN."""
