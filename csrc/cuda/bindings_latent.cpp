@@ -197,7 +197,11 @@ void latent_decode_attention(Tensor q, Tensor cache, Tensor w, Tensor block_tabl
   TORCH_CHECK(block_tables.dim() == 2 && block_tables.is_contiguous() &&
                   (table_rows.has_value() || block_tables.size(0) >= B) && (block_tables.size(1) >= 1 || B == 0),
               op, ": block_tables must be [B, max_blocks] contiguous");
-  TORCH_CHECK(block_tables.size(1) * cache.size(1) <= INT32_MAX, op, ": block_tables too wide");
+  // the kernels count tokens of a row, rounded up to a tile, and tiles of all rows in 32 bits
+  const int64_t tokens = block_tables.size(1) * cache.size(1);
+  TORCH_CHECK(tokens <= INT32_MAX - 128, op, ": block_tables too wide");
+  TORCH_CHECK(B * ((tokens + 63) / 64) <= 1 << 30, op, ": ", num(B), " rows of up to ", num(tokens),
+              " tokens are too many for one call");
   check(ctx_lens, at::kInt, q, op, "ctx_lens");
   TORCH_CHECK(ctx_lens.dim() == 1 && ctx_lens.is_contiguous() && ctx_lens.size(0) >= B, op,
               ": ctx_lens must hold an int32 per row");

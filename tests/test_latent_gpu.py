@@ -669,6 +669,30 @@ def test_one_row_of_any_pitch(dev, H):
         within(out[-1].view(H, 128), e, t)
 
 
+def test_decode_refuses_what_32_bits_do_not_count(dev):
+    """Tables so wide, or rows so many, that tokens rounded up to a tile or the tiles of all rows pass 32 bits."""
+    from kapsl_sdk_b200 import ops
+
+    k = Cache(dev, [40], 512, 64, 3)
+    w = k.randn(1, 256, 512, std=0.04)
+    wide = torch.zeros(1, 2 ** 31 // 64 - 1, dtype=torch.int32, device=dev)
+    with pytest.raises(RuntimeError, match="too wide"):
+        ops.latent_decode_attention(k.randn(1, 192), k.cache, w, wide, k.ctx, 1)
+    n, ctx = 65535, 2200000
+    plan = ops.latent_prefill_plan([n], [ctx], dev)
+    with pytest.raises(RuntimeError, match="too many"):
+        ops.latent_prefill_attention(k.randn(n, 192), k.cache, w, plan, wide[:, :ctx // 64 + 1].contiguous(), 1,
+                                     form="absorbed")
+    # a wide table by itself is in order: entries behind the context are not looked at
+    q = k.randn(1, 192)
+    far = wide[:, :2 ** 24].contiguous()
+    far[:, 2:] = -1
+    far[:, :2] = k.bt[:, :1].expand(1, 2)
+    exp, tol = decode64(q.view(1, 192), k.rows[0], w, 1 / math.sqrt(192))
+    within(ops.latent_decode_attention(q, k.cache, w, far, k.ctx, 1).view(1, 128), exp, tol)
+    no_error(dev)
+
+
 PREFILLS = [([1], [1]), ([17], [17]), ([130], [130]), ([128, 256], [128, 300]), ([300, 0, 1, 64], [557, 9, 900, 64]),
             ([257, 129, 5, 385], [257, 513, 1000, 400]), ([128, 3, 100, 1, 64], [128, 129, 640, 2500, 385])]
 
