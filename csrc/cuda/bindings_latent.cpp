@@ -3,6 +3,10 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <algorithm>
+#include <utility>
+#include <vector>
+
 #include "common.cuh"
 #include "kernels.h"
 
@@ -45,6 +49,23 @@ bool same_view(const Tensor& a, const Tensor& b) {
 // Strides of dims of one index never step, whatever they say.
 int64_t step(const Tensor& t, int64_t d) { return t.size(d) > 1 ? t.stride(d) : 0; }
 
+// Whether two indexes of a view may share an element: dim by dim, smallest stride first, each has to
+// step over everything inside it.
+bool overlaps_itself(const Tensor& t) {
+  std::vector<std::pair<int64_t, int64_t>> dims;  // stride, size
+  for (int64_t d = 0; d < t.dim(); ++d) {
+    if (t.size(d) == 0) return false;
+    if (t.size(d) > 1) dims.push_back({t.stride(d), t.size(d)});
+  }
+  std::sort(dims.begin(), dims.end());
+  int64_t extent = 1;
+  for (const auto& [stride, size] : dims) {
+    if (stride < extent) return true;
+    extent += (size - 1) * stride;
+  }
+  return false;
+}
+
 // Row pitch of a [rows, width] view, for kernels and tensor maps: that of a lone row never counts.
 int64_t pitch(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
 
@@ -61,8 +82,7 @@ kapsl::RopeArgs rope_args(const char* op, const Tensor& x, const Tensor& y, cons
   TORCH_CHECK(x.dim() == 3 && (x.size(2) <= 1 || x.stride(2) == 1), op, ": x must be [T, H, D] with contiguous heads");
   check(y, x.scalar_type(), x, op, "out");
   TORCH_CHECK(y.sizes() == x.sizes() && (y.size(2) <= 1 || y.stride(2) == 1), op, ": out must have x's shape");
-  for (int64_t d = 0; d < 2; ++d)
-    TORCH_CHECK(step(x, d) >= 0 && (y.size(d) <= 1 || y.stride(d) > 0), op, ": out must not be expanded");
+  TORCH_CHECK(!overlaps_itself(y), op, ": out must not be expanded or overlap itself");
   check(positions, at::kInt, x, op, "positions");
   TORCH_CHECK(positions.dim() == 1 && positions.is_contiguous() && positions.size(0) >= x.size(0), op,
               ": positions must hold an int32 per token");
@@ -83,8 +103,6 @@ kapsl::RopeArgs rope_args(const char* op, const Tensor& x, const Tensor& y, cons
   a.xs_h = step(x, 1);
   a.ys_t = step(y, 0);
   a.ys_h = step(y, 1);
-  TORCH_CHECK(!in_place || ((a.xs_t > 0 || x.size(0) <= 1) && (a.xs_h > 0 || x.size(1) <= 1)), op,
-              ": an expanded tensor cannot be rotated in place");
   a.positions = positions.data_ptr<int32_t>();
   a.cos_sin = cos_sin.data_ptr<float>();
   a.max_pos = (int)cos_sin.size(0);
@@ -175,7 +193,7 @@ void check_heads(const char* op, const Tensor& q, const Tensor& cache, const Ten
   TORCH_CHECK(out.dim() == 2 && out.size(1) == H * kVal && out.stride(1) == 1 && out.size(0) == q.size(0), op,
               ": out must be [T, ", num(H * kVal), "]");
   check_rows16(op, out, "out");
-  TORCH_CHECK(out.size(0) <= 1 || out.stride(0) > 0, op, ": out must not be expanded");
+  TORCH_CHECK(!overlaps_itself(out), op, ": out must not be expanded or overlap itself");
   check(w, at::kBFloat16, q, op, "w_kv_b");
   TORCH_CHECK(w.numel() == H * (kNope + kVal) * R && w.size(-1) == R && w.is_contiguous(), op, ": w_kv_b must be [", num(H),
               " * 256, ", num(R), "] contiguous");

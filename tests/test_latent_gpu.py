@@ -265,6 +265,38 @@ def test_write_padded_rows_need_no_position(dev):
     assert ops.check_errors(dev) == 80
 
 
+def test_refuses_outputs_that_overlap_themselves(dev):
+    """Rows or heads of an output that share memory would be written by several threads."""
+    from kapsl_sdk_b200 import ops
+    from kapsl_sdk_b200.ops import reference as ref
+
+    cs = ref.rope_cos_sin(10, 64, 1e4, device=dev)
+    pos = torch.zeros(4, dtype=torch.int32, device=dev)
+    flat = torch.randn(4096, device=dev).to(torch.bfloat16)
+    x = torch.randn(4, 3, 64, device=dev).to(torch.bfloat16)
+    k = Cache(dev, [40, 50], 512, 16, 3)
+    q, w = k.randn(2, 5 * 192), k.randn(5, 256, 512, std=0.04)
+    plan = ops.latent_prefill_plan([1, 1], [40, 50], dev)
+    kv, nw, slots = k.randn(4, 576), k.randn(512), torch.arange(4, device=dev)
+    shared = flat.as_strided((4, 3, 64), (64, 64, 1))  # a token's second head is the next one's first
+    rows = flat.as_strided((2, 640), (320, 1))
+    before = flat.clone()
+    for bad in (lambda: ops.rope(x, pos, cs, out=shared), lambda: ops.rope(shared, pos, cs, out=shared),
+                lambda: ops.rope(x, pos, cs, out=flat.as_strided((4, 3, 64), (192, 32, 1))),
+                lambda: ops.rope_latent_write(shared, kv, pos, slots, cs, nw, 1e-6, k.cache),
+                lambda: ops.rope_latent_write(x, kv, pos, slots, cs, nw, 1e-6, k.cache, q_out=shared),
+                lambda: ops.latent_decode_attention(q, k.cache, w, k.bt, k.ctx, 5, out=rows),
+                lambda: ops.latent_prefill_attention(q, k.cache, w, plan, k.bt, 5, out=rows)):
+        with pytest.raises(RuntimeError):
+            bad()
+    # heads outside tokens, and tokens outside heads, are both in order; so is reading shared memory
+    good = torch.empty(3, 4, 64, device=dev, dtype=torch.bfloat16).transpose(0, 1)
+    assert torch.equal(ops.rope(x, pos, cs, out=good), ops.rope(x, pos, cs))
+    assert torch.equal(ops.rope(shared, pos, cs), ops.rope(shared.clone(), pos, cs))
+    no_error(dev)
+    assert torch.equal(flat, before)
+
+
 # -------------------------------------------------------------------------- attention
 class Cache:
     """Ragged contexts in permuted pages; what no sequence owns is NaN."""
