@@ -210,7 +210,7 @@ template <int R, bool IL>
 __global__ void __launch_bounds__(256) rope_latent_write_kernel(
     const bf16* q, int64_t qs_t, int64_t qs_h, bf16* qo, int64_t qo_t, int64_t qo_h, const bf16* kv, int64_t kv_stride,
     const int32_t* positions, const int64_t* slots, const float* __restrict__ cos_sin, int max_pos,
-    const bf16* __restrict__ w, float eps, bf16* cache, int64_t num_slots, int T, int H, int latent_blocks, int* err) {
+    const bf16* w, float eps, bf16* cache, int64_t num_slots, int T, int H, int latent_blocks, int* err) {
   griddep_entry();
   constexpr int P = 64, N = 8, half = P / 2;
   constexpr int NU = IL ? P / N : half / N;  // rotating units a head
@@ -257,10 +257,12 @@ __global__ void __launch_bounds__(256) rope_latent_write_kernel(
   }
   const bf16* src = kv + (int64_t)t * kv_stride;
   bf16* dst = cache + slot * (R + P);
-  Vec<bf16, N> v[R / 256];
+  Vec<bf16, N> v[R / 256], ww[R / 256];
   Vec<bf16, N> a, b;
 #pragma unroll
   for (int i = 0; i < R / 256; ++i) v[i] = *reinterpret_cast<const Vec<bf16, N>*>(src + (i * 32 + lane) * N);
+#pragma unroll
+  for (int i = 0; i < R / 256; ++i) ww[i] = *reinterpret_cast<const Vec<bf16, N>*>(w + (i * 32 + lane) * N);
   if (lane < NU) {
     a = *reinterpret_cast<const Vec<bf16, N>*>(src + R + lane * N);
     if (!IL) b = *reinterpret_cast<const Vec<bf16, N>*>(src + R + half + lane * N);
@@ -273,9 +275,8 @@ __global__ void __launch_bounds__(256) rope_latent_write_kernel(
   const float inv = rsqrtf(warp_sum(ss) / (float)R + eps);
 #pragma unroll
   for (int i = 0; i < R / 256; ++i) {
-    const Vec<bf16, N> ww = *reinterpret_cast<const Vec<bf16, N>*>(w + (i * 32 + lane) * N);
 #pragma unroll
-    for (int k = 0; k < N; ++k) v[i].v[k] = from_f<bf16>(to_f(v[i].v[k]) * inv * to_f(ww.v[k]));
+    for (int k = 0; k < N; ++k) v[i].v[k] = from_f<bf16>(to_f(v[i].v[k]) * inv * to_f(ww[i].v[k]));
     *reinterpret_cast<Vec<bf16, N>*>(dst + (i * 32 + lane) * N) = v[i];
   }
   if (lane < NU) {

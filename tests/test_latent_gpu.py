@@ -297,6 +297,32 @@ def test_refuses_outputs_that_overlap_themselves(dev):
     assert torch.equal(flat, before)
 
 
+def test_write_reads_a_weight_just_written(dev):
+    """The norm weight may come from the kernel right before, which lets the write kernel start early."""
+    from kapsl_sdk_b200 import ops
+    from kapsl_sdk_b200.ops import reference as ref
+
+    R, T = 512, 2000
+    cs = ref.rope_cos_sin(10, 64, 1e4, device=dev)
+    pos, slots = torch.zeros(T, dtype=torch.int32, device=dev), torch.arange(T, device=dev)
+    kv = torch.ones(T, R + 64, device=dev, dtype=torch.bfloat16)  # normed: 1 / sqrt(1 + eps) = 1
+    q = torch.zeros(T, 1, 64, device=dev, dtype=torch.bfloat16)
+    w = torch.zeros(1, R, device=dev, dtype=torch.bfloat16)
+    # silu(30) = 30 to a part in 2^43, times 2^i
+    xs = [torch.cat([torch.full((1, R), 30.0), torch.full((1, R), 2.0 ** i)], 1).to(torch.bfloat16).to(dev) for i in range(8)]
+    caches = [torch.zeros(125, 16, R + 64, device=dev, dtype=torch.bfloat16) for _ in range(8)]
+    for _ in range(20):
+        torch.cuda.synchronize()
+        for x, cache in zip(xs, caches):
+            ops.silu_mul(x, out=w)
+            ops.rope_latent_write(q, kv, pos, slots, cs, w[0], 0.0, cache)
+        torch.cuda.synchronize()
+        for i, cache in enumerate(caches):
+            assert bool((cache[..., :R] == 30.0 * 2.0 ** i).all())
+            cache.zero_()
+    no_error(dev)
+
+
 # -------------------------------------------------------------------------- attention
 class Cache:
     """Ragged contexts in permuted pages; what no sequence owns is NaN."""
