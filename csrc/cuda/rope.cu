@@ -71,7 +71,6 @@ template <int N, bool IL>
 struct Angles {
   static constexpr int M = IL ? N / 2 : N;
   float c[M], s[M];
-  __device__ __forceinline__ Angles() {}
   __device__ __forceinline__ Angles(const float* cs, int half, int i) {
     load_cs<M>(cs + i, c);
     load_cs<M>(cs + half + i, s);
@@ -220,8 +219,17 @@ __global__ void __launch_bounds__(256) rope_latent_write_kernel(
     const bool ok = pos >= 0 && pos < max_pos;
     const bf16* src = q + t * qs_t + (int64_t)u * N;
     bf16* dst = qo + t * qo_t + (int64_t)u * N;
-    Angles<N, IL> angles;  // a position outside reads nothing (the table may have no rows at all)
-    if (ok) angles = Angles<N, IL>(cos_sin + (int64_t)pos * P, half, IL ? u * N / 2 : u * N);
+    if (!ok) {  // nothing is read from the table, which may have no rows at all
+      if (src != dst)
+        for (int h = threadIdx.x / NU; h < H; h += step) {
+          *reinterpret_cast<Vec<bf16, N>*>(dst + h * qo_h) = *reinterpret_cast<const Vec<bf16, N>*>(src + h * qs_h);
+          if (!IL)
+            *reinterpret_cast<Vec<bf16, N>*>(dst + h * qo_h + half) =
+                *reinterpret_cast<const Vec<bf16, N>*>(src + h * qs_h + half);
+        }
+      return;
+    }
+    const Angles<N, IL> angles(cos_sin + (int64_t)pos * P, half, IL ? u * N / 2 : u * N);
     for (int h = threadIdx.x / NU; h < H; h += 2 * step) {
       Vec<bf16, N> a[2], b[2];
 #pragma unroll
@@ -236,7 +244,7 @@ __global__ void __launch_bounds__(256) rope_latent_write_kernel(
       for (int k = 0; k < 2; ++k) {
         if (h + k * step < H) {
           bf16* at = dst + (h + k * step) * qo_h;
-          if (ok) angles.rotate(a[k], b[k]);
+          angles.rotate(a[k], b[k]);
           *reinterpret_cast<Vec<bf16, N>*>(at) = a[k];
           if (!IL) *reinterpret_cast<Vec<bf16, N>*>(at + half) = b[k];
         }
