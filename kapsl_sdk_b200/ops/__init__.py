@@ -72,7 +72,10 @@ def describe_error(code: int) -> str:
 
 
 def check_errors(device: torch.device) -> int:
-    """Return (and clear) the first non-zero kernel status word on ``device``."""
+    """Return (and clear) the first non-zero kernel status word on ``device`` (0 for a device that
+    runs no kernels)."""
+    if device.type != "cuda":
+        return 0
     buf = error_buffer(device)
     v = int(buf.max().item())
     if v:

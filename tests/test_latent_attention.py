@@ -126,3 +126,12 @@ def test_scratch_of_prefill_is_bounded(q_lens, ctx_lens, heads, ranges):
     assert room <= ops.LATENT_KV_BYTES
     assert step == 1 or step * (p.kv_rows * 512 + room) <= ops.LATENT_KV_BYTES
     assert p.passes(heads, 1)[1:] == (0, 0, 1)
+
+
+def test_check_errors_of_a_device_without_kernels():
+    """Asking for the CPU's status is answered, and keeps no buffer of it as a GPU's."""
+    before = dict(ops._err_bufs)
+    assert ops.check_errors(torch.device("cpu")) == 0
+    assert ops._err_bufs == before
+    with pytest.raises(RuntimeError):
+        ops.error_buffer(torch.device("cpu"))
