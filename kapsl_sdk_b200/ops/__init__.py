@@ -413,10 +413,10 @@ class LatentPrefillPlan:
         under LATENT_KV_BYTES (one head may take more keys and values than that).  Only row tiles longer
         than a part are cut: the others write no partial results.  One chunk of 256 tokens over 65,536 beside
         500 single tokens, 8 heads: 10 MB of them for one row tile; cutting all 501 took 4.8 GB."""
-        kv = self.kv_rows * 512
+        kv = max(1, self.kv_rows * 512)
         step = max(1, min(num_heads, LATENT_KV_BYTES // kv))
         ranges = key_ranges if key_ranges > 0 else self.key_ranges(step)
-        while ranges > 1:
+        while ranges > 1 and self.key_tiles:
             part = -(-self.key_tiles[0] // ranges)
             cut, slots = sum(n > part for n in self.key_tiles), -(-self.key_tiles[0] // part)
             room = cut * slots * LATENT_PART_BYTES

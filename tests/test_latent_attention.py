@@ -135,3 +135,8 @@ def test_check_errors_of_a_device_without_kernels():
     assert ops._err_bufs == before
     with pytest.raises(RuntimeError):
         ops.error_buffer(torch.device("cpu"))
+
+
+def test_passes_of_nothing():
+    p = ops.latent_prefill_plan([0], [0], device="cpu")
+    assert p.passes(7) == p.passes(7, 4) == (7, 0, 0, 1)
