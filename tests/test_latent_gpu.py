@@ -105,6 +105,26 @@ def test_rope(dev, dtype, interleaved, T, H, D, P, offset):
     no_error(dev)
 
 
+@pytest.mark.parametrize("interleaved,P,offset", [(False, 128, 0), (True, 64, 64)])
+def test_rope_of_a_prompt(dev, interleaved, P, offset):
+    """The served type at a prompt's size, in place and into another buffer."""
+    from kapsl_sdk_b200 import ops
+    from kapsl_sdk_b200.ops import reference as ref
+
+    T, H, D = 6001, 40, 128
+    g = torch.Generator(device=dev).manual_seed(1)
+    cs = ref.rope_cos_sin(8192, P, 1e4, device=dev)
+    pos = torch.arange(1000, 1000 + T, device=dev, dtype=torch.int32)
+    x = torch.randn(T, H, D, generator=g, device=dev).to(torch.bfloat16)
+    out = ops.rope(x, pos, cs, offset, interleaved)
+    for t0 in range(0, T, 1500):
+        part = slice(t0, t0 + 1500)
+        exp, mag = rope64(x[part], pos[part], cs, offset, interleaved)
+        within(out[part], exp, U * exp.abs() + 4 * 2.0 ** -24 * mag)
+    assert torch.equal(ops.rope(x, pos, cs, offset, interleaved, out=x), out)
+    no_error(dev)
+
+
 def test_rope_empty_and_positions_outside(dev):
     from kapsl_sdk_b200 import ops
     from kapsl_sdk_b200.ops import reference as ref
@@ -1129,6 +1149,73 @@ def test_graphs_streams_and_repeats(dev):
     for i in range(2):
         for o in got[i]:
             assert torch.equal(o, exp[i])
+    no_error(dev)
+
+
+@pytest.mark.parametrize("H,R", [(20, 512), (128, 512), (70, 256)])
+def test_captured_decode_follows_lengths_and_tables(dev, H, R):
+    """A captured call replayed with other lengths and block tables: longer and shorter contexts, rows that
+    became empty or filled, the eager results bit for bit."""
+    from kapsl_sdk_b200 import ops
+
+    k = Cache(dev, [900, 33, 400, 1, 700, 64], R, 16, H)
+    B = len(k.rows)
+    q, w = k.randn(B, H * 192), k.randn(H * 256, R, std=1 / math.sqrt(R))
+    bt, ctx = k.bt.clone(), torch.tensor([10, 0, 400, 1, 0, 64], dtype=torch.int32, device=dev)
+
+    def run():
+        return ops.latent_decode_attention(q, k.cache, w, bt, ctx, H)
+
+    run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    for order, lens in (((0, 1, 2, 3, 4, 5), (900, 33, 400, 1, 700, 64)), ((4, 2, 0, 5, 3, 1), (650, 0, 899, 17, 1, 33)),
+                        ((5, 4, 3, 2, 1, 0), (0, 0, 0, 0, 0, 0)), ((2, 2, 2, 2, 2, 2), (400, 128, 129, 1, 0, 16))):
+        bt.copy_(k.bt[list(order)])
+        ctx.copy_(torch.tensor(lens, dtype=torch.int32))
+        q.copy_(k.randn(B, H * 192))
+        for _ in range(2):
+            graph.replay()
+        torch.cuda.synchronize()
+        got = out.clone()
+        assert torch.equal(got, run())
+        for b in range(B):
+            exp, tol = decode64(q[b].view(H, 192), k.rows[order[b]][:lens[b]], w.view(H, 256, R), 1 / math.sqrt(192))
+            within(got[b].view(H, 128), exp, tol)
+    no_error(dev)
+
+
+def test_captured_prefill_in_parts(dev):
+    """A captured call whose long context is cut, replayed with other queries and beside eager calls on another
+    stream."""
+    from kapsl_sdk_b200 import ops
+
+    H, q_lens, ctx_lens = 4, [200, 30], [5000, 300]
+    k = Cache(dev, ctx_lens, 512, 16, 60)
+    q, w = k.randn(230, H * 192), k.randn(H * 256, 512, std=1 / math.sqrt(512))
+    plan = ops.latent_prefill_plan(q_lens, ctx_lens, dev)
+    assert plan.passes(H)[1] == 1 and plan.work.shape[0] == 2
+
+    def run():
+        return ops.latent_prefill_attention(q, k.cache, w, plan, k.bt, H, form="expanded")
+
+    run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    side = torch.cuda.Stream()
+    for _ in range(3):
+        q.copy_(k.randn(230, H * 192))
+        exp = run()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            other = [run() for _ in range(3)]
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, exp) and all(torch.equal(o, exp) for o in other)
     no_error(dev)
 
 
