@@ -12,9 +12,11 @@
 //
 // Roundings: qa and P become bf16 because the cache does not change its type and both
 // operands of an MMA share theirs; halves of more bits would cost a second pass over every key
-// tile's products, which bound the kernel.  The joined o keeps 16 bits in two bf16.  Each
-// rounding is 2^-9 of a value at most and 0.0017 in the mean square: an output is 0.0024-0.0028
-// from 64-bit arithmetic, where one rounded once at the end is 0.0017.
+// tile's products, which bound the kernel above some 32 heads.  With few heads it waits for DRAM
+// and such a pass might hide; one precision is kept, so that a model's accuracy does not depend on
+// how its heads are sharded.  The joined o keeps 16 bits in two bf16.  Each rounding is 2^-8 of
+// a value at most and 0.0017 in the mean square: an output is 0.0024-0.0028 from 64-bit
+// arithmetic, where one rounded once at the end is 0.0017.
 #include <algorithm>
 
 #include "common.cuh"
@@ -659,7 +661,9 @@ __global__ void __launch_bounds__(kAttnThreads<R>, 1)
 //
 // Whole calls, 64-head tiles and pairs: 192 x 8192 tokens x 128 heads 674 and 508 us, 64 x 4096 x 128 145
 // and 119, 64 x 500 x 128 56 and 51, 16 x 1000 x 80 31 and 30; at 64 heads and fewer, where half
-// of the MMA's rows would be empty, 151 and 189 (64 x 8192 x 64).  A tile takes 4,100 cycles where its
+// of the MMA's rows would be empty, 151 and 189 (64 x 8192 x 64).  With L2 flushed 8 x 2048 x 128 41 and
+// 41, 4 x 1000 x 128 37 and 35; a lone request loses by the pairs' longer set-up and piece's
+// end, 1 x 2048 x 128 33 and 34, 1 x 2048 x 80 29 and 31, 1 x 512 x 128 29 and 33.  A tile takes 4,100 cycles where its
 // MMAs alone would take 2,500 (S 1,460, second product 1,050): operands, arriving chunks and P
 // share the shared memory, and loads from L2 run at 5.9 TB/s over the GPU.  The end of a piece
 // (queries to tensor memory, partial result) takes 19,000 cycles; a form that turned the queries in
@@ -727,8 +731,8 @@ __device__ __forceinline__ bool try_wait_cluster(uint64_t* bar, uint32_t parity)
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     latent_attn_pair_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap c_map,
                             const bf16* qa, const bf16* cache, int64_t num_blocks, int page,
-                            const int32_t* block_tables, int max_blocks, const int32_t* table_rows, int num_tables, const int32_t* ctx_lens,
-                            const int32_t* table, float* part_o, float2* part_ml, int B, int H,
+                            const int32_t* block_tables, int max_blocks, const int32_t* table_rows, int num_tables,
+                            const int32_t* ctx_lens, const int32_t* table, float* part_o, float2* part_ml, int B, int H,
                             int heads_per_cta, int head_tiles, float scale_log2, int* err) {
   griddep_launch();
   constexpr int R = 512, W = R + kRot;
@@ -1664,8 +1668,8 @@ void run_pairs(const LatentDecode& a, const Plan& p, const bf16* qa, float* part
   const CUtensorMap tq = make_tmap_2d_bf16(qa, (uint64_t)a.B * a.H, W, W, 128, 64, true);
   const CUtensorMap tc = make_tmap_2d_bf16(a.cache, (uint64_t)a.num_blocks * a.page, W, W, a.page, 64, true);
   launch_k(latent_attn_pair_kernel, dim3(2 * p.ctas * p.head_tiles), kPairThreads, sizeof(PairSmem), st, tq, tc, qa,
-           static_cast<const bf16*>(a.cache), a.num_blocks, a.page, a.block_tables, a.max_blocks, a.table_rows, a.num_tables, a.ctx_lens, table, part_o,
-           part_ml, a.B, a.H, p.heads_per_cta, p.head_tiles, a.scale * kLog2e, a.err);
+           static_cast<const bf16*>(a.cache), a.num_blocks, a.page, a.block_tables, a.max_blocks, a.table_rows,
+           a.num_tables, a.ctx_lens, table, part_o, part_ml, a.B, a.H, p.heads_per_cta, p.head_tiles, a.scale * kLog2e, a.err);
   KAPSL_LAUNCH_CHECK();
 }
 

@@ -8,7 +8,7 @@
 // Roundings: the expanded keys and values are bf16, the type of the query's rows that the first
 // product takes and half the bytes of fp32, and so is P, the second product's operand (sums
 // are fp32).  fp16 would keep 3 bits more, but not every model's values are within its range.  With the
-// output's own, three roundings of 2^-9 at most: an output is 0.0029 from 64-bit arithmetic
+// output's own, three roundings of 2^-8 at most: an output is 0.0029 from 64-bit arithmetic
 // in the mean square, where one rounded once at the end is 0.0017.
 #include <algorithm>
 

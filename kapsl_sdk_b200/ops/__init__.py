@@ -360,8 +360,8 @@ def latent_decode_attention(q: torch.Tensor, cache: torch.Tensor, w_kv_b: torch.
     half is applied to the attended latents, so nothing is expanded per cached token.
     ``q`` [B, H * 192] has 128 position-free and 64 rotated dims a head; ``out`` is
     [B, H * 128].  Rows with ``ctx_lens`` 0 (a padded batch) and rows whose scores are all -inf give
-    zeros.  ``max_ctx`` (a host number, default the block tables' width) only bounds how many
-    CTAs are launched.
+    zeros; a context longer than its block table is cut to the table.  ``max_ctx`` (a host number,
+    default the block tables' width) only bounds how many CTAs are launched.
     The keys of a block table entry outside the cache read as zeros, and device error 82 is recorded."""
     if scale is None:
         scale = 1.0 / math.sqrt(192)
@@ -401,10 +401,10 @@ class LatentPrefillPlan:
     key_tiles: list[int]    # 128-key tiles of each row tile, in the order of work (most first)
 
     def key_ranges(self, num_heads: int) -> int:
-        """Parts into which the expanded form cuts every row tile's keys: as often as the longest row tile
-        by itself takes what all of them take spread over the 148 SMs, parts of 4 key tiles or
-        more.  512 new tokens over 16384, 20 heads: 331 us whole, 187 in three parts; row tiles that
-        fill the GPU stay whole, since parts cost fp32 partial results and a joining kernel."""
+        """Parts into which the expanded form cuts the longest row tile's keys: as often as it takes by
+        itself what all row tiles take spread over the 148 SMs, parts of 4 key tiles or more.  512
+        new tokens over 16384, 20 heads: 331 us whole, 188 in three parts; row tiles that fill the
+        GPU stay whole, since parts cost fp32 partial results and a joining kernel."""
         spread = max(4.0, 1.9 * self.row_tiles * num_heads / 148)
         return max(1, min(32, -(-self.max_ctx // 128) // 4, int(self.chain_us / spread)))
 
@@ -427,12 +427,15 @@ class LatentPrefillPlan:
 
     def absorbed_is_shorter(self, num_heads: int, rank: int = 512) -> bool:
         """Whether taking every new token by itself in the absorbed form is estimated to take less time
-        than expanding the contexts.  In microseconds, fitted to both forms' times on B200 (148
-        SMs) over some 40 ragged batches: absorbed, a 64-key tile of up to 64 heads 3.0 (rank 256: 1.4) of
-        an SM, of 65 - 128 heads 2.6 (rank 256: 2.8), and 2 for a thousand rows x heads of head products; expanded, 256 context rows of a head
-        4.5 (2.3) of an SM pair, a 128-key tile of 256 new tokens 1.9 of an SM, or the longest row
-        tile by itself, or a key range of it and 9 for the join.  20 new tokens over 4020, 8
-        heads: 37 and 46; five prompts of 17 to 300 tokens, 28 heads: 98 and 59."""
+        than expanding the contexts.  In microseconds, fitted to both forms' times on a B200's 148
+        SMs over some 40 ragged batches: absorbed, a 64-key tile of up to 64 heads 3.0 (rank 256:
+        1.4) of an SM, of 65 - 128 heads 2.6 (rank 256: 2.8), and 2 for a thousand rows x heads of
+        head products; expanded, 256 context rows of a head 4.5 (2.3) of an SM pair, a 128-key tile
+        of 256 new tokens 1.9 of an SM, or the longest row tile by itself, or a part of it and 9 for
+        the join.  20 new tokens over 4020, 8 heads: 37 and 46; five prompts of 17 to 300 tokens, 28
+        heads: 98 and 59.  Small absorbed calls of more than 64 heads take up to 1.5 times the
+        estimate (45 us for 30), where the choice was still right to a few percent.  One choice is made
+        for the whole call: a few tokens over a long context beside a long prompt take its form."""
         rows, wide, ranges = self.rows - self.q_start, rank > 256, self.key_ranges(num_heads)
         start = 19 if -(-rows // 16) * num_heads <= 256 else 26
         tile = (2.6 * -(-num_heads // 128) if wide and num_heads > 64 else
