@@ -66,6 +66,19 @@ bool overlaps_itself(const Tensor& t) {
   return false;
 }
 
+// Whether kv [T, n] shares elements with the heads q [T, H, D] of the same buffer's rows (a fused
+// projection's), each row's heads taken as one stretch.  Only views of one row pitch are judged.
+bool rows_meet(const Tensor& kv, const Tensor& q) {
+  if (!ranges_meet(kv, q)) return false;
+  const int64_t heads = step(q, 1) * (q.size(1) - 1) + q.size(2), width = kv.size(1);
+  int64_t at = ((const char*)kv.data_ptr() - (const char*)q.data_ptr()) / q.element_size();
+  if (q.size(0) == 1) return at < heads && at + width > 0;
+  const int64_t pitch = q.stride(0);
+  if (kv.stride(0) != pitch || heads > pitch) return false;
+  at = (at % pitch + pitch) % pitch;  // kv's start behind the heads', in a row
+  return at < heads || at + width > pitch;
+}
+
 // Row pitch of a [rows, width] view, for kernels and tensor maps: that of a lone row never counts.
 int64_t pitch(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
 
@@ -166,7 +179,7 @@ void rope_latent_write(Tensor q, Tensor q_out, Tensor kv, Tensor positions, Tens
   TORCH_CHECK((reinterpret_cast<uintptr_t>(cos_sin.data_ptr()) & 15) == 0, op, ": cos_sin must be 16-byte aligned");
   TORCH_CHECK(q.size(0) <= INT32_MAX, op, ": too many tokens");
   TORCH_CHECK(!ranges_meet(cache, kv) && !ranges_meet(cache, q_out), op, ": the cache must not overlap kv or q");
-  TORCH_CHECK(!ranges_meet(kv, q_out) || q_out.data_ptr() == q.data_ptr(), op, ": q_out must not overlap kv");
+  TORCH_CHECK(a.in_place ? !rows_meet(kv, q) : !ranges_meet(kv, q_out), op, ": the query heads written must not overlap kv");
   const c10::cuda::CUDAGuard g(q.device());
   kapsl::launch_rope_latent_write(a, bf(kv), kv.size(0) > 1 ? kv.stride(0) : 0, slots.data_ptr<int64_t>(), bf(w),
                                   (float)eps, bf(cache), cache.size(0) * cache.size(1), (int)R, cur_stream());

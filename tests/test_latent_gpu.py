@@ -343,6 +343,31 @@ def test_write_reads_a_weight_just_written(dev):
     no_error(dev)
 
 
+def test_write_refuses_latents_that_its_queries_overwrite(dev):
+    """In one projection's rows the latents may lie before or behind the heads, not among them."""
+    from kapsl_sdk_b200 import ops
+    from kapsl_sdk_b200.ops import reference as ref
+
+    T, H, R = 5, 2, 256
+    cs = ref.rope_cos_sin(10, 64, 1e4, device=dev)
+    pos, slots = torch.arange(T, dtype=torch.int32, device=dev), torch.arange(T, device=dev)
+    cache = torch.zeros(1, 16, R + 64, dtype=torch.bfloat16, device=dev)
+    w = torch.ones(R, dtype=torch.bfloat16, device=dev)
+    y = torch.randn(T, 2 * (R + 64) + H * 192, device=dev).to(torch.bfloat16)
+    q = y[:, R + 64:R + 64 + H * 192].view(T, H, 192)[..., 128:]
+    for at in (0, R + 64 + H * 192):
+        for n in (T, 1):
+            ops.rope_latent_write(q[:n], y[:n, at:at + R + 64], pos, slots, cs, w, 1e-6, cache)
+    no_error(dev)
+    before = y.clone()
+    for at in (R + 64, R + 64 + 192, R + 64 + H * 192 - 8):
+        for n in (T, 1):
+            with pytest.raises(RuntimeError, match="overlap kv"):
+                ops.rope_latent_write(q[:n], y[:n, at:at + R + 64], pos, slots, cs, w, 1e-6, cache)
+    assert torch.equal(y, before)
+    no_error(dev)
+
+
 # -------------------------------------------------------------------------- attention
 class Cache:
     """Ragged contexts in permuted pages; what no sequence owns is NaN."""
