@@ -67,7 +67,7 @@ bool overlaps_itself(const Tensor& t) {
 }
 
 // Whether kv [T, n] shares elements with the heads q [T, H, D] of the same buffer's rows (a fused
-// projection's), each row's heads taken as one stretch.  Only views of one row pitch are judged.
+// projection's), each row's heads taken as one stretch.  Views of other row pitches are not compared.
 bool rows_meet(const Tensor& kv, const Tensor& q) {
   if (!ranges_meet(kv, q)) return false;
   const int64_t heads = step(q, 1) * (q.size(1) - 1) + q.size(2), width = kv.size(1);
@@ -179,7 +179,8 @@ void rope_latent_write(Tensor q, Tensor q_out, Tensor kv, Tensor positions, Tens
   TORCH_CHECK((reinterpret_cast<uintptr_t>(cos_sin.data_ptr()) & 15) == 0, op, ": cos_sin must be 16-byte aligned");
   TORCH_CHECK(q.size(0) <= INT32_MAX, op, ": too many tokens");
   TORCH_CHECK(!ranges_meet(cache, kv) && !ranges_meet(cache, q_out), op, ": the cache must not overlap kv or q");
-  TORCH_CHECK(a.in_place ? !rows_meet(kv, q) : !ranges_meet(kv, q_out), op, ": the query heads written must not overlap kv");
+  TORCH_CHECK(a.in_place ? !rows_meet(kv, q) : !ranges_meet(kv, q_out), op,
+              ": the query heads written must not overlap kv");
   const c10::cuda::CUDAGuard g(q.device());
   kapsl::launch_rope_latent_write(a, bf(kv), kv.size(0) > 1 ? kv.stride(0) : 0, slots.data_ptr<int64_t>(), bf(w),
                                   (float)eps, bf(cache), cache.size(0) * cache.size(1), (int)R, cur_stream());
@@ -341,7 +342,8 @@ void check_latent_prefill(Tensor q, Tensor cache, Tensor w, Tensor block_tables,
 
 // attention of `heads` heads: q / out already narrowed to them
 void latent_prefill(Tensor q, Tensor kv, Tensor k_rope, Tensor work, Tensor seq_info, Tensor out, int64_t heads,
-                    double scale, int64_t cut, int64_t part_tiles, int64_t slots, c10::optional<Tensor> parts, Tensor err) {
+                    double scale, int64_t cut, int64_t part_tiles, int64_t slots, c10::optional<Tensor> parts,
+                    Tensor err) {
   const char* op = "latent_prefill";
   TORCH_CHECK(q.is_cuda(), op, ": q must be a CUDA tensor");
   check(q, at::kBFloat16, q, op, "q");

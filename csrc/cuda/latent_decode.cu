@@ -1669,7 +1669,8 @@ void run_pairs(const LatentDecode& a, const Plan& p, const bf16* qa, float* part
   const CUtensorMap tc = make_tmap_2d_bf16(a.cache, (uint64_t)a.num_blocks * a.page, W, W, a.page, 64, true);
   launch_k(latent_attn_pair_kernel, dim3(2 * p.ctas * p.head_tiles), kPairThreads, sizeof(PairSmem), st, tq, tc, qa,
            static_cast<const bf16*>(a.cache), a.num_blocks, a.page, a.block_tables, a.max_blocks, a.table_rows,
-           a.num_tables, a.ctx_lens, table, part_o, part_ml, a.B, a.H, p.heads_per_cta, p.head_tiles, a.scale * kLog2e, a.err);
+           a.num_tables, a.ctx_lens, table, part_o, part_ml, a.B, a.H, p.heads_per_cta, p.head_tiles,
+           a.scale * kLog2e, a.err);
   KAPSL_LAUNCH_CHECK();
 }
 
